@@ -37,6 +37,9 @@ SOURCES = [
     "gemm_f32.hip",
     "attn.hip",
     "attn_wave.hip",
+    "kvcache.hip",
+    "paged_attn.hip",
+    "logits.hip",
 ]
 
 COMMON_FLAGS = [
@@ -53,9 +56,11 @@ COMMON_FLAGS = [
 
 
 # Per-source extra flags.  RoPE reproduces the reference's separately rounded
-# products and sum, so multiply-add contraction is off for that file.
+# products and sum, so multiply-add contraction is off for that file, and for
+# the cache's, whose 8-bit values are those of the same sums.
 EXTRA_FLAGS = {
     "rope.hip": ["-ffp-contract=off"],
+    "kvcache.hip": ["-ffp-contract=off"],
 }
 
 

@@ -134,6 +134,11 @@ Slot kSlots[] = {
     LZ_ENTRY(lz_dropout),
     LZ_ENTRY(lz_dropout_mask),
     LZ_ENTRY(lz_attn_bwd),
+    LZ_ENTRY(lz_kv_write),
+    LZ_ENTRY(lz_kv_read),
+    LZ_ENTRY(lz_paged_attn_workspace),
+    LZ_ENTRY(lz_paged_attn),
+    LZ_ENTRY(lz_process_logits),
 };
 
 PyObject* bind(PyObject*, PyObject* args) {

@@ -21,6 +21,7 @@ LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
 F32 = 0
 BF16 = 1
 F16 = 2
+E4M3 = 8  # float8_e4m3fn storage of a key/value cache
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -132,6 +133,32 @@ SIGNATURES = {
         [
             _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
             _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _i32, _vp,
+        ],
+    ),
+    "lz_kv_write": (
+        _i32,
+        [
+            _vp, _i64, _i32, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _vp, _i64, _vp,
+            _vp, _i64, _i64, _i64, _i64, _vp,
+        ],
+    ),
+    "lz_kv_read": (
+        _i32,
+        [_vp, _vp, _vp, _vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i32, _i64, _vp],
+    ),
+    "lz_paged_attn_workspace": (_i64, [_i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "lz_paged_attn": (
+        _i32,
+        [
+            _vp, _i64, _i32, _i64, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
+            _i64, _i64, _f32, _vp, _i64, _vp, _i64, _vp,
+        ],
+    ),
+    "lz_process_logits": (
+        _i32,
+        [
+            _vp, _i64, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _f32, _vp, _f32, _vp, _f32, _vp, _i64, _vp,
+            _i32, _i64, _vp, _i64, _vp,
         ],
     ),
 }

@@ -1,0 +1,120 @@
+"""The paged key/value cache of generation.
+
+LayerCache and CacheStep are what the kernels take (ops.kv_cache_write,
+ops.paged_attention, ops.kv_cache_read); KVCache owns the pages of a model's
+layers and hands them to sequences.  The reference has no cache: its generate
+(model/llama.py:311-335) runs the whole window through the model for every
+token.
+"""
+from __future__ import annotations
+
+from typing import List, NamedTuple, Optional, Sequence, Tuple
+
+import torch
+
+from . import ops
+
+
+class LayerCache(NamedTuple):
+    """One layer's pages, [pages, KV heads, page size, head dim] each, in the
+    model's dtype, or float8_e4m3fn with int8 exponents [pages, KV heads, page
+    size]: the value is the stored number times 2^exponent."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_exp: Optional[torch.Tensor] = None
+    v_exp: Optional[torch.Tensor] = None
+
+
+class CacheStep(NamedTuple):
+    """The new tokens of one pass through the layers.  Device tensors, int32:
+    row_start [B + 1] (sequence b's new tokens are rows row_start[b] ..
+    row_start[b + 1] - 1), kv_len [B] (its length with them), page_table
+    [B, pages of the longest].  Host numbers: rows = row_start[B], and upper
+    bounds max_new and max_len of the new and of all tokens of a sequence."""
+
+    row_start: torch.Tensor
+    kv_len: torch.Tensor
+    page_table: torch.Tensor
+    rows: int
+    max_new: int
+    max_len: int
+
+
+class KVCache:
+    """Pages for n_layers layers and up to `batch` sequences.
+
+    storage: the model's dtype (None) or torch.float8_e4m3fn.  n_pages pages
+    are shared by all sequences: each takes pages as it grows, a page holding
+    page_size of its tokens in every layer, and free() gives them back."""
+
+    def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, *, batch: int, n_pages: int, page_size: int = 64,
+                 dtype: torch.dtype = torch.bfloat16, storage: Optional[torch.dtype] = None, device="cuda") -> None:
+        if head_dim not in (32, 64, 128):
+            raise ValueError(f"the cache's kernels take head dims 32, 64 and 128, not {head_dim}")
+        if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+            raise ValueError(f"page size must be a power of two from 16 to 1024, got {page_size}")
+        if min(n_layers, n_kv_heads, batch, n_pages) < 1:
+            raise ValueError("layers, heads, sequences and pages must be positive")
+        if dtype not in ops._DTYPES:
+            raise TypeError(f"a cache holds float32, bfloat16 or float16 rows, not {dtype}")
+        if storage not in (None, dtype, torch.float8_e4m3fn):
+            raise TypeError(f"a cache stores {dtype} or torch.float8_e4m3fn, not {storage}")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise RuntimeError(f"llama-zero HIP kernels run on a ROCm GPU; got device {self.device}")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.dtype, self.page_size, self.n_pages = dtype, page_size, n_pages
+        eight = storage == torch.float8_e4m3fn
+        shape = (n_layers, n_pages, n_kv_heads, page_size, head_dim)
+        store = torch.float8_e4m3fn if eight else dtype
+        self._k, self._v = (torch.empty(shape, dtype=store, device=self.device) for _ in range(2))
+        exps: List[Optional[torch.Tensor]] = [None, None]
+        if eight:
+            exps = [torch.empty(shape[:4], dtype=torch.int8, device=self.device) for _ in range(2)]
+        self.layers = [LayerCache(self._k[i], self._v[i], *(None if e is None else e[i] for e in exps))
+                       for i in range(n_layers)]
+        self.lengths = [0] * batch
+        self._pages: List[List[int]] = [[] for _ in range(batch)]
+        self._free = list(range(n_pages - 1, -1, -1))
+
+    def _page_table(self, which: Sequence[int]) -> List[List[int]]:
+        width = max(1, max(len(self._pages[b]) for b in which))
+        return [self._pages[b] + [-1] * (width - len(self._pages[b])) for b in which]
+
+    def step(self, new: Sequence[int]) -> CacheStep:
+        """Room for new[b] more tokens of every sequence b (0: none) and the
+        CacheStep that the layers' calls take.  Nothing changes if the pages
+        do not suffice."""
+        if len(new) != len(self.lengths):
+            raise ValueError(f"{len(new)} counts of new tokens for {len(self.lengths)} sequences")
+        if min(new) < 0:
+            raise ValueError("counts of new tokens must not be negative")
+        want = [-(-(n + l) // self.page_size) - len(p) for n, l, p in zip(new, self.lengths, self._pages)]
+        if sum(want) > len(self._free):
+            raise RuntimeError(f"the cache has {len(self._free)} free pages of {self.page_size} tokens; {sum(want)} "
+                               "more are needed: free() sequences or make it larger")
+        starts = [0]
+        for b, n in enumerate(new):
+            self._pages[b] += [self._free.pop() for _ in range(want[b])]
+            self.lengths[b] += n
+            starts.append(starts[-1] + n)
+        B, table = len(new), self._page_table(range(len(new)))
+        flat = torch.tensor(starts + self.lengths + [p for row in table for p in row], dtype=torch.int32)
+        flat = flat.to(self.device)
+        return CacheStep(flat[: B + 1], flat[B + 1 : 2 * B + 1], flat[2 * B + 1 :].view(B, -1), starts[-1], max(new),
+                         max(self.lengths))
+
+    def free(self, b: int) -> None:
+        """Ends sequence b: its pages go back, and its slot is empty."""
+        self._free += reversed(self._pages[b])
+        self._pages[b], self.lengths[b] = [], 0
+
+    def read(self, layer: int, b: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Sequence b's keys and values in one layer, [tokens, KV heads, head
+        dim] each, in the model's dtype."""
+        n, kv = self.lengths[b], self.layers[layer]
+        flat = torch.tensor([0, n] + self._page_table([b])[0], dtype=torch.int32).to(self.device)
+        k, v = ops.kv_cache_read(kv, flat[2:].view(1, -1), flat[:2], n, self.dtype)
+        return k.view(n, *kv.k.shape[1::2]), v.view(n, *kv.v.shape[1::2])

@@ -1201,3 +1201,240 @@ def attn_bwd(q2, k2, v2, o2, do2, lse, B, S, H, KV, hd, scale, dq2, dk2, dv2, qt
               _ptr(dot), dq2.data_ptr(), _row_stride(dq2), dk2.data_ptr(), _row_stride(dk2), dv2.data_ptr(),
               _row_stride(dv2), B, S, H, KV, hd, float(scale), _ptr(rc), _ptr(rs), dtype_code(q2),
               stream_ptr(q2.device))
+
+
+# ---------------------------------------------------------------------------
+# generation from a paged key/value cache (see lzhip/cache.py)
+# ---------------------------------------------------------------------------
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """_lib.call with `device` current (a kernel goes to the current device,
+    whatever its stream belongs to)."""
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, stream_ptr(device))
+
+
+def _int32_table(t: torch.Tensor, name: str, device: torch.device, dim: int = 1) -> None:
+    if t.dtype != torch.int32 or t.dim() != dim or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {dim} dimension(s), got {t.dtype} "
+                         f"{tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the rows on {device}")
+
+
+def _cache_args(layer, dtype: torch.dtype, device: torch.device) -> Tuple[tuple, int, int]:
+    """(pointer and shape arguments of a LayerCache, KV heads, head dim)."""
+    k, v, k_exp, v_exp = layer
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or v.dtype != k.dtype or not (k.is_contiguous() and v.is_contiguous()):
+        raise ValueError(f"cache pages must be two contiguous [pages, KV heads, page size, head dim] tensors of one "
+                         f"dtype, got {k.dtype} {tuple(shape)} and {v.dtype} {tuple(v.shape)}")
+    if k.device != device or v.device != device:
+        raise ValueError(f"the cache is on {k.device} and {v.device}, the rows on {device}")
+    if k.dtype == torch.float8_e4m3fn:
+        for e in (k_exp, v_exp):
+            if e is None or e.dtype != torch.int8 or e.shape != shape[:3] or not e.is_contiguous() or e.device != device:
+                raise ValueError("a float8_e4m3fn cache needs contiguous int8 exponents of its [pages, KV heads, page "
+                                 "size] beside it")
+        code, ke, ve = _lib.E4M3, k_exp.data_ptr(), v_exp.data_ptr()
+    else:
+        if k.dtype != dtype or k_exp is not None or v_exp is not None:
+            raise TypeError(f"a cache of {k.dtype} {'with' if k_exp is not None else 'without'} exponents does not "
+                            f"hold {dtype} rows")
+        code, ke, ve = _DTYPES[dtype], None, None
+    return (k.data_ptr(), v.data_ptr(), ke, ve, code, shape[0], shape[2]), shape[1], shape[3]
+
+
+def _step_rows(step, device: torch.device) -> int:
+    """B of a CacheStep, checked."""
+    _int32_table(step.row_start, "row_start", device)
+    _int32_table(step.kv_len, "kv_len", device)
+    _int32_table(step.page_table, "page_table", device, 2)
+    B = step.kv_len.numel()
+    if step.row_start.numel() != B + 1 or step.page_table.size(0) != B or B == 0 or step.page_table.size(1) == 0:
+        raise ValueError(f"a step of {B} sequences needs {B + 1} row starts and a page table of {B} rows, got "
+                         f"{step.row_start.numel()} and {tuple(step.page_table.shape)}")
+    return B
+
+
+def _aligned_rows(t: torch.Tensor, name: str, cols: int) -> torch.Tensor:
+    """t as 2-D rows of `cols` whose starts are 16-byte aligned (a copy if they
+    are not)."""
+    if t.dim() != 2 or t.size(1) != cols or (t.stride(1) != 1 and cols > 1):
+        raise ValueError(f"{name} must be rows of {cols} adjacent values, got {tuple(t.shape)} with strides {t.stride()}")
+    if t.size(0) > 1 and t.stride(0) < cols:
+        raise ValueError(f"{name}: rows overlap (stride {t.stride(0)})")
+    if t.data_ptr() % 16 or _row_stride(t) * t.element_size() % 16:
+        return copy2d(t, torch.empty(t.shape, dtype=t.dtype, device=t.device))
+    return t
+
+
+def _row_output(out: Optional[torch.Tensor], rows: int, cols: int, like: torch.Tensor, all_used: bool) -> torch.Tensor:
+    """The output rows: the caller's, whose rows of no sequence are left as
+    they are, or new ones, where those are zeros."""
+    if out is None:
+        if all_used:
+            return torch.empty((rows, cols), dtype=like.dtype, device=like.device)
+        return zeros((rows, cols), like.dtype, like.device)
+    if out.dtype != like.dtype or tuple(out.shape) != (rows, cols) or out.device != like.device or out.stride(1) != 1 \
+            or (rows > 1 and out.stride(0) < cols) or out.data_ptr() % 16 \
+            or _row_stride(out) * out.element_size() % 16:
+        raise ValueError(f"out must be {like.dtype} rows [{rows}, {cols}] on {like.device}, 16-byte aligned")
+    return out
+
+
+def kv_cache_write(qkv: torch.Tensor, layer, step, n_heads: int, cos: torch.Tensor, sin: torch.Tensor,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Writes a step's keys and values into a layer's pages and returns the
+    rotated queries [rows, n_heads * hd].
+
+    qkv: [rows, (n_heads + 2 * KV) * hd], the fused projection before RoPE;
+    layer: LayerCache, layer.k of qkv's dtype or float8_e4m3fn; step:
+    CacheStep; cos/sin: RoPE tables [>= step.max_len, hd] in qkv's dtype.
+    Rotation, rounding and 8-bit storage: lz_kv_write."""
+    require_gpu(qkv, cos, sin, layer.k, layer.v, step.row_start, step.kv_len, step.page_table, out)
+    dev, dtype = qkv.device, qkv.dtype
+    code = dtype_code(qkv)
+    cache, KV, hd = _cache_args(layer, dtype, dev)
+    B = _step_rows(step, dev)
+    rows = qkv.size(0)
+    qkv = _aligned_rows(qkv, "qkv", (n_heads + 2 * KV) * hd)
+    for t in (cos, sin):
+        if t.dtype != dtype or t.dim() != 2 or t.size(1) != hd or not t.is_contiguous() or t.device != dev \
+                or t.data_ptr() % 16:
+            raise ValueError(f"RoPE tables must be contiguous {dtype} [positions, {hd}] on {dev}")
+    if cos.size(0) < step.max_len or sin.size(0) != cos.size(0):
+        raise ValueError(f"RoPE tables of {cos.size(0)} and {sin.size(0)} positions for {step.max_len}")
+    q = _row_output(out, rows, n_heads * hd, qkv, rows == step.rows)
+    _call_on(dev, "lz_kv_write", qkv.data_ptr(), _row_stride(qkv), code, rows, cos.data_ptr(), sin.data_ptr(),
+             cos.size(0), q.data_ptr(), _row_stride(q), *cache, step.page_table.data_ptr(), step.page_table.size(1),
+             step.row_start.data_ptr(), step.kv_len.data_ptr(), B, n_heads, KV, hd)
+    return q
+
+
+def kv_cache_read(layer, page_table: torch.Tensor, start: torch.Tensor, rows: int, dtype: torch.dtype
+                  ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(k, v), each [rows, KV * hd] of dtype: the cached keys and values of
+    page_table's sequences one after another, rows start[b] .. start[b + 1] - 1
+    the first positions of sequence b (start: int32 [B + 1]; rows =
+    start[B]).  A float8_e4m3fn cache is read back in any dtype, others in
+    their own."""
+    require_gpu(page_table, start, layer.k, layer.v)
+    dev = page_table.device
+    if dtype not in _DTYPES:
+        raise TypeError(f"a cache is read back in float32, bfloat16 or float16, not in {dtype}")
+    cache, KV, hd = _cache_args(layer, dtype, dev)
+    _int32_table(page_table, "page_table", dev, 2)
+    _int32_table(start, "start", dev)
+    B = page_table.size(0)
+    if start.numel() != B + 1 or B == 0 or page_table.size(1) == 0 or rows < 0:
+        raise ValueError(f"{B} sequences need {B + 1} starts, got {start.numel()}")
+    k = torch.empty((rows, KV * hd), dtype=dtype, device=dev)
+    v = torch.empty((rows, KV * hd), dtype=dtype, device=dev)
+    _call_on(dev, "lz_kv_read", *cache, page_table.data_ptr(), page_table.size(1), start.data_ptr(), B, KV, hd,
+             k.data_ptr(), v.data_ptr(), _DTYPES[dtype], rows)
+    return k, v
+
+
+def paged_attention(q: torch.Tensor, layer, step, n_heads: int, scale: float,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of a step's rotated queries [rows, n_heads * hd] over the
+    cached keys and values of their sequences (a step's own tokens included:
+    kv_cache_write comes first); causal within the new tokens.  A row that
+    sees nothing is zero."""
+    require_gpu(q, layer.k, layer.v, step.row_start, step.kv_len, step.page_table, out)
+    dev = q.device
+    code = dtype_code(q)
+    cache, KV, hd = _cache_args(layer, q.dtype, dev)
+    B = _step_rows(step, dev)
+    rows = q.size(0)
+    if n_heads <= 0 or n_heads % KV:
+        raise ValueError(f"{n_heads} query heads do not divide over {KV} key/value heads")
+    q = _aligned_rows(q, "q", n_heads * hd)
+    o = _row_output(out, rows, n_heads * hd, q, rows == step.rows)
+    ws_bytes = _lib.query("lz_paged_attn_workspace", code, cache[4], rows, B, n_heads, KV, hd, step.max_new,
+                          step.max_len)
+    ws = torch.empty(((ws_bytes + 15) // 16) * 4, dtype=torch.float32, device=dev) if ws_bytes else None
+    _call_on(dev, "lz_paged_attn", q.data_ptr(), _row_stride(q), code, rows, *cache, step.page_table.data_ptr(),
+             step.page_table.size(1), step.row_start.data_ptr(), step.kv_len.data_ptr(), B, n_heads, KV, hd,
+             step.max_new, step.max_len, float(scale), o.data_ptr(), _row_stride(o), _ptr(ws), ws_bytes)
+    return o
+
+
+def _per_row(value, name: str, B: int, device: torch.device) -> Tuple[Optional[torch.Tensor], float]:
+    """A penalty as (one fp32 value a row, unused) or (None, one for all)."""
+    if not isinstance(value, torch.Tensor):
+        value = float(value)
+        if not math.isfinite(value) or (name == "repetition_penalty" and value <= 0.0):
+            raise ValueError(f"{name} must be finite{' and positive' if name == 'repetition_penalty' else ''}, got {value}")
+        return None, value
+    if value.dtype != torch.float32 or tuple(value.shape) != (B,) or not value.is_contiguous() or value.device != device:
+        raise ValueError(f"{name} must be a number or a contiguous float32 [{B}] tensor on {device}")
+    return value, 0.0
+
+
+def _row_lengths(t: Optional[torch.Tensor], name: str, B: int, device: torch.device) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (B,) or t.device != device:
+        raise ValueError(f"{name} must be an int32 or int64 [{B}] tensor on {device}")
+    return t.to(torch.int32).contiguous()
+
+
+def process_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = None,
+                   lengths: Optional[torch.Tensor] = None, prompt_lengths: Optional[torch.Tensor] = None,
+                   repetition_penalty=1.0, presence_penalty=0.0, frequency_penalty=0.0,
+                   bias: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Logits [B, V] adjusted before a token is chosen, as float32 [B, V].
+
+    In this order: tokens of the row's text (tokens [B, T] int64, of which the
+    first lengths[b] count) are divided by repetition_penalty where positive
+    and multiplied by it elsewhere; frequency_penalty times a token's
+    occurrences after the first prompt_lengths[b] tokens and presence_penalty
+    (if there are any) are subtracted; bias ([V] or [B, V] float32) is added;
+    what mask forbids becomes -inf (bool [V] or [B, V], True allows, or int32
+    words of 32 tokens, [ceil(V / 32)] or [B, ceil(V / 32)], lowest bit
+    first).  The penalties are numbers or float32 [B] tensors.  Ids outside
+    the vocabulary (padding) count for nothing."""
+    require_gpu(logits, tokens, lengths, prompt_lengths, bias, mask)
+    dev = logits.device
+    code = dtype_code(logits)
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [B, V], got {tuple(logits.shape)}")
+    B, V = logits.shape
+    if (V > 1 and logits.stride(1) != 1) or (B > 1 and logits.stride(0) < V):
+        raise ValueError(f"logits rows must be adjacent values, got strides {logits.stride()}")
+    n, ldt = 0, 0
+    if tokens is not None:
+        if tokens.dtype != torch.int64 or tokens.dim() != 2 or tokens.size(0) != B or tokens.device != dev or (
+                tokens.size(1) > 1 and tokens.stride(1) != 1):
+            raise ValueError(f"tokens must be int64 [{B}, T] rows on {dev}")
+        n, ldt = tokens.size(1), tokens.stride(0)
+    elif lengths is not None or prompt_lengths is not None:
+        raise ValueError("lengths and prompt_lengths say which tokens count: there are none")
+    lengths = _row_lengths(lengths, "lengths", B, dev)
+    prompts = _row_lengths(prompt_lengths, "prompt_lengths", B, dev)
+    rep, rep_s = _per_row(repetition_penalty, "repetition_penalty", B, dev)
+    pres, pres_s = _per_row(presence_penalty, "presence_penalty", B, dev)
+    freq, freq_s = _per_row(frequency_penalty, "frequency_penalty", B, dev)
+    ldb = ldm = kind = 0
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.device != dev or tuple(bias.shape) not in ((V,), (B, V)) or (
+                V > 1 and bias.stride(-1) != 1):
+            raise ValueError(f"bias must be float32 [{V}] or [{B}, {V}] on {dev}")
+        ldb = bias.stride(0) if bias.dim() == 2 else 0
+    if mask is not None:
+        kind = {torch.bool: 1, torch.int32: 2}.get(mask.dtype, 0)
+        cols = V if kind == 1 else (V + 31) // 32
+        if not kind or mask.device != dev or tuple(mask.shape) not in ((cols,), (B, cols)) or (
+                cols > 1 and mask.stride(-1) != 1):
+            raise ValueError(f"mask must be bool [{V}] or [{B}, {V}], or int32 words of {(V + 31) // 32}, on {dev}")
+        ldm = mask.stride(0) if mask.dim() == 2 else 0
+    out = torch.empty((B, V), dtype=torch.float32, device=dev)
+    _call_on(dev, "lz_process_logits", logits.data_ptr(), logits.stride(0) if B > 1 else V, code, B, V,
+             _ptr(tokens), ldt, n, _ptr(lengths), _ptr(prompts), _ptr(rep), rep_s, _ptr(pres), pres_s, _ptr(freq),
+             freq_s, _ptr(bias), ldb, _ptr(mask), kind, ldm, out.data_ptr(), V)
+    return out

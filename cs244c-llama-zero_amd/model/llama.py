@@ -12,7 +12,7 @@ no CPU compute path.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Any, Optional, Tuple
+from typing import Any, Callable, Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
@@ -20,6 +20,7 @@ from torch.utils.checkpoint import checkpoint as activation_checkpoint
 
 from lzhip import functional as LF
 from lzhip import ops
+from lzhip.cache import CacheStep, KVCache, LayerCache
 
 from .config import ModelConfig
 
@@ -185,6 +186,19 @@ class GroupedQueryAttention(nn.Module):
         )
         return self.o_proj(y, residual)
 
+    def forward_cached(self, x: torch.Tensor, layer: LayerCache, step: CacheStep,
+                       residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """forward() for a step's new tokens [rows, dim], whose keys and values
+        go into the layer's cache and which attend over all of it (no
+        gradients, no dropout)."""
+        ops.require_gpu(x)
+        qkv = ops.gemm(x, LF.fused_weight([self.q_proj.weight, self.k_proj.weight, self.v_proj.weight]))
+        # a position's rotation does not depend on the table's length: whole
+        # blocks, so that a growing sequence rarely rebuilds it
+        cos, sin = self.rotary.tables(-(-step.max_len // 256) * 256, x.device, x.dtype)
+        q = ops.kv_cache_write(qkv, layer, step, self.n_heads, cos, sin)
+        return self.o_proj(ops.paged_attention(q, layer, step, self.n_heads, float(self.scale)), residual)
+
 
 class SwiGLU(nn.Module):
     def __init__(self, cfg: ModelConfig) -> None:
@@ -222,6 +236,11 @@ class TransformerBlock(nn.Module):
         # the block's output is the MLP's: under output_unused() (the ZeRO-3
         # recompute) its value is not formed
         return self.mlp(h, residual=x, compute_output=not LF.output_is_unused())
+
+    def forward_cached(self, x: torch.Tensor, layer: LayerCache, step: CacheStep) -> torch.Tensor:
+        """forward() for a step's new tokens [rows, dim] over a cache."""
+        x = self.attn.forward_cached(self.input_norm(x), layer, step, residual=x)
+        return self.mlp(self.post_attn_norm(x), residual=x)
 
 
 @dataclass
@@ -357,6 +376,37 @@ class LlamaForCausalLM(nn.Module):
             return module(*args)
         return executor.call_module(module_name, module, *args)
 
+    def new_cache(self, batch: int, max_len: int, dtype: Optional[torch.dtype] = None, page_size: int = 64) -> KVCache:
+        """A cache for `batch` sequences of up to max_len tokens, on the
+        model's device; dtype torch.float8_e4m3fn stores it in 8 bits (None:
+        the model's dtype)."""
+        w = self.tok_embeddings.weight
+        return KVCache(self.cfg.n_layers, self.cfg.n_kv_heads, self.cfg.head_dim, batch=batch,
+                       n_pages=batch * -(-max_len // page_size), page_size=page_size, dtype=w.dtype, storage=dtype,
+                       device=w.device)
+
+    @torch.no_grad()
+    def forward_cached(self, ids: torch.Tensor, cache: KVCache, step: CacheStep) -> torch.Tensor:
+        """Logits [B, V] of each sequence's last new token.  ids: the step's
+        new tokens, sequence after sequence ([rows] int64); step: what
+        cache.step(counts) returned for them.  As in eval mode, without
+        dropout.  The row of a sequence that has no new tokens says nothing."""
+        if self._zero3_executor is not None:
+            raise RuntimeError("a ZeRO-3 sharded model has no cached forward: gather its parameters first "
+                               "(summon_full_params) or generate without use_cache")
+        if ids.dim() != 1 or ids.numel() != step.rows:
+            raise ValueError(f"ids should hold the step's {step.rows} tokens, got shape {tuple(ids.shape)}")
+        training = self.training
+        self.eval()
+        try:
+            x = self.tok_embeddings(ids)
+            for layer, block in zip(cache.layers, self.layers):
+                x = block.forward_cached(x, layer, step)
+            last = ops.embedding_fwd((step.row_start[1:] - 1).long(), x)  # rows of x
+            return self.lm_head(self.norm(last))
+        finally:
+            self.train(training)
+
     @torch.no_grad()
     def generate(
         self,
@@ -364,19 +414,53 @@ class LlamaForCausalLM(nn.Module):
         max_new_tokens: int,
         temperature: float = 1.0,
         top_k: Optional[int] = None,
+        *,
+        use_cache: bool = False,
+        cache_dtype: Optional[torch.dtype] = None,
+        repetition_penalty: float = 1.0,
+        presence_penalty: float = 0.0,
+        frequency_penalty: float = 0.0,
+        logit_bias: Optional[torch.Tensor] = None,
+        token_mask: Union[None, torch.Tensor, Callable[[torch.Tensor], torch.Tensor]] = None,
     ) -> torch.Tensor:
         """Autoregressive sampling with the reference's semantics
         (model/llama.py:311-335): each new token takes a full forward over the
         last max_seq_len tokens; temperature <= 0 picks the arg-max, otherwise
         the logits / temperature, cut to their top_k largest, are sampled.
-        The sequence grows in one preallocated buffer."""
+        The sequence grows in one preallocated buffer.
+
+        use_cache keeps every layer's keys and values (in cache_dtype; see
+        new_cache) and runs new tokens alone through the model, as long as the
+        sequence fits max_seq_len; past that the window moves, which a cache
+        cannot follow, and each token takes a full forward again.  The
+        penalties, logit_bias and token_mask (a mask, or a function that makes
+        one of the [B, t] tokens so far) adjust the logits first, as
+        ops.process_logits says, the prompt counting for repetition_penalty
+        alone."""
         self.eval()
         bsz, t0 = input_ids.shape
         seq = input_ids.new_empty((bsz, t0 + max_new_tokens))
         seq[:, :t0] = input_ids
         window = self.cfg.max_seq_len
+        adjust = (repetition_penalty != 1.0 or presence_penalty != 0.0 or frequency_penalty != 0.0
+                  or logit_bias is not None or token_mask is not None)
+        prompts = torch.full((bsz,), t0, dtype=torch.int32, device=seq.device) if adjust else None
+        cache, cached = None, 0
+        if use_cache and 0 < t0 <= window and max_new_tokens > 0:
+            cache = self.new_cache(bsz, min(t0 + max_new_tokens - 1, window), cache_dtype)
         for t in range(t0, t0 + max_new_tokens):
-            context = seq[:, max(0, t - window) : t].contiguous()
-            last = self(context).logits[:, -1, :].float()
-            seq[:, t] = _next_token(last, temperature, top_k)
+            if cache is not None and t <= window:
+                step = cache.step([t - cached] * bsz)
+                last = self.forward_cached(seq[:, cached:t].reshape(-1), cache, step)
+                cached = t
+            else:
+                cache = None
+                context = seq[:, max(0, t - window) : t].contiguous()
+                last = self(context).logits[:, -1, :]
+            if adjust:
+                last = ops.process_logits(
+                    last, tokens=seq[:, :t], prompt_lengths=prompts, repetition_penalty=repetition_penalty,
+                    presence_penalty=presence_penalty, frequency_penalty=frequency_penalty, bias=logit_bias,
+                    mask=token_mask(seq[:, :t]) if callable(token_mask) else token_mask)
+            seq[:, t] = _next_token(last.float(), temperature, top_k)
         return seq

@@ -382,6 +382,76 @@ int lz_attn_bwd_direct(const void* q, int64_t ldq, const void* k, int64_t ldk, c
 int lz_dropout(const void* x, void* y, int64_t n, float p, uint64_t seed, int dtype, void* stream);
 int lz_dropout_mask(uint8_t* keep, int64_t n, float p, uint64_t seed, void* stream);
 
+/* ---- generation from a paged key/value cache ----------------------------
+ * The reference has no cache: its generate (model/llama.py:311-335) runs the
+ * whole window through the model for every token.
+ *
+ * A layer's keys and values are [pages][KV][page_size][hd] each, contiguous,
+ * 16-byte aligned, of cache_dtype = the rows' dtype or LZ_E4M3
+ * (float8_e4m3fn) with one exponent e (int8, [pages][KV][page_size]) for each
+ * token and kv head: the value is the stored number times 2^e.  page_size is a
+ * power of two from 16 to 1024, hd 32, 64 or 128.  Position p of sequence b is
+ * in page table[b * width + p / page_size].  A step's rows are the new tokens,
+ * sequence after sequence: rows row_start[b] .. row_start[b+1]-1 (row_start:
+ * B + 1 ascending values, on the device) are the last tokens of sequence b,
+ * whose length with them is kv_len[b].  Rows of no sequence are left as they
+ * are.  What the tables say is checked on the device: a position outside the
+ * table and a page id outside [0, pages) are skipped, and the rows of tokens
+ * whose position is negative or past the table (or the cos/sin tables') come
+ * out as zeros. */
+#define LZ_E4M3 8
+
+/* q_out rows (H heads) = RoPE(q), and RoPE(k) and v of every row into its
+ * page.  qkv rows hold H + 2*KV heads; cos_t/sin_t are lz_rope_table's,
+ * [positions][hd] in the rows' dtype.  The rotation is formed in fp32 and
+ * rounded once to what it is stored in.  LZ_E4M3: e is the smallest integer
+ * with max |x| <= 448 * 2^e over a token's head (0 if all are zero; within
+ * -120..119, -15..7 for LZ_F16 rows, larger values becoming 448 * 2^e);
+ * infinities are stored as NaN.  Rows and tables must be 16-byte aligned. */
+int lz_kv_write(const void* qkv, int64_t ld, int dtype, int64_t rows, const void* cos_t, const void* sin_t,
+                int64_t positions, void* q_out, int64_t ldq, void* k, void* v, void* k_exp, void* v_exp,
+                int cache_dtype, int64_t pages, int64_t page_size, const int32_t* table, int64_t width,
+                const int32_t* row_start, const int32_t* kv_len, int64_t B, int64_t H, int64_t KV, int64_t hd,
+                void* stream);
+
+/* The cached keys and values of B sequences as rows [rows][KV * hd] of dtype:
+ * rows start[b] .. start[b+1]-1 are positions 0, 1, ... of sequence b.
+ * Positions without a page come out as zeros. */
+int lz_kv_read(const void* k, const void* v, const void* k_exp, const void* v_exp, int cache_dtype, int64_t pages,
+               int64_t page_size, const int32_t* table, int64_t width, const int32_t* start, int64_t B, int64_t KV,
+               int64_t hd, void* k_out, void* v_out, int dtype, int64_t rows, void* stream);
+
+/* Attention of a step's rows (q rows of H heads, rotated; kv head h / (H/KV))
+ * over their sequences' cached keys and values, their own tokens' included:
+ * the i-th of `new` rows sees positions 0 .. kv_len - new + i.  A row that
+ * sees nothing comes out as zeros.  max_new and max_len: at least the largest
+ * number of new tokens and of cached ones (max_new sizes the grid: rows past
+ * it would be left; max_len only how the work is split).  workspace:
+ * lz_paged_attn_workspace bytes, 16-byte aligned, for the joined parts of
+ * long sequences. */
+int64_t lz_paged_attn_workspace(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd,
+                                int64_t max_new, int64_t max_len);
+int lz_paged_attn(const void* q, int64_t ldq, int dtype, int64_t rows, const void* k, const void* v, const void* k_exp,
+                  const void* v_exp, int cache_dtype, int64_t pages, int64_t page_size, const int32_t* table,
+                  int64_t width, const int32_t* row_start, const int32_t* kv_len, int64_t B, int64_t H, int64_t KV,
+                  int64_t hd, int64_t max_new, int64_t max_len, float scale, void* o, int64_t ldo, void* workspace,
+                  int64_t ws_bytes, void* stream);
+
+/* out (fp32, B rows of V) = logits after, in this order: the repetition
+ * penalty of tokens in the row's text (x > 0 ? x / rep : x * rep), minus
+ * freq * (occurrences after the prompt) and pres (if there are any), plus the
+ * bias, and -inf where the mask forbids.  tokens: B rows of n_tokens ids,
+ * of which the first lengths[b] count (NULL: all) and the first prompts[b] of
+ * those are the prompt (NULL: none); ids outside [0, V) count for nothing.
+ * rep / pres / freq: one value a row, or NULL and the scalar.  bias and mask
+ * rows have strides ldb and ldm (0: one row for all); mask_kind 0: none, 1: a
+ * byte a token (0 forbids), 2: a bit a token in 32-bit words, lowest first. */
+int lz_process_logits(const void* logits, int64_t ld, int dtype, int64_t B, int64_t V, const int64_t* tokens,
+                      int64_t ldt, int64_t n_tokens, const int32_t* lengths, const int32_t* prompts, const float* rep,
+                      float rep_s, const float* pres, float pres_s, const float* freq, float freq_s, const float* bias,
+                      int64_t ldb, const void* mask, int mask_kind, int64_t ldm, float* out, int64_t ldo,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif
