@@ -86,6 +86,17 @@ __device__ __forceinline__ float sum_halves(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// exp(d) for d <= 0 to about 1 ulp: 2^hi * (1 + lo ln 2) with hi + lo =
+// d * log2(e) formed in two terms.  Below -150 (where the result is zero) d is
+// replaced, so that -inf does not meet inf - inf in lo; a NaN stays one.
+__device__ __forceinline__ float exp_accurate(float d) {
+  d = d < -150.f ? -150.f : d;
+  const float hi = d * kLog2e;
+  const float lo = fmaf(d, kLog2e, -hi) + d * 1.9259629911266175e-8f;  // log2(e) - float(log2(e))
+  const float p = __builtin_amdgcn_exp2f(hi);
+  return fmaf(p * kLn2, lo, p);
+}
+
 template <typename F = FmtBF16>
 __device__ __forceinline__ void store_bf16x4(uint16_t* p, float a, float b, float c, float d) {
   uint2 w;

@@ -53,17 +53,6 @@ __device__ __forceinline__ void wave_order() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// exp(d) for d <= 0 to about 1 ulp: 2^hi * (1 + lo ln 2) with hi + lo =
-// d * log2(e) formed in two terms.  Below -150 (where the result is zero) d is
-// replaced, so that -inf does not meet inf - inf in lo; a NaN stays one.
-__device__ __forceinline__ float exp_accurate(float d) {
-  d = d < -150.f ? -150.f : d;
-  const float hi = d * kLog2e;
-  const float lo = fmaf(d, kLog2e, -hi) + d * 1.9259629911266175e-8f;  // log2(e) - float(log2(e))
-  const float p = __builtin_amdgcn_exp2f(hi);
-  return fmaf(p * kLn2, lo, p);
-}
-
 // fp32 tiles: rows of HD + 4 floats (16 consecutive rows' 16-byte reads fall
 // on distinct banks).
 template <typename T, int HD_>

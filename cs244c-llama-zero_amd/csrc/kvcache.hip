@@ -16,8 +16,9 @@
 // relative) and makes the way back exact in bf16: four significant bits.  e is
 // kept in -120..119 (448 * 2^119 is the largest finite value of that form), and
 // in -15..7 for fp16 rows, so that every stored value is an fp16 number (a
-// multiple of 2^-24 up to 57344); larger inputs become the largest value.  All zeros take e = 0.  An infinity or NaN is stored as NaN and left
-// out of the maximum.
+// multiple of 2^-24 up to 57344); larger inputs become the largest value.  All
+// zeros take e = 0.  An infinity or NaN is stored as NaN and left out of the
+// maximum.
 #include <type_traits>
 
 #include "kvcache.h"
@@ -235,7 +236,8 @@ int lz_check_pages(const char* what, const void* k, const void* v, const void* k
                  KV > 0 && KV <= 65536,
              "%s: bad shape", what);
   LZ_REQUIRE(k && v && table && lz_aligned16(k) && lz_aligned16(v), "%s: pages must be 16-byte aligned", what);
-  LZ_REQUIRE(cache_dtype != LZ_E4M3 || (k_exp && v_exp), "%s: an e4m3 cache needs its exponents", what);
+  LZ_REQUIRE(cache_dtype != LZ_E4M3 || (k_exp && v_exp && lz_aligned16(k_exp) && lz_aligned16(v_exp)),
+             "%s: an e4m3 cache needs its exponents, 16-byte aligned", what);
   return LZ_OK;
 }
 

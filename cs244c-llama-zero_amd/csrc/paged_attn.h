@@ -1,0 +1,110 @@
+// What the kernels of attention over a paged cache share.
+#pragma once
+#include "attn_tiles.h"
+#include "kvcache.h"
+
+namespace {
+
+// Packed rows: the `new` tokens of a sequence times the G = H / KV query heads
+// of one kv head are one list of new * G rows, row m = token m / G, head m % G
+// of the group, so that one pass over a kv head's keys and values serves all
+// of them.  A block of rows goes over the keys in up to nsplit parts of
+// `chunk` keys (a multiple of 64); parts of one block meet in the workspace.
+struct PagedArgs {
+  const void* q;
+  int64_t ldq;
+  const void* k;
+  const void* v;
+  const int8_t* k_exp;
+  const int8_t* v_exp;
+  LzPages pg;
+  const int32_t* row_start;
+  const int32_t* kv_len;
+  void* o;
+  int64_t ldo;
+  float* part;  // [rows * H][nsplit][hd], then [rows * H][nsplit][2]: maximum and sum
+  float scale;
+  int rows, B, H, KV, nqb, nsplit, chunk;
+};
+
+// A workgroup's place: blocks of one (sequence, kv head) pair are dealt to one
+// XCD when the pairs split evenly over the eight, so that the keys and values
+// its row blocks share are fetched into one L2.
+struct PagedPlace {
+  int b, g, qb, split;
+  __device__ __forceinline__ PagedPlace(const PagedArgs& a, uint32_t bid) {
+    const uint32_t pairs = (uint32_t)(a.B * a.KV);
+    const uint32_t pair = bid % pairs, rest = bid / pairs;
+    b = (int)(pair / (uint32_t)a.KV);
+    g = (int)(pair % (uint32_t)a.KV);
+    split = (int)(rest / (uint32_t)a.nqb);
+    qb = a.nqb - 1 - (int)(rest % (uint32_t)a.nqb);  // the blocks with the most keys first
+  }
+};
+
+// Rows m0 .. m0 + BM - 1 of a pair's packed rows and the keys that they see:
+// row m's are 0 .. sees(m) - 1.
+struct PagedRows {
+  int m0, count;  // count: rows of the pair (0 or less: none)
+  int row0, base, G, cap;
+  __device__ __forceinline__ PagedRows(const PagedArgs& a, int b, int m0_) {
+    m0 = m0_;
+    G = a.H / a.KV;
+    const int lo = a.row_start[b], hi = a.row_start[b + 1];
+    base = a.kv_len[b] - hi + 1;  // keys that row r of q sees: base + r
+    row0 = max(lo, 0);
+    count = hi > row0 ? (min(hi, a.rows) - row0) * G : 0;
+    cap = a.pg.width << a.pg.log_size;
+  }
+  __device__ __forceinline__ int row(int m) const { return row0 + m / G; }
+  __device__ __forceinline__ int sees(int m) const { return min(max(base + row(m), 0), cap); }
+  // the keys that the block's rows see together, and the parts they make
+  template <int BM>
+  __device__ __forceinline__ int keys() const {
+    return sees(min(m0 + BM, count) - 1);
+  }
+  static __device__ __forceinline__ int parts(const PagedArgs& a, int keys) {
+    return min(max((keys + a.chunk - 1) / a.chunk, 1), a.nsplit);
+  }
+};
+
+// Two e4m3 values of a word, times 2^e (exact in bf16, and in fp16 for what
+// lz_kv_write stores of fp16 rows), as two values of the 16-bit format F.
+template <typename F, bool kHi>
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w, float unit) {
+  if constexpr (F::kDtype == LZ_F16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, unit, kHi));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, unit, kHi));
+}
+
+template <int BYTES>
+__device__ __forceinline__ void load_words(uint32_t* w, const void* p) {
+  if constexpr (BYTES == 2) {
+    w[0] = *static_cast<const uint16_t*>(p);
+  } else if constexpr (BYTES == 4) {
+    w[0] = *static_cast<const uint32_t*>(p);
+  } else if constexpr (BYTES == 8) {
+    const uint2 x = *static_cast<const uint2*>(p);
+    w[0] = x.x;
+    w[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint4 x = static_cast<const uint4*>(p)[i];
+      w[4 * i] = x.x;
+      w[4 * i + 1] = x.y;
+      w[4 * i + 2] = x.z;
+      w[4 * i + 3] = x.w;
+    }
+  }
+}
+
+// Whether a word of two 16-bit values of the format F, or an fp32 word, holds
+// an infinity or NaN.
+template <typename F>
+__device__ __forceinline__ bool nonfinite16(uint32_t w) {
+  constexpr uint32_t kExp = F::kDtype == LZ_F16 ? 0x7c00u : 0x7f80u;
+  return (w & kExp) == kExp || ((w >> 16) & kExp) == kExp;
+}
+__device__ __forceinline__ bool nonfinite32(uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u; }
+
+}  // namespace

@@ -1237,8 +1237,8 @@ def _cache_args(layer, dtype: torch.dtype, device: torch.device) -> Tuple[tuple,
     if k.dtype == torch.float8_e4m3fn:
         for e in (k_exp, v_exp):
             if e is None or e.dtype != torch.int8 or e.shape != shape[:3] or not e.is_contiguous() or e.device != device:
-                raise ValueError("a float8_e4m3fn cache needs contiguous int8 exponents of its [pages, KV heads, page "
-                                 "size] beside it")
+                raise ValueError("a float8_e4m3fn cache needs contiguous int8 exponents [pages, KV heads, page size] "
+                                 "beside it")
         code, ke, ve = _lib.E4M3, k_exp.data_ptr(), v_exp.data_ptr()
     else:
         if k.dtype != dtype or k_exp is not None or v_exp is not None:
