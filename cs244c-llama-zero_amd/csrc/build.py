@@ -39,6 +39,7 @@ SOURCES = [
     "attn_wave.hip",
     "kvcache.hip",
     "paged_attn.hip",
+    "paged_tile.hip",
     "logits.hip",
 ]
 

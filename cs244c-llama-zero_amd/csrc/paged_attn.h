@@ -3,14 +3,12 @@
 #include "attn_tiles.h"
 #include "kvcache.h"
 
-namespace {
-
 // Packed rows: the `new` tokens of a sequence times the G = H / KV query heads
 // of one kv head are one list of new * G rows, row m = token m / G, head m % G
 // of the group, so that one pass over a kv head's keys and values serves all
 // of them.  A block of rows goes over the keys in up to nsplit parts of
 // `chunk` keys (a multiple of 64); parts of one block meet in the workspace.
-struct PagedArgs {
+struct LzPagedArgs {
   const void* q;
   int64_t ldq;
   const void* k;
@@ -26,6 +24,14 @@ struct PagedArgs {
   float scale;
   int rows, B, H, KV, nqb, nsplit, chunk;
 };
+
+// paged_tile.hip: 16-bit rows in blocks of kPagedTileRows; LZ_OK or a status.
+constexpr int kPagedTileRows = 128;
+int lz_paged_tile(const LzPagedArgs& a, int dtype, bool e4m3, int64_t hd, uint32_t blocks, hipStream_t stream);
+
+namespace {
+
+typedef LzPagedArgs PagedArgs;
 
 // A workgroup's place: blocks of one (sequence, kv head) pair are dealt to one
 // XCD when the pairs split evenly over the eight, so that the keys and values
@@ -59,10 +65,7 @@ struct PagedRows {
   __device__ __forceinline__ int row(int m) const { return row0 + m / G; }
   __device__ __forceinline__ int sees(int m) const { return min(max(base + row(m), 0), cap); }
   // the keys that the block's rows see together, and the parts they make
-  template <int BM>
-  __device__ __forceinline__ int keys() const {
-    return sees(min(m0 + BM, count) - 1);
-  }
+  __device__ __forceinline__ int keys(int bm) const { return sees(min(m0 + bm, count) - 1); }
   static __device__ __forceinline__ int parts(const PagedArgs& a, int keys) {
     return min(max((keys + a.chunk - 1) / a.chunk, 1), a.nsplit);
   }

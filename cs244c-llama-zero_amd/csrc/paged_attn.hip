@@ -17,6 +17,7 @@
 // HD / 16 adjacent columns of eight keys and swaps rows and columns of that
 // 8 x (HD / 16) block in registers (v_perm).
 #include <algorithm>
+#include <cmath>
 
 #include "paged_attn.h"
 
@@ -238,7 +239,7 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
   const PagedPlace at(a, blockIdx.x);
   const PagedRows rw(a, at.b, at.qb * BM);
   if (rw.m0 >= rw.count) return;
-  const int n_keys = rw.keys<BM>(), n_parts = PagedRows::parts(a, n_keys);
+  const int n_keys = rw.keys(BM), n_parts = PagedRows::parts(a, n_keys);
   if (at.split >= n_parts) return;
   const int k_lo = at.split * a.chunk, k_hi = at.split + 1 == n_parts ? n_keys : k_lo + a.chunk;
 
@@ -452,8 +453,8 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
 }
 
 // The parts of rows that were split, joined: one group of HD / 4 lanes a row.
-template <typename T, int HD, int BM>
-__global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a) {
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm) {
   constexpr int kLanes = HD / 4;
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
   const uint32_t rh = idx / kLanes;
@@ -464,9 +465,9 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a) {
   if (b < 0) return;
   PagedRows rw(a, b, 0);
   const int m = (row - rw.row0) * rw.G + head % rw.G;
-  rw.m0 = m / BM * BM;
-  if (m / BM >= a.nqb) return;
-  const int n_parts = PagedRows::parts(a, rw.template keys<BM>());
+  rw.m0 = m / bm * bm;
+  if (m / bm >= a.nqb) return;
+  const int n_parts = PagedRows::parts(a, rw.keys(bm));
   if (n_parts == 1) return;
   const float* part = a.part + (int64_t)rh * a.nsplit * HD + d;
   const float* s2 = a.part + (int64_t)a.rows * a.H * a.nsplit * HD + (int64_t)rh * a.nsplit * 2;
@@ -490,19 +491,19 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a) {
 }
 
 struct Plan {
-  int nq;  // 16-row blocks of a wave
+  int bm;  // rows of a block: 16 or 32 (paged_wave_kernel) or kPagedTileRows
   int nqb, nsplit, chunk;
 };
 
-// Row blocks of 16 or 32, and parts so that about four workgroups come to a
-// CU, none under 256 keys.
-Plan make_plan(int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t max_new, int64_t max_len) {
+// Row blocks, and parts so that about four workgroups come to a CU (two of
+// the tile kernel's), none under 256 keys.
+Plan make_plan(int dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t max_new, int64_t max_len) {
   Plan p;
   const int64_t packed = std::max<int64_t>(1, std::min(max_new, rows)) * (H / KV);
-  p.nq = packed <= 16 ? 1 : 2;
-  p.nqb = (int)lz_cdiv(packed, 16 * p.nq);
+  p.bm = packed <= 16 ? 16 : packed <= 64 || dtype == LZ_F32 ? 32 : kPagedTileRows;
+  p.nqb = (int)lz_cdiv(packed, p.bm);
   const int64_t blocks = B * KV * p.nqb, len = std::max<int64_t>(1, max_len);
-  const int64_t want = std::max<int64_t>(1, lz_cdiv(4 * lz_num_cus(), blocks));
+  const int64_t want = std::max<int64_t>(1, (p.bm == kPagedTileRows ? 2 : 4) * lz_num_cus() / blocks);
   p.chunk = (int)std::max<int64_t>(256, lz_cdiv(lz_cdiv(len, want), 64) * 64);
   p.nsplit = (int)lz_cdiv(len, p.chunk);
   return p;
@@ -513,7 +514,7 @@ Plan make_plan(int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t max_new, 
 LZ_EXPORT int64_t lz_paged_attn_workspace(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV,
                                           int64_t hd, int64_t max_new, int64_t max_len) {
   if (rows <= 0 || B <= 0 || H <= 0 || KV <= 0 || H % KV || max_len < 0 || max_len > INT32_MAX - 1024) return 0;
-  const Plan p = make_plan(rows, B, H, KV, max_new, max_len);
+  const Plan p = make_plan(dtype, rows, B, H, KV, max_new, max_len);
   return p.nsplit > 1 ? rows * H * p.nsplit * (hd + 2) * 4 : 0;
 }
 
@@ -529,12 +530,13 @@ LZ_EXPORT int lz_paged_attn(const void* q, int64_t ldq, int dtype, int64_t rows,
   LZ_REQUIRE(H > 0 && H % KV == 0 && H <= 65536 && rows >= 0 && rows * H <= INT32_MAX / 64 && max_new >= 0 &&
                  max_len >= 0 && max_len <= INT32_MAX - 1024,
              "lz_paged_attn: bad shape");
+  LZ_REQUIRE(scale >= 0.f && scale < INFINITY, "lz_paged_attn: scale %g", (double)scale);
   LZ_REQUIRE(ldq >= H * hd && ldo >= H * hd, "lz_paged_attn: row strides shorter than the rows");
   LZ_REQUIRE(rows == 0 || (q && o && row_start && kv_len && lz_aligned16(q) && lz_aligned16(o) && ldq * esz % 16 == 0 &&
                            ldo * esz % 16 == 0),
              "lz_paged_attn: rows must be 16-byte aligned");
   if (rows == 0) return LZ_OK;
-  const Plan p = make_plan(rows, B, H, KV, max_new, max_len);
+  const Plan p = make_plan(dtype, rows, B, H, KV, max_new, max_len);
   const int64_t need = lz_paged_attn_workspace(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
   LZ_REQUIRE(need == 0 || (workspace && lz_aligned16(workspace) && ws_bytes >= need),
              "lz_paged_attn: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
@@ -544,16 +546,18 @@ LZ_EXPORT int lz_paged_attn(const void* q, int64_t ldq, int dtype, int64_t rows,
               LzPages{table, (int)width, (int)pages, lz_log2(page_size)}, row_start, kv_len, o, ldo, (float*)workspace,
               scale, (int)rows, (int)B, (int)H, (int)KV, p.nqb, p.nsplit, p.chunk};
   hipStream_t s = lz_stream(stream);
-#define RUN(T, HD, E8)                                                                     \
-  do {                                                                                     \
-    if (p.nq == 1) paged_wave_kernel<T, HD, E8, 1><<<(uint32_t)blocks, 256, 0, s>>>(a);    \
-    else paged_wave_kernel<T, HD, E8, 2><<<(uint32_t)blocks, 256, 0, s>>>(a);              \
-    if (p.nsplit > 1) {                                                                    \
-      if (p.nq == 1) paged_join_kernel<T, HD, 16><<<(uint32_t)joins, 256, 0, s>>>(a);      \
-      else paged_join_kernel<T, HD, 32><<<(uint32_t)joins, 256, 0, s>>>(a);                \
-    }                                                                                      \
+  const bool tiles = p.bm == kPagedTileRows;
+  if (tiles)
+    if (int rc = lz_paged_tile(a, dtype, cache_dtype == LZ_E4M3, hd, (uint32_t)blocks, s)) return rc;
+#define RUN(T, HD, E8)                                                                    \
+  do {                                                                                    \
+    if (p.bm == 16) paged_wave_kernel<T, HD, E8, 1><<<(uint32_t)blocks, 256, 0, s>>>(a);  \
+    else paged_wave_kernel<T, HD, E8, 2><<<(uint32_t)blocks, 256, 0, s>>>(a);             \
   } while (0)
-  LZ_CACHE_CASES(dtype, cache_dtype, hd, RUN);
+  if (!tiles) LZ_CACHE_CASES(dtype, cache_dtype, hd, RUN);
+#undef RUN
+#define RUN(T, HD, E8) paged_join_kernel<T, HD><<<(uint32_t)joins, 256, 0, s>>>(a, p.bm)
+  if (p.nsplit > 1) LZ_CACHE_CASES(dtype, 0, hd, RUN);
 #undef RUN
   return lz_check_launch("lz_paged_attn");
 }
