@@ -25,9 +25,10 @@ struct LzPagedArgs {
   int rows, B, H, KV, nqb, nsplit, chunk;
 };
 
-// paged_tile.hip: 16-bit rows in blocks of kPagedTileRows; LZ_OK or a status.
+// paged_tile.hip: 16-bit rows in blocks of kPagedTileRows; `groups`
+// (1 or 2) of its waves share a block's keys.  LZ_OK or a status.
 constexpr int kPagedTileRows = 128;
-int lz_paged_tile(const LzPagedArgs& a, int dtype, bool e4m3, int64_t hd, uint32_t blocks, hipStream_t stream);
+int lz_paged_tile(const LzPagedArgs& a, int dtype, bool e4m3, int64_t hd, int groups, uint32_t blocks, hipStream_t stream);
 
 namespace {
 

@@ -452,60 +452,91 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
   }
 }
 
-// The parts of rows that were split, joined: one group of HD / 4 lanes a row.
+// The parts of rows that were split, joined: `per` groups of HD / 4 lanes for
+// one (row, head), each with every per-th part, all loads of a thread
+// independent; the groups meet in LDS in a fixed order.
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm) {
+__global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm, int per) {
   constexpr int kLanes = HD / 4;
-  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
-  const uint32_t rh = idx / kLanes;
-  const int d = (int)(idx % kLanes) * 4;
-  if (rh >= (uint32_t)a.rows * (uint32_t)a.H) return;
+  __shared__ float4 ys[256];
+  __shared__ float ms[256], ls[256];
+  const int tid = threadIdx.x, d = tid % kLanes * 4, grp = tid / kLanes % per, rows = 256 / (kLanes * per);
+  const uint32_t rh = blockIdx.x * (uint32_t)rows + (uint32_t)(tid / (kLanes * per));
   const int row = (int)(rh / (uint32_t)a.H), head = (int)(rh % (uint32_t)a.H);
-  const int b = lz_seq_of_row(a.row_start, a.B, a.rows, row);
-  if (b < 0) return;
-  PagedRows rw(a, b, 0);
-  const int m = (row - rw.row0) * rw.G + head % rw.G;
-  rw.m0 = m / bm * bm;
-  if (m / bm >= a.nqb) return;
-  const int n_parts = PagedRows::parts(a, rw.keys(bm));
-  if (n_parts == 1) return;
+  int n_parts = 0;
+  if (row < a.rows) {
+    const int b = lz_seq_of_row(a.row_start, a.B, a.rows, row);
+    if (b >= 0) {
+      PagedRows rw(a, b, 0);
+      const int m = (row - rw.row0) * rw.G + head % rw.G;
+      rw.m0 = m / bm * bm;
+      if (m / bm < a.nqb) n_parts = PagedRows::parts(a, rw.keys(bm));
+    }
+  }
+  if (n_parts == 1) n_parts = 0;  // was written whole
   const float* part = a.part + (int64_t)rh * a.nsplit * HD + d;
   const float* s2 = a.part + (int64_t)a.rows * a.H * a.nsplit * HD + (int64_t)rh * a.nsplit * 2;
-  float top = -INFINITY;
-  for (int i = 0; i < n_parts; ++i) top = fmaxf(top, s2[2 * i]);
-  float l = 0.f;
+  float top = -INFINITY, l = 0.f;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int i = 0; i < n_parts; ++i) {
+  for (int i = grp; i < n_parts; i += per) {
     const float4 z = *reinterpret_cast<const float4*>(part + (int64_t)i * HD);
-    const float f = s2[2 * i] == -INFINITY ? 0.f : exp_of<T>(s2[2 * i] - top);
-    if (f == 0.f && s2[2 * i + 1] == 0.f) continue;
-    l = fmaf(f, s2[2 * i + 1], l);
-    y.x = fmaf(f, z.x, y.x);
-    y.y = fmaf(f, z.y, y.y);
-    y.z = fmaf(f, z.z, y.z);
-    y.w = fmaf(f, z.w, y.w);
+    const float2 t = *reinterpret_cast<const float2*>(s2 + 2 * i);
+    if (t.x == -INFINITY && t.y == 0.f) continue;  // saw nothing
+    const float m_new = fmaxf(top, t.x);
+    const float f = m_new == top ? 1.f : exp_of<T>(top - m_new), e = m_new == t.x ? 1.f : exp_of<T>(t.x - m_new);
+    top = m_new;
+    l = fmaf(l, f, e * t.y);
+    y.x = fmaf(y.x, f, e * z.x);
+    y.y = fmaf(y.y, f, e * z.y);
+    y.z = fmaf(y.z, f, e * z.z);
+    y.w = fmaf(y.w, f, e * z.w);
   }
+  if (per > 1) {
+    ys[tid] = y;
+    ms[tid] = top;
+    ls[tid] = l;
+    __syncthreads();
+    if (grp != 0) return;
+    for (int i = 1; i < per; ++i) top = fmaxf(top, ms[tid + i * kLanes]);
+    l = 0.f;
+    y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < per; ++i) {
+      const int at = tid + i * kLanes;
+      if (ms[at] == -INFINITY && ls[at] == 0.f) continue;
+      const float e = ms[at] == top ? 1.f : exp_of<T>(ms[at] - top);
+      const float4 z = ys[at];
+      l = fmaf(e, ls[at], l);
+      y.x = fmaf(e, z.x, y.x);
+      y.y = fmaf(e, z.y, y.y);
+      y.z = fmaf(e, z.z, y.z);
+      y.w = fmaf(e, z.w, y.w);
+    }
+  }
+  if (n_parts == 0) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   store_row4<T, HD>(a, row, head, d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
 }
 
 struct Plan {
   int bm;  // rows of a block: 16 or 32 (paged_wave_kernel) or kPagedTileRows
+  int groups;  // of the tile kernel's waves
   int nqb, nsplit, chunk;
 };
 
-// Row blocks, and parts so that about four workgroups come to a CU (two of
-// the tile kernel's), none under 256 keys.
+// Row blocks and parts.
 Plan make_plan(int dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t max_new, int64_t max_len) {
   Plan p;
-  const int64_t packed = std::max<int64_t>(1, std::min(max_new, rows)) * (H / KV);
-  p.bm = packed <= 16 ? 16 : packed <= 64 || dtype == LZ_F32 ? 32 : kPagedTileRows;
+  const int64_t G = H / KV, packed = std::max<int64_t>(1, std::min(max_new, rows)) * G, cus = lz_num_cus();
+  p.bm = packed <= 16 ? 16 : packed < 64 || dtype == LZ_F32 ? 32 : kPagedTileRows;
   p.nqb = (int)lz_cdiv(packed, p.bm);
-  const int64_t blocks = B * KV * p.nqb, len = std::max<int64_t>(1, max_len);
-  const int64_t want = std::max<int64_t>(1, (p.bm == kPagedTileRows ? 2 : 4) * lz_num_cus() / blocks);
+  const bool tiles = p.bm == kPagedTileRows;
+  // blocks that have rows: not every sequence has max_new of them
+  const int64_t blocks = KV * std::min(B * p.nqb, std::min(B, rows) + rows * G / p.bm);
+  const int64_t len = std::max<int64_t>(1, max_len), want = std::max<int64_t>(1, (tiles ? 1 : 4) * cus / blocks);
   p.chunk = (int)std::max<int64_t>(256, lz_cdiv(lz_cdiv(len, want), 64) * 64);
   p.nsplit = (int)lz_cdiv(len, p.chunk);
+  p.groups = blocks * p.nsplit <= cus ? 2 : 1;
   return p;
 }
 
@@ -540,7 +571,8 @@ LZ_EXPORT int lz_paged_attn(const void* q, int64_t ldq, int dtype, int64_t rows,
   const int64_t need = lz_paged_attn_workspace(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
   LZ_REQUIRE(need == 0 || (workspace && lz_aligned16(workspace) && ws_bytes >= need),
              "lz_paged_attn: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
-  const int64_t blocks = B * KV * p.nqb * p.nsplit, joins = lz_cdiv(rows * H * (hd / 4), 256);
+  const int64_t blocks = B * KV * p.nqb * p.nsplit, per = p.nsplit <= 4 ? 1 : p.nsplit <= 16 ? 4 : 8,
+                joins = lz_cdiv(rows * H * (hd / 4) * per, 256);
   LZ_REQUIRE(blocks <= INT32_MAX / 256 && joins <= INT32_MAX / 256, "lz_paged_attn: too many rows");
   PagedArgs a{q, ldq, k, v, (const int8_t*)k_exp, (const int8_t*)v_exp,
               LzPages{table, (int)width, (int)pages, lz_log2(page_size)}, row_start, kv_len, o, ldo, (float*)workspace,
@@ -548,7 +580,7 @@ LZ_EXPORT int lz_paged_attn(const void* q, int64_t ldq, int dtype, int64_t rows,
   hipStream_t s = lz_stream(stream);
   const bool tiles = p.bm == kPagedTileRows;
   if (tiles)
-    if (int rc = lz_paged_tile(a, dtype, cache_dtype == LZ_E4M3, hd, (uint32_t)blocks, s)) return rc;
+    if (int rc = lz_paged_tile(a, dtype, cache_dtype == LZ_E4M3, hd, p.groups, (uint32_t)blocks, s)) return rc;
 #define RUN(T, HD, E8)                                                                    \
   do {                                                                                    \
     if (p.bm == 16) paged_wave_kernel<T, HD, E8, 1><<<(uint32_t)blocks, 256, 0, s>>>(a);  \
@@ -556,7 +588,7 @@ LZ_EXPORT int lz_paged_attn(const void* q, int64_t ldq, int dtype, int64_t rows,
   } while (0)
   if (!tiles) LZ_CACHE_CASES(dtype, cache_dtype, hd, RUN);
 #undef RUN
-#define RUN(T, HD, E8) paged_join_kernel<T, HD><<<(uint32_t)joins, 256, 0, s>>>(a, p.bm)
+#define RUN(T, HD, E8) paged_join_kernel<T, HD><<<(uint32_t)joins, 256, 0, s>>>(a, p.bm, (int)per)
   if (p.nsplit > 1) LZ_CACHE_CASES(dtype, 0, hd, RUN);
 #undef RUN
   return lz_check_launch("lz_paged_attn");

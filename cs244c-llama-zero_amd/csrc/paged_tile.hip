@@ -11,6 +11,8 @@
 // lies in one page); e4m3 ones pass through registers, where the next step's
 // bytes wait while this one is computed, and become 16-bit values once for
 // all four waves.
+#include <type_traits>
+
 #include "paged_attn.h"
 
 namespace {
@@ -22,15 +24,16 @@ struct Tiles {
   // e4m3: 16-byte pieces of a tile and of a thread
   static constexpr int kPieces = 64 * HD / 16, kMine = (kPieces + 255) / 256;
 
-  char* ks;  // two K tiles, then two V tiles
-  int lane, wave, tid;
+  char* ks;  // this key group's two K tiles, then its two V tiles
+  int lane, wave, tid;  // wave, tid: in the group of four waves
   int ids;       // page of the 16-key tile ids_from + lane
   int ids_from;
   uint4 kr[kMine], vr[kMine];
   int kx[kMine], vx[kMine];
 
-  __device__ __forceinline__ char* k_tile(int it) const { return ks + (it & 1) * kTile; }
-  __device__ __forceinline__ char* v_tile(int it) const { return ks + (2 + (it & 1)) * kTile; }
+  int stage;  // of the step that is computed
+  __device__ __forceinline__ char* k_tile(int ahead = 0) const { return ks + (stage ^ ahead) * kTile; }
+  __device__ __forceinline__ char* v_tile(int ahead = 0) const { return ks + (2 + (stage ^ ahead)) * kTile; }
 
   // The pages of steps it .. it + 15 (64 keys each).
   __device__ __forceinline__ void look_up(const PagedArgs& a, int b, int it, int n_keys) {
@@ -38,28 +41,28 @@ struct Tiles {
     const int key = 64 * it + 16 * lane;
     ids = key < n_keys ? a.pg.page_of(b, key) : -1;
   }
-  // bit t: the 16-key tile t of step it has a page (or holds no key at all)
+  // bit t: the 16-key tile t from step it on has a page (or holds no key at all)
   __device__ __forceinline__ uint32_t present(int it, int n_keys) const {
     const uint64_t ok = __ballot(ids >= 0 || 16 * (ids_from + lane) >= n_keys);
-    return (uint32_t)(ok >> (4 * it - ids_from)) & 15u;
+    return (uint32_t)(ok >> (4 * it - ids_from));
   }
-  __device__ __forceinline__ int64_t token(const PagedArgs& a, int g, int it, int r) const {
-    const int id = max(__builtin_amdgcn_readlane(ids, 4 * it + r / 16 - ids_from), 0);  // no page: any, zeroed later
-    return (((int64_t)id * a.KV + g) << a.pg.log_size) + ((64 * it + r) & ((1 << a.pg.log_size) - 1));
-  }
-
-  __device__ __forceinline__ void issue(const PagedArgs& a, int g, int it) {
+  // Step it's rows into the stage `ahead` of this one.  Each wave copies 16,
+  // which lie in one page.
+  __device__ __forceinline__ void issue(const PagedArgs& a, int g, int it, int ahead) {
     if constexpr (!k8) {
+      const int id = max(__builtin_amdgcn_readlane(ids, 4 * it + wave - ids_from), 0);  // no page: any, zeroed later
+      const int64_t tok =
+          (((int64_t)id * a.KV + g) << a.pg.log_size) + ((64 * it + 16 * wave) & ((1 << a.pg.log_size) - 1));
 #pragma unroll
       for (int side = 0; side < 2; ++side) {
-        char* dst = side ? v_tile(it) : k_tile(it);
-        const char* src = static_cast<const char*>(side ? a.v : a.k);
+        char* dst = (side ? v_tile(ahead) : k_tile(ahead)) + wave * kPer * 1024;
+        const lz_v4i rsrc = lz_buffer_rsrc(static_cast<const char*>(side ? a.v : a.k) + tok * HD * 2);
 #pragma unroll
         for (int q = 0; q < kPer; ++q) {
-          const int blk = wave * kPer + q, r = blk * kRowsPerLoad + lane / kChunks;
-          const int c = (lane % kChunks) ^ tswz<HD>(r);
-          lz_dma16_first(lz_buffer_rsrc(src + token(a, g, it, blk * kRowsPerLoad) * HD * 2),
-                         (uint32_t)((lane / kChunks) * HD * 2 + c * 16), 0, dst + blk * 1024);
+          const int c = (lane % kChunks) ^ tswz<HD>(q * kRowsPerLoad + lane / kChunks);  // of the row in its 16
+          const uint32_t off = (uint32_t)(q * 1024 + (lane / kChunks) * HD * 2 + c * 16);
+          if (q == 0) lz_dma16_first(rsrc, off, 0, dst);
+          else lz_dma16(rsrc, off, 0, dst + q * 1024);
         }
       }
     } else {
@@ -86,14 +89,14 @@ struct Tiles {
           make_uint4(e4m3_pair<F, false>(w[2 * h], unit), e4m3_pair<F, true>(w[2 * h], unit),
                      e4m3_pair<F, false>(w[2 * h + 1], unit), e4m3_pair<F, true>(w[2 * h + 1], unit));
   }
-  // e4m3: the bytes of step it into its tiles
-  __device__ __forceinline__ void put(int it) const {
+  // e4m3: the bytes that issue() fetched into their tiles
+  __device__ __forceinline__ void put(int ahead) const {
 #pragma unroll
     for (int j = 0; j < kMine; ++j) {
       const int p = tid + 256 * j, r = p / (HD / 16), c = p % (HD / 16);
       if (kPieces % 256 && p >= kPieces) continue;
-      put(k_tile(it), r, c, kr[j], kx[j]);
-      put(v_tile(it), r, c, vr[j], vx[j]);
+      put(k_tile(ahead), r, c, kr[j], kx[j]);
+      put(v_tile(ahead), r, c, vr[j], vx[j]);
     }
   }
   // zeros into the V rows of step it that hold no token: their weights are
@@ -102,7 +105,7 @@ struct Tiles {
     for (int p = tid; p < 64 * kChunks; p += 256) {
       const int r = p / kChunks;
       if (64 * it + r >= n_keys || !((here >> (r / 16)) & 1))
-        *reinterpret_cast<uint4*>(v_tile(it) + toff<HD>(r, p % kChunks)) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(v_tile() + toff<HD>(r, p % kChunks)) = make_uint4(0, 0, 0, 0);
     }
   }
 };
@@ -133,14 +136,34 @@ __device__ __forceinline__ bf16x8_t finite_part(const bf16x8_t& x) {
   return __builtin_bit_cast(bf16x8_t, w);
 }
 
+// O^T += V^T . P^T of one step; vf: the fragments of V^T for its first 16
+// keys, read ahead as the others are here.  ODD: infinities and NaN left out.
+template <typename F, int HD, bool ODD>
+__device__ __forceinline__ void step_sum(f32x16_t (&o)[HD / 32], const f32x16_t (&s)[2], bf16x8_t (&vf)[2][HD / 32],
+                                         const TileOffsets<HD>& to, const char* vt) {
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    if (ks + 1 < 4)
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) vf[(ks + 1) & 1][i] = to.frag_t(vt, ks + 1, i);
+    const bf16x8_t pb = pack8<F>(s[ks >> 1], 8 * (ks & 1));
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i)
+      o[i] = mfma16<F>(ODD ? finite_part<F>(vf[ks & 1][i]) : vf[ks & 1][i], pb, o[i]);
+  }
+}
+
 // One step's softmax and its part of the sum.  s: scores of keys 32 t + 8 (r /
 // 4) + 4 half + r % 4 in register [t][r]; MASK: keys at or past `lim` (of this
 // lane's row, from the step's first key) and 16-key tiles without their bit in
-// `here` are not seen.
-template <typename F, int HD, bool MASK>
-__device__ __forceinline__ void step_sum(f32x16_t (&s)[2], f32x16_t (&o)[HD / 32], float& m, float& l,
-                                         const TileOffsets<HD>& to, const char* vt, float unit, int lim, uint32_t here,
-                                         bool odd, int half) {
+// `here` are not seen.  ODD: see step_sum().
+template <typename F, int HD, bool MASK, bool ODD>
+__device__ __forceinline__ void step_softmax(f32x16_t (&s)[2], f32x16_t (&o)[HD / 32], float& m, float& l,
+                                             const TileOffsets<HD>& to, const char* vt, float unit, int lim,
+                                             uint32_t here, int half) {
+  bf16x8_t vf[2][HD / 32];
+#pragma unroll
+  for (int i = 0; i < HD / 32; ++i) vf[0][i] = to.frag_t(vt, 0, i);
   float mx = -INFINITY;
 #pragma unroll
   for (int t = 0; t < 2; ++t)
@@ -172,17 +195,7 @@ __device__ __forceinline__ void step_sum(f32x16_t (&s)[2], f32x16_t (&o)[HD / 32
       s[t][r] = p;
       l += p;  // this lane's keys; the halves meet at the end
     }
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks) {
-    const bf16x8_t pb = pack8<F>(s[ks >> 1], 8 * (ks & 1));
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i) {
-      bf16x8_t f = to.frag_t(vt, ks, i);
-      if constexpr (MASK)
-        if (odd) f = finite_part<F>(f);
-      o[i] = mfma16<F>(f, pb, o[i]);
-    }
-  }
+  step_sum<F, HD, ODD>(o, s, vf, to, vt);
 }
 
 // Whether V rows lo .. hi - 1 of the tile hold an infinity or NaN.
@@ -226,23 +239,53 @@ __device__ __forceinline__ void add_odd(f32x16_t (&o)[HD / 32], const f32x16_t (
   }
 }
 
-template <typename F, int HD, bool k8>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 2 : 3, HD == 128 ? 2 : 3)))
+// The sequence with the r-th longest cache (of the first 64; the others keep
+// their places): blocks of long sequences are dealt out first, so that they do
+// not meet on a few CUs at the end.  1024 new tokens over 8192 beside a short
+// prompt: 224 us with the sequences' blocks dealt in turn, 170 so; eight prompts of up
+// to 2048 tokens (16 heads of 128) 110 and 80.
+__device__ __forceinline__ int by_length(const PagedArgs& a, int r, int lane) {
+  if (a.B > 64) return r;
+  const int len = lane < a.B ? a.kv_len[lane] : -1;
+  int rank = lane < a.B ? 0 : 64;
+  for (int i = 0; i < a.B; ++i) {
+    const int other = __builtin_amdgcn_readlane(len, i);
+    rank += other > len || (other == len && i < lane);
+  }
+  return __builtin_ctzll(__ballot(rank == r) | (1ull << 63));
+}
+
+// NG: groups of four waves that share the rows and take every NG-th step of
+// the keys, each with tiles of its own; they meet in LDS at the end.
+template <typename F, int HD, bool k8, int NG>
+__global__ void __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(HD == 128 || NG == 2 ? 2 : 3, HD == 128 || NG == 2 ? 2 : 3)))
 paged_tile_kernel(PagedArgs a) {
   typedef Tiles<F, HD, k8> T;
   constexpr int BM = kPagedTileRows;
-  __shared__ __attribute__((aligned(1024))) char smem[4 * T::kTile];
+  __shared__ __attribute__((aligned(1024))) char smem[NG * 4 * T::kTile];
+  __shared__ float stats[NG == 2 ? 4 : 1][64][2];
 
-  const PagedPlace at(a, blockIdx.x);
-  const PagedRows rw(a, at.b, at.qb * BM);
-  if (rw.m0 >= rw.count) return;
+  // kv heads go to the XCDs in turn, so that a head's keys and values are
+  // fetched into few L2s; then the row blocks of a sequence, most keys first
+  struct {
+    int b, g, split;
+  } at;
+  const uint32_t rest = blockIdx.x / (uint32_t)a.KV;
+  at.g = (int)(blockIdx.x % (uint32_t)a.KV);
+  at.b = by_length(a, (int)(rest / (uint32_t)(a.nqb * a.nsplit)), threadIdx.x & 63);
+  const int place = (int)(rest % (uint32_t)(a.nqb * a.nsplit));
+  at.split = place % a.nsplit;
+  PagedRows rw(a, at.b, 0);
+  rw.m0 = ((rw.count + BM - 1) / BM - 1 - place / a.nsplit) * BM;
+  if (rw.m0 < 0) return;
   const int n_keys = rw.keys(BM), n_parts = PagedRows::parts(a, n_keys);
   if (at.split >= n_parts) return;
   const int k_lo = at.split * a.chunk, k_hi = at.split + 1 == n_parts ? n_keys : k_lo + a.chunk;
 
+  const int grp = NG == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
   T tl;
-  tl.ks = smem;
-  tl.tid = threadIdx.x;
+  tl.ks = smem + grp * 4 * T::kTile;
+  tl.tid = threadIdx.x & 255;
   tl.lane = tl.tid & 63;
   tl.wave = __builtin_amdgcn_readfirstlane(tl.tid >> 6);
   const int lane = tl.lane, half = lane >> 5, l32 = lane & 31;
@@ -261,65 +304,110 @@ paged_tile_kernel(PagedArgs a) {
 #pragma unroll
   for (int kk = 0; kk < HD / 16; ++kk) qf[kk] = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(qp + kk * 16));
   f32x16_t o[HD / 32];
-#pragma unroll
-  for (int i = 0; i < HD / 32; ++i)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
-  float mx = -INFINITY, l = 0.f;
+  float mx, l;
   const float unit = a.scale * kLog2e;
-
-  int it = k_lo / 64;
   const int end = (k_hi + 63) / 64, free_end = min(all / 64, end), wave_end = min((most + 63) / 64, end);
-  tl.look_up(a, at.b, it, n_keys);
-  if (it < end) {
-    tl.issue(a, at.g, it);
-    if constexpr (k8) tl.put(it);
-  }
 
-  // Opens step it: its tiles are there and every wave is done with the other
-  // stage, into which the next step's go.
-  auto open_step = [&]() {
-    dma_barrier();
-    const uint32_t here = tl.present(it, n_keys);
-    if (64 * it + 64 > n_keys || here != 15u) {  // the same for all waves
-      tl.clear(it, n_keys, here);
-      __syncthreads();
+  // One pass over the keys, in rounds of NG steps; `rt` is a round's first
+  // step.  Returns whether V had an infinity or NaN in a step whose keys not
+  // all of this wave's rows see: its zero weights make it NaN in all of them.
+  // Then the pass is made again with ODD, which multiplies the finite part and
+  // adds the rest where it is seen; the other rows get the same bits as ever.
+  auto pass = [&](auto odd_pass) {
+    constexpr bool ODD = decltype(odd_pass)::value;
+    bool met = false;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+    mx = -INFINITY;
+    l = 0.f;
+    int rt = k_lo / 64;
+    tl.stage = 0;
+    tl.look_up(a, at.b, rt, n_keys);
+    if (rt + grp < end) {
+      tl.issue(a, at.g, rt + grp, 0);
+      if constexpr (k8) tl.put(0);
     }
-    if (it + 1 < end) tl.issue(a, at.g, it + 1);
-    return here;
-  };
-  auto close_step = [&]() {
-    if constexpr (k8)
-      if (it + 1 < end) tl.put(it + 1);
-  };
-
-  while (it < end) {
-    // fifteen steps: the pages looked up serve one more, which they issue
-    const int stop = min(it + 15, end);
-    const bool clean = __ballot(tl.ids >= 0 || 16 * (tl.ids_from + lane) >= n_keys) == ~0ull;
-    const int free_stop = clean ? min(stop, free_end) : it;
-    for (; it < free_stop; ++it) {
-      open_step();
-      f32x16_t s[2];
-      step_scores<F, HD>(s, to, tl.k_tile(it), qf);
-      step_sum<F, HD, false>(s, o, mx, l, to, tl.v_tile(it), unit, 0, 15u, false, half);
-      close_step();
-    }
-    for (; it < stop; ++it) {
-      const uint32_t here = open_step();
-      if (it < wave_end) {
-        f32x16_t s[2];
-        step_scores<F, HD>(s, to, tl.k_tile(it), qf);
-        const bool odd = rows_odd<F, HD>(tl.v_tile(it), max(all - 64 * it, 0), min(64, n_keys - 64 * it), lane);
-        step_sum<F, HD, true>(s, o, mx, l, to, tl.v_tile(it), unit, sees - 64 * it, here, odd, half);
-        if (odd) add_odd<F, HD>(o, s, tl.v_tile(it), sees - 64 * it, lane);
+    // Opens a round: its tiles are there and every wave is done with the other
+    // stage, into which the next round's go.
+    auto open_round = [&](auto full) {
+      dma_barrier();
+      uint32_t here = ~0u;
+      if constexpr (!decltype(full)::value) {
+        here = tl.present(rt, n_keys);
+        constexpr uint32_t kAll = NG == 2 ? 0xffu : 0xfu;
+        if (64 * (rt + NG) > n_keys || (here & kAll) != kAll) {  // the same for all waves
+          tl.clear(rt + grp, n_keys, here >> (4 * grp));
+          __syncthreads();
+        }
       }
-      close_step();
+      if (rt + grp + NG < end) tl.issue(a, at.g, rt + grp + NG, 1);
+      return here >> (4 * grp);
+    };
+    auto close_round = [&]() {
+      if constexpr (k8)
+        if (rt + grp + NG < end) tl.put(1);
+      tl.stage ^= 1;
+      rt += NG;
+    };
+    while (rt < end) {
+      // the pages looked up serve one more round than is computed, which it issues
+      const int stop = min(rt + 16 - NG, end);
+      const bool clean = __ballot(tl.ids >= 0 || 16 * (tl.ids_from + lane) >= n_keys) == ~0ull;
+      // rounds that lie before every row's diagonal and whose tiles are full
+      const int free_stop = clean && !ODD ? min(stop, min(free_end - grp, n_keys / 64 - NG + 1)) : rt;
+      while (rt < free_stop) {
+        open_round(std::true_type{});
+        f32x16_t s[2];
+        step_scores<F, HD>(s, to, tl.k_tile(), qf);
+        step_softmax<F, HD, false, false>(s, o, mx, l, to, tl.v_tile(), unit, 0, 15u, half);
+        close_round();
+      }
+      while (rt < stop) {
+        const uint32_t here = open_round(std::false_type{});
+        const int it = rt + grp;
+        if (it < wave_end) {
+          f32x16_t s[2];
+          step_scores<F, HD>(s, to, tl.k_tile(), qf);
+          if constexpr (!ODD)
+            met |= rows_odd<F, HD>(tl.v_tile(), max(all - 64 * it, 0), min(64, n_keys - 64 * it), lane);
+          step_softmax<F, HD, true, ODD>(s, o, mx, l, to, tl.v_tile(), unit, sees - 64 * it, here, half);
+          if constexpr (ODD) add_odd<F, HD>(o, s, tl.v_tile(), sees - 64 * it, lane);
+        }
+        close_round();
+      }
+      if (rt < end) tl.look_up(a, at.b, rt, n_keys);
     }
-    if (it < end) tl.look_up(a, at.b, it, n_keys);
-  }
+    return met;
+  };
+  if (__syncthreads_or(pass(std::false_type{}))) pass(std::true_type{});
 
   l = sum_halves(l);
+  if constexpr (NG == 2) {
+    // the second group's sums into LDS, the first adds them to its own
+    __syncthreads();
+    float* park = reinterpret_cast<float*>(smem) + tl.wave * (HD / 2) * 64 + lane;
+    if (grp == 1) {
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) park[(16 * i + r) * 64] = o[i][r];
+      stats[tl.wave][lane][0] = mx;
+      stats[tl.wave][lane][1] = l;
+    }
+    __syncthreads();
+    if (grp == 1) return;
+    const float m2 = stats[tl.wave][lane][0], l2 = stats[tl.wave][lane][1];
+    const float top = fmaxf(mx, m2);
+    const float f = mx == top ? 1.f : __builtin_amdgcn_exp2f(mx - top), f2 = m2 == top ? 1.f : __builtin_amdgcn_exp2f(m2 - top);
+    mx = top;
+    l = fmaf(l, f, l2 * f2);
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[i][r] = fmaf(o[i][r], f, park[(16 * i + r) * 64] * f2);
+  }
   if (m_first + l32 >= rw.count) return;
   if (n_parts == 1) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -349,11 +437,17 @@ paged_tile_kernel(PagedArgs a) {
 
 }  // namespace
 
-int lz_paged_tile(const LzPagedArgs& a, int dtype, bool e4m3, int64_t hd, uint32_t blocks, hipStream_t stream) {
+int lz_paged_tile(const LzPagedArgs& a, int dtype, bool e4m3, int64_t hd, int groups, uint32_t blocks, hipStream_t stream) {
 #define RUN(F, HD)                                                                      \
   do {                                                                                  \
-    if (e4m3) paged_tile_kernel<F, HD, true><<<blocks, 256, 0, stream>>>(a);            \
-    else paged_tile_kernel<F, HD, false><<<blocks, 256, 0, stream>>>(a);                \
+    if (groups == 2) {                                                                  \
+      if (e4m3) paged_tile_kernel<F, HD, true, 2><<<blocks, 512, 0, stream>>>(a);       \
+      else paged_tile_kernel<F, HD, false, 2><<<blocks, 512, 0, stream>>>(a);           \
+    } else if (e4m3) {                                                                  \
+      paged_tile_kernel<F, HD, true, 1><<<blocks, 256, 0, stream>>>(a);                 \
+    } else {                                                                            \
+      paged_tile_kernel<F, HD, false, 1><<<blocks, 256, 0, stream>>>(a);                \
+    }                                                                                   \
   } while (0)
   if (dtype == LZ_F16) {
     if (hd == 32) RUN(FmtF16, 32);
