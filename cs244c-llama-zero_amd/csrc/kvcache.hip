@@ -97,6 +97,8 @@ struct WriteArgs {
 // upper half): a head is HD / 2 / N neighbouring lanes.
 template <typename T, int HD, bool k8>
 __global__ void __launch_bounds__(256) kv_write_kernel(WriteArgs a) {
+  __shared__ LzSeqs seqs;
+  seqs.load(a.row_start, a.kv_len, a.B, a.rows, threadIdx.x);
   constexpr int N = Vec<T>::N, kLanes = HD / 2 / N;
   const int heads = a.H + 2 * a.KV, per_row = heads * kLanes;
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
@@ -109,9 +111,10 @@ __global__ void __launch_bounds__(256) kv_write_kernel(WriteArgs a) {
   const T* x = static_cast<const T*>(a.qkv) + row * a.ld + (int64_t)head * HD + i;
   Vec<T>::load(lo, x);
   Vec<T>::load(hi, x + HD / 2);
-  const int b = lz_seq_of_row(a.row_start, a.B, a.rows, row);
+  int base = 0;
+  const int b = seqs.find(a.row_start, a.kv_len, a.B, a.rows, row, base);
   if (b < 0) return;
-  const int pos = a.kv_len[b] - a.row_start[b + 1] + row;
+  const int pos = base + row;
   const bool there = pos >= 0 && pos < a.positions;
   if (head < a.H + a.KV) {
     if (there) {
@@ -158,7 +161,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(WriteArgs a) {
     }
 #pragma unroll
     for (int o = 1; o < kLanes; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-    const int e = exponent_of<(sizeof(T) == 2 && !std::is_same<T, uint16_t>::value)>(amax);
+    const int e = exponent_of<std::is_same<T, _Float16>::value>(amax);
     const float inv = lz_pow2(-e);
     uint8_t* dst = static_cast<uint8_t*>(is_k ? a.k : a.v) + token * HD + i;
     store_e4m3<N>(dst, lo, inv);
@@ -182,6 +185,8 @@ struct ReadArgs {
 // One thread per 16 bytes of an output row, keys and values alike.
 template <typename T, int HD, bool k8>
 __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
+  __shared__ LzSeqs seqs;
+  seqs.load(a.start, nullptr, a.B, a.rows, threadIdx.x);
   constexpr int N = Vec<T>::N, kLanes = HD / N;
   const int per_row = a.KV * kLanes;
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
@@ -189,9 +194,10 @@ __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
   if (row >= a.rows) return;
   const int rem = (int)(idx - (uint32_t)row * (uint32_t)per_row);
   const int g = rem / kLanes, i = (rem - g * kLanes) * N;
-  const int b = lz_seq_of_row(a.start, a.B, a.rows, row);
+  int base = 0;
+  const int b = seqs.find(a.start, nullptr, a.B, a.rows, row, base);
   if (b < 0) return;
-  const int pos = row - a.start[b];
+  const int pos = base + row;
   const int page = a.pg.page_of(b, pos);
   const int64_t token = (((int64_t)page * a.KV + g) << a.pg.log_size) + (pos & ((1 << a.pg.log_size) - 1));
   const int64_t out = ((int64_t)row * a.KV + g) * HD + i;

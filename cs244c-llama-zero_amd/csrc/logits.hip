@@ -33,38 +33,110 @@ struct LogitsArgs {
   int B, V, n_tokens, mask_kind;  // mask_kind 0: none, 1: a byte a token, 2: a bit a token
 };
 
-constexpr int kSlice = 4096;
-
-template <typename T>
+// NV * 2048 tokens of the vocabulary a workgroup: eight adjacent ones a thread
+// and vector, whose logits are in flight while the text is counted.  ALIGNED:
+// every row's vectors are 16-byte aligned.
+template <typename T, int NV, bool ALIGNED>
 __global__ void __launch_bounds__(256) process_logits_kernel(LogitsArgs a) {
-  __shared__ uint32_t cnt[kSlice];  // 2 * (times in the answer) + (1 if in the text)
+  constexpr int kSlice = NV * 2048;
+  __shared__ __attribute__((aligned(16))) uint32_t cnt[kSlice];  // 2 * (times in the answer) + (1 if in the text)
   const int slices = (a.V + kSlice - 1) / kSlice;
   const int b = blockIdx.x / slices, lo = (blockIdx.x % slices) * kSlice;
   const int n = min(kSlice, a.V - lo);
-  const int len = a.tokens ? (a.lengths ? min(max(a.lengths[b], 0), a.n_tokens) : a.n_tokens) : 0;
-  const int prompt = a.prompts ? a.prompts[b] : 0;
-  for (int i = threadIdx.x; i < n; i += 256) cnt[i] = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < len; i += 256) {
-    const int64_t t = a.tokens[b * a.ldt + i] - lo;
-    if (t >= 0 && t < n) {
-      atomicOr(&cnt[t], 1u);
-      if (i >= prompt) atomicAdd(&cnt[t], 2u);
+  const int tid = threadIdx.x;
+  const T* x_row = static_cast<const T*>(a.logits) + b * a.ld + lo;
+  const float* b_row = a.bias ? a.bias + b * a.ldb + lo : nullptr;
+
+  float x[NV][8];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int i = (k * 256 + tid) * 8;
+    if (ALIGNED && i + 8 <= n) {
+      T raw[8];
+#pragma unroll
+      for (int w = 0; w < (int)sizeof(T) / 2; ++w)
+        reinterpret_cast<uint4*>(raw)[w] = reinterpret_cast<const uint4*>(x_row + i)[w];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[k][e] = Elem<T>::load(raw, e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[k][e] = i + e < n ? Elem<T>::load(x_row, i + e) : 0.f;
     }
   }
-  __syncthreads();
+
+  const int len = a.tokens ? (a.lengths ? min(max(a.lengths[b], 0), a.n_tokens) : a.n_tokens) : 0;
+  const int prompt = a.prompts ? a.prompts[b] : 0;
+  if (len > 0) {  // the same for the whole workgroup
+    for (int i = tid; i < kSlice / 4; i += 256) reinterpret_cast<uint4*>(cnt)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    const int64_t* text = a.tokens + b * a.ldt;
+#pragma unroll 4
+    for (int i = tid; i < len; i += 256) {
+      const uint64_t t = (uint64_t)(text[i] - lo);
+      if (t < (uint64_t)n) {
+        atomicOr(&cnt[t], 1u);
+        if (i >= prompt) atomicAdd(&cnt[t], 2u);
+      }
+    }
+    __syncthreads();
+  }
   const float r = a.rep ? a.rep[b] : a.rep_s, p = a.pres ? a.pres[b] : a.pres_s, f = a.freq ? a.freq[b] : a.freq_s;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const int v = lo + i;
-    float x = Elem<T>::load(static_cast<const T*>(a.logits) + b * a.ld, v);
-    const uint32_t c = cnt[i];
-    if (c & 1) x = x > 0.f ? x / r : x * r;
-    if (c >> 1) x = x - f * (float)(c >> 1) - p;
-    if (a.bias) x += a.bias[b * a.ldb + v];
-    bool ok = true;
-    if (a.mask_kind == 1) ok = static_cast<const uint8_t*>(a.mask)[b * a.ldm + v] != 0;
-    else if (a.mask_kind == 2) ok = (static_cast<const uint32_t*>(a.mask)[b * a.ldm + (v >> 5)] >> (v & 31)) & 1;
-    a.out[b * a.ldo + v] = ok ? x : -INFINITY;
+
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int i = (k * 256 + tid) * 8;
+    if (i >= n) break;
+    if (len > 0) {
+      uint32_t c[8];
+      *reinterpret_cast<uint4*>(c) = reinterpret_cast<const uint4*>(cnt + i)[0];
+      *reinterpret_cast<uint4*>(c + 4) = reinterpret_cast<const uint4*>(cnt + i)[1];
+      if (c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (c[e] & 1) x[k][e] = x[k][e] > 0.f ? x[k][e] / r : x[k][e] * r;
+          if (c[e] >> 1) x[k][e] = x[k][e] - f * (float)(c[e] >> 1) - p;
+        }
+      }
+    }
+    float y[8] = {};
+    if (b_row) {
+      if (ALIGNED && i + 8 <= n) {
+        reinterpret_cast<float4*>(y)[0] = reinterpret_cast<const float4*>(b_row + i)[0];
+        reinterpret_cast<float4*>(y)[1] = reinterpret_cast<const float4*>(b_row + i)[1];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (i + e < n) y[e] = b_row[i + e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[k][e] += y[e];
+    }
+    uint32_t allowed = 0xffu;
+    if (a.mask_kind == 2) {  // i and lo are multiples of eight: the bits are in one word
+      allowed = static_cast<const uint32_t*>(a.mask)[b * a.ldm + ((lo + i) >> 5)] >> (i & 31);
+    } else if (a.mask_kind == 1) {
+      const uint8_t* m = static_cast<const uint8_t*>(a.mask) + b * a.ldm + lo + i;
+      uint8_t w[8] = {};
+      if (i + 8 <= n) __builtin_memcpy(w, m, 8);
+      else
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (i + e < n) w[e] = m[e];
+      allowed = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) allowed |= (w[e] != 0) << e;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (allowed >> e) & 1 ? x[k][e] : -INFINITY;
+    float* o = a.out + b * a.ldo + lo + i;
+    if (ALIGNED && i + 8 <= n) {
+      reinterpret_cast<float4*>(o)[0] = reinterpret_cast<const float4*>(y)[0];
+      reinterpret_cast<float4*>(o)[1] = reinterpret_cast<const float4*>(y)[1];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (i + e < n) o[e] = y[e];
+    }
   }
 }
 
@@ -82,14 +154,28 @@ LZ_EXPORT int lz_process_logits(const void* logits, int64_t ld, int dtype, int64
              "lz_process_logits: mask kind %d", mask_kind);
   if (B == 0 || V == 0) return LZ_OK;
   LZ_REQUIRE(logits && out && ldo >= V && (B == 1 || ld >= V) && (tokens || n_tokens == 0), "lz_process_logits: bad arguments");
-  const int64_t slices = lz_cdiv(V, kSlice);
+  const int esz = lz_esize(dtype);
+  const bool aligned = lz_aligned16(logits) && lz_aligned16(out) && (B == 1 || (ld * esz % 16 == 0 && ldo % 4 == 0)) &&
+                       (!bias || (lz_aligned16(bias) && ldb % 4 == 0));
+  // small slices where the rows are few and a slice's chain of loads is the
+  // time; large ones where each reads a long text again
+  const bool small = B * lz_cdiv(V, 8192) < 2 * lz_num_cus();
+  const int64_t slices = lz_cdiv(V, small ? 2048 : 8192);
   LZ_REQUIRE(B * slices <= INT32_MAX / 256, "lz_process_logits: too many rows");
   LogitsArgs a{logits, ld, n_tokens ? tokens : nullptr, ldt, lengths, prompts, rep, pres, freq, rep_s, pres_s, freq_s,
                bias, ldb, mask, ldm, out, ldo, (int)B, (int)V, (int)n_tokens, mask_kind};
   const uint32_t grid = (uint32_t)(B * slices);
   hipStream_t s = lz_stream(stream);
-  if (dtype == LZ_BF16) process_logits_kernel<uint16_t><<<grid, 256, 0, s>>>(a);
-  else if (dtype == LZ_F16) process_logits_kernel<_Float16><<<grid, 256, 0, s>>>(a);
-  else process_logits_kernel<float><<<grid, 256, 0, s>>>(a);
+#define RUN(T)                                                                           \
+  do {                                                                                   \
+    if (small && aligned) process_logits_kernel<T, 1, true><<<grid, 256, 0, s>>>(a);     \
+    else if (small) process_logits_kernel<T, 1, false><<<grid, 256, 0, s>>>(a);          \
+    else if (aligned) process_logits_kernel<T, 4, true><<<grid, 256, 0, s>>>(a);         \
+    else process_logits_kernel<T, 4, false><<<grid, 256, 0, s>>>(a);                     \
+  } while (0)
+  if (dtype == LZ_BF16) RUN(uint16_t);
+  else if (dtype == LZ_F16) RUN(_Float16);
+  else RUN(float);
+#undef RUN
   return lz_check_launch("lz_process_logits");
 }
