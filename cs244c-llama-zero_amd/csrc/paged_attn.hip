@@ -236,16 +236,22 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
   __shared__ __attribute__((aligned(16))) float park[4 * BM * RS];
   __shared__ float ml[4][BM][2];
 
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c16 = lane & 15, g4 = lane >> 4;
   const PagedPlace at(a, blockIdx.x);
+  const int k_lo = at.split * a.chunk;
+  // This wave's 16-key tiles: number x is at key k_lo + (x / NT * 4 + wave) *
+  // KT + 16 * (x % NT).  Their pages are looked up 64 at a time, one a lane, the
+  // first beside the sequence's length.
+  auto key_of = [&](int x) { return k_lo + ((x / NT) * 4 + wave) * KT + 16 * (x % NT); };
+  const int first_ids = a.pg.page_of(at.b, key_of(lane));
+
   const PagedRows rw(a, at.b, at.qb * BM);
   if (rw.m0 >= rw.count) return;
   const int n_keys = rw.keys(BM), n_parts = PagedRows::parts(a, n_keys);
   if (at.split >= n_parts) return;
-  const int k_lo = at.split * a.chunk, k_hi = at.split + 1 == n_parts ? n_keys : k_lo + a.chunk;
-
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c16 = lane & 15, g4 = lane >> 4;
+  const int k_hi = at.split + 1 == n_parts ? n_keys : k_lo + a.chunk;
 
   typename W::Query q[NQ];
   int sees[NQ];
@@ -268,11 +274,8 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
   }
   const float unit = sizeof(T) == 4 ? a.scale : a.scale * kLog2e;
 
-  // This wave's 16-key tiles: number x is at key k_lo + (x / NT * 4 + wave) *
-  // KT + 16 * (x % NT).  Their pages are looked up 64 at a time, one a lane.
-  int ids = -1, ids_from = -64;
+  int ids = key_of(lane) < k_hi ? first_ids : -1, ids_from = 0;
   const int size_mask = (1 << a.pg.log_size) - 1;
-  auto key_of = [&](int x) { return k_lo + ((x / NT) * 4 + wave) * KT + 16 * (x % NT); };
   auto tokens = [&](int64_t (&tok)[NT], int tile) {
     const int x = tile * NT;
     if (x - ids_from >= 64) {
@@ -463,6 +466,21 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm, in
   const int tid = threadIdx.x, d = tid % kLanes * 4, grp = tid / kLanes % per, rows = 256 / (kLanes * per);
   const uint32_t rh = blockIdx.x * (uint32_t)rows + (uint32_t)(tid / (kLanes * per));
   const int row = (int)(rh / (uint32_t)a.H), head = (int)(rh % (uint32_t)a.H);
+  const float* part = a.part + (int64_t)rh * a.nsplit * HD + d;
+  const float* s2 = a.part + (int64_t)a.rows * a.H * a.nsplit * HD + (int64_t)rh * a.nsplit * 2;
+  // A thread's first parts are fetched beside what says how many there are
+  // (parts that were not written hold anything and are not used).
+  constexpr int kAhead = 4;
+  float4 z[kAhead];
+  float2 zs[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    const int i = grp + k * per;
+    if (row < a.rows && i < a.nsplit) {
+      z[k] = *reinterpret_cast<const float4*>(part + (int64_t)i * HD);
+      zs[k] = *reinterpret_cast<const float2*>(s2 + 2 * i);
+    }
+  }
   int n_parts = 0;
   if (row < a.rows) {
     const int b = lz_seq_of_row(a.row_start, a.B, a.rows, row);
@@ -474,24 +492,25 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm, in
     }
   }
   if (n_parts == 1) n_parts = 0;  // was written whole
-  const float* part = a.part + (int64_t)rh * a.nsplit * HD + d;
-  const float* s2 = a.part + (int64_t)a.rows * a.H * a.nsplit * HD + (int64_t)rh * a.nsplit * 2;
   float top = -INFINITY, l = 0.f;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = grp; i < n_parts; i += per) {
-    const float4 z = *reinterpret_cast<const float4*>(part + (int64_t)i * HD);
-    const float2 t = *reinterpret_cast<const float2*>(s2 + 2 * i);
-    if (t.x == -INFINITY && t.y == 0.f) continue;  // saw nothing
+  auto add = [&](const float4& v, const float2& t) {
+    if (t.x == -INFINITY && t.y == 0.f) return;  // saw nothing
     const float m_new = fmaxf(top, t.x);
     const float f = m_new == top ? 1.f : exp_of<T>(top - m_new), e = m_new == t.x ? 1.f : exp_of<T>(t.x - m_new);
     top = m_new;
     l = fmaf(l, f, e * t.y);
-    y.x = fmaf(y.x, f, e * z.x);
-    y.y = fmaf(y.y, f, e * z.y);
-    y.z = fmaf(y.z, f, e * z.z);
-    y.w = fmaf(y.w, f, e * z.w);
-  }
+    y.x = fmaf(y.x, f, e * v.x);
+    y.y = fmaf(y.y, f, e * v.y);
+    y.z = fmaf(y.z, f, e * v.z);
+    y.w = fmaf(y.w, f, e * v.w);
+  };
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    if (grp + k * per < n_parts) add(z[k], zs[k]);
+#pragma unroll 4
+  for (int i = grp + kAhead * per; i < n_parts; i += per)
+    add(*reinterpret_cast<const float4*>(part + (int64_t)i * HD), *reinterpret_cast<const float2*>(s2 + 2 * i));
   if (per > 1) {
     ys[tid] = y;
     ms[tid] = top;
