@@ -543,17 +543,35 @@ struct Plan {
   int nqb, nsplit, chunk;
 };
 
-// Row blocks and parts.
-Plan make_plan(int dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t max_new, int64_t max_len) {
+// Row blocks and parts.  paged_wave_kernel: whole sequences where there is a
+// block for every CU (32 ragged sequences of up to 2048, 16/8 heads of 128: 33
+// us, in parts of 512 keys 37); else four workgroups a CU, so that lengths even
+// out (16 of up to 4096, 32/8 heads: 27 us in eight parts, 33 in four), but two
+// where that makes more than 16 parts to join (4 x 32768 in e4m3: 41 us in 16,
+// 48 in 32), and parts of 256 KiB at least, below which a part's lookups and
+// its end cost more than its keys (8 of up to 4096: 20 us, 23 in half as much),
+// while every CU has one (1 x 8192: 14 us in 32, 19 in 8).  The tile kernel:
+// one workgroup a CU, of two wave groups where that is all (1 x 512 new tokens
+// over 4096: 55 us in two parts, 70 whole, 89 whole with one group; in four
+// parts, with one group, 55).
+Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd, int64_t max_new,
+               int64_t max_len) {
   Plan p;
   const int64_t G = H / KV, packed = std::max<int64_t>(1, std::min(max_new, rows)) * G, cus = lz_num_cus();
   p.bm = packed <= 16 ? 16 : packed < 64 || dtype == LZ_F32 ? 32 : kPagedTileRows;
   p.nqb = (int)lz_cdiv(packed, p.bm);
-  const bool tiles = p.bm == kPagedTileRows;
   // blocks that have rows: not every sequence has max_new of them
   const int64_t blocks = KV * std::min(B * p.nqb, std::min(B, rows) + rows * G / p.bm);
-  const int64_t len = std::max<int64_t>(1, max_len), want = std::max<int64_t>(1, (tiles ? 1 : 4) * cus / blocks);
-  p.chunk = (int)std::max<int64_t>(256, lz_cdiv(lz_cdiv(len, want), 64) * 64);
+  const int64_t len = std::max<int64_t>(1, max_len), one = std::max<int64_t>(1, cus / blocks);
+  int64_t chunk;
+  if (p.bm == kPagedTileRows || blocks >= cus) {
+    chunk = lz_cdiv(len, one);
+  } else {
+    const int64_t key_bytes = 2 * hd * (cache_dtype == LZ_E4M3 ? 1 : lz_esize(dtype));
+    chunk = lz_cdiv(len, std::min(4 * cus / blocks, std::max<int64_t>(16, 2 * cus / blocks)));
+    chunk = std::max(chunk, std::min((256 << 10) / key_bytes, lz_cdiv(len, one)));
+  }
+  p.chunk = (int)std::max<int64_t>(256, lz_cdiv(chunk, 64) * 64);
   p.nsplit = (int)lz_cdiv(len, p.chunk);
   p.groups = blocks * p.nsplit <= cus ? 2 : 1;
   return p;
@@ -564,7 +582,7 @@ Plan make_plan(int dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_
 LZ_EXPORT int64_t lz_paged_attn_workspace(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV,
                                           int64_t hd, int64_t max_new, int64_t max_len) {
   if (rows <= 0 || B <= 0 || H <= 0 || KV <= 0 || H % KV || max_len < 0 || max_len > INT32_MAX - 1024) return 0;
-  const Plan p = make_plan(dtype, rows, B, H, KV, max_new, max_len);
+  const Plan p = make_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
   return p.nsplit > 1 ? rows * H * p.nsplit * (hd + 2) * 4 : 0;
 }
 
@@ -586,7 +604,7 @@ LZ_EXPORT int lz_paged_attn(const void* q, int64_t ldq, int dtype, int64_t rows,
                            ldo * esz % 16 == 0),
              "lz_paged_attn: rows must be 16-byte aligned");
   if (rows == 0) return LZ_OK;
-  const Plan p = make_plan(dtype, rows, B, H, KV, max_new, max_len);
+  const Plan p = make_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
   const int64_t need = lz_paged_attn_workspace(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
   LZ_REQUIRE(need == 0 || (workspace && lz_aligned16(workspace) && ws_bytes >= need),
              "lz_paged_attn: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
