@@ -239,21 +239,72 @@ __device__ __forceinline__ void add_odd(f32x16_t (&o)[HD / 32], const f32x16_t (
   }
 }
 
-// The sequence with the r-th longest cache (of the first 64; the others keep
-// their places): blocks of long sequences are dealt out first, so that they do
-// not meet on a few CUs at the end.  1024 new tokens over 8192 beside a short
-// prompt: 224 us with the sequences' blocks dealt in turn, 170 so; eight prompts of up
-// to 2048 tokens (16 heads of 128) 110 and 80.
-__device__ __forceinline__ int by_length(const PagedArgs& a, int r, int lane) {
-  if (a.B > 64) return r;
-  const int len = lane < a.B ? a.kv_len[lane] : -1;
-  int rank = lane < a.B ? 0 : 64;
-  for (int i = 0; i < a.B; ++i) {
-    const int other = __builtin_amdgcn_readlane(len, i);
-    rank += other > len || (other == len && i < lane);
+// The w-th row block of a kv head in the order of the keys that blocks go over,
+// most first: the long ones start at once and the short ones fill the gaps
+// (eight prompts of up to 2048 tokens, 16 heads of 128, fp16: 110 us dealt in
+// turn, 80 sequence after sequence, 72 so).  Lane b of a wave counts sequence b's blocks; a bisection finds the
+// step count of the w-th one.
+struct ByLength {
+  int b, m0;  // sequence and first row; b < 0: there are fewer blocks
+
+  static __device__ __forceinline__ int sum(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, false);  // row_ror 8, 4, 2, 1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x122, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, false);
+    const auto h = __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false);
+    const auto q = __builtin_amdgcn_permlane32_swap(h[0] + h[1], h[0] + h[1], false, false);
+    return __builtin_amdgcn_readfirstlane((int)(q[0] + q[1]));
   }
-  return __builtin_ctzll(__ballot(rank == r) | (1ull << 63));
-}
+
+  __device__ __forceinline__ ByLength(const PagedArgs& a, int w, int lane) {
+    constexpr int BM = kPagedTileRows;
+    if (a.B > 64) {  // sequence after sequence
+      b = w / a.nqb;
+      const PagedRows rw(a, b, 0);
+      m0 = ((rw.count + BM - 1) / BM - 1 - w % a.nqb) * BM;
+      if (m0 < 0) b = -1;
+      return;
+    }
+    int count = 0, base = 0, nq = 0;
+    const int G = a.H / a.KV, cap = a.pg.width << a.pg.log_size;
+    if (lane < a.B) {
+      const PagedRows rw(a, lane, 0);
+      count = max(rw.count, 0);
+      base = rw.base + rw.row0;  // keys that the sequence's first row sees
+      nq = (count + BM - 1) / BM;
+    }
+    // this lane's first block with more than 64 s keys, nq: none; -1: all blocks
+    auto first = [&](int s) {
+      const int t = 64 * s + 1;
+      if (s < 0) return 0;
+      const int d = t - base;  // token of its first row that sees t keys
+      if (t > cap || nq == 0 || d > (count - 1) / G) return nq;
+      return max(d, 0) * G / BM;
+    };
+    b = -1;
+    m0 = 0;
+    if (w >= sum(nq)) return;
+    int lo = -1, hi = cap / 64 + 1;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (w < sum(nq - first(mid))) lo = mid;
+      else hi = mid;
+    }
+    const int f0 = first(lo), f1 = first(hi), r = w - sum(nq - f1);
+    int before = f1 - f0;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(before, o, 64);
+      if (lane >= o) before += y;
+    }
+    before -= f1 - f0;
+    const uint64_t here = __ballot(before <= r && r < before + f1 - f0);
+    if (here == 0) return;
+    b = __builtin_ctzll(here);
+    m0 = __builtin_amdgcn_readlane(f0 + r - before, b) * BM;
+  }
+};
 
 // NG: groups of four waves that share the rows and take every NG-th step of
 // the keys, each with tiles of its own; they meet in LDS at the end.
@@ -266,18 +317,14 @@ paged_tile_kernel(PagedArgs a) {
   __shared__ float stats[NG == 2 ? 4 : 1][64][2];
 
   // kv heads go to the XCDs in turn, so that a head's keys and values are
-  // fetched into few L2s; then the row blocks of a sequence, most keys first
-  struct {
-    int b, g, split;
-  } at;
+  // fetched into few L2s
   const uint32_t rest = blockIdx.x / (uint32_t)a.KV;
-  at.g = (int)(blockIdx.x % (uint32_t)a.KV);
-  at.b = by_length(a, (int)(rest / (uint32_t)(a.nqb * a.nsplit)), threadIdx.x & 63);
-  const int place = (int)(rest % (uint32_t)(a.nqb * a.nsplit));
-  at.split = place % a.nsplit;
-  PagedRows rw(a, at.b, 0);
-  rw.m0 = ((rw.count + BM - 1) / BM - 1 - place / a.nsplit) * BM;
-  if (rw.m0 < 0) return;
+  const ByLength block(a, (int)(rest / (uint32_t)a.nsplit), threadIdx.x & 63);
+  if (block.b < 0) return;
+  const struct {
+    int b, g, split;
+  } at = {block.b, (int)(blockIdx.x % (uint32_t)a.KV), (int)(rest % (uint32_t)a.nsplit)};
+  const PagedRows rw(a, at.b, block.m0);
   const int n_keys = rw.keys(BM), n_parts = PagedRows::parts(a, n_keys);
   if (at.split >= n_parts) return;
   const int k_lo = at.split * a.chunk, k_hi = at.split + 1 == n_parts ? n_keys : k_lo + a.chunk;

@@ -255,6 +255,122 @@ def test_paged_attention_lengths(dtype, e4m3, n, length, H, KV, hd, page):
     _check_attention(c, H)
 
 
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("seqs,H,KV", [
+    ([(1, 1 + 7 * b % 40) for b in range(300)], 2, 1),                          # more sequences than threads
+    ([(1, 1 + b % 3) for b in range(1100)], 1, 1),                              # more than the tables in LDS hold
+    ([(1 + b % 5, 1 + b % 5 + b % 17) for b in range(1030)], 1, 1),
+    ([(b % 37, b % 37 + 11 * b % 50) for b in range(70)], 8, 2),                # chunks of more than 64 sequences
+    ([(3, 90), (70, 71), (0, 0), (33, 400), (1, 1)], 12, 3),                    # chunks beside single tokens
+])
+def test_many_sequences(seqs, H, KV, e4m3):
+    """Attention, write and read of long lists of sequences."""
+    c = Case(seqs, KV, 32, 16, BF16, e4m3, seed=len(seqs), fill=None if e4m3 else math.nan)
+    _check_attention(c, H)
+    n = [min(l, 20) for _, l in seqs]
+    start = torch.tensor([sum(n[:b]) for b in range(len(n) + 1)], dtype=torch.int32)
+    k, _ = ops.kv_cache_read(c.layer, c.step.page_table, start.to(DEV), int(start[-1]), BF16)
+    want = torch.cat([c.tokens(0, b, m) for b, m in enumerate(n)]).reshape(-1, KV * 32)
+    assert torch.equal(k.cpu(), want.to(BF16))
+    cos, sin = _tables(c.step.max_len, 32, BF16)
+    qkv = torch.randn(c.rows, (H + 2 * KV) * 32, generator=c.g).to(BF16)
+    q = ops.kv_cache_write(qkv.to(DEV), c.layer, c.step, H, cos.to(DEV), sin.to(DEV))
+    pos = torch.cat([torch.arange(l - m, l) for m, l in seqs])
+    x = _rotated(qkv.view(c.rows, -1, 32)[:, : H + KV], pos, cos, sin)
+    assert torch.equal(q.cpu(), x[:, :H].reshape(c.rows, -1).to(BF16))
+    start = torch.tensor([sum(l for _, l in seqs[:b]) for b in range(len(seqs) + 1)], dtype=torch.int32)
+    _, v = ops.kv_cache_read(c.layer, c.step.page_table, start.to(DEV), int(start[-1]), F32 if e4m3 else BF16)
+    new = torch.cat([torch.arange(int(start[b]) + l - m, int(start[b]) + l) for b, (m, l) in enumerate(seqs)])
+    want = qkv[:, (H + KV) * 32 :].reshape(-1, 32)
+    if e4m3:
+        y, e = _quantise(want.float(), BF16)
+        want = y.float() * torch.ldexp(torch.ones(1), e.int())[:, None]
+    assert torch.equal(v.cpu()[new].reshape(-1, 32), want)
+
+
+@pytest.mark.parametrize("new,bound", [(1, 100), (1, 5000), (40, 100), (40, 5000)])
+def test_bound_on_the_length_only_splits(new, bound):
+    """max_len below and above the sequences' lengths: the same attention."""
+    c = Case([(new, 1300), (1, 40)], 2, 64, 32, BF16, seed=bound)
+    c.step = c.step._replace(max_len=bound)
+    _check_attention(c, 8)
+
+
+@pytest.mark.parametrize("dtype,e4m3", [(BF16, False), (BF16, True), (F32, False), (F16, True)])
+@pytest.mark.parametrize("news", [[64, 1, 1, 30, 1], [1, 1, 1], [200, 90]])
+def test_steps_of_a_layer(news, dtype, e4m3):
+    """Write, then attend, step after step: each row against the attention of
+    the whole text over what the cache holds."""
+    H, KV, hd, page = 8, 2, 64, 32
+    total = sum(news)
+    g = torch.Generator().manual_seed(total)
+    cache = KVCache(1, KV, hd, batch=2, n_pages=2 * -(-total // page), page_size=page, dtype=dtype,
+                    storage=E4M3 if e4m3 else None, device=DEV)
+    cos, sin = (t.to(DEV) for t in _tables(total, hd, dtype))
+    done = 0
+    for n in news:
+        step = cache.step([n, n])
+        qkv = torch.randn(2 * n, (H + 2 * KV) * hd, generator=g).to(dtype).to(DEV)
+        q = ops.kv_cache_write(qkv, cache.layers[0], step, H, cos, sin)
+        o = ops.paged_attention(q, cache.layers[0], step, H, hd**-0.5).double().cpu().view(2, n, H, hd)
+        for b in range(2):
+            k, v = (t.double().cpu() for t in cache.read(0, b))
+            x = q.double().cpu().view(2, n, H, hd)[b]
+            for i in (0, n // 2, n - 1):
+                seen = done + i + 1
+                for h in range(H):
+                    kk, vv = k[:seen, h // 4], v[:seen, h // 4]
+                    p = torch.softmax(kk @ x[i, h] * hd**-0.5, 0)
+                    size = float((kk.abs() @ x[i, h].abs()).max()) * hd**-0.5
+                    u = _u(dtype)
+                    fp32 = (2 * (hd + 4) * size + 8 + seen) * U32
+                    tol = u * (p @ vv).abs() + ((u if dtype != F32 else 0.0) + fp32) * (p @ vv.abs())
+                    assert bool(((o[b, i, h] - p @ vv).abs() <= tol).all()), (n, b, i, h)
+        done += n
+
+
+def test_a_captured_step_follows_its_tables():
+    """One decoded token captured with its lengths on the device: every replay
+    one token further, against eager calls."""
+    H, KV, hd, page = 8, 2, 64, 16
+    caches = [KVCache(1, KV, hd, batch=3, n_pages=60, page_size=page, device=DEV) for _ in range(2)]
+    lens, most = [5, 250, 31], 320
+    g = torch.Generator().manual_seed(2)
+    cos, sin = (t.to(DEV) for t in _tables(most, hd, BF16))
+    first = torch.randn(sum(lens), (H + 2 * KV) * hd, generator=g).to(BF16).to(DEV)
+    filled = [cache.step(lens) for cache in caches]
+    # the captured side: pages for what comes, lengths and the input in place
+    cache = caches[0]
+    table = cache.step([40] * 3).page_table.clone()
+    kv = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    each = CacheStep(torch.arange(4, dtype=torch.int32, device=DEV), kv, table, 3, 1, most)
+    x = torch.zeros(3, (H + 2 * KV) * hd, dtype=BF16, device=DEV)
+    layer = cache.layers[0]
+
+    def once():
+        return ops.paged_attention(ops.kv_cache_write(x, layer, each, H, cos, sin), layer, each, H, 0.125)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        once()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = once()
+    for cache, step in zip(caches, filled):  # after the warm-up, which wrote its last tokens
+        ops.kv_cache_write(first, cache.layers[0], step, H, cos, sin)
+    for turn in range(6):
+        new = torch.randn(3, (H + 2 * KV) * hd, generator=g).to(BF16)
+        x.copy_(new)
+        kv += 1
+        graph.replay()
+        torch.cuda.synchronize()
+        s = caches[1].step([1] * 3)._replace(max_len=most)  # split alike
+        q = ops.kv_cache_write(new.to(DEV), caches[1].layers[0], s, H, cos, sin)
+        assert torch.equal(out, ops.paged_attention(q, caches[1].layers[0], s, H, 0.125)), turn
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("n,length", [(1, 600), (70, 300), (200, 200)])
 def test_paged_attention_large_scores(dtype, n, length):
@@ -385,7 +501,8 @@ def _logits_oracle(x, tokens, lengths, prompts, rep, pres, freq, bias, mask):
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("B,V,T,bias,mask", [(1, 1, 1, "", ""), (1, 32000, 37, "shared", ""), (3, 4097, 300, "rows", "bits"),
                                              (2, 8191, 5000, "", "bools"), (5, 100, 0, "rows", "shared bits"),
-                                             (2, 10007, 64, "shared", "shared bools")])
+                                             (2, 10007, 64, "shared", "shared bools"),
+                                             (64, 70001, 20, "rows", "bits"), (70, 65536, 9, "shared", "bools")])
 def test_process_logits(dtype, B, V, T, bias, mask):
     g = torch.Generator().manual_seed(B * V + T)
     wide = (3 * torch.randn(B, 2, V + 3, generator=g)).to(dtype)
