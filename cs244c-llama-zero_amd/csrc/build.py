@@ -1,8 +1,9 @@
 """Builds libllamazero_hip.so for gfx950 from the .hip sources in this folder.
 
 Each source is compiled to an object under csrc/_build/ (in parallel), then
-linked into ../lzhip/libllamazero_hip.so; pycall.cpp, the Python entry to it,
-becomes ../lzhip/_pycall.so.  Usage:
+linked into ../lzhip/libllamazero_hip.so; pycall.cpp and torchcall.cpp, the
+Python entries to it, become ../lzhip/_pycall.so and ../lzhip/_torchcall.so.
+Usage:
 
     python csrc/build.py [--jobs N] [--arch gfx950]
 """
@@ -21,6 +22,7 @@ HERE = Path(__file__).resolve().parent
 PKG = HERE.parent
 OUT_LIB = PKG / "lzhip" / "libllamazero_hip.so"
 OUT_CALL = PKG / "lzhip" / "_pycall.so"  # the Python entry to it (pycall.cpp)
+OUT_TORCH = PKG / "lzhip" / "_torchcall.so"  # tensor-level entries to it (torchcall.cpp)
 
 SOURCES = [
     "runtime.hip",
@@ -91,6 +93,7 @@ def build(arch: str = "gfx950", jobs: int | None = None, verbose: bool = False) 
     objs = []
     failures = []
     with cf.ThreadPoolExecutor(max_workers=jobs) as pool:
+        entries = [pool.submit(build_torchcall), pool.submit(build_pycall)]
         futs = [pool.submit(_compile, hipcc, arch, HERE / s, build_dir / (Path(s).stem + ".o")) for s in SOURCES]
         for fut in futs:
             obj, rc, msgs = fut.result()
@@ -100,6 +103,8 @@ def build(arch: str = "gfx950", jobs: int | None = None, verbose: bool = False) 
                 if msgs.strip() and verbose:
                     print(msgs)
                 objs.append(obj)
+    for entry in entries:
+        entry.result()
     if failures:
         raise RuntimeError("HIP compilation failed:\n" + "\n".join(failures))
     tmp = OUT_LIB.with_suffix(".so.tmp")
@@ -108,23 +113,38 @@ def build(arch: str = "gfx950", jobs: int | None = None, verbose: bool = False) 
     if proc.returncode != 0:
         raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
     os.replace(tmp, OUT_LIB)
-    build_pycall()
     return OUT_LIB
 
 
-def build_pycall() -> Path:
-    """The CPython extension that calls the library (host code only)."""
+def _extension(source: str, out: Path, *flags: str) -> Path:
+    """A CPython extension (host code only)."""
     cxx = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
     if cxx is None:
-        raise RuntimeError("no C++ compiler (g++) for pycall.cpp")
-    tmp = OUT_CALL.with_suffix(".so.tmp")
+        raise RuntimeError(f"no C++ compiler (g++) for {source}")
+    tmp = out.with_suffix(".so.tmp")
     cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-I",
-           sysconfig.get_paths()["include"], str(HERE / "pycall.cpp"), "-o", str(tmp)]
+           sysconfig.get_paths()["include"], str(HERE / source), "-o", str(tmp), *flags]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
-        raise RuntimeError(f"pycall.cpp failed:\n{proc.stdout}\n{proc.stderr}")
-    os.replace(tmp, OUT_CALL)
-    return OUT_CALL
+        raise RuntimeError(f"{source} failed:\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, out)
+    return out
+
+
+def build_pycall() -> Path:
+    """The extension that calls the library."""
+    return _extension("pycall.cpp", OUT_CALL)
+
+
+def build_torchcall() -> Path:
+    """The extension that calls the library on torch tensors."""
+    import torch
+    from torch.utils import cpp_extension
+
+    lib = Path(torch.__file__).resolve().parent / "lib"
+    return _extension("torchcall.cpp", OUT_TORCH, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                      *(f"-isystem{p}" for p in cpp_extension.include_paths()), f"-L{lib}", "-ltorch_python", "-ltorch_cpu",
+                      "-lc10")
 
 
 def main() -> None:

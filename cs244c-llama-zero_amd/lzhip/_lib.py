@@ -1,5 +1,6 @@
 """Binding of libllamazero_hip.so (declared in include/llamazero_hip.h): loaded
-with ctypes, its entry points called through _pycall.
+with ctypes, its entry points called through _pycall, generation's through
+_torchcall.
 
 The library is loaded after torch so that the process keeps a single HIP
 runtime (torch ships its own libamdhip64.so.7, which the dynamic loader then
@@ -166,6 +167,7 @@ SIGNATURES = {
 _lock = threading.Lock()
 _lib = None
 _calls = {}  # entry point name -> its _pycall callable, filled when the library is loaded
+torchcall = None  # the _torchcall extension, bound when the library is loaded
 
 
 class HipLibraryError(RuntimeError):
@@ -174,7 +176,7 @@ class HipLibraryError(RuntimeError):
 
 def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
     """Loads (once) and returns the library with its signatures applied."""
-    global _lib
+    global _lib, torchcall
     if _lib is not None:  # set once, complete, under the lock
         return _lib
     with _lock:
@@ -188,8 +190,9 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
             )
         try:
             from . import _pycall as pycall
+            from . import _torchcall
         except ImportError as e:
-            raise HipLibraryError(f"lzhip/_pycall.so is missing ({e}): build it with "
+            raise HipLibraryError(f"lzhip/_pycall.so or lzhip/_torchcall.so is missing ({e}): build them with "
                                   "`python cs244c-llama-zero_amd/csrc/build.py`") from e
         lib = ctypes.CDLL(str(p), mode=ctypes.RTLD_GLOBAL)
         for name, (res, args) in SIGNATURES.items():
@@ -198,6 +201,10 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
             fn.argtypes = args
             if res is not ctypes.c_char_p:
                 _calls[name] = pycall.bind(name, ctypes.cast(fn, _vp).value)
+        _torchcall.bind({name: ctypes.cast(getattr(lib, name), _vp).value for name in SIGNATURES},
+                        getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None),
+                        getattr(torch._C, "_cuda_setDevice", None), HipLibraryError)
+        torchcall = _torchcall
         _lib = lib
         return lib
 
@@ -226,3 +233,10 @@ def query(name: str, *args) -> int:
     if _lib is None:
         load()
     return _calls[name](*args)
+
+
+def tensor_calls():
+    """The _torchcall extension (its functions take tensors)."""
+    if torchcall is None:
+        load()
+    return torchcall

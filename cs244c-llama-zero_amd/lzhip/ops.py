@@ -1207,107 +1207,8 @@ def attn_bwd(q2, k2, v2, o2, do2, lse, B, S, H, KV, hd, scale, dq2, dk2, dv2, qt
 # generation from a paged key/value cache (see lzhip/cache.py)
 # ---------------------------------------------------------------------------
 
-_current_device = getattr(torch._C, "_cuda_getDevice", None)  # without the lazy initialisation that a GPU tensor has behind it
-
-
-def _call_on(index: int, name: str, *args) -> None:
-    """_lib.call with device `index` current (a kernel goes to the current
-    device, whatever its stream belongs to)."""
-    if index == _current_device():
-        _lib.call(name, *args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            _lib.call(name, *args, _raw_stream(index))
-
-
-# The checks of a decoded token's calls cost as much as its kernels: each looks
-# at everything in one expression and leaves it to a second function to say
-# what was wrong.
-
-def _int32_table(t: torch.Tensor, name: str, index: int, dim: int = 1) -> None:
-    if t.dtype is not torch.int32 or t.dim() != dim or not t.is_contiguous() or t.get_device() != index:
-        require_gpu(t)
-        raise ValueError(f"{name} must be a contiguous int32 tensor of {dim} dimension(s) on cuda:{index}, got {t.dtype} "
-                         f"{tuple(t.shape)} on {t.device}")
-
-
-def _refuse_cache(layer, dtype: torch.dtype, index: int) -> None:
-    k, v, k_exp, v_exp = layer
-    require_gpu(k, v, k_exp, v_exp)
-    if any(t is not None and t.get_device() != index for t in layer):
-        raise ValueError(f"the cache and the rows (on cuda:{index}) must be on one device")
-    if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or not (k.is_contiguous() and v.is_contiguous()):
-        raise ValueError(f"cache pages must be two contiguous [pages, KV heads, page size, head dim] tensors of one "
-                         f"dtype, got {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
-    if k.dtype == torch.float8_e4m3fn:
-        raise ValueError("a float8_e4m3fn cache needs contiguous int8 exponents [pages, KV heads, page size] beside it")
-    raise TypeError(f"a cache of {k.dtype} {'with' if k_exp is not None else 'without'} exponents does not hold {dtype} "
-                    "rows")
-
-
-def _cache_args(layer, dtype: torch.dtype, index: int) -> Tuple[tuple, int, int]:
-    """(pointer and shape arguments of a LayerCache, KV heads, head dim)."""
-    k, v, k_exp, v_exp = layer
-    shape, stored = k.shape, k.dtype
-    if (len(shape) != 4 or v.shape != shape or v.dtype is not stored or not k.is_contiguous() or not v.is_contiguous()
-            or k.get_device() != index or v.get_device() != index):
-        _refuse_cache(layer, dtype, index)
-    if stored is dtype and k_exp is None and v_exp is None:
-        return (k.data_ptr(), v.data_ptr(), None, None, _DTYPES[dtype], shape[0], shape[2]), shape[1], shape[3]
-    if stored is not torch.float8_e4m3fn or any(
-            e is None or e.dtype is not torch.int8 or e.shape != shape[:3] or not e.is_contiguous()
-            or e.get_device() != index for e in (k_exp, v_exp)):
-        _refuse_cache(layer, dtype, index)
-    return ((k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), _lib.E4M3, shape[0], shape[2]), shape[1],
-            shape[3])
-
-
-def _step_rows(step, index: int) -> Tuple[int, int]:
-    """(sequences, pages of a row of the table) of a CacheStep."""
-    row_start, kv_len, table = step[:3]
-    _int32_table(row_start, "row_start", index)
-    _int32_table(kv_len, "kv_len", index)
-    _int32_table(table, "page_table", index, 2)
-    (B,), (rows, width) = kv_len.shape, table.shape
-    if rows != B or B == 0 or width == 0 or row_start.numel() != B + 1:
-        raise ValueError(f"a step of {B} sequences needs {B + 1} row starts and a page table of {B} rows, got "
-                         f"{row_start.numel()} and {(rows, width)}")
-    return B, width
-
-
-def _aligned_rows(t: torch.Tensor, name: str, cols: int) -> Tuple[torch.Tensor, int]:
-    """t as 2-D rows of `cols` whose starts are 16-byte aligned (a copy if they
-    are not), and their stride."""
-    esz = t.element_size()
-    if t.dim() == 2 and t.size(1) == cols and t.is_contiguous():
-        ld = cols
-    else:
-        if t.dim() != 2 or t.size(1) != cols or (t.stride(1) != 1 and cols > 1):
-            raise ValueError(f"{name} must be rows of {cols} adjacent values, got {tuple(t.shape)} with strides "
-                             f"{t.stride()}")
-        if t.size(0) > 1 and t.stride(0) < cols:
-            raise ValueError(f"{name}: rows overlap (stride {t.stride(0)})")
-        ld = _row_stride(t)
-    if t.data_ptr() % 16 or ld * esz % 16:
-        return copy2d(t, torch.empty(t.shape, dtype=t.dtype, device=t.device)), cols
-    return t, ld
-
-
-def _row_output(out: Optional[torch.Tensor], rows: int, cols: int, like: torch.Tensor, used: int
-                ) -> Tuple[torch.Tensor, int]:
-    """The output rows and their stride: the caller's, whose rows of no
-    sequence are left as they are, or new ones, where those are zeros."""
-    if out is None:
-        if used == rows:
-            return like.new_empty((rows, cols)), cols
-        return zeros((rows, cols), like.dtype, like.device), cols
-    if out.dtype != like.dtype or tuple(out.shape) != (rows, cols) or out.get_device() != like.get_device() \
-            or out.stride(1) != 1 or (rows > 1 and out.stride(0) < cols) or out.data_ptr() % 16 \
-            or _row_stride(out) * out.element_size() % 16:
-        require_gpu(out)
-        raise ValueError(f"out must be {like.dtype} rows [{rows}, {cols}] on {like.device}, 16-byte aligned")
-    return out, _row_stride(out)
-
+# Arguments are checked, outputs allocated and the C ABI called in
+# csrc/torchcall.cpp, on the device and the current stream of the first tensor.
 
 def kv_cache_write(qkv: torch.Tensor, layer, step, n_heads: int, cos: torch.Tensor, sin: torch.Tensor,
                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -1316,28 +1217,10 @@ def kv_cache_write(qkv: torch.Tensor, layer, step, n_heads: int, cos: torch.Tens
 
     qkv: [rows, (n_heads + 2 * KV) * hd], the fused projection before RoPE;
     layer: LayerCache, layer.k of qkv's dtype or float8_e4m3fn; step:
-    CacheStep; cos/sin: RoPE tables [>= step.max_len, hd] in qkv's dtype.
-    Rotation, rounding and 8-bit storage: lz_kv_write."""
-    if not qkv.is_cuda:
-        require_gpu(qkv)
-    index, dtype = qkv.get_device(), qkv.dtype
-    code = dtype_code(qkv)
-    cache, KV, hd = _cache_args(layer, dtype, index)
-    B, width = _step_rows(step, index)
-    rows = qkv.size(0)
-    qkv, ld = _aligned_rows(qkv, "qkv", (n_heads + 2 * KV) * hd)
-    positions = cos.size(0)
-    if (cos.dtype is not dtype or sin.dtype is not dtype or cos.shape != (positions, hd) or sin.shape != cos.shape
-            or not cos.is_contiguous() or not sin.is_contiguous() or cos.get_device() != index
-            or sin.get_device() != index or cos.data_ptr() % 16 or sin.data_ptr() % 16 or positions < step.max_len):
-        require_gpu(cos, sin)
-        raise ValueError(f"RoPE tables must be contiguous {dtype} [{step.max_len} or more, {hd}] on cuda:{index}, got "
-                         f"{cos.dtype} {tuple(cos.shape)} and {sin.dtype} {tuple(sin.shape)}")
-    q, ldq = _row_output(out, rows, n_heads * hd, qkv, step.rows)
-    _call_on(index, "lz_kv_write", qkv.data_ptr(), ld, code, rows, cos.data_ptr(), sin.data_ptr(), positions,
-             q.data_ptr(), ldq, *cache, step.page_table.data_ptr(), width, step.row_start.data_ptr(),
-             step.kv_len.data_ptr(), B, n_heads, KV, hd)
-    return q
+    CacheStep; cos/sin: RoPE tables [>= step.max_len, hd] in qkv's dtype; out:
+    rows for the queries (those of no sequence are left as they are; new ones
+    are zeros there).  Rotation, rounding and 8-bit storage: lz_kv_write."""
+    return _lib.tensor_calls().kv_cache_write(qkv, layer, step, n_heads, cos, sin, out)
 
 
 def kv_cache_read(layer, page_table: torch.Tensor, start: torch.Tensor, rows: int, dtype: torch.dtype
@@ -1347,21 +1230,7 @@ def kv_cache_read(layer, page_table: torch.Tensor, start: torch.Tensor, rows: in
     the first positions of sequence b (start: int32 [B + 1]; rows =
     start[B]).  A float8_e4m3fn cache is read back in any dtype, others in
     their own."""
-    if not page_table.is_cuda:
-        require_gpu(page_table)
-    index = page_table.get_device()
-    if dtype not in _DTYPES:
-        raise TypeError(f"a cache is read back in float32, bfloat16 or float16, not in {dtype}")
-    cache, KV, hd = _cache_args(layer, dtype, index)
-    _int32_table(page_table, "page_table", index, 2)
-    _int32_table(start, "start", index)
-    B, width = page_table.shape
-    if start.numel() != B + 1 or B == 0 or width == 0 or rows < 0:
-        raise ValueError(f"{B} sequences need {B + 1} starts, got {start.numel()}")
-    k, v = (torch.empty((rows, KV * hd), dtype=dtype, device=page_table.device) for _ in range(2))
-    _call_on(index, "lz_kv_read", *cache, page_table.data_ptr(), width, start.data_ptr(), B, KV, hd, k.data_ptr(),
-             v.data_ptr(), _DTYPES[dtype], rows)
-    return k, v
+    return _lib.tensor_calls().kv_cache_read(layer, page_table, start, rows, dtype)
 
 
 def paged_attention(q: torch.Tensor, layer, step, n_heads: int, scale: float,
@@ -1369,48 +1238,9 @@ def paged_attention(q: torch.Tensor, layer, step, n_heads: int, scale: float,
     """Attention of a step's rotated queries [rows, n_heads * hd] over the
     cached keys and values of their sequences (a step's own tokens included:
     kv_cache_write comes first); causal within the new tokens.  A row that
-    sees nothing is zero."""
-    if not q.is_cuda:
-        require_gpu(q)
-    index = q.get_device()
-    code = dtype_code(q)
-    cache, KV, hd = _cache_args(layer, q.dtype, index)
-    B, width = _step_rows(step, index)
-    rows = q.size(0)
-    if n_heads <= 0 or n_heads % KV:
-        raise ValueError(f"{n_heads} query heads do not divide over {KV} key/value heads")
-    q, ld = _aligned_rows(q, "q", n_heads * hd)
-    o, ldo = _row_output(out, rows, n_heads * hd, q, step.rows)
-    ws_bytes = _lib.query("lz_paged_attn_workspace", code, cache[4], rows, B, n_heads, KV, hd, step.max_new,
-                          step.max_len)
-    ws = q.new_empty((ws_bytes + 3) // 4, dtype=torch.float32) if ws_bytes else None
-    _call_on(index, "lz_paged_attn", q.data_ptr(), ld, code, rows, *cache, step.page_table.data_ptr(), width,
-             step.row_start.data_ptr(), step.kv_len.data_ptr(), B, n_heads, KV, hd, step.max_new, step.max_len,
-             scale, o.data_ptr(), ldo, _ptr(ws), ws_bytes)
-    return o
-
-
-def _per_row(value, name: str, B: int, index: int) -> Tuple[Optional[int], float]:
-    """A penalty as (address of one fp32 value a row, unused) or (None, one
-    for all)."""
-    if not isinstance(value, torch.Tensor):
-        value = float(value)
-        if not math.isfinite(value) or (name == "repetition_penalty" and value <= 0.0):
-            raise ValueError(f"{name} must be finite{' and positive' if name == 'repetition_penalty' else ''}, got {value}")
-        return None, value
-    if value.dtype is not torch.float32 or value.shape != (B,) or not value.is_contiguous() or value.get_device() != index:
-        require_gpu(value)
-        raise ValueError(f"{name} must be a number or a contiguous float32 [{B}] tensor on cuda:{index}")
-    return value.data_ptr(), 0.0
-
-
-def _row_lengths(t: Optional[torch.Tensor], name: str, B: int, index: int) -> Optional[torch.Tensor]:
-    if t is None:
-        return None
-    if t.dtype not in (torch.int32, torch.int64) or t.shape != (B,) or t.get_device() != index:
-        require_gpu(t)
-        raise ValueError(f"{name} must be an int32 or int64 [{B}] tensor on cuda:{index}")
-    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    sees nothing is zero.  out: rows for the result (those of no sequence are
+    left as they are; new ones are zeros there)."""
+    return _lib.tensor_calls().paged_attention(q, layer, step, n_heads, scale, out)
 
 
 def process_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = None,
@@ -1428,47 +1258,5 @@ def process_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = Non
     words of 32 tokens, [ceil(V / 32)] or [B, ceil(V / 32)], lowest bit
     first).  The penalties are numbers or float32 [B] tensors.  Ids outside
     the vocabulary (padding) count for nothing."""
-    if not logits.is_cuda:
-        require_gpu(logits)
-    index = logits.get_device()
-    code = dtype_code(logits)
-    if logits.dim() != 2:
-        raise ValueError(f"logits must be [B, V], got {tuple(logits.shape)}")
-    B, V = logits.shape
-    ld, inner = logits.stride()
-    if (V > 1 and inner != 1) or (B > 1 and ld < V):
-        raise ValueError(f"logits rows must be adjacent values, got strides {logits.stride()}")
-    n = ldt = 0
-    if tokens is not None:
-        if tokens.dtype is not torch.int64 or tokens.dim() != 2 or tokens.size(0) != B or tokens.get_device() != index or (
-                tokens.size(1) > 1 and tokens.stride(1) != 1):
-            require_gpu(tokens)
-            raise ValueError(f"tokens must be int64 [{B}, T] rows on cuda:{index}")
-        n, ldt = tokens.size(1), tokens.stride(0)
-    elif lengths is not None or prompt_lengths is not None:
-        raise ValueError("lengths and prompt_lengths say which tokens count: there are none")
-    lengths = _row_lengths(lengths, "lengths", B, index)
-    prompts = _row_lengths(prompt_lengths, "prompt_lengths", B, index)
-    rep, rep_s = _per_row(repetition_penalty, "repetition_penalty", B, index)
-    pres, pres_s = _per_row(presence_penalty, "presence_penalty", B, index)
-    freq, freq_s = _per_row(frequency_penalty, "frequency_penalty", B, index)
-    ldb = ldm = kind = 0
-    if bias is not None:
-        if bias.dtype is not torch.float32 or bias.get_device() != index or tuple(bias.shape) not in ((V,), (B, V)) or (
-                V > 1 and bias.stride(-1) != 1):
-            require_gpu(bias)
-            raise ValueError(f"bias must be float32 [{V}] or [{B}, {V}] on cuda:{index}")
-        ldb = bias.stride(0) if bias.dim() == 2 else 0
-    if mask is not None:
-        kind = 1 if mask.dtype is torch.bool else 2 if mask.dtype is torch.int32 else 0
-        cols = V if kind == 1 else (V + 31) // 32
-        if not kind or mask.get_device() != index or tuple(mask.shape) not in ((cols,), (B, cols)) or (
-                cols > 1 and mask.stride(-1) != 1):
-            require_gpu(mask)
-            raise ValueError(f"mask must be bool [{V}] or [{B}, {V}], or int32 words of {(V + 31) // 32}, on cuda:{index}")
-        ldm = mask.stride(0) if mask.dim() == 2 else 0
-    out = torch.empty((B, V), dtype=torch.float32, device=logits.device)
-    _call_on(index, "lz_process_logits", logits.data_ptr(), ld if B > 1 else V, code, B, V, _ptr(tokens), ldt, n,
-             _ptr(lengths), _ptr(prompts), rep, rep_s, pres, pres_s, freq, freq_s, _ptr(bias), ldb, _ptr(mask), kind,
-             ldm, out.data_ptr(), V)
-    return out
+    return _lib.tensor_calls().process_logits(logits, tokens, lengths, prompt_lengths, repetition_penalty,
+                                              presence_penalty, frequency_penalty, bias, mask)
