@@ -72,6 +72,13 @@ struct PagedRows {
   }
 };
 
+// A row's reference m for its weights 2^(s - m) (log2 units) is its running
+// maximum, but moves only when that is more than kSlack above it: weights up to
+// 2^8 are as exact in 16 and 32 bits as those up to 1, and the sums are
+// multiplied down once or twice in a pass and not at every new maximum (chunks
+// FIXME).
+constexpr float kSlack = 8.f;
+
 // Two e4m3 values of a word, times 2^e (exact in bf16, and in fp16 for what
 // lz_kv_write stores of fp16 rows), as two values of the 16-bit format F.
 template <typename F, bool kHi>

@@ -326,9 +326,10 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, s[n][t][i]);
       top = max_of_row(top) * unit;
-      if (__ballot(top > mx[n])) {
-        const float m_new = fmaxf(mx[n], top);
-        const float alpha = m_new == mx[n] ? 1.f : exp_of<T>(mx[n] - m_new);
+      const bool moved = top > mx[n] + (sizeof(T) == 4 ? 0.f : kSlack);
+      if (__ballot(moved)) {
+        const float m_new = moved ? top : mx[n];
+        const float alpha = moved ? exp_of<T>(mx[n] - m_new) : 1.f;
         mx[n] = m_new;
         sum[n] *= alpha;
 #pragma unroll

@@ -176,9 +176,10 @@ __device__ __forceinline__ void step_softmax(f32x16_t (&s)[2], f32x16_t (&o)[HD 
       mx = fmaxf(mx, s[t][r]);
     }
   mx = max_halves(mx) * unit;
-  if (__ballot(mx > m)) {  // some row's maximum moved
-    const float m_new = fmaxf(m, mx);
-    const float alpha = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+  const bool moved = mx > m + kSlack;
+  if (__ballot(moved)) {
+    const float m_new = moved ? mx : m;
+    const float alpha = moved ? __builtin_amdgcn_exp2f(m - m_new) : 1.f;
     l *= alpha;
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i)
