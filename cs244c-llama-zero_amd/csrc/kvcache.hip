@@ -196,9 +196,8 @@ __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
   const int g = rem / kLanes, i = (rem - g * kLanes) * N;
   int base = 0;
   const int b = seqs.find(a.start, nullptr, a.B, a.rows, row, base);
-  if (b < 0) return;
   const int pos = base + row;
-  const int page = a.pg.page_of(b, pos);
+  const int page = b < 0 ? -1 : a.pg.page_of(b, pos);
   const int64_t token = (((int64_t)page * a.KV + g) << a.pg.log_size) + (pos & ((1 << a.pg.log_size) - 1));
   const int64_t out = ((int64_t)row * a.KV + g) * HD + i;
 #pragma unroll

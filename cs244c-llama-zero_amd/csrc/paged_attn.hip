@@ -18,6 +18,7 @@
 // 8 x (HD / 16) block in registers (v_perm).
 #include <algorithm>
 #include <cmath>
+#include <limits>
 
 #include "paged_attn.h"
 
@@ -599,7 +600,8 @@ LZ_EXPORT int lz_paged_attn(const void* q, int64_t ldq, int dtype, int64_t rows,
   LZ_REQUIRE(H > 0 && H % KV == 0 && H <= 65536 && rows >= 0 && rows * H <= INT32_MAX / 64 && max_new >= 0 &&
                  max_len >= 0 && max_len <= INT32_MAX - 1024,
              "lz_paged_attn: bad shape");
-  LZ_REQUIRE(scale >= 0.f && scale < INFINITY, "lz_paged_attn: scale %g", (double)scale);
+  // (-inf, a masked score, times 0 or a subnormal that is flushed would be NaN)
+  LZ_REQUIRE(scale >= std::numeric_limits<float>::min() && scale * kLog2e < INFINITY, "lz_paged_attn: scale %g", (double)scale);
   LZ_REQUIRE(ldq >= H * hd && ldo >= H * hd, "lz_paged_attn: row strides shorter than the rows");
   LZ_REQUIRE(rows == 0 || (q && o && row_start && kv_len && lz_aligned16(q) && lz_aligned16(o) && ldq * esz % 16 == 0 &&
                            ldo * esz % 16 == 0),

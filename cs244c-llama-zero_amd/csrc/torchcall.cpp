@@ -210,7 +210,8 @@ struct Step {
   const at::Tensor *start, *len, *table;
   int64_t rows, max_new, max_len, B, width;
 
-  Step(PyObject* step, const Place& at) {
+  // x: the call's rows, of which there may be more than the step has
+  Step(PyObject* step, const at::Tensor& x, const Place& at) {
     start = &tensor(item(step, 0, 6, "CacheStep"), "row_start");
     len = &tensor(item(step, 1, 6, "CacheStep"), "kv_len");
     table = &tensor(item(step, 2, 6, "CacheStep"), "page_table");
@@ -226,6 +227,11 @@ struct Step {
       refuse(PyExc_ValueError, "a step of %lld sequences needs %lld row starts and a page table of %lld rows, got %lld and "
                                "%s", (long long)B, (long long)B + 1, (long long)B, (long long)start->size(0),
              shape(*table).c_str());
+    const int64_t n = x.dim() == 2 ? x.size(0) : INT64_MAX;  // other shapes are refused as rows
+    if (rows < 0 || rows > n || max_new < 0 || max_len < 0 || (max_new < rows && B * max_new < rows))
+      refuse(PyExc_ValueError, "a step of %lld rows, at most %lld of each of %lld sequences and %lld cached, does not fit "
+                               "rows %s", (long long)rows, (long long)max_new, (long long)B, (long long)max_len,
+             shape(x).c_str());
   }
 };
 
@@ -298,7 +304,7 @@ PyObject* kv_cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Place at(x);
     const int code = code_of(x);
     const Cache c(a[1], x.scalar_type(), at);
-    const Step s(a[2], at);
+    const Step s(a[2], x, at);
     const int64_t H = integer(a[3]);
     const at::Tensor &cos = tensor(a[4], "cos"), &sin = tensor(a[5], "sin");
     const Rows qkv(x, "qkv", (H + 2 * c.KV) * c.hd, code, at);
@@ -354,7 +360,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Place at(x);
     const int code = code_of(x);
     const Cache c(a[1], x.scalar_type(), at);
-    const Step s(a[2], at);
+    const Step s(a[2], x, at);
     const int64_t H = integer(a[3]);
     const double scale = PyFloat_AsDouble(a[4]);
     if (scale == -1.0 && PyErr_Occurred()) throw Refused{};
@@ -392,9 +398,9 @@ struct Penalty {
     }
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) throw Refused{};
-    if (!std::isfinite(v) || (positive && v <= 0.0))
-      refuse(PyExc_ValueError, "%s must be finite%s, got %R", name, positive ? " and positive" : "", o);
     all = (float)v;
+    if (!std::isfinite(all) || (positive && all <= 0.f))
+      refuse(PyExc_ValueError, "%s must be finite%s in float32, got %R", name, positive ? " and positive" : "", o);
   }
 };
 

@@ -18,7 +18,10 @@ from . import ops
 class LayerCache(NamedTuple):
     """One layer's pages, [pages, KV heads, page size, head dim] each, in the
     model's dtype, or float8_e4m3fn with int8 exponents [pages, KV heads, page
-    size]: the value is the stored number times 2^exponent."""
+    size]: the value is the stored number times 2^exponent (-126 to 127).
+    8-bit pages are read in the dtype that they were written with: float16
+    keeps smaller exponents than the others.  Where two rows of one step are
+    given the same slot, either is kept."""
 
     k: torch.Tensor
     v: torch.Tensor
@@ -29,9 +32,12 @@ class LayerCache(NamedTuple):
 class CacheStep(NamedTuple):
     """The new tokens of one pass through the layers.  Device tensors, int32:
     row_start [B + 1] (sequence b's new tokens are rows row_start[b] ..
-    row_start[b + 1] - 1), kv_len [B] (its length with them), page_table
-    [B, pages of the longest].  Host numbers: rows = row_start[B], and upper
-    bounds max_new and max_len of the new and of all tokens of a sequence."""
+    row_start[b + 1] - 1, from row_start[0] = 0 on), kv_len [B] (its length with
+    them), page_table [B, pages of the longest].  Host numbers: rows =
+    row_start[B], and upper bounds max_new and max_len of the new and of all
+    tokens of a sequence.  Tables that change under a captured call keep within
+    them: rows behind max_new of a sequence, or of none, are not computed (what
+    they hold is left, in a tensor of the call's own undefined)."""
 
     row_start: torch.Tensor
     kv_len: torch.Tensor

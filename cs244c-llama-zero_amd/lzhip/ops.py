@@ -1228,7 +1228,8 @@ def kv_cache_read(layer, page_table: torch.Tensor, start: torch.Tensor, rows: in
     """(k, v), each [rows, KV * hd] of dtype: the cached keys and values of
     page_table's sequences one after another, rows start[b] .. start[b + 1] - 1
     the first positions of sequence b (start: int32 [B + 1]; rows =
-    start[B]).  A float8_e4m3fn cache is read back in any dtype, others in
+    start[B], what lies behind it is zeros).  A float8_e4m3fn cache is read
+    back in any dtype that holds its numbers (float16: up to 65504), others in
     their own."""
     return _lib.tensor_calls().kv_cache_read(layer, page_table, start, rows, dtype)
 
@@ -1237,9 +1238,9 @@ def paged_attention(q: torch.Tensor, layer, step, n_heads: int, scale: float,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of a step's rotated queries [rows, n_heads * hd] over the
     cached keys and values of their sequences (a step's own tokens included:
-    kv_cache_write comes first); causal within the new tokens.  A row that
-    sees nothing is zero.  out: rows for the result (those of no sequence are
-    left as they are; new ones are zeros there)."""
+    kv_cache_write comes first); causal within the new tokens; scale > 0.  A
+    row that sees nothing is zero.  out: rows for the result (those of no sequence are
+    left as they are; new ones are zeros there); it may be q itself."""
     return _lib.tensor_calls().paged_attention(q, layer, step, n_heads, scale, out)
 
 
@@ -1256,7 +1257,8 @@ def process_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = Non
     (if there are any) are subtracted; bias ([V] or [B, V] float32) is added;
     what mask forbids becomes -inf (bool [V] or [B, V], True allows, or int32
     words of 32 tokens, [ceil(V / 32)] or [B, ceil(V / 32)], lowest bit
-    first).  The penalties are numbers or float32 [B] tensors.  Ids outside
+    first).  The penalties are numbers or float32 [B] tensors (finite, the
+    repetition penalty positive; tensors are not checked).  Ids outside
     the vocabulary (padding) count for nothing."""
     return _lib.tensor_calls().process_logits(logits, tokens, lengths, prompt_lengths, repetition_penalty,
                                               presence_penalty, frequency_penalty, bias, mask)

@@ -186,6 +186,7 @@ class GroupedQueryAttention(nn.Module):
         )
         return self.o_proj(y, residual)
 
+    @torch.no_grad()
     def forward_cached(self, x: torch.Tensor, layer: LayerCache, step: CacheStep,
                        residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         """forward() for a step's new tokens [rows, dim], whose keys and values
@@ -237,10 +238,16 @@ class TransformerBlock(nn.Module):
         # recompute) its value is not formed
         return self.mlp(h, residual=x, compute_output=not LF.output_is_unused())
 
+    @torch.no_grad()
     def forward_cached(self, x: torch.Tensor, layer: LayerCache, step: CacheStep) -> torch.Tensor:
-        """forward() for a step's new tokens [rows, dim] over a cache."""
+        """forward() for a step's new tokens [rows, dim] over a cache (no
+        gradients, no dropout)."""
         x = self.attn.forward_cached(self.input_norm(x), layer, step, residual=x)
-        return self.mlp(self.post_attn_norm(x), residual=x)
+        training, self.mlp.training = self.mlp.training, False
+        try:
+            return self.mlp(self.post_attn_norm(x), residual=x)
+        finally:
+            self.mlp.training = training
 
 
 @dataclass
@@ -389,23 +396,22 @@ class LlamaForCausalLM(nn.Module):
     def forward_cached(self, ids: torch.Tensor, cache: KVCache, step: CacheStep) -> torch.Tensor:
         """Logits [B, V] of each sequence's last new token.  ids: the step's
         new tokens, sequence after sequence ([rows] int64); step: what
-        cache.step(counts) returned for them.  As in eval mode, without
-        dropout.  The row of a sequence that has no new tokens says nothing."""
+        cache.step(counts) returned for them.  Without dropout, whatever the
+        mode.  The row of a sequence that has no new tokens says nothing."""
         if self._zero3_executor is not None:
             raise RuntimeError("a ZeRO-3 sharded model has no cached forward: gather its parameters first "
                                "(summon_full_params) or generate without use_cache")
         if ids.dim() != 1 or ids.numel() != step.rows:
             raise ValueError(f"ids should hold the step's {step.rows} tokens, got shape {tuple(ids.shape)}")
-        training = self.training
-        self.eval()
-        try:
-            x = self.tok_embeddings(ids)
-            for layer, block in zip(cache.layers, self.layers):
-                x = block.forward_cached(x, layer, step)
-            last = ops.embedding_fwd((step.row_start[1:] - 1).long(), x)  # rows of x
-            return self.lm_head(self.norm(last))
-        finally:
-            self.train(training)
+        if step.rows == 0:
+            raise ValueError("a step without new tokens has no logits")
+        if len(cache.layers) != len(self.layers):
+            raise ValueError(f"a cache of {len(cache.layers)} layers for a model of {len(self.layers)}")
+        x = self.tok_embeddings(ids)
+        for layer, block in zip(cache.layers, self.layers):
+            x = block.forward_cached(x, layer, step)
+        last = ops.embedding_fwd((step.row_start[1:] - 1).long(), x)  # rows of x
+        return self.lm_head(self.norm(last))
 
     @torch.no_grad()
     def generate(
@@ -436,7 +442,9 @@ class LlamaForCausalLM(nn.Module):
         penalties, logit_bias and token_mask (a mask, or a function that makes
         one of the [B, t] tokens so far) adjust the logits first, as
         ops.process_logits says, the prompt counting for repetition_penalty
-        alone."""
+        alone; where they leave a row no token, that is a ValueError."""
+        if cache_dtype is not None and not use_cache:
+            raise ValueError("cache_dtype is for use_cache=True")
         self.eval()
         bsz, t0 = input_ids.shape
         seq = input_ids.new_empty((bsz, t0 + max_new_tokens))
@@ -462,5 +470,8 @@ class LlamaForCausalLM(nn.Module):
                     last, tokens=seq[:, :t], prompt_lengths=prompts, repetition_penalty=repetition_penalty,
                     presence_penalty=presence_penalty, frequency_penalty=frequency_penalty, bias=logit_bias,
                     mask=token_mask(seq[:, :t]) if callable(token_mask) else token_mask)
+                if not bool(torch.isfinite(last.amax(-1)).all()):  # sampling from such a row would end the process
+                    raise ValueError(f"token {t}: the largest logit of a row is not finite (does token_mask or "
+                                     "logit_bias allow it no token?)")
             seq[:, t] = _next_token(last.float(), temperature, top_k)
         return seq

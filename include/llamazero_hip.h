@@ -416,7 +416,7 @@ int lz_kv_write(const void* qkv, int64_t ld, int dtype, int64_t rows, const void
 
 /* The cached keys and values of B sequences as rows [rows][KV * hd] of dtype:
  * rows start[b] .. start[b+1]-1 are positions 0, 1, ... of sequence b.
- * Positions without a page come out as zeros. */
+ * Positions without a page and rows of no sequence come out as zeros. */
 int lz_kv_read(const void* k, const void* v, const void* k_exp, const void* v_exp, int cache_dtype, int64_t pages,
                int64_t page_size, const int32_t* table, int64_t width, const int32_t* start, int64_t B, int64_t KV,
                int64_t hd, void* k_out, void* v_out, int dtype, int64_t rows, void* stream);
@@ -426,7 +426,8 @@ int lz_kv_read(const void* k, const void* v, const void* k_exp, const void* v_ex
  * the i-th of `new` rows sees positions 0 .. kv_len - new + i.  A row that
  * sees nothing comes out as zeros.  max_new and max_len: at least the largest
  * number of new tokens and of cached ones (max_new sizes the grid: rows past
- * it would be left; max_len only how the work is split).  workspace:
+ * it would be left; max_len only how the work is split).  scale: positive, a
+ * normal number.  o may be q (rows and stride alike).  workspace:
  * lz_paged_attn_workspace bytes, 16-byte aligned, for the joined parts of
  * long sequences. */
 int64_t lz_paged_attn_workspace(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd,

@@ -52,7 +52,8 @@ PAGES = [dict(hd=48), dict(size=24), dict(size=8), dict(size=2048), dict(cache=0
                                     dict(qkv=20), dict(positions=0), dict(rows=2**31)]),
     ("lz_kv_read", READ, PAGES + [dict(rows=-1), dict(k_out=None), dict(v_out=20)]),
     ("lz_paged_attn", ATTEND, PAGES + [dict(H=3), dict(H=0), dict(ldq=60), dict(ldo=60), dict(q=8), dict(o=None),
-                                       dict(rows=-1), dict(max_new=-1), dict(kv_len=None), dict(scale=-1.0), dict(scale=float("nan"))]),
+                                       dict(rows=-1), dict(max_new=-1), dict(kv_len=None), dict(scale=-1.0), dict(scale=0.0), dict(scale=1e-40),
+                                       dict(scale=3e38), dict(scale=float("nan"))]),
     ("lz_process_logits", LOGITS, [dict(dtype=5), dict(kind=3), dict(kind=1), dict(mask=P), dict(ldo=7), dict(B=2, ld=7),
                                    dict(logits=None), dict(tokens=None), dict(n=-1), dict(V=2**40), dict(B=-1)]),
 ])

@@ -223,6 +223,17 @@ def test_cache_read(dtype, e4m3, out, KV, hd, page):
         assert torch.equal(got.cpu(), want.to(out))
 
 
+def test_cache_read_rows_of_no_sequence():
+    c = Case([(1, 20), (1, 20)], 2, 64, 16, BF16)
+    spare = torch.full((13, 128), 7.0, dtype=BF16, device=DEV)  # what new memory may hold
+    del spare
+    k, v = ops.kv_cache_read(c.layer, c.step.page_table, torch.tensor([2, 6, 9], dtype=torch.int32, device=DEV), 13, BF16)
+    for side, got in ((0, k), (1, v)):
+        want = torch.zeros(13, 2, 64, dtype=torch.float64)
+        want[2:6], want[6:9] = c.tokens(side, 0, 4), c.tokens(side, 1, 3)
+        assert torch.equal(got.cpu().double(), want.view(13, 128))
+
+
 def _check_attention(c, H, scale=None, q=None, **kw):
     scale = c.hd**-0.5 if scale is None else scale
     q = torch.randn(c.rows, H * c.hd, generator=c.g).to(c.dtype) if q is None else q
@@ -629,6 +640,17 @@ def test_unaligned_rows():
     assert torch.equal(a, ops.kv_cache_write(wide[:, 1:257].contiguous(), c.layer, c.step, 4, cos, sin))
 
 
+@pytest.mark.parametrize("seqs", [[(1, 5), (1, 900)], [(90, 300), (3, 3)], [(1, 4000)]])
+def test_output_in_place_of_the_queries(seqs):
+    c = Case(seqs, 2, 64, 16, BF16)
+    wide = torch.randn(c.rows, 4 * 256, generator=c.g).to(BF16).to(DEV)
+    want = ops.paged_attention(wide[:, 256:512], c.layer, c.step, 4, 0.2)
+    rest = wide.clone()
+    assert ops.paged_attention(wide[:, 256:512], c.layer, c.step, 4, 0.2, out=wide[:, 256:512]).data_ptr() == wide[:, 256:].data_ptr()
+    rest[:, 256:512] = want
+    assert torch.equal(wide, rest)
+
+
 def test_refusals():
     c = Case([(2, 20)], 2, 64, 16, BF16)
     q = torch.zeros(2, 256, dtype=BF16, device=DEV)
@@ -657,6 +679,10 @@ def test_refusals():
         (lambda: ops.process_logits(q, tokens=torch.zeros(2, 3, device=DEV)), ValueError),
         (lambda: ops.process_logits(q, lengths=S.kv_len), ValueError),
         (lambda: ops.process_logits(q, repetition_penalty=0.0), ValueError),
+        (lambda: ops.process_logits(q, repetition_penalty=1e-60), ValueError),
+        (lambda: ops.process_logits(q, frequency_penalty=1e60), ValueError),
+        (lambda: att(step=S._replace(rows=3)), ValueError), (lambda: wr(step=S._replace(rows=-1)), ValueError),
+        (lambda: att(step=S._replace(max_new=1)), ValueError), (lambda: wr(step=S._replace(max_len=-1)), ValueError),
         (lambda: ops.process_logits(q, presence_penalty=math.nan), ValueError),
         (lambda: ops.process_logits(q, bias=torch.zeros(255, device=DEV)), ValueError),
         (lambda: ops.process_logits(q, mask=torch.zeros(2, 7, dtype=torch.int32, device=DEV)), ValueError),
@@ -730,6 +756,21 @@ def test_cached_forward_is_the_forward(dtype, storage, most):
     assert k.shape == v.shape == (done[1], 2, 64) and k.dtype == dtype
 
 
+def test_cached_forward_has_no_dropout_and_no_gradients():
+    model = _model(F32, dropout=0.5)
+    ids = torch.randint(0, 500, (9,), generator=torch.Generator().manual_seed(6)).to(DEV)
+    want = model(ids[None]).logits[0, -1].detach()
+    model.train()
+    model.layers[0].mlp.eval()
+    modes = [m.training for m in model.modules()]
+    cache = model.new_cache(3, 16)
+    got = model.forward_cached(ids, cache, cache.step([0, 9, 0]))  # no new tokens before and after
+    assert [m.training for m in model.modules()] == modes and not got.requires_grad
+    assert float((got[1] - want).norm() / want.norm()) <= 1e-4  # as in test_cached_forward_is_the_forward
+    x = torch.randn(3, 256, device=DEV, requires_grad=True)
+    assert not model.layers[1].forward_cached(x, cache.layers[1], cache.step([1, 1, 1])).requires_grad
+
+
 def test_cached_forward_in_e4m3():
     """The first layer's keys and values, which no attention comes before, are
     the float32 cache's, each off by at most half a step: 2^-4 of it, or, where
@@ -774,6 +815,12 @@ def test_generate_with_a_cache(new):
         assert len(set(once[b, 42:].tolist())) == new
     assert model.generate(prompt, 2, temperature=0.0, use_cache=True, cache_dtype=E4M3).shape == (2, 44)
     assert torch.equal(model.generate(prompt, 0, use_cache=True), prompt)
+    # a row that may take nothing
+    nothing = torch.ones(2, 500, dtype=torch.bool, device=DEV)
+    nothing[1] = False
+    for how in (dict(temperature=0.0), dict(temperature=1.0), dict(temperature=1.0, top_k=3, use_cache=True)):
+        with pytest.raises(ValueError, match="token 42"):
+            model.generate(prompt, new, token_mask=nothing, **how)
     torch.manual_seed(9)
     a = model.generate(prompt, 3, temperature=0.8, top_k=5, use_cache=True)
     torch.manual_seed(9)
@@ -789,6 +836,13 @@ def test_model_refusals():
     step = cache.step([4])
     with pytest.raises(ValueError):
         model.forward_cached(torch.zeros(3, dtype=torch.int64, device=DEV), cache, step)
+    with pytest.raises(ValueError):
+        model.forward_cached(torch.zeros(0, dtype=torch.int64, device=DEV), cache, cache.step([0]))
+    other = _model(F32, n_layers=3).new_cache(1, 16)
+    with pytest.raises(ValueError):
+        model.forward_cached(torch.zeros(4, dtype=torch.int64, device=DEV), other, other.step([4]))
+    with pytest.raises(ValueError):
+        model.generate(torch.zeros(1, 4, dtype=torch.int64, device=DEV), 2, cache_dtype=E4M3)
     model._zero3_executor = object()
     with pytest.raises(RuntimeError):
         model.forward_cached(torch.zeros(4, dtype=torch.int64, device=DEV), cache, step)
