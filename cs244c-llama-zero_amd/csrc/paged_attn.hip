@@ -545,33 +545,39 @@ struct Plan {
   int nqb, nsplit, chunk;
 };
 
-// Row blocks and parts.  paged_wave_kernel: whole sequences where there is a
-// block for every CU (32 ragged sequences of up to 2048, 16/8 heads of 128: 33
-// us, in parts of 512 keys 37); else four workgroups a CU, so that lengths even
-// out (16 of up to 4096, 32/8 heads: 27 us in eight parts, 33 in four), but two
-// where that makes more than 16 parts to join (4 x 32768 in e4m3: 41 us in 16,
-// 48 in 32), and parts of 256 KiB at least, below which a part's lookups and
-// its end cost more than its keys (8 of up to 4096: 20 us, 23 in half as much),
-// while every CU has one (1 x 8192: 14 us in 32, 19 in 8).  The tile kernel:
-// one workgroup a CU, of two wave groups where that is all (1 x 512 new tokens
-// over 4096: 55 us in two parts, 70 whole, 89 whole with one group; in four
-// parts, with one group, 55).
+// Row blocks and parts.  Tiles of 128 rows where a sequence has 64 packed rows
+// or more and the work is not little: at most 1.5 blocks of 32 rows a CU which
+// go over at most 512 keys a CU, where the tile kernel's longer start and steps
+// are the time (12/4 heads of 64: 3 prompts of up to 182 tokens 7.3 us, 9.3 in
+// tiles; 4 of up to 400 17, 14 in tiles; 16 of up to 256 18 and 11).
+// paged_wave_kernel: whole sequences where there is a block for every CU (32
+// ragged sequences of up to 2048, 16/8 heads of 128: 33 us, in parts of 512
+// keys 37); else four workgroups a CU, so that lengths even out (16 of up to
+// 4096, 32/8 heads: 27 us in eight parts, 33 in four), but two where that makes
+// more than 16 parts to join (4 x 32768 in e4m3: 41 us in 16, 48 in 32), and
+// parts of 512 keys at least, four of each wave's tiles (8 of up to 4096: 20 us,
+// 23 in parts of 256; in e4m3 15.3, 17.3 and, in parts of 1024, 16.6), while
+// every CU has one (1 x 8192: 13 us in 32, 19 in 8).  The tile kernel: one
+// workgroup a CU, of two wave groups where that is all (1 x 512 new tokens over
+// 4096: 55 us in two parts, 70 whole, 89 whole with one group; in four parts,
+// with one group, 55).
 Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd, int64_t max_new,
                int64_t max_len) {
   Plan p;
   const int64_t G = H / KV, packed = std::max<int64_t>(1, std::min(max_new, rows)) * G, cus = lz_num_cus();
-  p.bm = packed <= 16 ? 16 : packed < 64 || dtype == LZ_F32 ? 32 : kPagedTileRows;
+  const int64_t len = std::max<int64_t>(1, max_len), small = KV * lz_cdiv(rows * G, 32);
+  const bool little = 2 * small <= 3 * cus && small * std::min<int64_t>(len, 1 << 20) <= 512 * cus;
+  p.bm = packed <= 16 ? 16 : packed < 64 || little || dtype == LZ_F32 ? 32 : kPagedTileRows;
   p.nqb = (int)lz_cdiv(packed, p.bm);
   // blocks that have rows: not every sequence has max_new of them
   const int64_t blocks = KV * std::min(B * p.nqb, std::min(B, rows) + rows * G / p.bm);
-  const int64_t len = std::max<int64_t>(1, max_len), one = std::max<int64_t>(1, cus / blocks);
+  const int64_t one = std::max<int64_t>(1, cus / blocks);
   int64_t chunk;
   if (p.bm == kPagedTileRows || blocks >= cus) {
     chunk = lz_cdiv(len, one);
   } else {
-    const int64_t key_bytes = 2 * hd * (cache_dtype == LZ_E4M3 ? 1 : lz_esize(dtype));
     chunk = lz_cdiv(len, std::min(4 * cus / blocks, std::max<int64_t>(16, 2 * cus / blocks)));
-    chunk = std::max(chunk, std::min((256 << 10) / key_bytes, lz_cdiv(len, one)));
+    chunk = std::max(chunk, std::min<int64_t>(512, lz_cdiv(len, one)));
   }
   p.chunk = (int)std::max<int64_t>(256, lz_cdiv(chunk, 64) * 64);
   p.nsplit = (int)lz_cdiv(len, p.chunk);

@@ -199,21 +199,6 @@ __device__ __forceinline__ void step_softmax(f32x16_t (&s)[2], f32x16_t (&o)[HD 
   step_sum<F, HD, ODD>(o, s, vf, to, vt);
 }
 
-// Whether V rows lo .. hi - 1 of the tile hold an infinity or NaN.
-template <typename F, int HD>
-__device__ __forceinline__ bool rows_odd(const char* vt, int lo, int hi, int lane) {
-  constexpr int kChunks = HD / 8, kRows = 64 / kChunks;
-  bool odd = false;
-  for (int r0 = lo; r0 < hi; r0 += kRows) {
-    const int r = r0 + lane / kChunks;
-    if (r < hi) {
-      const uint4 x = *reinterpret_cast<const uint4*>(vt + r * HD * 2 + (lane % kChunks) * 16);
-      odd |= nonfinite16<F>(x.x) || nonfinite16<F>(x.y) || nonfinite16<F>(x.z) || nonfinite16<F>(x.w);
-    }
-  }
-  return __ballot(odd) != 0;
-}
-
 // What finite_part took out, added to the rows that see it.
 template <typename F, int HD>
 __device__ __forceinline__ void add_odd(f32x16_t (&o)[HD / 32], const f32x16_t (&s)[2], const char* vt, int lim,
@@ -357,13 +342,12 @@ paged_tile_kernel(PagedArgs a) {
   const int end = (k_hi + 63) / 64, free_end = min(all / 64, end), wave_end = min((most + 63) / 64, end);
 
   // One pass over the keys, in rounds of NG steps; `rt` is a round's first
-  // step.  Returns whether V had an infinity or NaN in a step whose keys not
-  // all of this wave's rows see: its zero weights make it NaN in all of them.
-  // Then the pass is made again with ODD, which multiplies the finite part and
-  // adds the rest where it is seen; the other rows get the same bits as ever.
+  // step.  Returns whether a sum is not finite: an infinity or NaN of V may
+  // have met the zero weight of a row that does not see it.  Then the pass is
+  // made again with ODD, which multiplies the finite part and adds the rest
+  // where it is seen; the other rows get the same bits as ever.
   auto pass = [&](auto odd_pass) {
     constexpr bool ODD = decltype(odd_pass)::value;
-    bool met = false;
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i)
 #pragma unroll
@@ -418,8 +402,6 @@ paged_tile_kernel(PagedArgs a) {
         if (it < wave_end) {
           f32x16_t s[2];
           step_scores<F, HD>(s, to, tl.k_tile(), qf);
-          if constexpr (!ODD)
-            met |= rows_odd<F, HD>(tl.v_tile(), max(all - 64 * it, 0), min(64, n_keys - 64 * it), lane);
           step_softmax<F, HD, true, ODD>(s, o, mx, l, to, tl.v_tile(), unit, sees - 64 * it, here, half);
           if constexpr (ODD) add_odd<F, HD>(o, s, tl.v_tile(), sees - 64 * it, lane);
         }
@@ -427,7 +409,12 @@ paged_tile_kernel(PagedArgs a) {
       }
       if (rt < end) tl.look_up(a, at.b, rt, n_keys);
     }
-    return met;
+    float zero = 0.f;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) zero = fmaf(o[i][r], 0.f, zero);
+    return zero != 0.f;  // NaN
   };
   if (__syncthreads_or(pass(std::false_type{}))) pass(std::true_type{});
 
