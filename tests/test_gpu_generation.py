@@ -19,6 +19,9 @@ pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda")
 BF16, F16, F32, E4M3 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
 U32 = 2.0**-24
+# A bound on the lengths (CacheStep.max_len) with which sequences of 64 packed
+# rows or more take 128-row tiles, however short they are.
+MUCH = 2**20
 
 
 def _u(dtype):
@@ -50,7 +53,7 @@ class Case:
     """A cache layer in random pages, the step of (new, length) sequences and
     the same on the CPU in float64."""
 
-    def __init__(self, seqs, KV, hd, page, dtype, e4m3=False, seed=0, spare=2, fill=None):
+    def __init__(self, seqs, KV, hd, page, dtype, e4m3=False, seed=0, spare=2, fill=None, most=0):
         self.seqs, self.KV, self.hd, self.page, self.dtype, self.e4m3 = seqs, KV, hd, page, dtype, e4m3
         g = torch.Generator().manual_seed(seed)
         self.g = g
@@ -86,7 +89,7 @@ class Case:
         self.layer = LayerCache(*dev, *(None if e is None else e.to(DEV) for e in self.exps))
         self.step = CacheStep(torch.tensor(starts, dtype=torch.int32, device=DEV),
                               torch.tensor([l for _, l in seqs], dtype=torch.int32, device=DEV), self.table.to(DEV),
-                              self.rows, max(n for n, _ in seqs), max(l for _, l in seqs))
+                              self.rows, max(n for n, _ in seqs), max(most, max(l for _, l in seqs)))
 
     def tokens(self, side, b, length=None):
         """[length, KV, hd] float64 of sequence b's keys (0) or values (1)."""
@@ -248,8 +251,9 @@ def _check_attention(c, H, scale=None, q=None, **kw):
 @pytest.mark.parametrize("seqs", sorted(SEQS))
 @pytest.mark.parametrize("dtype,e4m3", [(BF16, False), (F16, False), (F32, False), (BF16, True), (F16, True), (F32, True)])
 @pytest.mark.parametrize("H,KV,hd,page", [(10, 2, 32, 16), (12, 4, 64, 32), (5, 5, 128, 16), (32, 8, 128, 64)])
-def test_paged_attention(seqs, dtype, e4m3, H, KV, hd, page):
-    _check_attention(Case(SEQS[seqs], KV, hd, page, dtype, e4m3, seed=H + hd, fill=None if e4m3 else math.nan), H)
+@pytest.mark.parametrize("most", [0, MUCH])
+def test_paged_attention(seqs, dtype, e4m3, H, KV, hd, page, most):
+    _check_attention(Case(SEQS[seqs], KV, hd, page, dtype, e4m3, seed=H + hd, fill=None if e4m3 else math.nan, most=most), H)
 
 
 @pytest.mark.parametrize("dtype,e4m3", [(BF16, False), (F16, True), (F32, False)])
@@ -261,8 +265,9 @@ def test_paged_attention(seqs, dtype, e4m3, H, KV, hd, page):
     (64, 700, 4, 2, 128, 16),     # a chunk whose first rows end inside a page
     (33, 257, 33, 1, 32, 128),    # 33 heads on one
 ])
-def test_paged_attention_lengths(dtype, e4m3, n, length, H, KV, hd, page):
-    c = Case([(n, length), (min(n, 3), 3)], KV, hd, page, dtype, e4m3, seed=length, fill=None if e4m3 else math.inf)
+@pytest.mark.parametrize("most", [0, MUCH])
+def test_paged_attention_lengths(dtype, e4m3, n, length, H, KV, hd, page, most):
+    c = Case([(n, length), (min(n, 3), 3)], KV, hd, page, dtype, e4m3, seed=length, fill=None if e4m3 else math.inf, most=most)
     _check_attention(c, H)
 
 
@@ -278,6 +283,9 @@ def test_many_sequences(seqs, H, KV, e4m3):
     """Attention, write and read of long lists of sequences."""
     c = Case(seqs, KV, 32, 16, BF16, e4m3, seed=len(seqs), fill=None if e4m3 else math.nan)
     _check_attention(c, H)
+    step, c.step = c.step, c.step._replace(max_len=MUCH)
+    _check_attention(c, H)
+    c.step = step
     n = [min(l, 20) for _, l in seqs]
     start = torch.tensor([sum(n[:b]) for b in range(len(n) + 1)], dtype=torch.int32)
     k, _ = ops.kv_cache_read(c.layer, c.step.page_table, start.to(DEV), int(start[-1]), BF16)
@@ -299,17 +307,19 @@ def test_many_sequences(seqs, H, KV, e4m3):
     assert torch.equal(v.cpu()[new].reshape(-1, 32), want)
 
 
-@pytest.mark.parametrize("new,bound", [(1, 100), (1, 5000), (40, 100), (40, 5000)])
-def test_bound_on_the_length_only_splits(new, bound):
+@pytest.mark.parametrize("new,bound", [(1, 100), (1, 5000), (40, 100), (40, 5000), (40, 12000), (130, 12000), (130, 6000)])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_bound_on_the_length_only_splits(new, bound, e4m3):
     """max_len below and above the sequences' lengths: the same attention."""
-    c = Case([(new, 1300), (1, 40)], 2, 64, 32, BF16, seed=bound)
+    c = Case([(new, 1300), (1, 40)], 2, 64, 32, BF16, e4m3, seed=bound)
     c.step = c.step._replace(max_len=bound)
     _check_attention(c, 8)
 
 
 @pytest.mark.parametrize("dtype,e4m3", [(BF16, False), (BF16, True), (F32, False), (F16, True)])
 @pytest.mark.parametrize("news", [[64, 1, 1, 30, 1], [1, 1, 1], [200, 90]])
-def test_steps_of_a_layer(news, dtype, e4m3):
+@pytest.mark.parametrize("most", [0, MUCH])
+def test_steps_of_a_layer(news, dtype, e4m3, most):
     """Write, then attend, step after step: each row against the attention of
     the whole text over what the cache holds."""
     H, KV, hd, page = 8, 2, 64, 32
@@ -323,6 +333,7 @@ def test_steps_of_a_layer(news, dtype, e4m3):
         step = cache.step([n, n])
         qkv = torch.randn(2 * n, (H + 2 * KV) * hd, generator=g).to(dtype).to(DEV)
         q = ops.kv_cache_write(qkv, cache.layers[0], step, H, cos, sin)
+        step = step._replace(max_len=max(most, step.max_len))
         o = ops.paged_attention(q, cache.layers[0], step, H, hd**-0.5).double().cpu().view(2, n, H, hd)
         for b in range(2):
             k, v = (t.double().cpu() for t in cache.read(0, b))
@@ -383,21 +394,21 @@ def test_a_captured_step_follows_its_tables():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
-@pytest.mark.parametrize("n,length", [(1, 600), (70, 300), (200, 200)])
-def test_paged_attention_large_scores(dtype, n, length):
+@pytest.mark.parametrize("n,length,most", [(1, 600, 0), (70, 300, 0), (200, 200, 0), (70, 300, MUCH), (200, 200, MUCH)])
+def test_paged_attention_large_scores(dtype, n, length, most):
     """Scores in the hundreds: one key takes nearly all the weight, and the
     running maximum moves late."""
-    c = Case([(n, length)], 2, 64, 32, dtype, seed=n)
+    c = Case([(n, length)], 2, 64, 32, dtype, seed=n, most=most)
     q = (torch.randn(c.rows, 4 * 64, generator=c.g) * 12).to(dtype)
     _check_attention(c, 4, scale=0.5, q=q)
 
 
 @pytest.mark.parametrize("dtype,e4m3", [(BF16, False), (F16, False), (F32, False), (BF16, True)])
-@pytest.mark.parametrize("n,length", [(1, 200), (150, 200), (16, 40)])
-def test_paged_attention_nonfinite_reaches_only_who_sees_it(dtype, e4m3, n, length):
+@pytest.mark.parametrize("n,length,most", [(1, 200, 0), (150, 200, 0), (16, 40, 0), (150, 200, MUCH), (40, 40, MUCH)])
+def test_paged_attention_nonfinite_reaches_only_who_sees_it(dtype, e4m3, n, length, most):
     """An infinity or NaN among the last new token's keys and values leaves
     the rows before it as they were."""
-    c = Case([(n, length), (1, 9)], 2, 64, 32, dtype, e4m3, seed=7)
+    c = Case([(n, length), (1, 9)], 2, 64, 32, dtype, e4m3, seed=7, most=most)
     q = torch.randn(c.rows, 4 * 64, generator=c.g).to(dtype).to(DEV)
     before = ops.paged_attention(q, c.layer, c.step, 4, 0.125)
     p = length - 1
@@ -456,6 +467,32 @@ def test_bad_pages_are_left_out():
     k, _ = ops.kv_cache_read(c.layer, step.page_table, start, 100, F32)
     assert bool((k[16:32] == 0).all()) and bool((k[64:80] == 0).all()) and bool((k[96:] == 0).all())
     assert torch.equal(k[:16].cpu().double(), c.tokens(0, 0)[:16, 0])
+
+
+@pytest.mark.parametrize("most", [0, MUCH])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_chunks_that_see_nothing_and_bad_pages(e4m3, most):
+    """Chunks with more new tokens than the sequence has, one of no sequence at
+    all and one over pages outside the pool."""
+    c = Case([(90, 90), (40, 40), (70, 200)], 1, 64, 16, BF16, e4m3, most=most)
+    table = c.table.clone()
+    table[2, 1], table[2, 4], table[2, 9] = -5, 10_000_000, 2**31 - 1
+    step = c.step._replace(kv_len=torch.tensor([50, 0, 200], dtype=torch.int32, device=DEV), page_table=table.to(DEV))
+    q = torch.randn(c.rows + 3, 64, generator=c.g).to(BF16)
+    got = ops.paged_attention(q.to(DEV), c.layer, step, 1, 0.125, out=torch.full((c.rows + 3, 64), 7.0, dtype=BF16, device=DEV))
+    got = got.cpu().double()
+    assert bool((got[:40] == 0).all()) and bool((got[90:130] == 0).all()) and bool((got[c.rows :] == 7).all())
+    u = _u(BF16)
+    for row in range(c.rows):
+        b, keep = (0, range(row - 40 + 1)) if row < 90 else (2, [p for p in range(row + 1) if p // 16 not in (1, 4, 9)])
+        if len(keep) == 0 or 90 <= row < 130:
+            continue
+        k, v = c.tokens(0, b)[list(keep), 0], c.tokens(1, b)[list(keep), 0]
+        p = torch.softmax(k @ q[row].double() * 0.125, 0)
+        want, size = p @ v, p @ v.abs()
+        top = float((k.abs() @ q[row].double().abs()).max()) * 0.125
+        fp32 = (2 * (64 + 4) * top + 8 + len(keep)) * U32  # as in Case.attention
+        assert bool(((got[row] - want).abs() <= u * want.abs() + (u + fp32) * size).all()), row
 
 
 def test_pages_past_two_to_the_31_elements():
@@ -577,7 +614,7 @@ def _pass(c, H, qkv, cos, sin, logits, tokens):
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
-@pytest.mark.parametrize("seqs", [[(1, 900), (1, 3)], [(150, 300), (7, 90)]])
+@pytest.mark.parametrize("seqs", [[(1, 900), (1, 3)], [(150, 300), (7, 90)], [(400, 1200), (70, 90)]])
 def test_two_graphs_and_eager_calls_in_turn(seqs, e4m3):
     """Two captured passes and eager ones between their replays, on contents
     that change: every replay gives what the eager call gives."""
@@ -614,8 +651,9 @@ def test_two_graphs_and_eager_calls_in_turn(seqs, e4m3):
                 assert torch.equal(a, b), turn
 
 
-def test_calls_on_another_stream():
-    c = Case([(1, 700), (30, 64)], 2, 64, 32, BF16)
+@pytest.mark.parametrize("most", [0, MUCH])
+def test_calls_on_another_stream(most):
+    c = Case([(1, 700), (30, 64)], 2, 64, 32, BF16, most=most)
     q = torch.randn(c.rows, 4 * 64, generator=c.g).to(BF16).to(DEV)
     want = ops.paged_attention(q, c.layer, c.step, 4, 0.125)
     side = torch.cuda.Stream()
@@ -641,8 +679,9 @@ def test_unaligned_rows():
 
 
 @pytest.mark.parametrize("seqs", [[(1, 5), (1, 900)], [(90, 300), (3, 3)], [(1, 4000)]])
-def test_output_in_place_of_the_queries(seqs):
-    c = Case(seqs, 2, 64, 16, BF16)
+@pytest.mark.parametrize("most", [0, MUCH])
+def test_output_in_place_of_the_queries(seqs, most):
+    c = Case(seqs, 2, 64, 16, BF16, most=most)
     wide = torch.randn(c.rows, 4 * 256, generator=c.g).to(BF16).to(DEV)
     want = ops.paged_attention(wide[:, 256:512], c.layer, c.step, 4, 0.2)
     rest = wide.clone()
