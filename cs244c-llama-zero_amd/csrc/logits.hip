@@ -33,10 +33,13 @@ struct LogitsArgs {
   int B, V, n_tokens, mask_kind;  // mask_kind 0: none, 1: a byte a token, 2: a bit a token
 };
 
+typedef uint32_t Words4 __attribute__((ext_vector_type(4), aligned(2)));  // of any rows
+
 // NV * 2048 tokens of the vocabulary a workgroup: eight adjacent ones a thread
-// and vector, whose logits are in flight while the text is counted.  ALIGNED:
-// every row's vectors are 16-byte aligned.
-template <typename T, int NV, bool ALIGNED>
+// and vector, whose logits are in flight while the text is counted.  Rows start
+// at any element: loads and stores of 16 bytes need no alignment here (36 rows
+// of 53151 in fp16 with a bias each: 6.7 us, 13.6 one element at a time).
+template <typename T, int NV>
 __global__ void __launch_bounds__(256) process_logits_kernel(LogitsArgs a) {
   constexpr int kSlice = NV * 2048;
   __shared__ __attribute__((aligned(16))) uint32_t cnt[kSlice];  // 2 * (times in the answer) + (1 if in the text)
@@ -51,11 +54,11 @@ __global__ void __launch_bounds__(256) process_logits_kernel(LogitsArgs a) {
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int i = (k * 256 + tid) * 8;
-    if (ALIGNED && i + 8 <= n) {
+    if (i + 8 <= n) {
       T raw[8];
 #pragma unroll
       for (int w = 0; w < (int)sizeof(T) / 2; ++w)
-        reinterpret_cast<uint4*>(raw)[w] = reinterpret_cast<const uint4*>(x_row + i)[w];
+        reinterpret_cast<Words4*>(raw)[w] = reinterpret_cast<const Words4*>(x_row + i)[w];
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[k][e] = Elem<T>::load(raw, e);
     } else {
@@ -100,9 +103,9 @@ __global__ void __launch_bounds__(256) process_logits_kernel(LogitsArgs a) {
     }
     float y[8] = {};
     if (b_row) {
-      if (ALIGNED && i + 8 <= n) {
-        reinterpret_cast<float4*>(y)[0] = reinterpret_cast<const float4*>(b_row + i)[0];
-        reinterpret_cast<float4*>(y)[1] = reinterpret_cast<const float4*>(b_row + i)[1];
+      if (i + 8 <= n) {
+        reinterpret_cast<Words4*>(y)[0] = reinterpret_cast<const Words4*>(b_row + i)[0];
+        reinterpret_cast<Words4*>(y)[1] = reinterpret_cast<const Words4*>(b_row + i)[1];
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -129,9 +132,9 @@ __global__ void __launch_bounds__(256) process_logits_kernel(LogitsArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = (allowed >> e) & 1 ? x[k][e] : -INFINITY;
     float* o = a.out + b * a.ldo + lo + i;
-    if (ALIGNED && i + 8 <= n) {
-      reinterpret_cast<float4*>(o)[0] = reinterpret_cast<const float4*>(y)[0];
-      reinterpret_cast<float4*>(o)[1] = reinterpret_cast<const float4*>(y)[1];
+    if (i + 8 <= n) {
+      reinterpret_cast<Words4*>(o)[0] = reinterpret_cast<const Words4*>(y)[0];
+      reinterpret_cast<Words4*>(o)[1] = reinterpret_cast<const Words4*>(y)[1];
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -154,9 +157,6 @@ LZ_EXPORT int lz_process_logits(const void* logits, int64_t ld, int dtype, int64
              "lz_process_logits: mask kind %d", mask_kind);
   if (B == 0 || V == 0) return LZ_OK;
   LZ_REQUIRE(logits && out && ldo >= V && (B == 1 || ld >= V) && (tokens || n_tokens == 0), "lz_process_logits: bad arguments");
-  const int esz = lz_esize(dtype);
-  const bool aligned = lz_aligned16(logits) && lz_aligned16(out) && (B == 1 || (ld * esz % 16 == 0 && ldo % 4 == 0)) &&
-                       (!bias || (lz_aligned16(bias) && ldb % 4 == 0));
   // small slices where the rows are few and a slice's chain of loads is the
   // time; large ones where each reads a long text again
   const bool small = B * lz_cdiv(V, 8192) < 2 * lz_num_cus();
@@ -168,10 +168,8 @@ LZ_EXPORT int lz_process_logits(const void* logits, int64_t ld, int dtype, int64
   hipStream_t s = lz_stream(stream);
 #define RUN(T)                                                                           \
   do {                                                                                   \
-    if (small && aligned) process_logits_kernel<T, 1, true><<<grid, 256, 0, s>>>(a);     \
-    else if (small) process_logits_kernel<T, 1, false><<<grid, 256, 0, s>>>(a);          \
-    else if (aligned) process_logits_kernel<T, 4, true><<<grid, 256, 0, s>>>(a);         \
-    else process_logits_kernel<T, 4, false><<<grid, 256, 0, s>>>(a);                     \
+    if (small) process_logits_kernel<T, 1><<<grid, 256, 0, s>>>(a);                      \
+    else process_logits_kernel<T, 4><<<grid, 256, 0, s>>>(a);                            \
   } while (0)
   if (dtype == LZ_BF16) RUN(uint16_t);
   else if (dtype == LZ_F16) RUN(_Float16);

@@ -557,10 +557,11 @@ struct Plan {
 // more than 16 parts to join (4 x 32768 in e4m3: 41 us in 16, 48 in 32), and
 // parts of 512 keys at least, four of each wave's tiles (8 of up to 4096: 20 us,
 // 23 in parts of 256; in e4m3 15.3, 17.3 and, in parts of 1024, 16.6), while
-// every CU has one (1 x 8192: 13 us in 32, 19 in 8).  The tile kernel: one
-// workgroup a CU, of two wave groups where that is all (1 x 512 new tokens over
-// 4096: 55 us in two parts, 70 whole, 89 whole with one group; in four parts,
-// with one group, 55).
+// every CU has one (1 x 8192: 13 us in 32, 19 in 8); short sequences whole,
+// where the join costs more than their keys (1 x 512 over heads of 64: 6.4 us,
+// 8.6 in parts; of 128: 8.4 and 9.1).  The tile kernel: one workgroup a CU, of
+// two wave groups where that is all (1 x 512 new tokens over 4096: 55 us in two
+// parts, 70 whole, 89 whole with one group; in four parts, with one group, 55).
 Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd, int64_t max_new,
                int64_t max_len) {
   Plan p;
@@ -578,6 +579,7 @@ Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, i
   } else {
     chunk = lz_cdiv(len, std::min(4 * cus / blocks, std::max<int64_t>(16, 2 * cus / blocks)));
     chunk = std::max(chunk, std::min<int64_t>(512, lz_cdiv(len, one)));
+    if (dtype != LZ_F32 && len <= (hd > 64 ? 512 : 768)) chunk = len;
   }
   p.chunk = (int)std::max<int64_t>(256, lz_cdiv(chunk, 64) * 64);
   p.nsplit = (int)lz_cdiv(len, p.chunk);
