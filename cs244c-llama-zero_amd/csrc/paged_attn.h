@@ -54,11 +54,13 @@ struct PagedPlace {
 struct PagedRows {
   int m0, count;  // count: rows of the pair (0 or less: none)
   int row0, base, G, cap;
-  __device__ __forceinline__ PagedRows(const PagedArgs& a, int b, int m0_) {
+  __device__ __forceinline__ PagedRows(const PagedArgs& a, int b, int m0_)
+      : PagedRows(a, a.row_start[b], a.row_start[b + 1], a.kv_len[b], m0_) {}
+  // of a sequence whose rows are lo .. hi - 1, len tokens long
+  __device__ __forceinline__ PagedRows(const PagedArgs& a, int lo, int hi, int len, int m0_) {
     m0 = m0_;
     G = a.H / a.KV;
-    const int lo = a.row_start[b], hi = a.row_start[b + 1];
-    base = a.kv_len[b] - hi + 1;  // keys that row r of q sees: base + r
+    base = len - hi + 1;  // keys that row r of q sees: base + r
     row0 = max(lo, 0);
     count = hi > row0 ? (min(hi, a.rows) - row0) * G : 0;
     cap = a.pg.width << a.pg.log_size;

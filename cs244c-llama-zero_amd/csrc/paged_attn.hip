@@ -485,9 +485,18 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm, in
   }
   int n_parts = 0;
   if (row < a.rows) {
-    const int b = lz_seq_of_row(a.row_start, a.B, a.rows, row);
+    // the guess that serves single tokens, with all that it needs in one round
+    int b = (int)((int64_t)row * a.B / a.rows), lo = a.row_start[b], hi = a.row_start[b + 1], len = a.kv_len[b];
+    if (row < lo || row >= hi) {
+      b = lz_seq_of_row(a.row_start, a.B, a.rows, row);
+      if (b >= 0) {
+        lo = a.row_start[b];
+        hi = a.row_start[b + 1];
+        len = a.kv_len[b];
+      }
+    }
     if (b >= 0) {
-      PagedRows rw(a, b, 0);
+      PagedRows rw(a, lo, hi, len, 0);
       const int m = (row - rw.row0) * rw.G + head % rw.G;
       rw.m0 = m / bm * bm;
       if (m / bm < a.nqb) n_parts = PagedRows::parts(a, rw.keys(bm));
