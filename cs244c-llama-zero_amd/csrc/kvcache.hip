@@ -43,13 +43,15 @@ struct Vec {
   }
 };
 
-// Four floats to four e4m3 bytes (round to nearest even; |x| <= 448 or NaN).
+// Four floats to four e4m3 bytes (round to nearest even; |x| <= 448, or not
+// finite: NaN).
 __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
-template <int N>
+// CAP: finite values past 448 / inv become that.
+template <int N, bool CAP>
 __device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&x)[N], float inv) {
   uint32_t w[N / 4];
 #pragma unroll
@@ -57,9 +59,9 @@ __device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&x)[N], floa
     float y[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float t = x[4 * i + e] * inv;
-      const bool finite = fabsf(x[4 * i + e]) < INFINITY;
-      y[e] = finite ? fminf(fmaxf(t, -448.f), 448.f) : __builtin_nanf("");
+      y[e] = x[4 * i + e] * inv;
+      if constexpr (CAP)
+        if (fabsf(x[4 * i + e]) < INFINITY) y[e] = fminf(fmaxf(y[e], -448.f), 448.f);
     }
     w[i] = pack_e4m3(y[0], y[1], y[2], y[3]);
   }
@@ -164,8 +166,13 @@ __global__ void __launch_bounds__(256) kv_write_kernel(WriteArgs a) {
     const int e = exponent_of<std::is_same<T, _Float16>::value>(amax);
     const float inv = lz_pow2(-e);
     uint8_t* dst = static_cast<uint8_t*>(is_k ? a.k : a.v) + token * HD + i;
-    store_e4m3<N>(dst, lo, inv);
-    store_e4m3<N>(dst + HD / 2, hi, inv);
+    if (amax * inv > 448.f) {  // the exponent is at its limit
+      store_e4m3<N, true>(dst, lo, inv);
+      store_e4m3<N, true>(dst + HD / 2, hi, inv);
+    } else {
+      store_e4m3<N, false>(dst, lo, inv);
+      store_e4m3<N, false>(dst + HD / 2, hi, inv);
+    }
     if (i == 0) (is_k ? a.k_exp : a.v_exp)[token] = (int8_t)e;
   }
 }

@@ -70,7 +70,7 @@ struct PagedRows {
   // the keys that the block's rows see together, and the parts they make
   __device__ __forceinline__ int keys(int bm) const { return sees(min(m0 + bm, count) - 1); }
   static __device__ __forceinline__ int parts(const PagedArgs& a, int keys) {
-    return min(max((keys + a.chunk - 1) / a.chunk, 1), a.nsplit);
+    return min(max((int)(((uint32_t)keys + (uint32_t)a.chunk - 1) / (uint32_t)a.chunk), 1), a.nsplit);
   }
 };
 
