@@ -561,16 +561,19 @@ struct Plan {
 // tiles; 4 of up to 400 17, 14 in tiles; 16 of up to 256 18 and 11).
 // paged_wave_kernel: whole sequences where there is a block for every CU (32
 // ragged sequences of up to 2048, 16/8 heads of 128: 33 us, in parts of 512
-// keys 37); else four workgroups a CU, so that lengths even out (16 of up to
-// 4096, 32/8 heads: 27 us in eight parts, 33 in four), but two where that makes
-// more than 16 parts to join (4 x 32768 in e4m3: 41 us in 16, 48 in 32), and
-// parts of 512 keys at least, four of each wave's tiles (8 of up to 4096: 20 us,
-// 23 in parts of 256; in e4m3 15.3, 17.3 and, in parts of 1024, 16.6), while
-// every CU has one (1 x 8192: 13 us in 32, 19 in 8); short sequences whole,
-// where the join costs more than their keys (1 x 512 over heads of 64: 6.4 us,
-// 8.6 in parts; of 128: 8.4 and 9.1).  The tile kernel: one workgroup a CU, of
-// two wave groups where that is all (1 x 512 new tokens over 4096: 55 us in two
-// parts, 70 whole, 89 whole with one group; in four parts, with one group, 55).
+// keys 37), but four parts where some CUs would have one more than others and a
+// third of the CUs' time would go by (36 of them: 42 us, whole 51; 58: 52 and
+// 53; all 2048 long: 60 and 71 of 36, 93 and 85 of 58); fewer blocks than CUs:
+// four workgroups a CU, so that lengths even out (16 of up to 4096, 32/8 heads:
+// 27 us in eight parts, 33 in four), but two where that makes more than 16 parts
+// to join (4 x 32768 in e4m3: 41 us in 16, 48 in 32), and parts of 512 keys at
+// least, four of each wave's tiles (8 of up to 4096: 20 us, 23 in parts of 256;
+// in e4m3 15.3, 17.3 and, in parts of 1024, 16.6), while every CU has one
+// (1 x 8192: 13 us in 32, 19 in 8); short sequences whole, where the join costs
+// more than their keys (1 x 512 over heads of 64: 6.4 us, 8.6 in parts; of 128:
+// 8.4 and 9.1).  The tile kernel: one workgroup a CU, of two wave groups where
+// that is all (1 x 512 new tokens over 4096: 55 us in two parts, 70 whole, 89
+// whole with one group; in four parts, with one group, 55).
 Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd, int64_t max_new,
                int64_t max_len) {
   Plan p;
@@ -582,12 +585,14 @@ Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, i
   // blocks that have rows: not every sequence has max_new of them
   const int64_t blocks = KV * std::min(B * p.nqb, std::min(B, rows) + rows * G / p.bm);
   const int64_t one = std::max<int64_t>(1, cus / blocks);
-  int64_t chunk;
-  if (p.bm == kPagedTileRows || blocks >= cus) {
-    chunk = lz_cdiv(len, one);
-  } else {
-    chunk = lz_cdiv(len, std::min(4 * cus / blocks, std::max<int64_t>(16, 2 * cus / blocks)));
-    chunk = std::max(chunk, std::min<int64_t>(512, lz_cdiv(len, one)));
+  int64_t chunk = lz_cdiv(len, one);
+  if (p.bm != kPagedTileRows) {
+    if (blocks < cus) {
+      const int64_t even = lz_cdiv(len, std::min(4 * cus / blocks, std::max<int64_t>(16, 2 * cus / blocks)));
+      chunk = std::max(even, std::min<int64_t>(512, chunk));
+    } else if (3 * lz_cdiv(blocks, cus) * cus > 4 * blocks) {
+      chunk = std::max<int64_t>(512, lz_cdiv(len, 4));
+    }
     if (dtype != LZ_F32 && len <= (hd > 64 ? 512 : 768)) chunk = len;
   }
   p.chunk = (int)std::max<int64_t>(256, lz_cdiv(chunk, 64) * 64);

@@ -278,6 +278,7 @@ def test_paged_attention_lengths(dtype, e4m3, n, length, H, KV, hd, page, most):
     ([(1 + b % 5, 1 + b % 5 + b % 17) for b in range(1030)], 1, 1),
     ([(b % 37, b % 37 + 11 * b % 50) for b in range(70)], 8, 2),                # chunks of more than 64 sequences
     ([(3, 90), (70, 71), (0, 0), (33, 400), (1, 1)], 12, 3),                    # chunks beside single tokens
+    ([(1, 1 + 237 * b % 1500) for b in range(40)], 8, 8),                       # a few more heads than CUs
 ])
 def test_many_sequences(seqs, H, KV, e4m3):
     """Attention, write and read of long lists of sequences."""
