@@ -573,7 +573,10 @@ struct Plan {
 // more than their keys (1 x 512 over heads of 64: 6.4 us, 8.6 in parts; of 128:
 // 8.4 and 9.1).  The tile kernel: one workgroup a CU, of two wave groups where
 // that is all (1 x 512 new tokens over 4096: 55 us in two parts, 70 whole, 89
-// whole with one group; in four parts, with one group, 55).
+// whole with one group; in four parts, with one group, 55), and for up to a third
+// more blocks where their keys are uneven, so that those of a second turn are
+// short (a prompt of 2600, 16/8 heads: 46 us, 56 with one group; 3 chunks of 800
+// over 4096 alike: 119 and 104).
 Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd, int64_t max_new,
                int64_t max_len) {
   Plan p;
@@ -597,7 +600,8 @@ Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, i
   }
   p.chunk = (int)std::max<int64_t>(256, lz_cdiv(chunk, 64) * 64);
   p.nsplit = (int)lz_cdiv(len, p.chunk);
-  p.groups = blocks * p.nsplit <= cus ? 2 : 1;
+  const bool uneven = len >= 1024 && (2 * max_new >= len || 10 * rows < 9 * B * std::min(max_new, rows));
+  p.groups = blocks * p.nsplit <= cus || (uneven && 10 * blocks <= 13 * cus) ? 2 : 1;
   return p;
 }
 
