@@ -78,7 +78,8 @@ struct PagedRows {
 // maximum, but moves only when that is more than kSlack above it: weights up to
 // 2^8 are as exact in 16 and 32 bits as those up to 1, and the sums are
 // multiplied down once or twice in a pass and not at every new maximum (2 x up
-// to 1024 new tokens over up to 8192, 32/8 heads of 128: 161 and 171 us).
+// to 1024 new tokens over up to 8192, 32/8 heads of 128, one wave group a block:
+// 161 and 171 us).
 constexpr float kSlack = 8.f;
 
 // Two e4m3 values of a word, times 2^e (exact in bf16, and in fp16 for what
