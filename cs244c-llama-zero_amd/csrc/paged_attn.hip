@@ -576,7 +576,10 @@ struct Plan {
 // whole with one group; in four parts, with one group, 55), and for up to a third
 // more blocks where their keys are uneven, so that those of a second turn are
 // short (a prompt of 2600, 16/8 heads: 46 us, 56 with one group; 3 chunks of 800
-// over 4096 alike: 119 and 104).
+// over 4096 alike: 119 and 104); three parts of one group, two workgroups a CU,
+// where a block each would leave a third of the CUs idle for long (1 x 600 over
+// 8192, 32/8 heads: 99 us, whole 119; 1 x 1100 over 2200, 16/8 heads: 41 and 41;
+// 1 x 700 over 3000, 32/8 heads, with blocks for two thirds: 64 and 52).
 Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd, int64_t max_new,
                int64_t max_len) {
   Plan p;
@@ -597,6 +600,8 @@ Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, i
       chunk = std::max<int64_t>(512, lz_cdiv(len, 4));
     }
     if (dtype != LZ_F32 && len <= (hd > 64 ? 512 : 768)) chunk = len;
+  } else if (one == 1 && 3 * blocks <= 2 * cus && len >= 4096) {
+    chunk = lz_cdiv(len, 3);
   }
   p.chunk = (int)std::max<int64_t>(256, lz_cdiv(chunk, 64) * 64);
   p.nsplit = (int)lz_cdiv(len, p.chunk);
