@@ -34,14 +34,17 @@ namespace {
 
 typedef LzPagedArgs PagedArgs;
 
-// A workgroup's place: blocks of one (sequence, kv head) pair are dealt to one
-// XCD when the pairs split evenly over the eight, so that the keys and values
-// its row blocks share are fetched into one L2.
+// A workgroup's place.  With kv heads for the eight XCDs the blocks of one
+// (sequence, kv head) pair go to one of them, so that the keys and values its
+// row blocks share are fetched into one L2.  With fewer heads that would leave a
+// long sequence to some of the XCDs: its blocks go round all of them (4 x up to
+// 188 new tokens over up to 8979 in fp32, 2 heads of 32: 66 us, on two XCDs
+// 115).
 struct PagedPlace {
   int b, g, qb, split;
   __device__ __forceinline__ PagedPlace(const PagedArgs& a, uint32_t bid) {
     const uint32_t pairs = (uint32_t)(a.B * a.KV);
-    const uint32_t pair = bid % pairs, rest = bid / pairs;
+    const uint32_t rest = bid / pairs, pair = (bid + (a.KV % 8 ? rest : 0)) % pairs;
     b = (int)(pair / (uint32_t)a.KV);
     g = (int)(pair % (uint32_t)a.KV);
     split = (int)(rest / (uint32_t)a.nqb);
