@@ -85,6 +85,52 @@ struct PagedRows {
 // 161 and 171 us).
 constexpr float kSlack = 8.f;
 
+// Two fp32 weights of the second product as N packed terms of the 16-bit format
+// F, largest first.  Rounded to F once they would cost as much as the output's
+// own rounding (1.1 to 1.4 times the error against float64); so:
+//   paged_wave_kernel, bf16: three terms of eight significant bits, cut and not
+//     rounded, so that each remainder is exact and the three add up to the
+//     weight.  It is bound by memory: 16 x up to 4096 tokens, 32/8 heads of 128,
+//     30.7 us, with one rounded term 30.5; 8 x up to 15 new over 4096 44, 38.
+//   paged_tile_kernel, bf16: the cut weight and the rounded rest, off by 2^-16 of
+//     the weight at most.  It is bound by the matrix cores: 2 x up to 1024 new
+//     over up to 8192, 32/8 heads of 128, 199 us, with one term 155, three 244.
+//   fp16: the cut weight and the rounded rest, off by 2^-22 at most.  The weights
+//     are formed 2^7 times as large (kLift, in log2 units; so is their sum): up to
+//     2^15, and what the smallest subnormal cuts off is 2^-32 of the reference.
+template <typename F>
+constexpr float kLift = F::kDtype == LZ_F16 ? 7.f : 0.f;
+template <typename F, int N>
+__device__ __forceinline__ void weight_terms(uint32_t (&w)[N], float a, float b) {
+  if constexpr (F::kDtype == LZ_F16) {
+    static_assert(N == 2);
+    const auto cut = __builtin_amdgcn_cvt_pkrtz(a, b);
+    w[0] = __builtin_bit_cast(uint32_t, cut);
+    w[1] = F::pack2(a - (float)cut[0], b - (float)cut[1]);
+  } else {
+#pragma unroll
+    for (int t = 0; t < N; ++t) {
+      if (t == 1 && N == 2) {
+        w[t] = F::pack2(a, b);
+        break;
+      }
+      const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+      w[t] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+      a -= __uint_as_float(x & 0xffff0000u);
+      b -= __uint_as_float(y & 0xffff0000u);
+    }
+  }
+}
+// Four pairs: the operand words of N MFMAs.
+template <typename F, int N, typename Pair>
+__device__ __forceinline__ void weight_words(uint4 (&w)[N], const Pair& pair) {
+  uint32_t y[4][N];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) weight_terms<F, N>(y[e], pair(2 * e), pair(2 * e + 1));
+#pragma unroll
+  for (int t = 0; t < N; ++t) w[t] = make_uint4(y[0][t], y[1][t], y[2][t], y[3][t]);
+}
+
 // Two e4m3 values of a word, times 2^e (exact in bf16, and in fp16 for what
 // lz_kv_write stores of fp16 rows), as two values of the 16-bit format F.
 template <typename F, bool kHi>

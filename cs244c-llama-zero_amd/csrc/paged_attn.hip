@@ -60,6 +60,7 @@ struct Wave {
   static constexpr int NL = HD / 4 / CE, KW = CE * kEsz / 4;          // pieces of a lane, words of a piece
   static constexpr int VE = HD / 16, VB = VE * kEsz, VW = (VB + 3) / 4;  // columns, bytes and words of a lane's V
   static constexpr int NS = kWide ? HD / 4 : HD / 32;  // contraction steps of a score
+  static constexpr int kTerms = F::kDtype == LZ_F16 ? 2 : 3;  // of a weight (16-bit rows)
 
   uint32_t k[NT][NL][KW];
   uint32_t v[NT][4][VW];
@@ -177,11 +178,10 @@ struct Wave {
             for (int n = 0; n < NQ; ++n)
               acc[n][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.w[t][i][j]), p[n][t][i], acc[n][j], 0, 0, 0);
     } else {
-      uint4 pb[NQ];
+      uint4 pb[NQ][kTerms];
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
-        pb[n] = make_uint4(F::pack2(p[n][0][0], p[n][0][1]), F::pack2(p[n][0][2], p[n][0][3]),
-                           F::pack2(p[n][1][0], p[n][1][1]), F::pack2(p[n][1][2], p[n][1][3]));
+        weight_words<F>(pb[n], [&](int e) { return p[n][e >> 2][e & 3]; });
 #pragma unroll
       for (int j = 0; j < VE; ++j) {
         const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
@@ -189,8 +189,11 @@ struct Wave {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           w[e] = __builtin_amdgcn_perm(x.w[e >> 1][2 * (e & 1) + 1][j >> 1], x.w[e >> 1][2 * (e & 1)][j >> 1], sel);
+        const uint4 v = make_uint4(w[0], w[1], w[2], w[3]);
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) acc[n][j] = mfma32<F>(make_uint4(w[0], w[1], w[2], w[3]), pb[n], acc[n][j]);
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int t = kTerms - 1; t >= 0; --t) acc[n][j] = mfma32<F>(v, pb[n][t], acc[n][j]);  // the smallest first
       }
     }
   }
@@ -274,6 +277,7 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
     for (int j = 0; j < VE; ++j) acc[n][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
   const float unit = sizeof(T) == 4 ? a.scale : a.scale * kLog2e;
+  constexpr float lift = sizeof(T) == 4 ? 0.f : kLift<typename W::F>;
 
   int ids = key_of(lane) < k_hi ? first_ids : -1, ids_from = 0;
   const int size_mask = (1 << a.pg.log_size) - 1;
@@ -341,7 +345,7 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p = exp_of<T>(fmaf(s[n][t][i], unit, -m0));
+          const float p = exp_of<T>(fmaf(s[n][t][i], unit, lift - m0));
           s[n][t][i] = p;
           sum[n] += p;
         }

@@ -136,8 +136,9 @@ __device__ __forceinline__ bf16x8_t finite_part(const bf16x8_t& x) {
   return __builtin_bit_cast(bf16x8_t, w);
 }
 
-// O^T += V^T . P^T of one step; vf: the fragments of V^T for its first 16
-// keys, read ahead as the others are here.  ODD: infinities and NaN left out.
+// O^T += V^T . P^T of one step, each weight as two terms (weight_terms); vf: the
+// fragments of V^T for its first 16 keys, read ahead as the others are here.
+// ODD: infinities and NaN left out.
 template <typename F, int HD, bool ODD>
 __device__ __forceinline__ void step_sum(f32x16_t (&o)[HD / 32], const f32x16_t (&s)[2], bf16x8_t (&vf)[2][HD / 32],
                                          const TileOffsets<HD>& to, const char* vt) {
@@ -146,10 +147,13 @@ __device__ __forceinline__ void step_sum(f32x16_t (&o)[HD / 32], const f32x16_t 
     if (ks + 1 < 4)
 #pragma unroll
       for (int i = 0; i < HD / 32; ++i) vf[(ks + 1) & 1][i] = to.frag_t(vt, ks + 1, i);
-    const bf16x8_t pb = pack8<F>(s[ks >> 1], 8 * (ks & 1));
+    uint4 pb[2];
+    weight_words<F>(pb, [&](int e) { return s[ks >> 1][8 * (ks & 1) + e]; });
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i)
-      o[i] = mfma16<F>(ODD ? finite_part<F>(vf[ks & 1][i]) : vf[ks & 1][i], pb, o[i]);
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i)
+        o[i] = mfma16<F>(ODD ? finite_part<F>(vf[ks & 1][i]) : vf[ks & 1][i], __builtin_bit_cast(bf16x8_t, pb[t]), o[i]);
   }
 }
 
@@ -187,7 +191,7 @@ __device__ __forceinline__ void step_softmax(f32x16_t (&s)[2], f32x16_t (&o)[HD 
       for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
     m = m_new;
   }
-  const float nm = m == -INFINITY ? 0.f : -m;
+  const float nm = kLift<F> - (m == -INFINITY ? 0.f : m);
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll

@@ -1,0 +1,69 @@
+"""Generation from a paged key/value cache: what random steps do not reach.
+
+Tolerances count roundings, as in test_gpu_generation.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from lzhip import ops
+from test_gpu_generation import BF16, DEV, F16, MUCH, U32, Case, _u
+
+pytestmark = pytest.mark.gpu
+
+
+def _attention(c, q, H, scale, weights, terms):
+    """(o, bound) in float64: the output rounded to the type once, each weight
+    off by `weights` of it, sums of `terms` terms a key in fp32."""
+    q = q.double().view(-1, H, c.hd)
+    o, tol = torch.zeros_like(q), torch.zeros_like(q)
+    for b, (n, l) in enumerate(c.seqs):
+        k, v = c.tokens(0, b), c.tokens(1, b)
+        for i in range(n):
+            seen, r = l - n + i + 1, c.starts[b] + i
+            for h in range(H):
+                g = h // (H // c.KV)
+                p = torch.softmax(k[:seen, g] @ q[r, h] * scale, 0)
+                size = float((k[:seen, g].abs() @ q[r, h].abs()).max()) * scale
+                o[r, h] = p @ v[:seen, g]
+                # a score is hd products and adds and a few units of the
+                # exponent's argument
+                fp32 = (2 * (c.hd + 4) * size + 8 + terms * seen) * U32
+                tol[r, h] = _u(c.dtype) * o[r, h].abs() + (weights + fp32) * (p @ v[:seen, g].abs())
+    return o.view(-1, H * c.hd), tol.view(-1, H * c.hd)
+
+
+@pytest.mark.parametrize("dtype,e4m3", [(BF16, False), (F16, False), (BF16, True), (F16, True)])
+@pytest.mark.parametrize("seqs,H,KV,hd,page", [
+    ([(1, 900), (1, 40)], 8, 4, 64, 32),  # single tokens, one in parts
+    ([(1, 300)] * 3, 16, 8, 128, 16),
+    ([(15, 700), (3, 3)], 10, 2, 32, 16),  # short chunks
+    ([(40, 333)], 6, 2, 64, 64),
+])
+def test_weights_of_few_rows_keep_their_fp32_bits(seqs, H, KV, hd, page, dtype, e4m3):
+    """Single tokens and short chunks: the only rounding to the type is the
+    output's.  A weight enters the second product as two or three terms that
+    add up to it (in fp16 to u^2 of it)."""
+    c = Case(seqs, KV, hd, page, dtype, e4m3, seed=hd)
+    q = torch.randn(c.rows, H * hd, generator=c.g).to(dtype)
+    got = ops.paged_attention(q.to(DEV), c.layer, c.step, H, hd**-0.5).cpu().double()
+    want, tol = _attention(c, q, H, hd**-0.5, weights=_u(F16) ** 2 if dtype == F16 else 0.0, terms=3)
+    assert float(((got - want).abs() - tol).max()) <= 0
+
+
+@pytest.mark.parametrize("dtype,e4m3", [(BF16, False), (F16, False), (BF16, True), (F16, True)])
+@pytest.mark.parametrize("seqs,H,KV,hd,page", [
+    ([(150, 300), (70, 90)], 8, 2, 64, 32),
+    ([(129, 129)], 4, 4, 128, 16),
+    ([(200, 1000)], 5, 1, 32, 64),
+])
+def test_weights_of_tiles_keep_sixteen_bits(seqs, H, KV, hd, page, dtype, e4m3):
+    """Chunks in 128-row tiles: a weight 2^e (1 <= x < 2) is two terms, x cut to
+    the type (the rest is below 2 u) and the rest rounded (off by u of what is
+    below 2 u, so by u^2 2^e: half a step of the rest's)."""
+    c = Case(seqs, KV, hd, page, dtype, e4m3, seed=hd, most=MUCH)
+    q = torch.randn(c.rows, H * hd, generator=c.g).to(dtype)
+    got = ops.paged_attention(q.to(DEV), c.layer, c.step, H, hd**-0.5).cpu().double()
+    want, tol = _attention(c, q, H, hd**-0.5, weights=_u(dtype) ** 2, terms=2)
+    assert float(((got - want).abs() - tol).max()) <= 0
