@@ -55,24 +55,24 @@ struct PagedPlace {
 // Rows m0 .. m0 + BM - 1 of a pair's packed rows and the keys that they see:
 // row m's are 0 .. sees(m) - 1.
 struct PagedRows {
-  int m0, count;  // count: rows of the pair (0 or less: none)
+  int m0, count;  // count: rows of the pair
   int row0, base, G, cap;
-  __device__ __forceinline__ PagedRows(const PagedArgs& a, int b, int m0_)
+  __host__ __device__ __forceinline__ PagedRows(const PagedArgs& a, int b, int m0_)
       : PagedRows(a, a.row_start[b], a.row_start[b + 1], a.kv_len[b], m0_) {}
   // of a sequence whose rows are lo .. hi - 1, len tokens long
-  __device__ __forceinline__ PagedRows(const PagedArgs& a, int lo, int hi, int len, int m0_) {
+  __host__ __device__ __forceinline__ PagedRows(const PagedArgs& a, int lo, int hi, int len, int m0_) {
     m0 = m0_;
     G = a.H / a.KV;
-    base = len - hi + 1;  // keys that row r of q sees: base + r
-    row0 = max(lo, 0);
-    count = hi > row0 ? (min(hi, a.rows) - row0) * G : 0;
+    base = (int)((uint32_t)len - (uint32_t)hi + 1u);  // keys that row r of q sees: base + r
+    row0 = min(max(lo, 0), a.rows);  // both ends inside the call before the product
+    count = (min(max(hi, row0), a.rows) - row0) * G;
     cap = a.pg.width << a.pg.log_size;
   }
-  __device__ __forceinline__ int row(int m) const { return row0 + m / G; }
-  __device__ __forceinline__ int sees(int m) const { return min(max(base + row(m), 0), cap); }
+  __host__ __device__ __forceinline__ int row(int m) const { return row0 + m / G; }
+  __host__ __device__ __forceinline__ int sees(int m) const { return min(max((int)((uint32_t)base + (uint32_t)row(m)), 0), cap); }
   // the keys that the block's rows see together, and the parts they make
-  __device__ __forceinline__ int keys(int bm) const { return sees(min(m0 + bm, count) - 1); }
-  static __device__ __forceinline__ int parts(const PagedArgs& a, int keys) {
+  __host__ __device__ __forceinline__ int keys(int bm) const { return sees(min(m0 + bm, count) - 1); }
+  static __host__ __device__ __forceinline__ int parts(const PagedArgs& a, int keys) {
     return min(max((int)(((uint32_t)keys + (uint32_t)a.chunk - 1) / (uint32_t)a.chunk), 1), a.nsplit);
   }
 };

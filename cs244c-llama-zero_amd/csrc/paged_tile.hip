@@ -261,16 +261,16 @@ struct ByLength {
     const int G = a.H / a.KV, cap = a.pg.width << a.pg.log_size;
     if (lane < a.B) {
       const PagedRows rw(a, lane, 0);
-      count = max(rw.count, 0);
-      base = rw.base + rw.row0;  // keys that the sequence's first row sees
+      count = rw.count;
+      base = (int)((uint32_t)rw.base + (uint32_t)rw.row0);  // keys that the sequence's first row sees
       nq = (count + BM - 1) / BM;
     }
     // this lane's first block with more than 64 s keys, nq: none; -1: all blocks
     auto first = [&](int s) {
-      const int t = 64 * s + 1;
+      const uint32_t t = 64u * (uint32_t)s + 1u;
       if (s < 0) return 0;
-      const int d = t - base;  // token of its first row that sees t keys
-      if (t > cap || nq == 0 || d > (count - 1) / G) return nq;
+      const int d = (int)(t - (uint32_t)base);  // token of its first row that sees t keys
+      if (t > (uint32_t)cap || nq == 0 || d > (count - 1) / G) return nq;
       return max(d, 0) * G / BM;
     };
     b = -1;

@@ -67,3 +67,16 @@ def test_weights_of_tiles_keep_sixteen_bits(seqs, H, KV, hd, page, dtype, e4m3):
     got = ops.paged_attention(q.to(DEV), c.layer, c.step, H, hd**-0.5).cpu().double()
     want, tol = _attention(c, q, H, hd**-0.5, weights=_u(dtype) ** 2, terms=2)
     assert float(((got - want).abs() - tol).max()) <= 0
+
+
+@pytest.mark.parametrize("most", [0, MUCH])
+def test_starts_past_the_last_row(most):
+    """Sequences whose rows the tables put far behind the call's: nothing is
+    computed for them, the others are as ever."""
+    c = Case([(80, 100), (5, 30), (9, 9)], 2, 64, 16, BF16, most=most)
+    q = torch.randn(c.rows, 16 * 64, generator=c.g).to(BF16).to(DEV)
+    want = ops.paged_attention(q, c.layer, c.step, 16, 0.125)
+    start = torch.tensor([0, 80, 10**9, 2 * 10**9], dtype=torch.int32, device=DEV)
+    out = torch.full_like(q, 7.0)
+    ops.paged_attention(q, c.layer, c.step._replace(row_start=start), 16, 0.125, out=out)
+    assert torch.equal(out[:80], want[:80])
