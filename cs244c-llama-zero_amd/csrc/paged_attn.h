@@ -77,6 +77,18 @@ struct PagedRows {
   }
 };
 
+// Whether a row that sees `sees` keys sees one of k_lo .. k_hi - 1 (of pages
+// that there are).  A maximum of -inf says that it does not or that all its
+// scores are -inf: the former's output is zeros, the latter's NaN (0 / 0).  The
+// latter's maximum is kept as kAllInf, beside which any finite score takes all
+// the weight.
+constexpr float kAllInf = -3.402823466e38f;
+__device__ __forceinline__ bool sees_any(const PagedArgs& a, int b, int k_lo, int k_hi, int sees) {
+  for (int key = k_lo; key < min(k_hi, sees); key += 16)
+    if (a.pg.page_of(b, key) >= 0) return true;
+  return false;
+}
+
 // A row's reference m for its weights 2^(s - m) (log2 units) is its running
 // maximum, but moves only when that is more than kSlack above it: weights up to
 // 2^8 are as exact in 16 and 32 bits as those up to 1, and the sums are

@@ -445,9 +445,10 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
       y.z = fmaf(f, z.z, y.z);
       y.w = fmaf(f, z.w, y.w);
     }
+    if (top == -INFINITY && sees_any(a, at.b, k_lo, k_hi, rw.sees(m))) top = kAllInf;
     const int row = rw.row(m), head = at.g * rw.G + m % rw.G;
     if (n_parts == 1) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = top == -INFINITY ? 0.f : 1.f / l;
       store_row4<T, HD>(a, row, head, d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
     } else {
       const int64_t at_row = ((int64_t)row * a.H + head) * a.nsplit + at.split;
@@ -510,7 +511,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm, in
   float top = -INFINITY, l = 0.f;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](const float4& v, const float2& t) {
-    if (t.x == -INFINITY && t.y == 0.f) return;  // saw nothing
+    if (t.x == -INFINITY) return;  // saw nothing
     const float m_new = fmaxf(top, t.x);
     const float f = m_new == top ? 1.f : exp_of<T>(top - m_new), e = m_new == t.x ? 1.f : exp_of<T>(t.x - m_new);
     top = m_new;
@@ -537,7 +538,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm, in
     y = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i = 0; i < per; ++i) {
       const int at = tid + i * kLanes;
-      if (ms[at] == -INFINITY && ls[at] == 0.f) continue;
+      if (ms[at] == -INFINITY) continue;
       const float e = ms[at] == top ? 1.f : exp_of<T>(ms[at] - top);
       const float4 z = ys[at];
       l = fmaf(e, ls[at], l);
@@ -548,7 +549,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm, in
     }
   }
   if (n_parts == 0) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = top == -INFINITY ? 0.f : 1.f / l;
   store_row4<T, HD>(a, row, head, d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
 }
 

@@ -449,8 +449,9 @@ paged_tile_kernel(PagedArgs a) {
       for (int r = 0; r < 16; ++r) o[i][r] = fmaf(o[i][r], f, park[(16 * i + r) * 64] * f2);
   }
   if (m_first + l32 >= rw.count) return;
+  if (mx == -INFINITY && sees_any(a, at.b, k_lo, k_hi, sees)) mx = kAllInf;
   if (n_parts == 1) {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = mx == -INFINITY ? 0.f : 1.f / l;
     uint16_t* op = static_cast<uint16_t*>(a.o) + (int64_t)row * a.ldo + head * HD;
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i)

@@ -1239,7 +1239,8 @@ def paged_attention(q: torch.Tensor, layer, step, n_heads: int, scale: float,
     """Attention of a step's rotated queries [rows, n_heads * hd] over the
     cached keys and values of their sequences (a step's own tokens included:
     kv_cache_write comes first); causal within the new tokens; scale > 0.  A
-    row that sees nothing is zero.  out: rows for the result (those of no sequence are
+    row that sees nothing is zero, one whose scores are all -inf is NaN, as a
+    softmax of them.  out: rows for the result (those of no sequence are
     left as they are; new ones are zeros there); it may be q itself."""
     return _lib.tensor_calls().paged_attention(q, layer, step, n_heads, scale, out)
 

@@ -424,7 +424,7 @@ int lz_kv_read(const void* k, const void* v, const void* k_exp, const void* v_ex
 /* Attention of a step's rows (q rows of H heads, rotated; kv head h / (H/KV))
  * over their sequences' cached keys and values, their own tokens' included:
  * the i-th of `new` rows sees positions 0 .. kv_len - new + i.  A row that
- * sees nothing comes out as zeros.  max_new and max_len: at least the largest
+ * sees nothing comes out as zeros, one whose scores are all -inf as NaN.  max_new and max_len: at least the largest
  * number of new tokens and of cached ones (max_new sizes the grid: rows past
  * it would be left; max_len only how the work is split).  scale: positive, a
  * normal number.  o may be q (rows and stride alike).  workspace:

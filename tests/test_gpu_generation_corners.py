@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from lzhip import ops
-from test_gpu_generation import BF16, DEV, F16, MUCH, U32, Case, _u
+from test_gpu_generation import BF16, DEV, F16, F32, MUCH, U32, Case, _u
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +80,56 @@ def test_starts_past_the_last_row(most):
     out = torch.full_like(q, 7.0)
     ops.paged_attention(q, c.layer, c.step._replace(row_start=start), 16, 0.125, out=out)
     assert torch.equal(out[:80], want[:80])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n,length,most", [(1, 40, 0), (1, 3000, 0), (20, 90, 0), (20, 2500, 0), (90, 300, MUCH), (130, 3000, MUCH)])
+def test_scores_of_minus_infinity(dtype, n, length, most):
+    """A row that sees keys whose scores are all -inf is NaN, as a softmax is;
+    one that sees others too gives them all the weight; one that sees no key
+    (or none with a page) is zeros."""
+    H, KV, hd, page = 4, 2, 64, 16
+    seqs = [(n, length), (n, length), (n, n + 20), (n, length)]
+    c = Case(seqs, KV, hd, page, dtype, seed=length, most=most)
+    q = torch.randn(c.rows, H * hd, generator=c.g)
+    q.view(-1, H, hd)[..., 5] = 1.0 + q.view(-1, H, hd)[..., 5].abs()
+    q = q.to(dtype)
+    k = c.cpu[0]
+    low = [length, length - n // 2 - 1, 0, length]  # of each sequence, the first tokens whose keys overflowed (kv head 1)
+    for b, m in enumerate(low):
+        p = torch.arange(m)
+        k[c.table[b, p // page].long(), 1, p % page, 5] = -float("inf")
+    c.layer.k.copy_(k)
+    table = c.table.clone()
+    table[2] = -1  # no page at all
+    table[3, : (length - n) // page] = 10**6  # pages of the last tokens alone
+    step = c.step._replace(page_table=table.to(DEV))
+    got = ops.paged_attention(q.to(DEV), c.layer, step, H, 0.125).cpu().view(-1, H, hd)
+    own = got[: c.starts[2]].view(2, n, H, hd)
+    assert bool(torch.isfinite(own[:, :, :2]).all())
+    assert bool(torch.isnan(own[0, :, 2:]).all())
+    assert bool((got[c.starts[2] : c.starts[3]] == 0).all())
+    assert bool(torch.isnan(got[c.starts[3] :][:, 2:]).all()) and bool(torch.isfinite(got[c.starts[3] :][:, :2]).all())
+    kk, vv = c.tokens(0, 1)[:, 1], c.tokens(1, 1)[:, 1]
+    for i in range(n):
+        seen = length - n + i + 1
+        for h in (2, 3):
+            x = q[c.starts[1] + i].view(H, hd)[h].double()
+            if seen <= low[1]:
+                assert bool(torch.isnan(own[1, i, h]).all()), i
+                continue
+            keys, vals = kk[low[1] : seen], vv[low[1] : seen]
+            p = torch.softmax(keys @ x * 0.125, 0)
+            size = float((keys.abs() @ x.abs()).max()) * 0.125
+            tol = _u(dtype) * (p @ vals).abs() + (_u(dtype) ** 2 + (2 * (hd + 4) * size + 8 + 3 * len(p)) * U32) * (p @ vals.abs())
+            assert bool(((own[1, i, h].double() - p @ vals).abs() <= tol).all()), (i, h)
+
+
+def test_no_key_at_all_beside_scores_of_minus_infinity():
+    """Rows before a sequence's first token are zeros, those after it NaN."""
+    c = Case([(6, 6)], 1, 32, 16, F32)
+    c.layer.k[..., 0] = -float("inf")
+    q = torch.ones(6, 32, device=DEV)
+    step = c.step._replace(kv_len=torch.tensor([2], dtype=torch.int32, device=DEV))
+    got = ops.paged_attention(q, c.layer, step, 1, 0.5)
+    assert bool((got[:4] == 0).all()) and bool(torch.isnan(got[4:]).all())
