@@ -210,11 +210,12 @@ class SwiGLU(nn.Module):
         self.dropout = nn.Dropout(cfg.dropout)
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None,
-                compute_output: bool = True) -> torch.Tensor:
+                compute_output: bool = True, dropout: bool = True) -> torch.Tensor:
         """compute_output=False (the caller only takes gradients through the
-        result): the down projection's product is left uncomputed."""
+        result): the down projection's product is left uncomputed.
+        dropout=False: none, in training mode too."""
         ops.require_gpu(x)
-        p = float(self.dropout.p) if self.training else 0.0  # nn.Dropout on the gated activations
+        p = float(self.dropout.p) if self.training and dropout else 0.0  # nn.Dropout on the gated activations
         seed = ops.dropout_seed(x.device) if p > 0.0 else 0
         return LF.MLPFn.apply(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight, residual,
                               torch.is_grad_enabled(), p, seed, compute_output)
@@ -243,11 +244,7 @@ class TransformerBlock(nn.Module):
         """forward() for a step's new tokens [rows, dim] over a cache (no
         gradients, no dropout)."""
         x = self.attn.forward_cached(self.input_norm(x), layer, step, residual=x)
-        training, self.mlp.training = self.mlp.training, False
-        try:
-            return self.mlp(self.post_attn_norm(x), residual=x)
-        finally:
-            self.mlp.training = training
+        return self.mlp(self.post_attn_norm(x), residual=x, dropout=False)
 
 
 @dataclass
