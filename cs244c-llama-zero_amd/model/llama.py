@@ -36,6 +36,24 @@ def _next_token(logits: torch.Tensor, temperature: float, top_k: Optional[int]) 
     return torch.multinomial(torch.softmax(scaled, dim=-1), num_samples=1).squeeze(-1)
 
 
+def _require_choice(logits: torch.Tensor, t: int, temperature: float) -> None:
+    """Refuses adjusted logits that leave a row no token t to choose (sampling
+    from such a row would end the process).  Waits for the device."""
+    top = logits.amax(-1)
+    fine = top > float("-inf")  # not for NaN
+    if temperature > 0:
+        fine &= top < float("inf")
+    if bool(fine.all()):
+        return
+    if bool(top.isnan().any()):
+        why = "a row's logits hold NaN"
+    elif bool((top == float("-inf")).any()):
+        why = "token_mask or logit_bias allows a row no token"
+    else:
+        why = "a row's largest logit is infinite: it can be chosen (temperature 0) but not sampled"
+    raise ValueError(f"token {t}: {why}")
+
+
 class HipLinear(nn.Linear):
     """nn.Linear (same parameters, initialisation and state_dict) whose
     forward is the MFMA GEMM; bias is not supported (the model has none)."""
@@ -439,7 +457,9 @@ class LlamaForCausalLM(nn.Module):
         penalties, logit_bias and token_mask (a mask, or a function that makes
         one of the [B, t] tokens so far) adjust the logits first, as
         ops.process_logits says, the prompt counting for repetition_penalty
-        alone; where they leave a row no token, that is a ValueError."""
+        alone.  They are then looked at, for which the host waits for the
+        device: a row without a token to choose (all -inf, or NaN; infinite
+        where a token is sampled) is a ValueError."""
         if cache_dtype is not None and not use_cache:
             raise ValueError("cache_dtype is for use_cache=True")
         self.eval()
@@ -467,8 +487,6 @@ class LlamaForCausalLM(nn.Module):
                     last, tokens=seq[:, :t], prompt_lengths=prompts, repetition_penalty=repetition_penalty,
                     presence_penalty=presence_penalty, frequency_penalty=frequency_penalty, bias=logit_bias,
                     mask=token_mask(seq[:, :t]) if callable(token_mask) else token_mask)
-                if not bool(torch.isfinite(last.amax(-1)).all()):  # sampling from such a row would end the process
-                    raise ValueError(f"token {t}: the largest logit of a row is not finite (does token_mask or "
-                                     "logit_bias allow it no token?)")
+                _require_choice(last, t, temperature)
             seq[:, t] = _next_token(last.float(), temperature, top_k)
         return seq

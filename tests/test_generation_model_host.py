@@ -34,3 +34,46 @@ def test_a_cached_block_leaves_the_modes_alone(monkeypatch):
     x = torch.ones(3, 64)
     assert block.forward_cached(x, None, None) is x
     assert seen == [(True, 0.0)] and block.mlp.training
+
+
+class Fixed(LlamaForCausalLM):
+    """A model whose last logits are given."""
+
+    def __init__(self, rows):
+        super().__init__(_config(dropout=0.0, vocab_size=len(rows[0])))
+        self.rows = torch.tensor(rows)
+
+    def forward(self, ids):
+        return type("Out", (), {"logits": self.rows[:, None].expand(-1, ids.shape[1], -1)})
+
+
+@pytest.fixture
+def plain_adjustments(monkeypatch):
+    """process_logits' bias and mask on the CPU."""
+    def process(x, *, bias=None, mask=None, **_):
+        x = x.float() if bias is None else x.float() + bias
+        return x if mask is None else x.masked_fill(~mask, -float("inf"))
+
+    monkeypatch.setattr(ops, "process_logits", process)
+
+
+def test_an_infinite_bias_forces_a_token(plain_adjustments):
+    model = Fixed([[0.0, 1.0, 2.0, 3.0], [3.0, 2.0, 1.0, 0.0]])
+    bias = torch.tensor([0.0, float("inf"), 0.0, 0.0])
+    ids = torch.zeros(2, 3, dtype=torch.int64)
+    assert model.generate(ids, 2, temperature=0.0, logit_bias=bias)[:, 3:].tolist() == [[1, 1], [1, 1]]
+    # there is no distribution to sample from
+    with pytest.raises(ValueError, match="token 3.*infinite"):
+        model.generate(ids, 2, temperature=1.0, logit_bias=bias)
+
+
+def test_rows_without_a_token_are_refused(plain_adjustments):
+    model = Fixed([[0.0, 1.0, 2.0, 3.0], [3.0, 2.0, 1.0, 0.0]])
+    ids = torch.zeros(2, 3, dtype=torch.int64)
+    mask = torch.ones(2, 4, dtype=torch.bool)
+    mask[1] = False
+    for how in (dict(temperature=0.0), dict(temperature=1.0, top_k=2)):
+        with pytest.raises(ValueError, match="token 3.*no token"):
+            model.generate(ids, 2, token_mask=mask, **how)
+        with pytest.raises(ValueError, match="token 3.*NaN"):
+            model.generate(ids, 2, logit_bias=torch.tensor([0.0, float("nan"), 0.0, 0.0]), **how)
