@@ -167,7 +167,7 @@ SIGNATURES = {
 _lock = threading.Lock()
 _lib = None
 _calls = {}  # entry point name -> its _pycall callable, filled when the library is loaded
-torchcall = None  # the _torchcall extension, bound when the library is loaded
+torchcall = None  # the _torchcall extension, bound when tensor_calls() is first called
 
 
 class HipLibraryError(RuntimeError):
@@ -176,7 +176,7 @@ class HipLibraryError(RuntimeError):
 
 def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
     """Loads (once) and returns the library with its signatures applied."""
-    global _lib, torchcall
+    global _lib
     if _lib is not None:  # set once, complete, under the lock
         return _lib
     with _lock:
@@ -190,9 +190,8 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
             )
         try:
             from . import _pycall as pycall
-            from . import _torchcall
         except ImportError as e:
-            raise HipLibraryError(f"lzhip/_pycall.so or lzhip/_torchcall.so is missing ({e}): build them with "
+            raise HipLibraryError(f"lzhip/_pycall.so is missing ({e}): build it with "
                                   "`python cs244c-llama-zero_amd/csrc/build.py`") from e
         lib = ctypes.CDLL(str(p), mode=ctypes.RTLD_GLOBAL)
         for name, (res, args) in SIGNATURES.items():
@@ -201,10 +200,6 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
             fn.argtypes = args
             if res is not ctypes.c_char_p:
                 _calls[name] = pycall.bind(name, ctypes.cast(fn, _vp).value)
-        _torchcall.bind({name: ctypes.cast(getattr(lib, name), _vp).value for name in SIGNATURES},
-                        getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None),
-                        getattr(torch._C, "_cuda_setDevice", None), HipLibraryError)
-        torchcall = _torchcall
         _lib = lib
         return lib
 
@@ -236,7 +231,23 @@ def query(name: str, *args) -> int:
 
 
 def tensor_calls():
-    """The _torchcall extension (its functions take tensors)."""
-    if torchcall is None:
-        load()
+    """The _torchcall extension (its functions take tensors), which is tied to
+    torch's C++ interface and loaded when generation first asks for it: nothing
+    else needs it."""
+    global torchcall
+    if torchcall is not None:
+        return torchcall
+    lib = load()
+    with _lock:
+        if torchcall is None:
+            try:
+                from . import _torchcall
+            except ImportError as e:
+                raise HipLibraryError(f"lzhip/_torchcall.so is missing or of another torch ({e}): build it with "
+                                      "`python cs244c-llama-zero_amd/csrc/build.py`") from e
+            _torchcall.bind({name: ctypes.cast(getattr(lib, name), _vp).value for name in SIGNATURES},
+                            getattr(torch._C, "_cuda_getCurrentRawStream", None),
+                            getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_setDevice", None),
+                            HipLibraryError)
+            torchcall = _torchcall
     return torchcall
