@@ -413,9 +413,9 @@ class LlamaForCausalLM(nn.Module):
         new tokens, sequence after sequence ([rows] int64); step: what
         cache.step(counts) returned for them.  Without dropout, whatever the
         mode.  The row of a sequence that has no new tokens says nothing."""
-        if self._zero3_executor is not None:
+        if self._zero3_executor is not None and not getattr(self._zero3_executor, "params_materialized", False):
             raise RuntimeError("a ZeRO-3 sharded model has no cached forward: gather its parameters first "
-                               "(summon_full_params) or generate without use_cache")
+                               "(summon_full_params; a forward within it hands them back) or generate without use_cache")
         if ids.dim() != 1 or ids.numel() != step.rows:
             raise ValueError(f"ids should hold the step's {step.rows} tokens, got shape {tuple(ids.shape)}")
         if step.rows == 0:

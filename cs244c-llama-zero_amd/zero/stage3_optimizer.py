@@ -495,6 +495,12 @@ class ZeROStage3Optimizer:
         for h in self._handle_order:
             h.reshard()
 
+    @property
+    def params_materialized(self) -> bool:
+        """Whether every parameter is whole now (within summon_full_params until
+        a module is called, always with recompute=False)."""
+        return all(h.materialized for h in self._handle_order)
+
     @contextmanager
     def summon_full_params(self) -> Iterator[nn.Module]:
         self._summon_depth += 1

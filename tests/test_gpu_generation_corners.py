@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from lzhip import ops
-from test_gpu_generation import BF16, DEV, F16, F32, MUCH, U32, Case, _u
+from test_gpu_generation import BF16, DEV, F16, F32, MUCH, U32, Case, _model, _u
 
 pytestmark = pytest.mark.gpu
 
@@ -133,3 +133,26 @@ def test_no_key_at_all_beside_scores_of_minus_infinity():
     step = c.step._replace(kv_len=torch.tensor([2], dtype=torch.int32, device=DEV))
     got = ops.paged_attention(q, c.layer, step, 1, 0.5)
     assert bool((got[:4] == 0).all()) and bool(torch.isnan(got[4:]).all())
+
+
+@pytest.mark.parametrize("recompute", [True, False])
+def test_a_sharded_model_generates_from_a_cache_where_its_parameters_are_gathered(recompute):
+    """As the refusal of a ZeRO-3 model says: within summon_full_params, and
+    at all times where the engine keeps the parameters."""
+    from zero import ZeROStage3Optimizer
+
+    ids = torch.randint(0, 500, (2, 7), generator=torch.Generator().manual_seed(1)).to(DEV)
+    want = _model(BF16).generate(ids, 3, temperature=0.0, use_cache=True)
+    model = _model(BF16)
+    engine = ZeROStage3Optimizer(model=model, lr=1e-3, recompute=recompute)
+    if recompute:
+        with pytest.raises(RuntimeError, match="summon_full_params"):
+            model.generate(ids, 3, temperature=0.0, use_cache=True)
+    with engine.summon_full_params():
+        assert torch.equal(model.generate(ids, 3, temperature=0.0, use_cache=True), want)
+        assert model.generate(ids, 3, temperature=0.0).shape == (2, 10)
+        if recompute:  # a forward of its own hands each module's parameters back
+            with pytest.raises(RuntimeError, match="summon_full_params"):
+                model.generate(ids, 3, temperature=0.0, use_cache=True)
+    if not recompute:
+        assert torch.equal(model.generate(ids, 3, temperature=0.0, use_cache=True), want)
