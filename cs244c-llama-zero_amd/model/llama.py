@@ -152,16 +152,19 @@ class RotaryEmbedding(nn.Module):
             self._build_cache(seq_len=seq_len, device=device, dtype=dtype)
         return self.cos_cached[:, :, :seq_len, :], self.sin_cached[:, :, :seq_len, :]
 
-    def tables(self, seq_len: int, device: torch.device, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+    def tables(self, seq_len: int, device: torch.device, dtype: torch.dtype, block: int = 1
+               ) -> Tuple[torch.Tensor, torch.Tensor]:
         """[S, hd] views of the cache for the fused kernels (of what forward()
-        returns where that is replaced)."""
+        returns where that is replaced).  A position's rotation does not depend
+        on the table's length: with block > 1 the cache grows to multiples of
+        it, so that a growing sequence rarely rebuilds it."""
         forward = self.forward
         if getattr(forward, "__func__", None) is not RotaryEmbedding.forward:
             cos, sin = forward(seq_len, device, dtype)
             return cos.reshape(-1, self.dim), sin.reshape(-1, self.dim)
         cos, sin = self.cos_cached, self.sin_cached
         if seq_len > self.max_seq_len_cached or cos.device != device or cos.dtype != dtype:
-            self._build_cache(seq_len=seq_len, device=device, dtype=dtype)
+            self._build_cache(seq_len=-(-seq_len // block) * block, device=device, dtype=dtype)
             cos, sin = self.cos_cached, self.sin_cached
         return cos.view(-1, self.dim).narrow(0, 0, seq_len), sin.view(-1, self.dim).narrow(0, 0, seq_len)
 
@@ -212,9 +215,7 @@ class GroupedQueryAttention(nn.Module):
         gradients, no dropout)."""
         ops.require_gpu(x)
         qkv = ops.gemm(x, LF.fused_weight([self.q_proj.weight, self.k_proj.weight, self.v_proj.weight]))
-        # a position's rotation does not depend on the table's length: whole
-        # blocks, so that a growing sequence rarely rebuilds it
-        cos, sin = self.rotary.tables(-(-step.max_len // 256) * 256, x.device, x.dtype)
+        cos, sin = self.rotary.tables(step.max_len, x.device, x.dtype, block=256)
         q = ops.kv_cache_write(qkv, layer, step, self.n_heads, cos, sin)
         return self.o_proj(ops.paged_attention(q, layer, step, self.n_heads, float(self.scale)), residual)
 

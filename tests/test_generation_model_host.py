@@ -77,3 +77,43 @@ def test_rows_without_a_token_are_refused(plain_adjustments):
             model.generate(ids, 2, token_mask=mask, **how)
         with pytest.raises(ValueError, match="token 3.*NaN"):
             model.generate(ids, 2, logit_bias=torch.tensor([0.0, float("nan"), 0.0, 0.0]), **how)
+
+
+def _cached_attention(monkeypatch, attn):
+    """attn.forward_cached with its kernels replaced: the tables of each call."""
+    tables = []
+
+    def write(qkv, layer, step, heads, cos, sin, out=None):
+        tables.append((cos, sin))
+        return qkv[:, : heads * 32]
+
+    monkeypatch.setattr(ops, "require_gpu", lambda *t: None)
+    monkeypatch.setattr(ops, "gemm", lambda x, w: x.new_zeros(x.shape[0], w.shape[0]))
+    monkeypatch.setattr(ops, "copy2d", lambda a, b: b.copy_(a))
+    monkeypatch.setattr(ops, "kv_cache_write", write)
+    monkeypatch.setattr(ops, "paged_attention", lambda q, *a: q)
+    attn.o_proj.forward = lambda y, residual=None: y
+    return tables
+
+
+def _step(max_len):
+    return CacheStep(None, None, None, 2, 1, max_len)
+
+
+def test_replaced_rotary_tables_are_asked_for_the_sequence_alone(monkeypatch):
+    """A rotary of the user's own may depend on the length or end at the
+    model's: it gets the longest sequence's, as the uncached forward gives
+    it its own."""
+    attn = LlamaForCausalLM(_config()).layers[0].attn
+    asked = []
+
+    def forward(seq_len, device, dtype):
+        asked.append(seq_len)
+        assert seq_len <= 48
+        return torch.ones(1, 1, seq_len, 32), torch.zeros(1, 1, seq_len, 32)
+
+    attn.rotary.forward = forward
+    tables = _cached_attention(monkeypatch, attn)
+    for n in (1, 7, 48):
+        attn.forward_cached(torch.ones(2, 64), None, _step(n))
+    assert asked == [1, 7, 48] and [t[0].shape for t in tables] == [(1, 32), (7, 32), (48, 32)]
