@@ -39,6 +39,11 @@ def require_gpu(*tensors: Optional[torch.Tensor]) -> None:
             )
 
 
+def capturing() -> bool:
+    """Whether the current stream records a graph."""
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
 def stream_ptr(device: Optional[torch.device] = None) -> int:
     """torch's current stream on the device (default: the current one) as a
     hipStream_t, without building a torch.cuda.Stream object for it."""

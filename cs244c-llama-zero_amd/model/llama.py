@@ -131,6 +131,7 @@ class RotaryEmbedding(nn.Module):
         inv_freq = 1.0 / (base ** (torch.arange(0, dim, 2).float() / dim))
         self.register_buffer("inv_freq", inv_freq, persistent=False)
         self.max_seq_len_cached = 0
+        self._captured = []  # tables that a captured call reads
         self.register_buffer("cos_cached", torch.empty(0), persistent=False)
         self.register_buffer("sin_cached", torch.empty(0), persistent=False)
 
@@ -143,14 +144,27 @@ class RotaryEmbedding(nn.Module):
         self.sin_cached = sin[None, None]
         self.max_seq_len_cached = seq_len
 
+    def _tables(self, seq_len: int, device: torch.device, dtype: torch.dtype, block: int = 1
+                ) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The cache, at least seq_len long.  Under capture: tables that the
+        graph keeps an address of stay, whatever replaces them in the cache;
+        what is built there (and by each replay) is the graph's alone, since it
+        holds nothing before a replay."""
+        cos, sin = self.cos_cached, self.sin_cached
+        if seq_len <= self.max_seq_len_cached and cos.device == device and cos.dtype == dtype:
+            if ops.capturing() and not any(kept is cos for kept, _ in self._captured):
+                self._captured.append((cos, sin))
+            return cos, sin
+        old = cos, sin, self.max_seq_len_cached
+        self._build_cache(seq_len=-(-seq_len // block) * block, device=device, dtype=dtype)
+        cos, sin = self.cos_cached, self.sin_cached
+        if ops.capturing():
+            self.cos_cached, self.sin_cached, self.max_seq_len_cached = old
+        return cos, sin
+
     def forward(self, seq_len: int, device: torch.device, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
-        if (
-            seq_len > self.max_seq_len_cached
-            or self.cos_cached.device != device
-            or self.cos_cached.dtype != dtype
-        ):
-            self._build_cache(seq_len=seq_len, device=device, dtype=dtype)
-        return self.cos_cached[:, :, :seq_len, :], self.sin_cached[:, :, :seq_len, :]
+        cos, sin = self._tables(seq_len, device, dtype)
+        return cos[:, :, :seq_len, :], sin[:, :, :seq_len, :]
 
     def tables(self, seq_len: int, device: torch.device, dtype: torch.dtype, block: int = 1
                ) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -162,10 +176,7 @@ class RotaryEmbedding(nn.Module):
         if getattr(forward, "__func__", None) is not RotaryEmbedding.forward:
             cos, sin = forward(seq_len, device, dtype)
             return cos.reshape(-1, self.dim), sin.reshape(-1, self.dim)
-        cos, sin = self.cos_cached, self.sin_cached
-        if seq_len > self.max_seq_len_cached or cos.device != device or cos.dtype != dtype:
-            self._build_cache(seq_len=-(-seq_len // block) * block, device=device, dtype=dtype)
-            cos, sin = self.cos_cached, self.sin_cached
+        cos, sin = self._tables(seq_len, device, dtype, block)
         return cos.view(-1, self.dim).narrow(0, 0, seq_len), sin.view(-1, self.dim).narrow(0, 0, seq_len)
 
 

@@ -117,3 +117,44 @@ def test_replaced_rotary_tables_are_asked_for_the_sequence_alone(monkeypatch):
     for n in (1, 7, 48):
         attn.forward_cached(torch.ones(2, 64), None, _step(n))
     assert asked == [1, 7, 48] and [t[0].shape for t in tables] == [(1, 32), (7, 32), (48, 32)]
+
+
+def test_rotary_tables_of_a_captured_call_stay(monkeypatch):
+    """A graph keeps the tables' addresses: they live on where an eager call
+    needs longer ones.  What is built under capture holds nothing before a
+    replay, so no other call gets it."""
+    import gc
+    import weakref
+
+    rotary = LlamaForCausalLM(_config()).layers[0].attn.rotary
+    capturing = [False]
+    monkeypatch.setattr(ops, "capturing", lambda: capturing[0])
+    monkeypatch.setattr(ops, "rope_table", lambda n, dim, inv, dtype: (torch.zeros(n, dim), torch.zeros(n, dim)))
+    cpu = torch.device("cpu")
+
+    def call(n, captured, how):
+        capturing[0] = captured
+        try:
+            return (rotary.tables if how else rotary.forward)(n, cpu, torch.float32)[0]
+        finally:
+            capturing[0] = False
+
+    for how in (True, False):
+        rotary.max_seq_len_cached = 0
+        eager = call(8, False, how).data_ptr()
+        assert call(5, True, how).data_ptr() == eager
+        kept = weakref.ref(rotary.cos_cached)
+        assert call(16, False, how).data_ptr() != eager  # grown
+        gc.collect()
+        assert kept() is not None
+        inside = call(32, True, how)
+        assert inside.shape[-2] == 32 and rotary.max_seq_len_cached == 16
+        assert call(20, False, how).data_ptr() != inside.data_ptr() and rotary.max_seq_len_cached == 20
+        assert call(8, True, how).data_ptr() == call(9, True, how).data_ptr()
+    gone = weakref.ref(rotary.cos_cached)  # in no graph: not kept
+    rotary.max_seq_len_cached = 0
+    call(8, False, True)
+    first = weakref.ref(rotary.cos_cached)
+    call(64, False, True)
+    gc.collect()
+    assert gone() is not None and first() is None

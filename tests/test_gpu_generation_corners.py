@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from lzhip import ops
+from lzhip.cache import CacheStep
 from test_gpu_generation import BF16, DEV, F16, F32, MUCH, U32, Case, _model, _u
 
 pytestmark = pytest.mark.gpu
@@ -156,3 +157,42 @@ def test_a_sharded_model_generates_from_a_cache_where_its_parameters_are_gathere
                 model.generate(ids, 3, temperature=0.0, use_cache=True)
     if not recompute:
         assert torch.equal(model.generate(ids, 3, temperature=0.0, use_cache=True), want)
+
+
+def test_a_captured_model_step_outlives_longer_eager_ones():
+    """A decoded token captured once for all layers: eager calls of longer
+    sequences, which need longer rotary tables, between its replays."""
+    model = _model(BF16, max_seq_len=600)
+    g = torch.Generator().manual_seed(3)
+    lens, most = [5, 40], 200
+    prompt = torch.randint(0, 500, (sum(lens),), generator=g).to(DEV)
+    caches = [model.new_cache(2, 256) for _ in range(2)]
+    for cache in caches:
+        model.forward_cached(prompt, cache, cache.step(lens))
+    table = caches[0].step([most - 40] * 2).page_table.clone()  # pages for what comes
+    kv = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    step = CacheStep(torch.arange(3, dtype=torch.int32, device=DEV), kv, table, 2, 1, most)
+    ids = torch.zeros(2, dtype=torch.int64, device=DEV)
+    kv += 1
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        model.forward_cached(ids, caches[0], step)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = model.forward_cached(ids, caches[0], step)
+    kv -= 1
+    for turn in range(5):
+        other = model.new_cache(1, 300 + 256 * turn)
+        model.forward_cached(torch.randint(0, 500, (260 + 256 * turn,), generator=g).to(DEV), other,
+                             other.step([260 + 256 * turn]))
+        junk = [torch.full((256 * 64,), 3.0, dtype=BF16, device=DEV) for _ in range(40)]
+        new = torch.randint(0, 500, (2,), generator=g).to(DEV)
+        ids.copy_(new)
+        kv += 1
+        graph.replay()
+        torch.cuda.synchronize()
+        s = caches[1].step([1, 1])._replace(max_len=most)  # split alike
+        assert torch.equal(out, model.forward_cached(new, caches[1], s)), turn
+        del junk
