@@ -411,7 +411,8 @@ at::Tensor row_lengths(const at::Tensor* t, const char* name, int64_t B, const P
     require_gpu(*t);
     refuse(PyExc_ValueError, "%s must be an int32 or int64 [%lld] tensor on cuda:%d", name, (long long)B, (int)at.index);
   }
-  return narrow && t->is_contiguous() ? *t : t->to(at::kInt).contiguous();
+  if (narrow) return t->contiguous();
+  return t->clamp(0, INT32_MAX).to(at::kInt).contiguous();  // a text is shorter than that
 }
 
 // Rows of `cols` of a [cols] or [B, cols] tensor: their stride, 0 for one row

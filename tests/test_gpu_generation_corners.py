@@ -196,3 +196,18 @@ def test_a_captured_model_step_outlives_longer_eager_ones():
         s = caches[1].step([1, 1])._replace(max_len=most)  # split alike
         assert torch.equal(out, model.forward_cached(new, caches[1], s)), turn
         del junk
+
+
+def test_process_logits_lengths_past_32_bits():
+    """int64 lengths larger than any text: all of it counts; prompts as long:
+    nothing is the answer."""
+    g = torch.Generator().manual_seed(4)
+    x, tokens = torch.randn(3, 50, generator=g).to(DEV), torch.randint(0, 50, (3, 9), generator=g).to(DEV)
+    far = torch.tensor([2**63 - 1, 2**32, 2**31], device=DEV)
+    how = dict(tokens=tokens, repetition_penalty=1.5, presence_penalty=2.0, frequency_penalty=0.5)
+    got = ops.process_logits(x, lengths=far, **how)
+    assert torch.equal(got, ops.process_logits(x, **how)) and not torch.equal(got, x)
+    got = ops.process_logits(x, prompt_lengths=far, **how)
+    assert torch.equal(got, ops.process_logits(x, tokens=tokens, repetition_penalty=1.5))
+    none = ops.process_logits(x, lengths=torch.tensor([-(2**63), -(2**32) + 5, -1], device=DEV), **how)
+    assert torch.equal(none, x)
