@@ -23,6 +23,7 @@ struct LzPagedArgs {
   float* part;  // [rows * H][nsplit][hd], then [rows * H][nsplit][2]: maximum and sum
   float scale;
   int rows, B, H, KV, nqb, nsplit, chunk;
+  int most;  // packed rows of a sequence that the grid is for; those behind them are left
 };
 
 // paged_tile.hip: 16-bit rows in blocks of kPagedTileRows; `groups`
@@ -55,7 +56,7 @@ struct PagedPlace {
 // Rows m0 .. m0 + BM - 1 of a pair's packed rows and the keys that they see:
 // row m's are 0 .. sees(m) - 1.
 struct PagedRows {
-  int m0, count;  // count: rows of the pair
+  int m0, count;  // count: rows of the pair that are computed
   int row0, base, G, cap;
   __host__ __device__ __forceinline__ PagedRows(const PagedArgs& a, int b, int m0_)
       : PagedRows(a, a.row_start[b], a.row_start[b + 1], a.kv_len[b], m0_) {}
@@ -65,7 +66,7 @@ struct PagedRows {
     G = a.H / a.KV;
     base = (int)((uint32_t)len - (uint32_t)hi + 1u);  // keys that row r of q sees: base + r
     row0 = min(max(lo, 0), a.rows);  // both ends inside the call before the product
-    count = (min(max(hi, row0), a.rows) - row0) * G;
+    count = min((min(max(hi, row0), a.rows) - row0) * G, a.most);
     cap = a.pg.width << a.pg.log_size;
   }
   __host__ __device__ __forceinline__ int row(int m) const { return row0 + m / G; }

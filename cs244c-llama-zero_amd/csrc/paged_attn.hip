@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm, in
       PagedRows rw(a, lo, hi, len, 0);
       const int m = (row - rw.row0) * rw.G + head % rw.G;
       rw.m0 = m / bm * bm;
-      if (m / bm < a.nqb) n_parts = PagedRows::parts(a, rw.keys(bm));
+      if (m < rw.count) n_parts = PagedRows::parts(a, rw.keys(bm));
     }
   }
   if (n_parts == 1) n_parts = 0;  // was written whole
@@ -652,7 +652,8 @@ LZ_EXPORT int lz_paged_attn(const void* q, int64_t ldq, int dtype, int64_t rows,
   LZ_REQUIRE(blocks <= INT32_MAX / 256 && joins <= INT32_MAX / 256, "lz_paged_attn: too many rows");
   PagedArgs a{q, ldq, k, v, (const int8_t*)k_exp, (const int8_t*)v_exp,
               LzPages{table, (int)width, (int)pages, lz_log2(page_size)}, row_start, kv_len, o, ldo, (float*)workspace,
-              scale, (int)rows, (int)B, (int)H, (int)KV, p.nqb, p.nsplit, p.chunk};
+              scale, (int)rows, (int)B, (int)H, (int)KV, p.nqb, p.nsplit, p.chunk,
+              (int)(std::min(max_new, rows) * (H / KV))};
   hipStream_t s = lz_stream(stream);
   const bool tiles = p.bm == kPagedTileRows;
   if (tiles)

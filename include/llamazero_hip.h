@@ -424,12 +424,12 @@ int lz_kv_read(const void* k, const void* v, const void* k_exp, const void* v_ex
 /* Attention of a step's rows (q rows of H heads, rotated; kv head h / (H/KV))
  * over their sequences' cached keys and values, their own tokens' included:
  * the i-th of `new` rows sees positions 0 .. kv_len - new + i.  A row that
- * sees nothing comes out as zeros, one whose scores are all -inf as NaN.  max_new and max_len: at least the largest
- * number of new tokens and of cached ones (max_new sizes the grid: rows past
- * it would be left; max_len only how the work is split).  scale: positive, a
- * normal number.  o may be q (rows and stride alike).  workspace:
- * lz_paged_attn_workspace bytes, 16-byte aligned, for the joined parts of
- * long sequences. */
+ * sees nothing comes out as zeros, one whose scores are all -inf as NaN.
+ * max_new and max_len: at least the largest number of new tokens and of cached
+ * ones (max_new sizes the grid: a sequence's rows past it are left; max_len
+ * only how the work is split).  scale: positive, a normal number.  o may be q
+ * (rows and stride alike).  workspace: lz_paged_attn_workspace bytes, 16-byte
+ * aligned, for the joined parts of long sequences. */
 int64_t lz_paged_attn_workspace(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd,
                                 int64_t max_new, int64_t max_len);
 int lz_paged_attn(const void* q, int64_t ldq, int dtype, int64_t rows, const void* k, const void* v, const void* k_exp,

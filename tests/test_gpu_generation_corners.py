@@ -211,3 +211,28 @@ def test_process_logits_lengths_past_32_bits():
     assert torch.equal(got, ops.process_logits(x, tokens=tokens, repetition_penalty=1.5))
     none = ops.process_logits(x, lengths=torch.tensor([-(2**63), -(2**32) + 5, -1], device=DEV), **how)
     assert torch.equal(none, x)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("seqs,bound,most", [
+    ([(200, 300), (3, 50), (1, 9)], 128, MUCH),           # tiles, in the order of their keys
+    ([(300, 2000), (3, 50), (260, 700)], 250, MUCH),
+    ([(150, 150)] + [(b % 7, 20 + b) for b in range(70)], 130, MUCH),  # tiles, sequence after sequence
+    ([(60, 80), (3, 50)], 40, 0),                         # waves
+    ([(20, 3000), (1, 50)], 12, 0),                       # in parts
+])
+def test_rows_past_max_new_are_left(seqs, bound, most, e4m3):
+    """Tables that grew past a step's bound: a sequence's first max_new rows
+    are computed, the others left as they are."""
+    c = Case(seqs, 2, 64, 16, BF16, e4m3, seed=bound, most=most)
+    c.step = c.step._replace(max_new=bound)
+    q = torch.randn(c.rows, 2 * 64, generator=c.g).to(BF16)
+    out = torch.full_like(q, 7.0).to(DEV)
+    ops.paged_attention(q.to(DEV), c.layer, c.step, 2, 0.125, out=out)
+    got = out.cpu().double()
+    want, tol = c.attention(q, 2, 0.125)
+    for b, (n, _) in enumerate(seqs):
+        lo, hi = c.starts[b], c.starts[b + 1]
+        mid = min(lo + bound, hi)
+        assert bool(((got - want).abs() <= tol)[lo:mid].all()), b
+        assert bool((got[mid:hi] == 7).all()), b
