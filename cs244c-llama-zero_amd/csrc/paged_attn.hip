@@ -617,9 +617,20 @@ Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, i
 
 }  // namespace
 
+static bool plannable(int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t max_len) {
+  return rows > 0 && B > 0 && H > 0 && KV > 0 && H % KV == 0 && max_len >= 0 && max_len <= INT32_MAX - 1024;
+}
+
+LZ_EXPORT int64_t lz_paged_attn_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV,
+                                     int64_t hd, int64_t max_new, int64_t max_len) {
+  if (!plannable(rows, B, H, KV, max_len)) return 0;
+  const Plan p = make_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
+  return p.bm | (p.bm == kPagedTileRows ? p.groups : 1) << 8 | (int64_t)p.nsplit << 16;
+}
+
 LZ_EXPORT int64_t lz_paged_attn_workspace(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV,
                                           int64_t hd, int64_t max_new, int64_t max_len) {
-  if (rows <= 0 || B <= 0 || H <= 0 || KV <= 0 || H % KV || max_len < 0 || max_len > INT32_MAX - 1024) return 0;
+  if (!plannable(rows, B, H, KV, max_len)) return 0;
   const Plan p = make_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
   return p.nsplit > 1 ? rows * H * p.nsplit * (hd + 2) * 4 : 0;
 }

@@ -137,6 +137,7 @@ Slot kSlots[] = {
     LZ_ENTRY(lz_kv_write),
     LZ_ENTRY(lz_kv_read),
     LZ_ENTRY(lz_paged_attn_workspace),
+    LZ_ENTRY(lz_paged_attn_plan),
     LZ_ENTRY(lz_paged_attn),
     LZ_ENTRY(lz_process_logits),
 };

@@ -148,6 +148,7 @@ SIGNATURES = {
         [_vp, _vp, _vp, _vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i32, _i64, _vp],
     ),
     "lz_paged_attn_workspace": (_i64, [_i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "lz_paged_attn_plan": (_i64, [_i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
     "lz_paged_attn": (
         _i32,
         [

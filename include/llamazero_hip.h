@@ -432,6 +432,11 @@ int lz_kv_read(const void* k, const void* v, const void* k_exp, const void* v_ex
  * aligned, for the joined parts of long sequences. */
 int64_t lz_paged_attn_workspace(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd,
                                 int64_t max_new, int64_t max_len);
+/* How a call is computed: packed rows of a block (16 or 32: a wave's own tiles;
+ * 128: tiles in LDS) | wave groups of a block (tiles: 1 or 2) << 8 | parts of a
+ * long sequence << 16; 0 for shapes that are refused.  Diagnostic only. */
+int64_t lz_paged_attn_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd,
+                           int64_t max_new, int64_t max_len);
 int lz_paged_attn(const void* q, int64_t ldq, int dtype, int64_t rows, const void* k, const void* v, const void* k_exp,
                   const void* v_exp, int cache_dtype, int64_t pages, int64_t page_size, const int32_t* table,
                   int64_t width, const int32_t* row_start, const int32_t* kv_len, int64_t B, int64_t H, int64_t KV,
