@@ -36,8 +36,9 @@ class CacheStep(NamedTuple):
     them), page_table [B, pages of the longest].  Host numbers: rows =
     row_start[B], and upper bounds max_new and max_len of the new and of all
     tokens of a sequence.  Tables that change under a captured call keep within
-    them: rows behind max_new of a sequence, or of none, are not computed (what
-    they hold is left, in a tensor of the call's own undefined)."""
+    them: rows behind max_new of a sequence, or of none, are not computed (the
+    caller's tensor keeps what it holds there, one of the call's own holds
+    anything but in the rows from `rows` on, which are zeros)."""
 
     row_start: torch.Tensor
     kv_len: torch.Tensor

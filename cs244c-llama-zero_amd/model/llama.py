@@ -223,7 +223,8 @@ class GroupedQueryAttention(nn.Module):
                        residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         """forward() for a step's new tokens [rows, dim], whose keys and values
         go into the layer's cache and which attend over all of it (no
-        gradients, no dropout)."""
+        gradients, no dropout; a method, so the module's own hooks do not
+        run, those of o_proj do)."""
         ops.require_gpu(x)
         qkv = ops.gemm(x, LF.fused_weight([self.q_proj.weight, self.k_proj.weight, self.v_proj.weight]))
         cos, sin = self.rotary.tables(step.max_len, x.device, x.dtype, block=256)
@@ -272,7 +273,7 @@ class TransformerBlock(nn.Module):
     @torch.no_grad()
     def forward_cached(self, x: torch.Tensor, layer: LayerCache, step: CacheStep) -> torch.Tensor:
         """forward() for a step's new tokens [rows, dim] over a cache (no
-        gradients, no dropout)."""
+        gradients, no dropout, no hooks of the block or its attention)."""
         x = self.attn.forward_cached(self.input_norm(x), layer, step, residual=x)
         return self.mlp(self.post_attn_norm(x), residual=x, dropout=False)
 
@@ -424,7 +425,8 @@ class LlamaForCausalLM(nn.Module):
         """Logits [B, V] of each sequence's last new token.  ids: the step's
         new tokens, sequence after sequence ([rows] int64); step: what
         cache.step(counts) returned for them.  Without dropout, whatever the
-        mode.  The row of a sequence that has no new tokens says nothing."""
+        mode; forward hooks of the model, its blocks and their attention do not
+        run.  The row of a sequence that has no new tokens says nothing."""
         if self._zero3_executor is not None and not getattr(self._zero3_executor, "params_materialized", False):
             raise RuntimeError("a ZeRO-3 sharded model has no cached forward: gather its parameters first "
                                "(summon_full_params; a forward within it hands them back) or generate without use_cache")

@@ -396,9 +396,9 @@ int lz_dropout_mask(uint8_t* keep, int64_t n, float p, uint64_t seed, void* stre
  * B + 1 ascending values, on the device) are the last tokens of sequence b,
  * whose length with them is kv_len[b].  Rows of no sequence are left as they
  * are.  What the tables say is checked on the device: a position outside the
- * table and a page id outside [0, pages) are skipped, and the rows of tokens
- * whose position is negative or past the table (or the cos/sin tables') come
- * out as zeros. */
+ * table or on a page id outside [0, pages) is not written, read as zeros and
+ * not seen by attention; lz_kv_write's queries at a negative position or one
+ * past the cos/sin tables come out as zeros. */
 #define LZ_E4M3 8
 
 /* q_out rows (H heads) = RoPE(q), and RoPE(k) and v of every row into its

@@ -236,3 +236,49 @@ def test_rows_past_max_new_are_left(seqs, bound, most, e4m3):
         mid = min(lo + bound, hi)
         assert bool(((got - want).abs() <= tol)[lo:mid].all()), b
         assert bool((got[mid:hi] == 7).all()), b
+
+
+@pytest.mark.parametrize("most", [0, MUCH])
+def test_rows_between_the_last_sequence_and_the_step(most):
+    """Tables that cover fewer rows than the step was made for: the caller's
+    rows of no sequence stay, and new outputs are zeros from step.rows on."""
+    c = Case([(70, 90), (1, 5), (9, 20)], 2, 64, 16, BF16, most=most)
+    start = torch.tensor([0, 70, 71, 71], dtype=torch.int32, device=DEV)
+    step = c.step._replace(row_start=start)
+    wide = torch.randn(c.rows + 4, 8 * 64, generator=c.g).to(BF16).to(DEV)
+    cos, sin = (torch.randn(c.step.max_len if not most else 90, 64, generator=c.g).to(BF16).to(DEV) for _ in range(2))
+    out = torch.full((c.rows + 4, 256), 7.0, dtype=BF16, device=DEV)
+    q = ops.kv_cache_write(wide, c.layer, step._replace(max_len=90), 4, cos, sin, out=out)
+    assert q.data_ptr() == out.data_ptr() and bool((out[71:] == 7).all()) and not bool((out[:71] == 7).any())
+    o = ops.paged_attention(q, c.layer, step, 4, 0.125, out=torch.full_like(out, 7.0))
+    assert bool((o[71:] == 7).all()) and bool(torch.isfinite(o[:71]).all())
+    fresh = ops.kv_cache_write(wide, c.layer, step._replace(max_len=90), 4, cos, sin)
+    assert torch.equal(fresh[:71], q[:71]) and bool((fresh[c.rows :] == 0).all())
+    fresh = ops.paged_attention(q, c.layer, step, 4, 0.125)
+    assert torch.equal(fresh[:71], o[:71]) and bool((fresh[c.rows :] == 0).all())
+
+
+def test_positions_past_the_page_table():
+    """A sequence longer than its row of pages: its tokens there are not
+    written and not seen, their queries are rotated and see what is there."""
+    c = Case([(3, 64)], 1, 32, 16, F32)
+    step = c.step._replace(kv_len=torch.tensor([66], dtype=torch.int32, device=DEV), max_len=66)
+    cos, sin = (torch.randn(66, 32, generator=c.g) for _ in range(2))
+    qkv = torch.randn(3, 3 * 32, generator=c.g)
+    before = c.layer.k.clone()
+    q = ops.kv_cache_write(qkv.to(DEV), c.layer, step, 1, cos.to(DEV), sin.to(DEV))
+    pos = torch.tensor([63, 64, 65])
+    x = qkv[:, :64].view(3, 2, 32)
+    y = x * cos[pos][:, None] + torch.cat([-x[..., 16:], x[..., :16]], -1) * sin[pos][:, None]
+    assert torch.equal(q.cpu(), y[:, 0])
+    k = before.cpu()
+    k[c.table[0, 3], 0, 15] = y[0, 1]
+    assert torch.equal(c.layer.k.cpu(), k)
+    got = ops.paged_attention(q, c.layer, step, 1, 0.25).cpu()
+    kk = k[c.table[0].long(), 0].reshape(64, 32).double()
+    vv = c.layer.v.cpu()[c.table[0].long(), 0].reshape(64, 32).double()
+    for i in range(3):
+        p = torch.softmax(kk @ y[i, 0].double() * 0.25, 0)
+        size = float((kk.abs() @ y[i, 0].double().abs()).max()) * 0.25
+        tol = U32 * (p @ vv).abs() + (2 * 36 * size + 8 + 64) * U32 * (p @ vv.abs())
+        assert bool(((got[i].double() - p @ vv).abs() <= tol).all()), i
