@@ -452,9 +452,9 @@ class LlamaForCausalLM(nn.Module):
         *,
         use_cache: bool = False,
         cache_dtype: Optional[torch.dtype] = None,
-        repetition_penalty: float = 1.0,
-        presence_penalty: float = 0.0,
-        frequency_penalty: float = 0.0,
+        repetition_penalty: Union[float, torch.Tensor] = 1.0,
+        presence_penalty: Union[float, torch.Tensor] = 0.0,
+        frequency_penalty: Union[float, torch.Tensor] = 0.0,
         logit_bias: Optional[torch.Tensor] = None,
         token_mask: Union[None, torch.Tensor, Callable[[torch.Tensor], torch.Tensor]] = None,
     ) -> torch.Tensor:
@@ -481,7 +481,8 @@ class LlamaForCausalLM(nn.Module):
         seq = input_ids.new_empty((bsz, t0 + max_new_tokens))
         seq[:, :t0] = input_ids
         window = self.cfg.max_seq_len
-        adjust = (repetition_penalty != 1.0 or presence_penalty != 0.0 or frequency_penalty != 0.0
+        penalties = ((repetition_penalty, 1.0), (presence_penalty, 0.0), (frequency_penalty, 0.0))
+        adjust = (any(torch.is_tensor(p) or p != none for p, none in penalties)
                   or logit_bias is not None or token_mask is not None)
         prompts = torch.full((bsz,), t0, dtype=torch.int32, device=seq.device) if adjust else None
         cache, cached = None, 0

@@ -158,3 +158,22 @@ def test_rotary_tables_of_a_captured_call_stay(monkeypatch):
     call(64, False, True)
     gc.collect()
     assert gone() is not None and first() is None
+
+
+def test_penalties_may_be_one_for_each_row(monkeypatch):
+    """generate hands them on as process_logits takes them: numbers or
+    tensors."""
+    got = []
+
+    def process(x, **kw):
+        got.append({k: kw[k] for k in ("repetition_penalty", "presence_penalty", "frequency_penalty")})
+        return x.float()
+
+    monkeypatch.setattr(ops, "process_logits", process)
+    model = Fixed([[0.0, 1.0, 2.0, 3.0], [3.0, 2.0, 1.0, 0.0]])
+    ids, each = torch.zeros(2, 3, dtype=torch.int64), torch.tensor([1.0, 1.5])
+    for name in ("repetition_penalty", "presence_penalty", "frequency_penalty"):
+        model.generate(ids, 1, temperature=0.0, **{name: each})
+        assert len(got) == 1 and got.pop()[name] is each
+    model.generate(ids, 1, temperature=0.0, repetition_penalty=1, presence_penalty=0)  # nothing to adjust
+    assert not got
