@@ -8,6 +8,8 @@ token.
 """
 from __future__ import annotations
 
+import itertools
+import operator
 from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
@@ -86,32 +88,38 @@ class KVCache:
         self._pages: List[List[int]] = [[] for _ in range(batch)]
         self._free = list(range(n_pages - 1, -1, -1))
 
-    def _page_table(self, which: Sequence[int]) -> List[List[int]]:
-        width = max(1, max(len(self._pages[b]) for b in which))
-        return [self._pages[b] + [-1] * (width - len(self._pages[b])) for b in which]
+    @staticmethod
+    def _page_table(pages: Sequence[List[int]]) -> List[List[int]]:
+        width = max(1, max(map(len, pages)))
+        return [p + [-1] * (width - len(p)) for p in pages]
 
     def step(self, new: Sequence[int]) -> CacheStep:
         """Room for new[b] more tokens of every sequence b (0: none) and the
-        CacheStep that the layers' calls take.  Nothing changes if the pages
-        do not suffice."""
+        CacheStep that the layers' calls take.  A call that fails (the pages do
+        not suffice, say) changes nothing."""
+        new = [operator.index(n) for n in new]
         if len(new) != len(self.lengths):
             raise ValueError(f"{len(new)} counts of new tokens for {len(self.lengths)} sequences")
         if min(new) < 0:
             raise ValueError("counts of new tokens must not be negative")
-        want = [-(-(n + l) // self.page_size) - len(p) for n, l, p in zip(new, self.lengths, self._pages)]
-        if sum(want) > len(self._free):
+        lengths = [n + l for n, l in zip(new, self.lengths)]
+        want = [-(-l // self.page_size) - len(p) for l, p in zip(lengths, self._pages)]
+        left = len(self._free) - sum(want)
+        if left < 0:
             raise RuntimeError(f"the cache has {len(self._free)} free pages of {self.page_size} tokens; {sum(want)} "
                                "more are needed: free() sequences or make it larger")
-        starts = [0]
-        for b, n in enumerate(new):
-            self._pages[b] += [self._free.pop() for _ in range(want[b])]
-            self.lengths[b] += n
-            starts.append(starts[-1] + n)
-        B, table = len(new), self._page_table(range(len(new)))
-        flat = torch.tensor(starts + self.lengths + [p for row in table for p in row], dtype=torch.int32)
+        taken = iter(self._free[: left - 1 if left else None : -1])
+        more = [list(itertools.islice(taken, n)) for n in want]
+        B, starts = len(new), [0, *itertools.accumulate(new)]
+        table = self._page_table([p + m for p, m in zip(self._pages, more)])
+        flat = torch.tensor(starts + lengths + [p for row in table for p in row], dtype=torch.int32)
         flat = flat.to(self.device)
+        self.lengths[:] = lengths
+        del self._free[left:]
+        for p, m in zip(self._pages, more):
+            p += m
         return CacheStep(flat[: B + 1], flat[B + 1 : 2 * B + 1], flat[2 * B + 1 :].view(B, -1), starts[-1], max(new),
-                         max(self.lengths))
+                         max(lengths))
 
     def free(self, b: int) -> None:
         """Ends sequence b: its pages go back, and its slot is empty."""
@@ -122,6 +130,6 @@ class KVCache:
         """Sequence b's keys and values in one layer, [tokens, KV heads, head
         dim] each, in the model's dtype."""
         n, kv = self.lengths[b], self.layers[layer]
-        flat = torch.tensor([0, n] + self._page_table([b])[0], dtype=torch.int32).to(self.device)
+        flat = torch.tensor([0, n] + self._page_table([self._pages[b]])[0], dtype=torch.int32).to(self.device)
         k, v = ops.kv_cache_read(kv, flat[2:].view(1, -1), flat[:2], n, self.dtype)
         return k.view(n, *kv.k.shape[1::2]), v.view(n, *kv.v.shape[1::2])

@@ -177,3 +177,32 @@ def test_penalties_may_be_one_for_each_row(monkeypatch):
         assert len(got) == 1 and got.pop()[name] is each
     model.generate(ids, 1, temperature=0.0, repetition_penalty=1, presence_penalty=0)  # nothing to adjust
     assert not got
+
+
+def _cpu_cache(batch, n_pages):
+    from lzhip.cache import KVCache
+
+    cache = object.__new__(KVCache)  # its tables alone
+    cache.device, cache.page_size, cache.n_pages = torch.device("cpu"), 16, n_pages
+    cache.lengths, cache._pages = [0] * batch, [[] for _ in range(batch)]
+    cache._free = list(range(n_pages - 1, -1, -1))
+    return cache
+
+
+def test_a_step_that_fails_changes_nothing():
+    cache = _cpu_cache(3, 6)
+    s = cache.step([20, 0, 3])
+    assert s.row_start.tolist() == [0, 20, 20, 23] and s.kv_len.tolist() == [20, 0, 3]
+    before = (list(cache.lengths), [list(p) for p in cache._pages], list(cache._free))
+    for bad, err in (([1, 1.5, 1], TypeError), ([1, 20, "2"], TypeError), ([1, 1], ValueError), ([1, -1, 1], ValueError),
+                     ([0, 70, 0], RuntimeError)):
+        with pytest.raises(err):
+            cache.step(bad)
+    cache.device = torch.device("cuda:0")  # the tables do not arrive
+    with pytest.raises(Exception):
+        cache.step([20, 1, 1])
+    cache.device = torch.device("cpu")
+    assert (cache.lengths, cache._pages, cache._free) == before
+    s = cache.step([20, 1, 1])
+    used = [p for row in s.page_table.tolist() for p in row if p >= 0]
+    assert len(used) == len(set(used)) == 5 and cache.lengths == [40, 1, 4] and len(cache._free) == 1
