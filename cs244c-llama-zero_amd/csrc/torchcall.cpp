@@ -278,6 +278,25 @@ struct Out {
   }
 };
 
+// Refuses an output that lies over values of the input rows x which other
+// threads may read after it is written.  The same rows from their first column
+// on are fine (a thread reads what it writes there first: `first` columns), and so
+// are columns beside x's.
+void require_apart(const Out& out, const Rows& x, int64_t cols, int64_t first) {
+  const at::Tensor &o = out.t, &t = x.t;
+  const int64_t n = o.size(1), esz = t.element_size();
+  if (x.rows == 0 || n == 0) return;
+  const char *a = static_cast<const char*>(t.data_ptr()), *b = static_cast<const char*>(o.data_ptr());
+  const int64_t a_end = ((x.rows - 1) * x.ld + cols) * esz, b_end = ((x.rows - 1) * out.ld + n) * esz;
+  if (a + a_end <= b || b + b_end <= a) return;
+  if (x.ld == out.ld || x.rows == 1) {
+    if (a == b && n <= first) return;
+    const int64_t ld = x.ld * esz, off = ((b - a) % ld + ld) % ld;
+    if (x.rows > 1 && off >= cols * esz && off + n * esz <= ld) return;
+  }
+  refuse(PyExc_ValueError, "out overlaps the rows that the call reads");
+}
+
 // Runs a call's body; nothing but a Python exception leaves it.
 template <typename F>
 PyObject* guarded(const F& body) {
@@ -316,6 +335,7 @@ PyObject* kv_cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
                (long long)s.max_len, (long long)c.hd, (int)at.index, type_name(*t), shape(*t).c_str());
     }
     const Out q(a[6], x, qkv.rows, H * c.hd, s.rows, code, at);
+    require_apart(q, qkv, (H + 2 * c.KV) * c.hd, H * c.hd);
     call("lz_kv_write", p_write, (const void*)qkv.t.data_ptr(), qkv.ld, code, qkv.rows, (const void*)cos.data_ptr(),
          (const void*)sin.data_ptr(), cos.size(0), q.t.data_ptr(), q.ld, address(c.k), address(c.v), address(c.ke),
          address(c.ve), c.code, c.pages, c.size, (const int32_t*)address<int32_t>(s.table), s.width,
@@ -368,6 +388,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       refuse(PyExc_ValueError, "%lld query heads do not divide over %lld key/value heads", (long long)H, (long long)c.KV);
     const Rows q(x, "q", H * c.hd, code, at);
     const Out o(a[5], x, q.rows, H * c.hd, s.rows, code, at);
+    require_apart(o, q, H * c.hd, H * c.hd);
     const int64_t bytes = p_attn_ws(code, c.code, q.rows, s.B, H, c.KV, c.hd, s.max_new, s.max_len);
     at::Tensor ws;
     if (bytes) ws = fresh(x, {(bytes + 3) / 4}, at::kFloat);

@@ -23,7 +23,7 @@ class LayerCache(NamedTuple):
     size]: the value is the stored number times 2^exponent (-126 to 127).
     8-bit pages are read in the dtype that they were written with: float16
     keeps smaller exponents than the others.  Where two rows of one step are
-    given the same slot, either is kept."""
+    given the same slot, it holds parts of both."""
 
     k: torch.Tensor
     v: torch.Tensor

@@ -282,3 +282,33 @@ def test_positions_past_the_page_table():
         size = float((kk.abs() @ y[i, 0].double().abs()).max()) * 0.25
         tol = U32 * (p @ vv).abs() + (2 * 36 * size + 8 + 64) * U32 * (p @ vv.abs())
         assert bool(((got[i].double() - p @ vv).abs() <= tol).all()), i
+
+
+def test_outputs_over_other_inputs_are_refused():
+    """out may be q itself, or the q columns of qkv, or columns beside them;
+    what would be written over values still to be read is refused."""
+    c = Case([(5, 50)], 2, 32, 16, BF16)
+    cos, sin = (torch.randn(50, 32, generator=c.g).to(BF16).to(DEV) for _ in range(2))
+    first = torch.randn(12, 640, generator=c.g).to(BF16).to(DEV)
+    wide = first.clone()
+    q, qkv = wide[:5, :128], wide[:5, :256]
+
+    def attend(out):
+        return ops.paged_attention(q, c.layer, c.step, 4, 0.2, out=out)
+
+    def write(out):
+        return ops.kv_cache_write(qkv, c.layer, c.step, 4, cos, sin, out=out)
+
+    want = write(None), attend(None)
+    for out in (wide[:5, 8:136], wide[1:6, :128], wide.view(-1)[520 : 520 + 5 * 640].view(5, 640)[:, :128],
+                wide.view(-1)[: 5 * 128].view(5, 128)):
+        for call in (attend, write):
+            with pytest.raises(ValueError, match="overlap"):
+                call(out)
+    with pytest.raises(ValueError, match="overlap"):  # the keys' columns
+        write(wide[:5, 128:256])
+    assert torch.equal(wide, first)
+    for out in (wide[:5, 256:384], wide[:5, 512:], wide[5:10, 64:192], wide[:5, :128]):
+        for call, result in ((write, want[0]), (attend, want[1])):
+            assert torch.equal(call(out), result)
+            wide.copy_(first)
