@@ -40,7 +40,8 @@ typedef LzPagedArgs PagedArgs;
 // row blocks share are fetched into one L2.  With fewer heads that would leave a
 // long sequence to some of the XCDs: its blocks go round all of them (4 x up to
 // 188 new tokens over up to 8979 in fp32, 2 heads of 32: 66 us, on two XCDs
-// 115).
+// 115; where the pairs are many it can lose: single tokens of 4 x up to 5720, 18/6
+// heads of 64, 13.2 and 12.2).
 struct PagedPlace {
   int b, g, qb, split;
   __device__ __forceinline__ PagedPlace(const PagedArgs& a, uint32_t bid) {
@@ -95,7 +96,7 @@ __device__ __forceinline__ bool sees_any(const PagedArgs& a, int b, int k_lo, in
 // 2^8 are as exact in 16 and 32 bits as those up to 1, and the sums are
 // multiplied down once or twice in a pass and not at every new maximum (2 x up
 // to 1024 new tokens over up to 8192, 32/8 heads of 128, one wave group a block:
-// 161 and 171 us).
+// 208 and 218 us).
 constexpr float kSlack = 8.f;
 
 // Two fp32 weights of the second product as N packed terms of the 16-bit format

@@ -562,29 +562,29 @@ struct Plan {
 // Row blocks and parts.  Tiles of 128 rows where a sequence has 64 packed rows
 // or more and the work is not little: at most 1.5 blocks of 32 rows a CU which
 // go over at most 512 keys a CU, where the tile kernel's longer start and steps
-// are the time (12/4 heads of 64: 3 prompts of up to 182 tokens 7.3 us, 9.3 in
-// tiles; 4 of up to 400 17, 14 in tiles; 16 of up to 256 18 and 11).
+// are the time (12/4 heads of 64: 3 prompts of up to 182 tokens 8.1 us, 9.6 in
+// tiles; 4 of up to 400 16.3, 15.4 in tiles; 16 of up to 256 16 and 12).
 // paged_wave_kernel: whole sequences where there is a block for every CU (32
-// ragged sequences of up to 2048, 16/8 heads of 128: 33 us, in parts of 512
+// ragged sequences of up to 2048, 16/8 heads of 128: 34 us, in parts of 512
 // keys 37), but four parts where some CUs would have one more than others and a
-// third of the CUs' time would go by (36 of them: 42 us, whole 51; 58: 52 and
-// 53; all 2048 long: 60 and 71 of 36, 93 and 85 of 58); fewer blocks than CUs:
+// third of the CUs' time would go by (36 of them: 42 us, whole 52; 58: 53 and
+// 52; all 2048 long: 60 and 71 of 36, 93 and 84 of 58); fewer blocks than CUs:
 // four workgroups a CU, so that lengths even out (16 of up to 4096, 32/8 heads:
 // 27 us in eight parts, 33 in four), but two where that makes more than 16 parts
-// to join (4 x 32768 in e4m3: 41 us in 16, 48 in 32), and parts of 512 keys at
+// to join (4 x 32768 in e4m3: 43 us in 16, 48 in 32), and parts of 512 keys at
 // least, four of each wave's tiles (8 of up to 4096: 20 us, 23 in parts of 256;
-// in e4m3 15.3, 17.3 and, in parts of 1024, 16.6), while every CU has one
+// in e4m3 16.0, 19.2 and, in parts of 1024, 16.9), while every CU has one
 // (1 x 8192: 13 us in 32, 19 in 8); short sequences whole, where the join costs
-// more than their keys (1 x 512 over heads of 64: 6.4 us, 8.6 in parts; of 128:
-// 8.4 and 9.1).  The tile kernel: one workgroup a CU, of two wave groups where
-// that is all (1 x 512 new tokens over 4096: 55 us in two parts, 70 whole, 89
-// whole with one group; in four parts, with one group, 55), and for up to a third
+// more than their keys (1 x 512 over heads of 64: 6.7 us, 8.8 in parts; of 128:
+// 8.8 and 9.3).  The tile kernel: one workgroup a CU, of two wave groups where
+// that is all (1 x 512 new tokens over 4096: 64 us in two parts, 83 whole, 96
+// whole with one group; in four parts, with one group, 65), and for up to a third
 // more blocks where their keys are uneven, so that those of a second turn are
-// short (a prompt of 2600, 16/8 heads: 46 us, 56 with one group; 3 chunks of 800
-// over 4096 alike: 119 and 104); three parts of one group, two workgroups a CU,
+// short (a prompt of 2600, 16/8 heads: 58 us, 68 with one group; 3 chunks of 800
+// over 4096 alike: 151 and 135); three parts of one group, two workgroups a CU,
 // where a block each would leave a third of the CUs idle for long (1 x 600 over
-// 8192, 32/8 heads: 99 us, whole 119; 1 x 1100 over 2200, 16/8 heads: 41 and 41;
-// 1 x 700 over 3000, 32/8 heads, with blocks for two thirds: 64 and 52).
+// 8192, 32/8 heads: 125 us, whole 145; 1 x 1100 over 2200, 16/8 heads: 47 and 48;
+// 1 x 700 over 3000, 32/8 heads, with blocks for two thirds: 76 and 62).
 Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd, int64_t max_new,
                int64_t max_len) {
   Plan p;

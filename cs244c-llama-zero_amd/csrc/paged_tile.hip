@@ -231,10 +231,9 @@ __device__ __forceinline__ void add_odd(f32x16_t (&o)[HD / 32], const f32x16_t (
 
 // The w-th row block of a kv head in the order of the keys that blocks go over,
 // most first: the long ones start at once and the short ones fill the gaps
-// (eight prompts of up to 2048 tokens, 16 heads of 128, fp16: 110 us dealt in
-// turn, 80 sequence after sequence, 72 so; 66 with the steps since).  Lane b of
-// a wave counts sequence b's blocks; a bisection finds the step count of the
-// w-th one.
+// (eight prompts of up to 2048 tokens, 16 heads of 128, fp16: 121 us dealt in
+// turn, 102 sequence after sequence, 87 so).  Lane b of a wave counts sequence
+// b's blocks; a bisection finds the step count of the w-th one.
 struct ByLength {
   int b, m0;  // sequence and first row; b < 0: there are fewer blocks
 

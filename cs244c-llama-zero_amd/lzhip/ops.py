@@ -1224,9 +1224,10 @@ def kv_cache_write(qkv: torch.Tensor, layer, step, n_heads: int, cos: torch.Tens
     layer: LayerCache, layer.k of qkv's dtype or float8_e4m3fn; step:
     CacheStep; cos/sin: RoPE tables [>= step.max_len, hd] in qkv's dtype; out:
     rows for the queries, where those of no sequence are left as they are; they
-    may be qkv's own q columns, and otherwise must not overlap qkv.  In new ones the rows from step.rows on are zeros; others of no sequence
-    (row_start may cover less than step.rows) hold anything.  Rotation,
-    rounding and 8-bit storage: lz_kv_write.  No gradients."""
+    may be qkv's own q columns and must not overlap it otherwise.  In new ones
+    the rows from step.rows on are zeros; others of no sequence (row_start may
+    cover less than step.rows) hold anything.  Rotation, rounding and 8-bit
+    storage: lz_kv_write.  No gradients."""
     return _lib.tensor_calls().kv_cache_write(qkv, layer, step, n_heads, cos, sin, out)
 
 
@@ -1248,7 +1249,8 @@ def paged_attention(q: torch.Tensor, layer, step, n_heads: int, scale: float,
     kv_cache_write comes first); causal within the new tokens; scale > 0.  A
     row that sees nothing is zero, one whose scores are all -inf is NaN, as a
     softmax of them.  out: rows for the result, as kv_cache_write's; it may be
-    q itself and must not overlap it otherwise.  No gradients: the result of a q that needs them does not."""
+    q itself and must not overlap it otherwise.  No gradients: the result of a
+    q that needs them does not."""
     return _lib.tensor_calls().paged_attention(q, layer, step, n_heads, scale, out)
 
 

@@ -8,8 +8,8 @@ import pytest
 import torch
 
 from lzhip import ops
-from lzhip.cache import CacheStep
-from test_gpu_generation import BF16, DEV, F16, F32, MUCH, U32, Case, _model, _u
+from lzhip.cache import CacheStep, LayerCache
+from test_gpu_generation import BF16, DEV, E4M3, F16, F32, MUCH, U32, Case, _model, _u
 
 pytestmark = pytest.mark.gpu
 
@@ -312,3 +312,32 @@ def test_outputs_over_other_inputs_are_refused():
         for call, result in ((write, want[0]), (attend, want[1])):
             assert torch.equal(call(out), result)
             wide.copy_(first)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("new", [1, 70])
+def test_chunks_on_pages_past_two_to_the_31_elements(new, e4m3):
+    """Page ids whose element offsets need 64 bits, in the 128-row tiles and in
+    8 bits."""
+    pages, page, hd = 2**15 + 40, 1024, 64
+    store = E4M3 if e4m3 else BF16
+    k, v = (torch.empty(pages, 1, page, hd, dtype=store, device=DEV) for _ in range(2))
+    e = [torch.zeros(pages, 1, page, dtype=torch.int8, device=DEV) for _ in range(2)] if e4m3 else [None, None]
+    far = [pages - 1, 2**15 - 1, 2**15 + 1]
+    g = torch.Generator().manual_seed(8)
+    for p in far:
+        for t in (k, v):
+            t[p] = torch.randn(1, page, hd, generator=g).to(DEV).to(store)
+    length = 2 * page + 100
+    step = CacheStep(*(torch.tensor(t, dtype=torch.int32, device=DEV) for t in ([0, new], [length], [far])), new, new, MUCH)
+    q = torch.randn(new, 2 * hd, generator=g).to(BF16)
+    got = ops.paged_attention(q.to(DEV), LayerCache(k, v, *e), step, 2, 0.125).cpu().double()
+    kk, vv = (torch.cat([t[p, 0] for p in far])[:length].cpu().double() for t in (k, v))
+    for i in range(new):
+        for h in range(2):
+            seen, x = length - new + i + 1, q[i, h * hd : (h + 1) * hd].double()
+            p = torch.softmax(kk[:seen] @ x * 0.125, 0)
+            size = float((kk[:seen].abs() @ x.abs()).max()) * 0.125
+            want, a = p @ vv[:seen], p @ vv[:seen].abs()
+            tol = _u(BF16) * want.abs() + (_u(BF16) ** 2 + (2 * (hd + 4) * size + 8 + 3 * seen) * U32) * a
+            assert bool(((got[i, h * hd : (h + 1) * hd] - want).abs() <= tol).all()), (i, h)
