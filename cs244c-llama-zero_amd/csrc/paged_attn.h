@@ -105,7 +105,7 @@ constexpr float kSlack = 8.f;
 //   paged_wave_kernel, bf16: three terms of eight significant bits, cut and not
 //     rounded, so that each remainder is exact and the three add up to the
 //     weight.  It is bound by memory: 16 x up to 4096 tokens, 32/8 heads of 128,
-//     30.7 us, with one rounded term 30.5; 8 x up to 15 new over 4096 44, 38.
+//     31.0 us, with one rounded term 30.5; 8 x up to 15 new over 4096 46, 38.
 //   paged_tile_kernel, bf16: the cut weight and the rounded rest, off by 2^-16 of
 //     the weight at most.  It is bound by the matrix cores: 2 x up to 1024 new
 //     over up to 8192, 32/8 heads of 128, 199 us, with one term 155, three 244.

@@ -269,17 +269,10 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
 
   f32x4_t acc[NQ][VE];
   float mx[NQ], sum[NQ];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    mx[n] = -INFINITY;
-    sum[n] = 0.f;
-#pragma unroll
-    for (int j = 0; j < VE; ++j) acc[n][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  }
   const float unit = sizeof(T) == 4 ? a.scale : a.scale * kLog2e;
   constexpr float lift = sizeof(T) == 4 ? 0.f : kLift<typename W::F>;
 
-  int ids = key_of(lane) < k_hi ? first_ids : -1, ids_from = 0;
+  int ids, ids_from;
   const int size_mask = (1 << a.pg.log_size) - 1;
   auto tokens = [&](int64_t (&tok)[NT], int tile) {
     const int x = tile * NT;
@@ -298,117 +291,141 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
   W w;
   int64_t tok[NT], next[NT];
   const int n_tiles = max(0, (k_hi - k_lo - wave * KT + 4 * KT - 1) / (4 * KT));
-  if (n_tiles > 0) {
-    tokens(tok, 0);
-    w.load_k(a, tok, c16, g4);
-    w.load_v(a, tok, c16, g4);
-  }
-  for (int tile = 0; tile < n_tiles; ++tile) {
-    const int key0 = key_of(tile * NT);
-    const bool more = tile + 1 < n_tiles;
-    f32x4_t s[NQ][NT];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) w.scores(s[n], q[n]);
-    if (more) {
-      tokens(next, tile + 1);
-      w.load_k(a, next, c16, g4);
-    }
-    bool holes = key0 + KT > all_see;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) holes |= tok[t] < 0;
+  // An infinity of V that all rows see multiplies a weight's terms one by one: a
+  // zero among them would make it NaN.  Where a sum is not finite the pass is
+  // made again with such values out of the product, as in tiles with holes; the
+  // others get the same bits.
+  for (bool odd_pass = false;; odd_pass = true) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      if (holes) {
+      mx[n] = -INFINITY;
+      sum[n] = 0.f;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (tok[t] < 0 || key0 + 16 * t + 4 * g4 + i >= sees[n]) s[n][t][i] = -INFINITY;
-      }
-      float top = s[n][0][0];
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[n][t][i]);
-      top = max_of_row(top) * unit;
-      const bool moved = top > mx[n] + (sizeof(T) == 4 ? 0.f : kSlack);
-      if (__ballot(moved)) {
-        const float m_new = moved ? top : mx[n];
-        const float alpha = moved ? exp_of<T>(mx[n] - m_new) : 1.f;
-        mx[n] = m_new;
-        sum[n] *= alpha;
-#pragma unroll
-        for (int j = 0; j < VE; ++j) acc[n][j] *= alpha;
-      }
-      const float m0 = mx[n] == -INFINITY ? 0.f : mx[n];
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = exp_of<T>(fmaf(s[n][t][i], unit, lift - m0));
-          s[n][t][i] = p;
-          sum[n] += p;
-        }
+      for (int j = 0; j < VE; ++j) acc[n][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
-    typename W::Value x;
-    w.widen(x);
-    bool odd = false;
-    if (holes) {
-      // slots past the sequence hold anything: out, before they meet a zero
-      // weight.  An infinity or NaN that only some of the rows see is taken
-      // out too and added to those rows below.
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool there = key0 + 16 * t + 4 * g4 + i < n_keys;
-#pragma unroll
-          for (int e = 0; e < W::Value::N; ++e) {
-            uint32_t& y = x.w[t][i][e];
-            if (!there) y = 0;
-            if constexpr (W::kWide) {
-              if (nonfinite32(y)) {
-                y = 0;
-                odd = true;
-              }
-            } else if (nonfinite16<typename W::F>(y)) {
-              if (nonfinite16<typename W::F>(y & 0xffffu)) y &= 0xffff0000u;
-              if (nonfinite16<typename W::F>(y & 0xffff0000u)) y &= 0xffffu;
-              odd = true;
-            }
-          }
-        }
-      odd = __ballot(odd) != 0;
+    ids = key_of(lane) < k_hi ? first_ids : -1;
+    ids_from = 0;
+    if (n_tiles > 0) {
+      tokens(tok, 0);
+      w.load_k(a, tok, c16, g4);
+      w.load_v(a, tok, c16, g4);
     }
-    if (more) w.load_v(a, next, c16, g4);
-    W::pv(acc, x, s);
-    if (odd) {
-#pragma unroll 1
-      for (int kk = 0; kk < KT; ++kk) {
-        const int64_t tk = tok[kk / 16] + kk % 16;
-        if (tok[kk / 16] < 0 || key0 + kk >= n_keys) continue;
+    for (int tile = 0; tile < n_tiles; ++tile) {
+      const int key0 = key_of(tile * NT);
+      const bool more = tile + 1 < n_tiles;
+      f32x4_t s[NQ][NT];
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-          float p = 0.f;
+      for (int n = 0; n < NQ; ++n) w.scores(s[n], q[n]);
+      if (more) {
+        tokens(next, tile + 1);
+        w.load_k(a, next, c16, g4);
+      }
+      bool holes = odd_pass || key0 + KT > all_see;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) holes |= tok[t] < 0;
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        if (holes) {
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p = kk / 16 == t && kk % 4 == i ? s[n][t][i] : p;
-          p = __shfl(p, c16 + 16 * (kk % 16 / 4), 64);
-          if (key0 + kk < sees[n]) {
+            for (int i = 0; i < 4; ++i)
+              if (tok[t] < 0 || key0 + 16 * t + 4 * g4 + i >= sees[n]) s[n][t][i] = -INFINITY;
+        }
+        float top = s[n][0][0];
 #pragma unroll
-            for (int j = 0; j < VE; ++j)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float y = W::v_elem(a, tk, (4 * g4 + i) * VE + j);
-                if (!(fabsf(y) < INFINITY)) acc[n][j][i] = fmaf(p, y, acc[n][j][i]);
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, s[n][t][i]);
+        top = max_of_row(top) * unit;
+        const bool moved = top > mx[n] + (sizeof(T) == 4 ? 0.f : kSlack);
+        if (__ballot(moved)) {
+          const float m_new = moved ? top : mx[n];
+          const float alpha = moved ? exp_of<T>(mx[n] - m_new) : 1.f;
+          mx[n] = m_new;
+          sum[n] *= alpha;
+#pragma unroll
+          for (int j = 0; j < VE; ++j) acc[n][j] *= alpha;
+        }
+        const float m0 = mx[n] == -INFINITY ? 0.f : mx[n];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = exp_of<T>(fmaf(s[n][t][i], unit, lift - m0));
+            s[n][t][i] = p;
+            sum[n] += p;
+          }
+      }
+      typename W::Value x;
+      w.widen(x);
+      bool odd = false;
+      if (holes) {
+        // slots past the sequence hold anything: out, before they meet a zero
+        // weight.  An infinity or NaN that only some of the rows see is taken
+        // out too and added to those rows below.
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool there = key0 + 16 * t + 4 * g4 + i < n_keys;
+#pragma unroll
+            for (int e = 0; e < W::Value::N; ++e) {
+              uint32_t& y = x.w[t][i][e];
+              if (!there) y = 0;
+              if constexpr (W::kWide) {
+                if (nonfinite32(y)) {
+                  y = 0;
+                  odd = true;
+                }
+              } else if (nonfinite16<typename W::F>(y)) {
+                if (nonfinite16<typename W::F>(y & 0xffffu)) y &= 0xffff0000u;
+                if (nonfinite16<typename W::F>(y & 0xffff0000u)) y &= 0xffffu;
+                odd = true;
               }
+            }
+          }
+        odd = __ballot(odd) != 0;
+      }
+      if (more) w.load_v(a, next, c16, g4);
+      W::pv(acc, x, s);
+      if (odd) {
+#pragma unroll 1
+        for (int kk = 0; kk < KT; ++kk) {
+          const int64_t tk = tok[kk / 16] + kk % 16;
+          if (tok[kk / 16] < 0 || key0 + kk >= n_keys) continue;
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            float p = 0.f;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) p = kk / 16 == t && kk % 4 == i ? s[n][t][i] : p;
+            p = __shfl(p, c16 + 16 * (kk % 16 / 4), 64);
+            if (key0 + kk < sees[n]) {
+#pragma unroll
+              for (int j = 0; j < VE; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float y = W::v_elem(a, tk, (4 * g4 + i) * VE + j);
+                  if (!(fabsf(y) < INFINITY)) acc[n][j][i] = fmaf(p, y, acc[n][j][i]);
+                }
+            }
           }
         }
       }
-    }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) tok[t] = next[t];
+      for (int t = 0; t < NT; ++t) tok[t] = next[t];
+    }
+    if (W::kWide || odd_pass) break;
+    float zero = 0.f;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int j = 0; j < VE; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) zero = fmaf(acc[n][j][i], 0.f, zero);
+    if (__ballot(zero != 0.f) == 0) break;  // NaN
   }
 
   // the four waves' parts, joined in a fixed order

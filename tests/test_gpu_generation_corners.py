@@ -4,6 +4,8 @@ Tolerances count roundings, as in test_gpu_generation.
 """
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -341,3 +343,27 @@ def test_chunks_on_pages_past_two_to_the_31_elements(new, e4m3):
             want, a = p @ vv[:seen], p @ vv[:seen].abs()
             tol = _u(BF16) * want.abs() + (_u(BF16) ** 2 + (2 * (hd + 4) * size + 8 + 3 * seen) * U32) * a
             assert bool(((got[i, h * hd : (h + 1) * hd] - want).abs() <= tol).all()), (i, h)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n,length,most", [(1, 1, 0), (1, 40, 0), (1, 3000, 0), (20, 90, 0), (20, 2500, 0), (90, 300, MUCH),
+                                           (130, 3000, MUCH)])
+def test_infinities_that_rows_see(dtype, n, length, most):
+    """An infinite value of a token that every row sees: the weighted sum's, of
+    its sign, and NaN where both signs meet; the other columns as ever."""
+    H, KV, hd, page = 4, 2, 64, 16
+    c = Case([(n, length), (1, 3)], KV, hd, page, dtype, seed=length, most=most)
+    q = (torch.randn(c.rows, H * hd, generator=c.g) * 0.1).to(dtype)
+    first = 0 if length == n else length - n  # the last token that all rows see
+    for tok, col, sign in ((0, 5, 1), (first, 6, -1), (first // 2, 7, 1), (0, 9, 1), (first, 9, -1), (first // 3, 20, 1)):
+        if length == 1 and col == 9 and sign < 0:
+            continue
+        c.cpu[1][c.table[0, tok // page], :, tok % page, col] = sign * math.inf
+    c.layer.v.copy_(c.cpu[1])
+    got = ops.paged_attention(q.to(DEV), c.layer, c.step, H, 0.125).cpu().double()
+    want, tol = c.attention(q, H, 0.125)
+    assert bool(torch.isposinf(want.view(-1, H, hd)[:n, :, 5]).all())
+    assert torch.equal(got.nan_to_num(nan=7e30, posinf=8e30, neginf=-8e30)[~torch.isfinite(want)],
+                       want.nan_to_num(nan=7e30, posinf=8e30, neginf=-8e30)[~torch.isfinite(want)])
+    fine = torch.isfinite(want)
+    assert bool(((got - want).abs() <= tol)[fine].all())
