@@ -367,3 +367,41 @@ def test_infinities_that_rows_see(dtype, n, length, most):
                        want.nan_to_num(nan=7e30, posinf=8e30, neginf=-8e30)[~torch.isfinite(want)])
     fine = torch.isfinite(want)
     assert bool(((got - want).abs() <= tol)[fine].all())
+
+
+def test_two_threads_generate_at_once():
+    """Cached steps of one model in training mode, with dropout, from two
+    threads on streams of their own: the bits of the same steps alone, and the
+    modes as they were."""
+    import threading
+
+    model = _model(BF16, dropout=0.5).train()
+    modes = [m.training for m in model.modules()]
+    g = torch.Generator().manual_seed(2)
+    texts = [torch.randint(0, 500, (2, 30), generator=g).to(DEV) for _ in range(2)]
+
+    def steps(text, out):
+        cache = model.new_cache(2, 48)
+        out.append(model.forward_cached(text[:, :20].reshape(-1), cache, cache.step([20, 20])))
+        for t in range(20, 30):
+            out.append(model.forward_cached(text[:, t].contiguous(), cache, cache.step([1, 1])))
+
+    want = [[], []]
+    for text, out in zip(texts, want):
+        steps(text, out)
+    torch.cuda.synchronize()
+    got, streams = [[], []], [torch.cuda.Stream() for _ in range(2)]
+
+    def run(i):
+        with torch.cuda.stream(streams[i]):
+            steps(texts[i], got[i])
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert [m.training for m in model.modules()] == modes
+    for a, b in zip(want, got):
+        assert len(a) == len(b) == 11 and all(torch.equal(x, y) for x, y in zip(a, b))

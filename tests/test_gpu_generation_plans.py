@@ -54,12 +54,15 @@ def _reference(c, q, H, scale, hidden=()):
 
 
 CHUNKS = [(400, 500), (333, 333), (300, 1100), (257, 260), (129, 700)]
+MIXED = [(1, 1 + 41 * b % 700) for b in range(30)] + [(700, 900)] + [(b % 3, 200 + b) for b in range(33)]  # 64 sequences
 MANY = [(b % 37, b % 37 + 11 * b % 50) for b in range(70)]
 PLANS = {
     # name: (sequences, query heads, kv heads, page, bound on the lengths, plan)
     "one group": (CHUNKS, 32, 8, 32, 0, (128, 1, 1)),
     "one group, equal": ([(352, 1500)] * 3, 32, 8, 64, 0, (128, 1, 1)),
     "one group, many sequences": (MANY, 16, 4, 16, MUCH, (128, 1, 1)),
+    "one group, a chunk beside 63 others": (MIXED, 16, 8, 32, 0, (128, 1, 1)),
+    "one group, a chunk beside 64 others": ([(1, 77)] + MIXED, 16, 8, 32, 0, (128, 1, 1)),
     "three parts": ([(600, 4200)], 32, 8, 64, 0, (128, 1, 3)),
     "two groups, a few more blocks than CUs": ([(1056, 1056)], 32, 8, 32, 0, (128, 2, 1)),
     "two groups": ([(600, 800)], 32, 8, 16, 0, (128, 2, 1)),
