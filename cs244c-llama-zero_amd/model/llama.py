@@ -11,6 +11,7 @@ no CPU compute path.
 """
 from __future__ import annotations
 
+import threading
 from dataclasses import dataclass
 from typing import Any, Callable, Optional, Tuple, Union
 
@@ -117,6 +118,34 @@ def apply_rotary_pos_emb(
     return LF.RopeFn.apply(q, c2, s2), LF.RopeFn.apply(k, c2, s2)
 
 
+_tables_lock = threading.Lock()  # of every module's rotary tables
+
+
+class _Built:
+    """The streams that may use tensors which the current one is building: the
+    others wait for it once, and their work is waited for before the memory
+    goes to another tensor.  A copy of a module copies its tensors, not this."""
+
+    def __init__(self, device: torch.device) -> None:
+        self.event = torch.cuda.current_stream(device).record_event()
+        self.streams = {ops.stream_ptr(device)}
+
+    def reach(self, device: torch.device, *tensors: torch.Tensor) -> None:
+        if ops.stream_ptr(device) in self.streams:
+            return
+        stream = torch.cuda.current_stream(device)
+        stream.wait_event(self.event)
+        for t in tensors:
+            t.record_stream(stream)
+        self.streams.add(ops.stream_ptr(device))
+
+    def __deepcopy__(self, memo) -> None:
+        return None
+
+    def __reduce__(self):
+        return type(None), ()
+
+
 class RotaryEmbedding(nn.Module):
     """cos/sin cache [1, 1, S, hd] in the activation dtype, rebuilt when the
     sequence grows or the device/dtype changes (model/llama.py:42-69); the
@@ -132,6 +161,7 @@ class RotaryEmbedding(nn.Module):
         self.register_buffer("inv_freq", inv_freq, persistent=False)
         self.max_seq_len_cached = 0
         self._captured = []  # tables that a captured call reads
+        self._built: Optional[_Built] = None
         self.register_buffer("cos_cached", torch.empty(0), persistent=False)
         self.register_buffer("sin_cached", torch.empty(0), persistent=False)
 
@@ -146,21 +176,27 @@ class RotaryEmbedding(nn.Module):
 
     def _tables(self, seq_len: int, device: torch.device, dtype: torch.dtype, block: int = 1
                 ) -> Tuple[torch.Tensor, torch.Tensor]:
-        """The cache, at least seq_len long.  Under capture: tables that the
-        graph keeps an address of stay, whatever replaces them in the cache;
-        what is built there (and by each replay) is the graph's alone, since it
-        holds nothing before a replay."""
-        cos, sin = self.cos_cached, self.sin_cached
-        if seq_len <= self.max_seq_len_cached and cos.device == device and cos.dtype == dtype:
-            if ops.capturing() and not any(kept is cos for kept, _ in self._captured):
-                self._captured.append((cos, sin))
+        """The cache, at least seq_len long, for the current stream.  Under
+        capture: tables that the graph keeps an address of stay, whatever
+        replaces them in the cache; what is built there (and by each replay) is
+        the graph's alone, since it holds nothing before a replay."""
+        with _tables_lock:
+            cos, sin = self.cos_cached, self.sin_cached
+            if seq_len <= self.max_seq_len_cached and cos.device == device and cos.dtype == dtype:
+                if ops.capturing():
+                    if not any(kept is cos for kept, _ in self._captured):
+                        self._captured.append((cos, sin))
+                elif self._built is not None:
+                    self._built.reach(device, cos, sin)
+                return cos, sin
+            old = cos, sin, self.max_seq_len_cached
+            self._build_cache(seq_len=-(-seq_len // block) * block, device=device, dtype=dtype)
+            cos, sin = self.cos_cached, self.sin_cached
+            if ops.capturing():
+                self.cos_cached, self.sin_cached, self.max_seq_len_cached = old
+            else:
+                self._built = _Built(device) if device.type == "cuda" else None
             return cos, sin
-        old = cos, sin, self.max_seq_len_cached
-        self._build_cache(seq_len=-(-seq_len // block) * block, device=device, dtype=dtype)
-        cos, sin = self.cos_cached, self.sin_cached
-        if ops.capturing():
-            self.cos_cached, self.sin_cached, self.max_seq_len_cached = old
-        return cos, sin
 
     def forward(self, seq_len: int, device: torch.device, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
         cos, sin = self._tables(seq_len, device, dtype)

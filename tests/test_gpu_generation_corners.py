@@ -14,6 +14,7 @@ from lzhip.cache import CacheStep, LayerCache
 from test_gpu_generation import BF16, DEV, E4M3, F16, F32, MUCH, U32, Case, _model, _u
 
 pytestmark = pytest.mark.gpu
+DEV0 = torch.device("cuda", 0)
 
 
 def _attention(c, q, H, scale, weights, terms):
@@ -405,3 +406,36 @@ def test_two_threads_generate_at_once():
     assert [m.training for m in model.modules()] == modes
     for a, b in zip(want, got):
         assert len(a) == len(b) == 11 and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("grow", [False, True])
+def test_rotary_tables_on_another_stream_than_they_were_built_on(grow):
+    """Tables that one stream has still to build, used by another; and old
+    ones, which another stream has still to read, replaced by longer ones."""
+    import copy
+
+    from model.llama import RotaryEmbedding
+
+    def rotary():
+        return RotaryEmbedding(64, 10_000.0).to(DEV)
+
+    want = [t.clone() for t in rotary().tables(100, DEV0, F32)]
+    rope, side = rotary(), torch.cuda.Stream()
+    if grow:
+        rope.tables(100, DEV0, F32)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            got = [t.clone() for t in rope.tables(100, DEV0, F32)]
+        rope.tables(5000, DEV0, F32)  # the old ones are free for what comes
+        junk = [torch.full((100, 64), 9.0, device=DEV) for _ in range(64)]
+    else:
+        junk = [torch.full((100, 64), 9.0, device=DEV) for _ in range(64)]
+        del junk
+        torch.cuda._sleep(20_000_000)
+        rope.tables(100, DEV0, F32)
+        with torch.cuda.stream(side):
+            got = [t.clone() for t in rope.tables(100, DEV0, F32)]
+            assert all(torch.equal(a, b) for a, b in zip(copy.deepcopy(rope).tables(100, DEV0, F32), got))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
