@@ -85,8 +85,8 @@ struct PagedRows {
 // latter's maximum is kept as kAllInf, beside which any finite score takes all
 // the weight.
 constexpr float kAllInf = -3.402823466e38f;
-__device__ __forceinline__ bool sees_any(const PagedArgs& a, int b, int k_lo, int k_hi, int sees) {
-  for (int key = k_lo; key < min(k_hi, sees); key += 16)
+__host__ __device__ __forceinline__ bool sees_any(const PagedArgs& a, int b, int k_lo, int k_hi, int sees) {
+  for (int key = k_lo; key < min(k_hi, sees); key = ((key >> a.pg.log_size) + 1) << a.pg.log_size)  // a page at a time
     if (a.pg.page_of(b, key) >= 0) return true;
   return false;
 }

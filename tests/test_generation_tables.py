@@ -63,3 +63,41 @@ def test_rows_of_any_table_are_rows_of_the_call(tmp_path):
     """Starts far past the last row, descending, negative: no row outside q
     and no more rows than there are."""
     run_on_host(tmp_path, ROWS)
+
+
+SEES = r"""
+#include "paged_attn.h"
+#include <cstdio>
+#include <vector>
+int main() {
+  int bad = 0;
+  for (int log_size : {4, 5, 8, 10})
+    for (int there = -1; there < 7; ++there) {  // the one page that there is
+      std::vector<int> table(14, -1);
+      if (there >= 0) table[7 + there] = 3;
+      PagedArgs a{};
+      a.pg = LzPages{table.data(), 7, 10, log_size};
+      for (int k_lo = 0; k_lo <= 7 << log_size; k_lo += 64)
+        for (int k_hi : {k_lo, k_lo + 1, k_lo + 64, 5 << log_size, 7 << log_size, 2147483647})
+          for (int sees : {0, 1, 63, 64, 65, 3 << log_size, (3 << log_size) + 1, 7 << log_size}) {
+            bool want = false;
+            for (int key = k_lo; key < k_hi && key < sees; ++key) want |= key >> log_size == there;
+            bad += sees_any(a, 1, k_lo, k_hi, sees) != want;
+          }
+    }
+  // the longest table there can be
+  std::vector<int> longest(2147483647 / 1024, -1);
+  PagedArgs a{};
+  a.pg = LzPages{longest.data(), (int)longest.size(), 10, 10};
+  const int cap = a.pg.width << 10;
+  bad += sees_any(a, 0, 0, 2147483647, cap);
+  longest.back() = 0;
+  bad += !sees_any(a, 0, cap - 1024, cap, cap) || sees_any(a, 0, 0, cap, cap - 1024);
+  printf("%d\n", bad);
+  return bad != 0;
+}
+"""
+
+
+def test_whether_a_row_sees_a_key(tmp_path):
+    run_on_host(tmp_path, SEES)
