@@ -43,6 +43,8 @@ SOURCES = [
     "paged_attn.hip",
     "paged_tile.hip",
     "logits.hip",
+    "tables.hip",
+    "verify.hip",
 ]
 
 COMMON_FLAGS = [

@@ -1,4 +1,5 @@
-// Writing a paged key/value cache and reading it back.
+// Writing a paged key/value cache, reading it back, and moving the tokens that
+// are kept of a draft.
 //
 // lz_kv_write takes the rows of a fused QKV product, rotates q and k at each
 // row's own position (NeoX half split: y1 = x1 c1 - x2 s1, y2 = x2 c2 + x1 s2,
@@ -93,11 +94,13 @@ struct WriteArgs {
   const int32_t* row_start;
   const int32_t* kv_len;
   int rows, positions, B, H, KV;
+  const int32_t* turn;  // kTurn: the position that each row is rotated to
 };
 
 // One thread per (row, head, 16 bytes of its lower half and the same of its
-// upper half): a head is HD / 2 / N neighbouring lanes.
-template <typename T, int HD, bool k8>
+// upper half): a head is HD / 2 / N neighbouring lanes.  kTurn: a drafted token's
+// position is its depth in its tree, not the place where it is cached.
+template <typename T, int HD, bool k8, bool kTurn>
 __global__ void __launch_bounds__(256) kv_write_kernel(WriteArgs a) {
   __shared__ LzSeqs seqs;
   seqs.load(a.row_start, a.kv_len, a.B, a.rows, threadIdx.x);
@@ -116,12 +119,12 @@ __global__ void __launch_bounds__(256) kv_write_kernel(WriteArgs a) {
   int base = 0;
   const int b = seqs.find(a.row_start, a.kv_len, a.B, a.rows, row, base);
   if (b < 0) return;
-  const int pos = base + row;
-  const bool there = pos >= 0 && pos < a.positions;
+  const int pos = base + row, turn = kTurn ? a.turn[row] : pos;
+  const bool there = turn >= 0 && turn < a.positions;
   if (head < a.H + a.KV) {
     if (there) {
-      const T* cp = static_cast<const T*>(a.cos) + (int64_t)pos * HD + i;
-      const T* sp = static_cast<const T*>(a.sin) + (int64_t)pos * HD + i;
+      const T* cp = static_cast<const T*>(a.cos) + (int64_t)turn * HD + i;
+      const T* sp = static_cast<const T*>(a.sin) + (int64_t)turn * HD + i;
       float c1[N], c2[N], s1[N], s2[N];
       Vec<T>::load(c1, cp);
       Vec<T>::load(c2, cp + HD / 2);
@@ -189,6 +192,70 @@ struct ReadArgs {
   int rows, B, KV;
 };
 
+struct KeepArgs {
+  void* k;
+  void* v;
+  int8_t* k_exp;
+  int8_t* v_exp;
+  const int64_t* slots;      // [rows]: page * page size + place in it, -1 without one
+  const int32_t* row_start;
+  const int32_t* kept;       // [B][ldk]
+  const int32_t* counts;
+  int64_t ldk, slots_all;    // slots of a layer
+  int rows, layers, KV, log_size, nodes;
+};
+
+// Moves the kept nodes of each sequence to its first slots of the step: node
+// kept[j]'s keys and values to slot j.  One thread per (layer, keys or values, kv
+// head, 16 bytes of a token), and gridDim.y for the sequences: it goes over the
+// nodes in their order, eight at a time, whose loads are in flight together.
+// kept ascends, so kept[j] >= j: what a thread still has to read lies behind what
+// it has written, and no other thread touches its bytes.
+template <bool k8>
+__global__ void __launch_bounds__(256) kv_keep_kernel(KeepArgs a, int chunks) {
+  const int b = blockIdx.y;
+  const int lo = min(max(a.row_start[b], 0), a.rows), hi = min(max(a.row_start[b + 1], lo), a.rows), n = hi - lo;
+  const int count = min(min(a.counts[b], n), a.nodes);
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t per_layer = 2u * (uint32_t)a.KV * (uint32_t)chunks;
+  const uint32_t layer = idx / per_layer, rem = idx - layer * per_layer;
+  if (layer >= (uint32_t)a.layers) return;
+  const int side = rem >= per_layer / 2, at = (int)(rem - side * (per_layer / 2));
+  const int g = at / chunks, c = at - g * chunks;
+  const int64_t token = (int64_t)layer * a.slots_all * a.KV;  // of the layer's first page and head
+  char* x = static_cast<char*>(side ? a.v : a.k) + (token * chunks + c) * 16;
+  int8_t* e = k8 ? (side ? a.v_exp : a.k_exp) + token : nullptr;
+  const int mask = (1 << a.log_size) - 1;
+  auto place = [&](int64_t slot) {  // of this head, in tokens
+    return ((((slot >> a.log_size) * a.KV + g) << a.log_size) + (slot & mask));
+  };
+  constexpr int kAhead = 8;
+  for (int j0 = 0; j0 < count; j0 += kAhead) {
+    int64_t dst[kAhead];
+    uint4 w[kAhead];
+    int8_t we[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int j = j0 + i;
+      dst[i] = -1;
+      const int node = j < count ? a.kept[b * a.ldk + j] : -1;
+      if (node < 0 || node >= n || node == j) continue;
+      const int64_t from = a.slots[lo + node], to = a.slots[lo + j];
+      if (from < 0 || from >= a.slots_all || to < 0 || to >= a.slots_all) continue;
+      dst[i] = place(to);
+      const int64_t src = place(from);
+      w[i] = *reinterpret_cast<const uint4*>(x + src * chunks * 16);
+      if (k8 && c == 0) we[i] = e[src];
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (dst[i] >= 0) {
+        *reinterpret_cast<uint4*>(x + dst[i] * chunks * 16) = w[i];
+        if (k8 && c == 0) e[dst[i]] = we[i];
+      }
+  }
+}
+
 // One thread per 16 bytes of an output row, keys and values alike.
 template <typename T, int HD, bool k8>
 __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
@@ -253,34 +320,85 @@ int lz_check_pages(const char* what, const void* k, const void* v, const void* k
   return LZ_OK;
 }
 
+static int write(const char* what, const void* qkv, int64_t ld, int dtype, int64_t rows, const void* cos_t,
+                 const void* sin_t, int64_t positions, void* q_out, int64_t ldq, void* k, void* v, void* k_exp, void* v_exp,
+                 int cache_dtype, int64_t pages, int64_t page_size, const int32_t* table, int64_t width,
+                 const int32_t* row_start, const int32_t* kv_len, const int32_t* turn, int64_t B, int64_t H, int64_t KV,
+                 int64_t hd, void* stream) {
+  if (int rc = lz_check_pages(what, k, v, k_exp, v_exp, cache_dtype, dtype, pages, page_size, table, width, B, KV,
+                           hd))
+    return rc;
+  const int esz = lz_esize(dtype);
+  LZ_REQUIRE(rows >= 0 && rows <= INT32_MAX && H > 0 && H <= 65536 && positions > 0 && positions <= INT32_MAX,
+             "%s: bad shape", what);
+  LZ_REQUIRE(ld >= (H + 2 * KV) * hd && ldq >= H * hd, "%s: row strides shorter than the rows", what);
+  LZ_REQUIRE(rows == 0 || (qkv && q_out && cos_t && sin_t && row_start && kv_len && lz_aligned16(qkv) &&
+                           lz_aligned16(q_out) && lz_aligned16(cos_t) && lz_aligned16(sin_t) && ld * esz % 16 == 0 &&
+                           ldq * esz % 16 == 0),
+             "%s: rows and tables must be 16-byte aligned", what);
+  if (rows == 0) return LZ_OK;
+  const int64_t threads = rows * (H + 2 * KV) * (hd * esz / 32);
+  LZ_REQUIRE(threads <= (int64_t)UINT32_MAX - 255, "%s: too many rows", what);
+  WriteArgs a{qkv, ld, cos_t, sin_t, q_out, ldq, k, v, (int8_t*)k_exp, (int8_t*)v_exp,
+              LzPages{table, (int)width, (int)pages, lz_log2(page_size)}, row_start, kv_len,
+              (int)rows, (int)positions, (int)B, (int)H, (int)KV, turn};
+  const uint32_t grid = (uint32_t)lz_cdiv(threads, 256);
+  hipStream_t s = lz_stream(stream);
+#define RUN(T, HD, E8)                                                   \
+  do {                                                                   \
+    if (turn) kv_write_kernel<T, HD, E8, true><<<grid, 256, 0, s>>>(a);  \
+    else kv_write_kernel<T, HD, E8, false><<<grid, 256, 0, s>>>(a);      \
+  } while (0)
+  LZ_CACHE_CASES(dtype, cache_dtype, hd, RUN);
+#undef RUN
+  return lz_check_launch(what);
+}
+
 LZ_EXPORT int lz_kv_write(const void* qkv, int64_t ld, int dtype, int64_t rows, const void* cos_t, const void* sin_t,
                           int64_t positions, void* q_out, int64_t ldq, void* k, void* v, void* k_exp, void* v_exp,
                           int cache_dtype, int64_t pages, int64_t page_size, const int32_t* table, int64_t width,
                           const int32_t* row_start, const int32_t* kv_len, int64_t B, int64_t H, int64_t KV, int64_t hd,
                           void* stream) {
-  if (int rc = lz_check_pages("lz_kv_write", k, v, k_exp, v_exp, cache_dtype, dtype, pages, page_size, table, width, B, KV,
-                           hd))
-    return rc;
-  const int esz = lz_esize(dtype);
-  LZ_REQUIRE(rows >= 0 && rows <= INT32_MAX && H > 0 && H <= 65536 && positions > 0 && positions <= INT32_MAX,
-             "lz_kv_write: bad shape");
-  LZ_REQUIRE(ld >= (H + 2 * KV) * hd && ldq >= H * hd, "lz_kv_write: row strides shorter than the rows");
-  LZ_REQUIRE(rows == 0 || (qkv && q_out && cos_t && sin_t && row_start && kv_len && lz_aligned16(qkv) &&
-                           lz_aligned16(q_out) && lz_aligned16(cos_t) && lz_aligned16(sin_t) && ld * esz % 16 == 0 &&
-                           ldq * esz % 16 == 0),
-             "lz_kv_write: rows and tables must be 16-byte aligned");
-  if (rows == 0) return LZ_OK;
-  const int64_t threads = rows * (H + 2 * KV) * (hd * esz / 32);
-  LZ_REQUIRE(threads <= (int64_t)UINT32_MAX - 255, "lz_kv_write: too many rows");
-  WriteArgs a{qkv, ld, cos_t, sin_t, q_out, ldq, k, v, (int8_t*)k_exp, (int8_t*)v_exp,
-              LzPages{table, (int)width, (int)pages, lz_log2(page_size)}, row_start, kv_len,
-              (int)rows, (int)positions, (int)B, (int)H, (int)KV};
-  const uint32_t grid = (uint32_t)lz_cdiv(threads, 256);
-#define RUN(T, HD, E8) kv_write_kernel<T, HD, E8><<<grid, 256, 0, lz_stream(stream)>>>(a)
-  LZ_CACHE_CASES(dtype, cache_dtype, hd, RUN);
-#undef RUN
-  return lz_check_launch("lz_kv_write");
+  return write("lz_kv_write", qkv, ld, dtype, rows, cos_t, sin_t, positions, q_out, ldq, k, v, k_exp, v_exp, cache_dtype,
+               pages, page_size, table, width, row_start, kv_len, nullptr, B, H, KV, hd, stream);
 }
+
+LZ_EXPORT int lz_kv_write_at(const void* qkv, int64_t ld, int dtype, int64_t rows, const void* cos_t, const void* sin_t,
+                             int64_t positions, void* q_out, int64_t ldq, void* k, void* v, void* k_exp, void* v_exp,
+                             int cache_dtype, int64_t pages, int64_t page_size, const int32_t* table, int64_t width,
+                             const int32_t* row_start, const int32_t* kv_len, const int32_t* row_position, int64_t B,
+                             int64_t H, int64_t KV, int64_t hd, void* stream) {
+  LZ_REQUIRE(rows == 0 || row_position, "lz_kv_write_at: no positions");
+  return write("lz_kv_write_at", qkv, ld, dtype, rows, cos_t, sin_t, positions, q_out, ldq, k, v, k_exp, v_exp, cache_dtype,
+               pages, page_size, table, width, row_start, kv_len, row_position, B, H, KV, hd, stream);
+}
+
+LZ_EXPORT int lz_kv_keep(void* k, void* v, void* k_exp, void* v_exp, int cache_dtype, int64_t layers, int64_t pages,
+                         int64_t page_size, int64_t KV, int64_t hd, const int64_t* slots, int64_t rows,
+                         const int32_t* row_start, int64_t B, const int32_t* kept, int64_t ldk, int64_t nodes,
+                         const int32_t* counts, void* stream) {
+  LZ_REQUIRE(cache_dtype == LZ_BF16 || cache_dtype == LZ_F16 || cache_dtype == LZ_F32 || cache_dtype == LZ_E4M3,
+             "lz_kv_keep: bad dtype %d", cache_dtype);
+  LZ_REQUIRE(hd == 32 || hd == 64 || hd == 128, "lz_kv_keep: head dim %lld (32, 64 or 128)", (long long)hd);
+  LZ_REQUIRE(lz_page_size_ok(page_size), "lz_kv_keep: page size %lld (a power of two, 16 to 1024)", (long long)page_size);
+  LZ_REQUIRE(layers > 0 && layers <= 65536 && pages > 0 && pages <= INT32_MAX && KV > 0 && KV <= 65536 && B > 0 &&
+                 B <= 65535 && rows >= 0 && rows <= INT32_MAX && nodes >= 0 && nodes <= INT32_MAX,
+             "lz_kv_keep: bad shape");
+  LZ_REQUIRE(k && v && lz_aligned16(k) && lz_aligned16(v), "lz_kv_keep: pages must be 16-byte aligned");
+  LZ_REQUIRE(cache_dtype != LZ_E4M3 || (k_exp && v_exp), "lz_kv_keep: an e4m3 cache needs its exponents");
+  if (rows == 0 || nodes == 0) return LZ_OK;
+  LZ_REQUIRE(slots && row_start && kept && counts && ldk >= nodes, "lz_kv_keep: bad arguments");
+  const bool e8 = cache_dtype == LZ_E4M3;
+  const int64_t chunks = hd * (e8 ? 1 : lz_esize(cache_dtype)) / 16, threads = layers * 2 * KV * chunks;
+  LZ_REQUIRE(threads <= (int64_t)UINT32_MAX - 255, "lz_kv_keep: too many heads");
+  KeepArgs a{k, v, (int8_t*)k_exp, (int8_t*)v_exp, slots, row_start, kept, counts, ldk, pages * page_size,
+             (int)rows, (int)layers, (int)KV, lz_log2(page_size), (int)nodes};
+  const dim3 grid((uint32_t)lz_cdiv(threads, 256), (uint32_t)B);
+  if (e8) kv_keep_kernel<true><<<grid, 256, 0, lz_stream(stream)>>>(a, (int)chunks);
+  else kv_keep_kernel<false><<<grid, 256, 0, lz_stream(stream)>>>(a, (int)chunks);
+  return lz_check_launch("lz_kv_keep");
+}
+
 
 LZ_EXPORT int lz_kv_read(const void* k, const void* v, const void* k_exp, const void* v_exp, int cache_dtype,
                          int64_t pages, int64_t page_size, const int32_t* table, int64_t width, const int32_t* start,

@@ -24,10 +24,15 @@ struct LzPagedArgs {
   float scale;
   int rows, B, H, KV, nqb, nsplit, chunk;
   int most;  // packed rows of a sequence that the grid is for; those behind them are left
+  // trees of drafted tokens (null: the rows are causal, each seeing those before it)
+  const int32_t* base;    // [B]: the tokens that every row of the sequence sees
+  const uint32_t* mask;   // [rows][words]: bit j of a row: it sees token base + j
+  int words;
 };
 
 // paged_tile.hip: 16-bit rows in blocks of kPagedTileRows; `groups`
-// (1 or 2) of its waves share a block's keys.  LZ_OK or a status.
+// (1 or 2) of its waves share a block's keys; trees where a.mask is set.  LZ_OK
+// or a status.
 constexpr int kPagedTileRows = 128;
 int lz_paged_tile(const LzPagedArgs& a, int dtype, bool e4m3, int64_t hd, int groups, uint32_t blocks, hipStream_t stream);
 
@@ -72,12 +77,41 @@ struct PagedRows {
   }
   __host__ __device__ __forceinline__ int row(int m) const { return row0 + m / G; }
   __host__ __device__ __forceinline__ int sees(int m) const { return min(max((int)((uint32_t)base + (uint32_t)row(m)), 0), cap); }
+  // the keys that every row from m on sees, all of them
+  __host__ __device__ __forceinline__ int all(int m) const { return sees(m); }
   // the keys that the block's rows see together, and the parts they make
   __host__ __device__ __forceinline__ int keys(int bm) const { return sees(min(m0 + bm, count) - 1); }
   static __host__ __device__ __forceinline__ int parts(const PagedArgs& a, int keys) {
     return min(max((int)(((uint32_t)keys + (uint32_t)a.chunk - 1) / (uint32_t)a.chunk), 1), a.nsplit);
   }
 };
+
+// The same of a tree: every row sees the sequence's first `ctx` keys, and of the
+// others, up to the last of `len`, those whose bits are set in its mask.
+struct TreeRows : PagedRows {
+  int len, ctx;
+  __host__ __device__ __forceinline__ TreeRows(const PagedArgs& a, int b, int m0_)
+      : TreeRows(a, b, a.row_start[b], a.row_start[b + 1], a.kv_len[b], m0_) {}
+  __host__ __device__ __forceinline__ TreeRows(const PagedArgs& a, int b, int lo, int hi, int n, int m0_)
+      : PagedRows(a, lo, hi, n, m0_) {
+    len = min(max(n, 0), cap);
+    ctx = min(max(a.base[b], 0), len);
+  }
+  __host__ __device__ __forceinline__ int sees(int) const { return len; }
+  __host__ __device__ __forceinline__ int all(int) const { return ctx; }
+  __host__ __device__ __forceinline__ int keys(int) const { return len; }
+};
+
+// Bit k: a row of a tree sees the key `off` + k, counted from the first that not
+// all rows see (those before it are seen).  `row`: its mask.
+__host__ __device__ __forceinline__ uint32_t tree_bits(const uint32_t* row, int words, int off) {
+  if (off <= -32) return ~0u;
+  const int i = off >> 5, s = off & 31;  // word -1: keys that all rows see
+  const uint32_t lo = i < 0 ? ~0u : i < words ? row[i] : 0u;
+  if (s == 0) return lo;
+  const uint32_t hi = i + 1 < words ? row[i + 1] : 0u;
+  return lo >> s | hi << (32 - s);
+}
 
 // Whether a row that sees `sees` keys sees one of k_lo .. k_hi - 1 (of pages
 // that there are).  A maximum of -inf says that it does not or that all its
@@ -89,6 +123,21 @@ __host__ __device__ __forceinline__ bool sees_any(const PagedArgs& a, int b, int
   for (int key = k_lo; key < min(k_hi, sees); key = ((key >> a.pg.log_size) + 1) << a.pg.log_size)  // a page at a time
     if (a.pg.page_of(b, key) >= 0) return true;
   return false;
+}
+
+// The same of a tree's row.
+__host__ __device__ __forceinline__ bool sees_any(const PagedArgs& a, int b, int k_lo, int k_hi, const TreeRows& rw, int row) {
+  if (sees_any(a, b, k_lo, k_hi, rw.ctx)) return true;
+  const uint32_t* mask = a.mask + (int64_t)row * a.words;
+  for (int key = max(k_lo, rw.ctx); key < min(k_hi, rw.len); ++key)
+    if ((tree_bits(mask, a.words, key - rw.ctx) & 1) && a.pg.page_of(b, key) >= 0) return true;
+  return false;
+}
+__host__ __device__ __forceinline__ bool sees_any(const PagedArgs& a, int b, int k_lo, int k_hi, const PagedRows& rw, int, int m) {
+  return sees_any(a, b, k_lo, k_hi, rw.sees(m));
+}
+__host__ __device__ __forceinline__ bool sees_any(const PagedArgs& a, int b, int k_lo, int k_hi, const TreeRows& rw, int row, int) {
+  return sees_any(a, b, k_lo, k_hi, rw, row);
 }
 
 // A row's reference m for its weights 2^(s - m) (log2 units) is its running

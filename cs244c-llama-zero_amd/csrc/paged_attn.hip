@@ -3,7 +3,8 @@
 //   o_i = sum_j softmax_j(scale * q_i . k_j) v_j,  j <= kv_len - new + i
 //
 // for the i-th of a sequence's `new` last tokens, whose keys and values are in
-// the cache already.  One pass over the keys with a running maximum and sum:
+// the cache already; or, for a tree of drafted tokens, j < base and those j after
+// them whose bits are set in row i's mask.  One pass over the keys with a running maximum and sum:
 // per tile, S^T = K . Q^T, so that a lane owns one row's column and the
 // probabilities are the B operand of O^T += V^T . P^T as they stand.
 //
@@ -232,8 +233,11 @@ __device__ __forceinline__ void store_row4(const PagedArgs& a, int row, int head
   }
 }
 
-template <typename T, int HD, bool k8, int NQ>
+// Rows: PagedRows, or TreeRows, whose tiles from the first key that not all rows
+// see on take each row's bits of its mask.
+template <typename T, int HD, bool k8, int NQ, typename Rows>
 __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
+  constexpr bool kTree = std::is_same<Rows, TreeRows>::value;
   typedef Wave<T, HD, k8, NQ> W;
   constexpr int BM = 16 * NQ, KT = W::KT, NT = W::NT, VE = W::VE;
   constexpr int RS = HD + 4;  // floats of a parked row
@@ -251,7 +255,7 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
   auto key_of = [&](int x) { return k_lo + ((x / NT) * 4 + wave) * KT + 16 * (x % NT); };
   const int first_ids = a.pg.page_of(at.b, key_of(lane));
 
-  const PagedRows rw(a, at.b, at.qb * BM);
+  const Rows rw(a, at.b, at.qb * BM);
   if (rw.m0 >= rw.count) return;
   const int n_keys = rw.keys(BM), n_parts = PagedRows::parts(a, n_keys);
   if (at.split >= n_parts) return;
@@ -259,13 +263,15 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
 
   typename W::Query q[NQ];
   int sees[NQ];
+  const uint32_t* mask[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int m = min(rw.m0 + 16 * n + c16, rw.count - 1);  // rows past the last repeat it and are not stored
     sees[n] = rw.sees(m);
+    if constexpr (kTree) mask[n] = a.mask + (int64_t)rw.row(m) * a.words;
     q[n].load(static_cast<const T*>(a.q) + (int64_t)rw.row(m) * a.ldq + (at.g * rw.G + m % rw.G) * HD, g4);
   }
-  const int all_see = rw.sees(rw.m0);  // keys that every row of the block sees
+  const int all_see = rw.all(rw.m0);  // keys that every row of the block sees
 
   f32x4_t acc[NQ][VE];
   float mx[NQ], sum[NQ];
@@ -326,11 +332,14 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
         if (holes) {
+          uint32_t bits = 0;
+          if constexpr (kTree) bits = tree_bits(mask[n], a.words, key0 - all_see) >> (4 * g4);
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (tok[t] < 0 || key0 + 16 * t + 4 * g4 + i >= sees[n]) s[n][t][i] = -INFINITY;
+              if (tok[t] < 0 || key0 + 16 * t + 4 * g4 + i >= sees[n] || (kTree && !((bits >> (16 * t + i)) & 1)))
+                s[n][t][i] = -INFINITY;
         }
         float top = s[n][0][0];
 #pragma unroll
@@ -402,7 +411,9 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) p = kk / 16 == t && kk % 4 == i ? s[n][t][i] : p;
             p = __shfl(p, c16 + 16 * (kk % 16 / 4), 64);
-            if (key0 + kk < sees[n]) {
+            bool seen = key0 + kk < sees[n];
+            if constexpr (kTree) seen = seen && (tree_bits(mask[n], a.words, key0 + kk - all_see) & 1);
+            if (seen) {
 #pragma unroll
               for (int j = 0; j < VE; ++j)
 #pragma unroll
@@ -462,8 +473,8 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
       y.z = fmaf(f, z.z, y.z);
       y.w = fmaf(f, z.w, y.w);
     }
-    if (top == -INFINITY && sees_any(a, at.b, k_lo, k_hi, rw.sees(m))) top = kAllInf;
     const int row = rw.row(m), head = at.g * rw.G + m % rw.G;
+    if (top == -INFINITY && sees_any(a, at.b, k_lo, k_hi, rw, row, m)) top = kAllInf;
     if (n_parts == 1) {
       const float inv = top == -INFINITY ? 0.f : 1.f / l;
       store_row4<T, HD>(a, row, head, d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
@@ -482,7 +493,7 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
 // The parts of rows that were split, joined: `per` groups of HD / 4 lanes for
 // one (row, head), each with every per-th part, all loads of a thread
 // independent; the groups meet in LDS in a fixed order.
-template <typename T, int HD>
+template <typename T, int HD, typename Rows>
 __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm, int per) {
   constexpr int kLanes = HD / 4;
   __shared__ float4 ys[256];
@@ -518,7 +529,10 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm, in
       }
     }
     if (b >= 0) {
-      PagedRows rw(a, lo, hi, len, 0);
+      Rows rw = [&] {
+        if constexpr (std::is_same<Rows, TreeRows>::value) return TreeRows(a, b, lo, hi, len, 0);
+        else return PagedRows(a, lo, hi, len, 0);
+      }();
       const int m = (row - rw.row0) * rw.G + head % rw.G;
       rw.m0 = m / bm * bm;
       if (m < rw.count) n_parts = PagedRows::parts(a, rw.keys(bm));
@@ -652,49 +666,89 @@ LZ_EXPORT int64_t lz_paged_attn_workspace(int dtype, int cache_dtype, int64_t ro
   return p.nsplit > 1 ? rows * H * p.nsplit * (hd + 2) * 4 : 0;
 }
 
-LZ_EXPORT int lz_paged_attn(const void* q, int64_t ldq, int dtype, int64_t rows, const void* k, const void* v,
-                            const void* k_exp, const void* v_exp, int cache_dtype, int64_t pages, int64_t page_size,
-                            const int32_t* table, int64_t width, const int32_t* row_start, const int32_t* kv_len,
-                            int64_t B, int64_t H, int64_t KV, int64_t hd, int64_t max_new, int64_t max_len, float scale,
-                            void* o, int64_t ldo, void* workspace, int64_t ws_bytes, void* stream) {
-  if (int rc = lz_check_pages("lz_paged_attn", k, v, k_exp, v_exp, cache_dtype, dtype, pages, page_size, table, width, B,
+LZ_EXPORT int64_t lz_tree_attn_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd,
+                                    int64_t max_new, int64_t max_len) {
+  return lz_paged_attn_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
+}
+
+LZ_EXPORT int64_t lz_tree_attn_workspace(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV,
+                                         int64_t hd, int64_t max_new, int64_t max_len) {
+  return lz_paged_attn_workspace(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
+}
+
+template <typename Rows>
+static void launch(const PagedArgs& a, const Plan& p, int dtype, int cache_dtype, int64_t hd, uint32_t blocks, uint32_t joins,
+                   int per, hipStream_t s) {
+#define RUN(T, HD, E8)                                                              \
+  do {                                                                              \
+    if (p.bm == 16) paged_wave_kernel<T, HD, E8, 1, Rows><<<blocks, 256, 0, s>>>(a); \
+    else paged_wave_kernel<T, HD, E8, 2, Rows><<<blocks, 256, 0, s>>>(a);           \
+  } while (0)
+  if (p.bm != kPagedTileRows) LZ_CACHE_CASES(dtype, cache_dtype, hd, RUN);
+#undef RUN
+#define RUN(T, HD, E8) paged_join_kernel<T, HD, Rows><<<joins, 256, 0, s>>>(a, p.bm, per)
+  if (p.nsplit > 1) LZ_CACHE_CASES(dtype, 0, hd, RUN);
+#undef RUN
+}
+
+static int attend(const char* what, const void* q, int64_t ldq, int dtype, int64_t rows, const void* k, const void* v,
+                  const void* k_exp, const void* v_exp, int cache_dtype, int64_t pages, int64_t page_size,
+                  const int32_t* table, int64_t width, const int32_t* row_start, const int32_t* kv_len, int64_t B,
+                  int64_t H, int64_t KV, int64_t hd, int64_t max_new, int64_t max_len, float scale, void* o, int64_t ldo,
+                  void* workspace, int64_t ws_bytes, void* stream, const int32_t* base, const uint32_t* mask,
+                  int64_t words) {
+  if (int rc = lz_check_pages(what, k, v, k_exp, v_exp, cache_dtype, dtype, pages, page_size, table, width, B,
                               KV, hd))
     return rc;
   const int esz = lz_esize(dtype);
   LZ_REQUIRE(H > 0 && H % KV == 0 && H <= 65536 && rows >= 0 && rows * H <= INT32_MAX / 64 && max_new >= 0 &&
                  max_len >= 0 && max_len <= INT32_MAX - 1024,
-             "lz_paged_attn: bad shape");
+             "%s: bad shape", what);
   // (-inf, a masked score, times 0 or a subnormal that is flushed would be NaN)
-  LZ_REQUIRE(scale >= std::numeric_limits<float>::min() && scale * kLog2e < INFINITY, "lz_paged_attn: scale %g", (double)scale);
-  LZ_REQUIRE(ldq >= H * hd && ldo >= H * hd, "lz_paged_attn: row strides shorter than the rows");
+  LZ_REQUIRE(scale >= std::numeric_limits<float>::min() && scale * kLog2e < INFINITY, "%s: scale %g", what, (double)scale);
+  LZ_REQUIRE(ldq >= H * hd && ldo >= H * hd, "%s: row strides shorter than the rows", what);
   LZ_REQUIRE(rows == 0 || (q && o && row_start && kv_len && lz_aligned16(q) && lz_aligned16(o) && ldq * esz % 16 == 0 &&
                            ldo * esz % 16 == 0),
-             "lz_paged_attn: rows must be 16-byte aligned");
+             "%s: rows must be 16-byte aligned", what);
   if (rows == 0) return LZ_OK;
   const Plan p = make_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
   const int64_t need = lz_paged_attn_workspace(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
   LZ_REQUIRE(need == 0 || (workspace && lz_aligned16(workspace) && ws_bytes >= need),
-             "lz_paged_attn: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
+             "%s: workspace of %lld bytes, %lld needed", what, (long long)ws_bytes, (long long)need);
   const int64_t blocks = B * KV * p.nqb * p.nsplit, per = p.nsplit <= 4 ? 1 : p.nsplit <= 16 ? 4 : 8,
                 joins = lz_cdiv(rows * H * (hd / 4) * per, 256);
-  LZ_REQUIRE(blocks <= INT32_MAX / 256 && joins <= INT32_MAX / 256, "lz_paged_attn: too many rows");
+  LZ_REQUIRE(blocks <= INT32_MAX / 256 && joins <= INT32_MAX / 256, "%s: too many rows", what);
   PagedArgs a{q, ldq, k, v, (const int8_t*)k_exp, (const int8_t*)v_exp,
               LzPages{table, (int)width, (int)pages, lz_log2(page_size)}, row_start, kv_len, o, ldo, (float*)workspace,
               scale, (int)rows, (int)B, (int)H, (int)KV, p.nqb, p.nsplit, p.chunk,
-              (int)(std::min(max_new, rows) * (H / KV))};
+              (int)(std::min(max_new, rows) * (H / KV)), base, mask, (int)words};
   hipStream_t s = lz_stream(stream);
-  const bool tiles = p.bm == kPagedTileRows;
-  if (tiles)
+  if (p.bm == kPagedTileRows)
     if (int rc = lz_paged_tile(a, dtype, cache_dtype == LZ_E4M3, hd, p.groups, (uint32_t)blocks, s)) return rc;
-#define RUN(T, HD, E8)                                                                    \
-  do {                                                                                    \
-    if (p.bm == 16) paged_wave_kernel<T, HD, E8, 1><<<(uint32_t)blocks, 256, 0, s>>>(a);  \
-    else paged_wave_kernel<T, HD, E8, 2><<<(uint32_t)blocks, 256, 0, s>>>(a);             \
-  } while (0)
-  if (!tiles) LZ_CACHE_CASES(dtype, cache_dtype, hd, RUN);
-#undef RUN
-#define RUN(T, HD, E8) paged_join_kernel<T, HD><<<(uint32_t)joins, 256, 0, s>>>(a, p.bm, (int)per)
-  if (p.nsplit > 1) LZ_CACHE_CASES(dtype, 0, hd, RUN);
-#undef RUN
-  return lz_check_launch("lz_paged_attn");
+  if (mask) launch<TreeRows>(a, p, dtype, cache_dtype, hd, (uint32_t)blocks, (uint32_t)joins, (int)per, s);
+  else launch<PagedRows>(a, p, dtype, cache_dtype, hd, (uint32_t)blocks, (uint32_t)joins, (int)per, s);
+  return lz_check_launch(what);
+}
+
+LZ_EXPORT int lz_paged_attn(const void* q, int64_t ldq, int dtype, int64_t rows, const void* k, const void* v,
+                            const void* k_exp, const void* v_exp, int cache_dtype, int64_t pages, int64_t page_size,
+                            const int32_t* table, int64_t width, const int32_t* row_start, const int32_t* kv_len,
+                            int64_t B, int64_t H, int64_t KV, int64_t hd, int64_t max_new, int64_t max_len, float scale,
+                            void* o, int64_t ldo, void* workspace, int64_t ws_bytes, void* stream) {
+  return attend("lz_paged_attn", q, ldq, dtype, rows, k, v, k_exp, v_exp, cache_dtype, pages, page_size, table, width,
+                row_start, kv_len, B, H, KV, hd, max_new, max_len, scale, o, ldo, workspace, ws_bytes, stream, nullptr,
+                nullptr, 0);
+}
+
+LZ_EXPORT int lz_tree_attn(const void* q, int64_t ldq, int dtype, int64_t rows, const void* k, const void* v,
+                           const void* k_exp, const void* v_exp, int cache_dtype, int64_t pages, int64_t page_size,
+                           const int32_t* table, int64_t width, const int32_t* row_start, const int32_t* kv_len,
+                           const int32_t* base, const int32_t* mask, int64_t words, int64_t B, int64_t H, int64_t KV,
+                           int64_t hd, int64_t max_new, int64_t max_len, float scale, void* o, int64_t ldo,
+                           void* workspace, int64_t ws_bytes, void* stream) {
+  LZ_REQUIRE(words > 0 && words <= (1 << 20), "lz_tree_attn: %lld mask words a row", (long long)words);
+  LZ_REQUIRE(rows == 0 || (base && mask), "lz_tree_attn: no mask");
+  return attend("lz_tree_attn", q, ldq, dtype, rows, k, v, k_exp, v_exp, cache_dtype, pages, page_size, table, width,
+                row_start, kv_len, B, H, KV, hd, max_new, max_len, scale, o, ldo, workspace, ws_bytes, stream, base,
+                (const uint32_t*)mask, words);
 }

@@ -140,6 +140,14 @@ Slot kSlots[] = {
     LZ_ENTRY(lz_paged_attn_plan),
     LZ_ENTRY(lz_paged_attn),
     LZ_ENTRY(lz_process_logits),
+    LZ_ENTRY(lz_kv_write_at),
+    LZ_ENTRY(lz_kv_keep),
+    LZ_ENTRY(lz_tree_attn_workspace),
+    LZ_ENTRY(lz_tree_attn_plan),
+    LZ_ENTRY(lz_tree_attn),
+    LZ_ENTRY(lz_cache_tables),
+    LZ_ENTRY(lz_verify_workspace),
+    LZ_ENTRY(lz_verify_draft),
 };
 
 PyObject* bind(PyObject*, PyObject* args) {

@@ -1,5 +1,6 @@
 // Tensor-level entry of generation's operators (lzhip/ops.py: kv_cache_write,
-// kv_cache_read, paged_attention, process_logits): arguments checked, outputs
+// kv_cache_read, paged_attention, process_logits, and for drafted tokens
+// cache_tables, verify_draft, kv_cache_keep): arguments checked, outputs
 // and workspaces allocated and the C ABI called in compiled code.  A decoded
 // token's kernels run for 4 to 5 us each; with the checks and allocations in
 // Python a call took 9.6 us of host time, so it takes 4.8, 3 of them the launch.
@@ -38,6 +39,13 @@ decltype(&lz_kv_read) p_read = nullptr;
 decltype(&lz_paged_attn) p_attn = nullptr;
 decltype(&lz_paged_attn_workspace) p_attn_ws = nullptr;
 decltype(&lz_process_logits) p_logits = nullptr;
+decltype(&lz_kv_write_at) p_write_at = nullptr;
+decltype(&lz_kv_keep) p_keep = nullptr;
+decltype(&lz_tree_attn) p_tree = nullptr;
+decltype(&lz_tree_attn_workspace) p_tree_ws = nullptr;
+decltype(&lz_cache_tables) p_tables = nullptr;
+decltype(&lz_verify_draft) p_verify = nullptr;
+decltype(&lz_verify_workspace) p_verify_ws = nullptr;
 decltype(&lz_copy2d) p_copy = nullptr;
 decltype(&lz_fill) p_fill = nullptr;
 decltype(&lz_last_error) p_error = nullptr;
@@ -205,19 +213,26 @@ struct Cache {
   }
 };
 
-// A CacheStep, checked.
+constexpr Py_ssize_t kDraft = 10;  // fields of a DraftStep
+bool is_draft(PyObject* step) { return PyTuple_Check(step) && PyTuple_GET_SIZE(step) == kDraft; }
+
+// A CacheStep or a DraftStep, checked.
 struct Step {
   const at::Tensor *start, *len, *table;
+  const at::Tensor *base = nullptr, *positions = nullptr, *mask = nullptr;  // of a DraftStep
   int64_t rows, max_new, max_len, B, width;
 
   // x: the call's rows, of which there may be more than the step has
   Step(PyObject* step, const at::Tensor& x, const Place& at) {
-    start = &tensor(item(step, 0, 6, "CacheStep"), "row_start");
-    len = &tensor(item(step, 1, 6, "CacheStep"), "kv_len");
-    table = &tensor(item(step, 2, 6, "CacheStep"), "page_table");
-    rows = integer(item(step, 3, 6, "CacheStep"));
-    max_new = integer(item(step, 4, 6, "CacheStep"));
-    max_len = integer(item(step, 5, 6, "CacheStep"));
+    const bool draft = is_draft(step);
+    const Py_ssize_t fields = draft ? kDraft : 6;
+    const char* type = draft ? "DraftStep" : "CacheStep";
+    start = &tensor(item(step, 0, fields, type), "row_start");
+    len = &tensor(item(step, 1, fields, type), "kv_len");
+    table = &tensor(item(step, 2, fields, type), "page_table");
+    rows = integer(item(step, 3, fields, type));
+    max_new = integer(item(step, 4, fields, type));
+    max_len = integer(item(step, 5, fields, type));
     int32_table(*start, "row_start", at, 1);
     int32_table(*len, "kv_len", at, 1);
     int32_table(*table, "page_table", at, 2);
@@ -232,6 +247,17 @@ struct Step {
       refuse(PyExc_ValueError, "a step of %lld rows, at most %lld of each of %lld sequences and %lld cached, does not fit "
                                "rows %s", (long long)rows, (long long)max_new, (long long)B, (long long)max_len,
              shape(x).c_str());
+    if (!draft) return;
+    base = &tensor(PyTuple_GET_ITEM(step, 6), "base");
+    positions = &tensor(PyTuple_GET_ITEM(step, 7), "positions");
+    mask = maybe(PyTuple_GET_ITEM(step, 9), "mask");
+    int32_table(*base, "base", at, 1);
+    int32_table(*positions, "positions", at, 1);
+    if (mask) int32_table(*mask, "mask", at, 2);
+    if (base->size(0) != B || positions->size(0) < rows || (mask && (mask->size(0) < rows || mask->size(1) == 0)))
+      refuse(PyExc_ValueError, "a draft of %lld sequences and %lld rows does not fit base %s, positions %s and mask %s",
+             (long long)B, (long long)rows, shape(*base).c_str(), shape(*positions).c_str(),
+             mask ? shape(*mask).c_str() : "None");
   }
 };
 
@@ -314,7 +340,7 @@ void expect(Py_ssize_t got, Py_ssize_t want) {
   if (got != want) refuse(PyExc_TypeError, "this function takes %zd arguments (%zd given)", want, got);
 }
 
-// ---- the four calls -------------------------------------------------------
+// ---- the cache's and the logits' calls -------------------------------------------------------
 
 PyObject* kv_cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -336,6 +362,14 @@ PyObject* kv_cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     const Out q(a[6], x, qkv.rows, H * c.hd, s.rows, code, at);
     require_apart(q, qkv, (H + 2 * c.KV) * c.hd, H * c.hd);
+    if (s.positions) {
+      call("lz_kv_write_at", p_write_at, (const void*)qkv.t.data_ptr(), qkv.ld, code, s.rows, (const void*)cos.data_ptr(),
+           (const void*)sin.data_ptr(), cos.size(0), q.t.data_ptr(), q.ld, address(c.k), address(c.v), address(c.ke),
+           address(c.ve), c.code, c.pages, c.size, (const int32_t*)address<int32_t>(s.table), s.width,
+           (const int32_t*)address<int32_t>(s.start), (const int32_t*)address<int32_t>(s.len),
+           (const int32_t*)address<int32_t>(s.positions), s.B, H, c.KV, c.hd, at.stream);
+      return THPVariable_Wrap(q.t);
+    }
     call("lz_kv_write", p_write, (const void*)qkv.t.data_ptr(), qkv.ld, code, qkv.rows, (const void*)cos.data_ptr(),
          (const void*)sin.data_ptr(), cos.size(0), q.t.data_ptr(), q.ld, address(c.k), address(c.v), address(c.ke),
          address(c.ve), c.code, c.pages, c.size, (const int32_t*)address<int32_t>(s.table), s.width,
@@ -389,9 +423,19 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Rows q(x, "q", H * c.hd, code, at);
     const Out o(a[5], x, q.rows, H * c.hd, s.rows, code, at);
     require_apart(o, q, H * c.hd, H * c.hd);
-    const int64_t bytes = p_attn_ws(code, c.code, q.rows, s.B, H, c.KV, c.hd, s.max_new, s.max_len);
+    const int64_t bytes = s.mask ? p_tree_ws(code, c.code, s.rows, s.B, H, c.KV, c.hd, s.max_new, s.max_len)
+                                 : p_attn_ws(code, c.code, q.rows, s.B, H, c.KV, c.hd, s.max_new, s.max_len);
     at::Tensor ws;
     if (bytes) ws = fresh(x, {(bytes + 3) / 4}, at::kFloat);
+    if (s.mask) {
+      call("lz_tree_attn", p_tree, (const void*)q.t.data_ptr(), q.ld, code, s.rows, (const void*)address(c.k),
+           (const void*)address(c.v), (const void*)address(c.ke), (const void*)address(c.ve), c.code, c.pages, c.size,
+           (const int32_t*)address<int32_t>(s.table), s.width, (const int32_t*)address<int32_t>(s.start),
+           (const int32_t*)address<int32_t>(s.len), (const int32_t*)address<int32_t>(s.base),
+           (const int32_t*)address<int32_t>(s.mask), s.mask->size(1), s.B, H, c.KV, c.hd, s.max_new, s.max_len,
+           (float)scale, o.t.data_ptr(), o.ld, bytes ? ws.data_ptr() : nullptr, bytes, at.stream);
+      return THPVariable_Wrap(o.t);
+    }
     call("lz_paged_attn", p_attn, (const void*)q.t.data_ptr(), q.ld, code, q.rows, (const void*)address(c.k),
          (const void*)address(c.v), (const void*)address(c.ke), (const void*)address(c.ve), c.code, c.pages, c.size,
          (const int32_t*)address<int32_t>(s.table), s.width, (const int32_t*)address<int32_t>(s.start),
@@ -504,6 +548,195 @@ PyObject* process_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- drafted tokens -------------------------------------------------------
+
+// An int32 [B] tensor.
+const at::Tensor& per_sequence(const at::Tensor& t, const char* name, int64_t B, const Place& at) {
+  int32_table(t, name, at, 1);
+  if (t.size(0) != B) refuse(PyExc_ValueError, "%s must hold %lld values, got %lld", name, (long long)B, (long long)t.size(0));
+  return t;
+}
+
+// The parents of trees: int32 [nodes], for all sequences, or [B, nodes].
+struct Parents {
+  const int32_t* at = nullptr;
+  int64_t nodes = 0, ld = 0;
+
+  Parents(PyObject* o, int64_t B, int64_t max_new, const Place& place) {
+    const at::Tensor* t = maybe(o, "parents");
+    if (!t) return;
+    int32_table(*t, "parents", place, t->dim() == 1 ? 1 : 2);
+    nodes = t->size(-1);
+    if (nodes == 0 || nodes < max_new || (t->dim() == 2 && t->size(0) != B))
+      refuse(PyExc_ValueError, "parents must be [nodes] or [%lld, nodes], of at least %lld nodes, got %s", (long long)B,
+             (long long)max_new, shape(*t).c_str());
+    at = static_cast<const int32_t*>(t->data_ptr());
+    ld = t->dim() == 2 ? nodes : 0;
+  }
+};
+
+PyObject* tuple_of(std::initializer_list<const at::Tensor*> tensors) {
+  PyObject* t = PyTuple_New((Py_ssize_t)tensors.size());
+  if (!t) throw Refused{};
+  Py_ssize_t i = 0;
+  for (const at::Tensor* x : tensors) {
+    PyObject* o = x->defined() ? THPVariable_Wrap(*x) : Py_NewRef(Py_None);
+    if (!o) {
+      Py_DECREF(t);
+      throw Refused{};
+    }
+    PyTuple_SET_ITEM(t, i++, o);
+  }
+  return t;
+}
+
+PyObject* cache_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect(n, 8);
+    const at::Tensor &table = tensor(item(a[0], 0, 5, "PageTables"), "page_table"),
+                     &lengths = tensor(item(a[0], 1, 5, "PageTables"), "lengths"),
+                     &free = tensor(item(a[0], 2, 5, "PageTables"), "free"),
+                     &n_free = tensor(item(a[0], 3, 5, "PageTables"), "n_free");
+    const int64_t size = integer(item(a[0], 4, 5, "PageTables"));
+    const Place at(table);
+    int32_table(table, "page_table", at, 2);
+    int32_table(free, "free", at, 1);
+    const int64_t B = table.size(0), width = table.size(1);
+    if (B == 0 || width == 0 || free.size(0) == 0)
+      refuse(PyExc_ValueError, "tables of %lld sequences, %lld pages each, %lld in all", (long long)B, (long long)width,
+             (long long)free.size(0));
+    per_sequence(lengths, "lengths", B, at);
+    per_sequence(n_free, "n_free", 1, at);
+    const at::Tensor& add = per_sequence(tensor(a[1], "new"), "new", B, at);
+    const int64_t rows = integer(a[2]), max_new = integer(a[3]), max_len = integer(a[4]);
+    if (rows < 0 || max_new < 0 || max_len < 0)
+      refuse(PyExc_ValueError, "a step of %lld rows, %lld new tokens a sequence and %lld in all", (long long)rows,
+             (long long)max_new, (long long)max_len);
+    const at::Tensor *keep = maybe(a[5], "keep"), *first = maybe(a[6], "base");
+    if (keep) per_sequence(*keep, "keep", B, at);
+    if (first) per_sequence(*first, "base", B, at);
+    const Parents parents(a[7], B, first ? 0 : max_new, at);
+    const int64_t words = (parents.nodes + 31) / 32;
+    const at::Tensor start = fresh(table, {B + 1}, at::kInt), len = fresh(table, {B}, at::kInt),
+                     base = fresh(table, {B}, at::kInt), positions = fresh(table, {rows}, at::kInt),
+                     slots = fresh(table, {rows}, at::kLong);
+    at::Tensor mask;
+    if (parents.at) mask = fresh(table, {rows, words}, at::kInt);
+    // an empty mask has no address, and is asked for all the same
+    int32_t* mask_at = parents.at ? (rows ? static_cast<int32_t*>(mask.data_ptr()) : start.data_ptr<int32_t>()) : nullptr;
+    call("lz_cache_tables", p_tables, address<int32_t>(&table), width, address<int32_t>(&lengths), address<int32_t>(&free),
+         free.size(0), address<int32_t>(&n_free), size, (const int32_t*)address<int32_t>(&add),
+         (const int32_t*)address<int32_t>(keep), (const int32_t*)address<int32_t>(first), parents.at, parents.ld,
+         parents.nodes, B, rows, max_new, max_len, address<int32_t>(&start), address<int32_t>(&len),
+         address<int32_t>(&base), address<int32_t>(&positions), address<int64_t>(&slots), mask_at, words, at.stream);
+    return tuple_of({&start, &len, &base, &positions, &slots, &mask});
+  });
+}
+
+PyObject* verify_draft(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect(n, 8);
+    const at::Tensor& x = tensor(a[0], "logits");
+    const Place at(x);
+    const int code = code_of(x);
+    if (x.dim() != 2 || x.size(1) == 0) refuse(PyExc_ValueError, "logits must be [rows, V], got %s", shape(x).c_str());
+    const int64_t rows = x.size(0), V = x.size(1);
+    if ((V > 1 && x.stride(1) != 1) || (rows > 1 && x.stride(0) < V))
+      refuse(PyExc_ValueError, "logits rows must be adjacent values, got strides (%lld, %lld)", (long long)x.stride(0),
+             (long long)x.stride(1));
+    const at::Tensor &tokens = tensor(a[1], "tokens"), &start = tensor(a[2], "row_start"), &uniform = tensor(a[4], "uniform");
+    const int64_t max_new = integer(a[3]);
+    int32_table(start, "row_start", at, 1);
+    const int64_t B = start.size(0) - 1;
+    if (B < 1 || max_new < 1) refuse(PyExc_ValueError, "no sequence's tokens to verify");
+    if (tokens.scalar_type() != at::kLong || tokens.dim() != 1 || tokens.size(0) != rows || !tokens.is_contiguous() ||
+        !at.here(tokens)) {
+      require_gpu(tokens);
+      refuse(PyExc_ValueError, "tokens must be a contiguous int64 [%lld] tensor on cuda:%d, got %s %s", (long long)rows,
+             (int)at.index, type_name(tokens), shape(tokens).c_str());
+    }
+    const bool wide = uniform.scalar_type() == at::kDouble;
+    if ((!wide && uniform.scalar_type() != at::kFloat) || uniform.dim() != 1 || uniform.size(0) != rows ||
+        !uniform.is_contiguous() || !at.here(uniform)) {
+      require_gpu(uniform);
+      refuse(PyExc_ValueError, "uniform must be a contiguous float32 or float64 [%lld] tensor on cuda:%d, got %s %s",
+             (long long)rows, (int)at.index, type_name(uniform), shape(uniform).c_str());
+    }
+    const Penalty heat(a[5], "temperature", B, false, at);
+    const Parents parents(a[6], B, max_new, at);
+    const at::Tensor* probs = maybe(a[7], "draft_probs");
+    if (probs) {
+      if (parents.at) refuse(PyExc_ValueError, "draft_probs are for chains: with parents, tokens are matched");
+      if (probs->scalar_type() != at::kFloat || probs->dim() != 2 || probs->size(0) != rows || probs->size(1) != V ||
+          (V > 1 && probs->stride(1) != 1) || (rows > 1 && probs->stride(0) < V) || !at.here(*probs)) {
+        require_gpu(*probs);
+        refuse(PyExc_ValueError, "draft_probs must be float32 rows [%lld, %lld] on cuda:%d, got %s %s", (long long)rows,
+               (long long)V, (int)at.index, type_name(*probs), shape(*probs).c_str());
+      }
+    }
+    const at::Tensor counts = fresh(x, {B}, at::kInt), kept = fresh(x, {B, max_new}, at::kInt),
+                     chosen = fresh(x, {B, max_new}, at::kLong);
+    const int64_t bytes = p_verify_ws(rows, B, V, probs != nullptr);
+    at::Tensor ws;
+    if (bytes) ws = fresh(x, {(bytes + 7) / 8}, at::kLong);
+    call("lz_verify_draft", p_verify, (const void*)x.data_ptr(), rows > 1 ? x.stride(0) : V, code, rows, V,
+         (const int64_t*)address<int64_t>(&tokens), (const void*)uniform.data_ptr(), (int)wide,
+         (const int32_t*)address<int32_t>(&start), B, max_new, heat.rows, heat.all, parents.at, parents.ld, parents.nodes,
+         (const float*)address<float>(probs), probs && rows > 1 ? probs->stride(0) : V, address<int32_t>(&counts),
+         address<int32_t>(&kept), address<int64_t>(&chosen), bytes ? ws.data_ptr() : nullptr, bytes, at.stream);
+    return tuple_of({&counts, &kept, &chosen});
+  });
+}
+
+PyObject* kv_cache_keep(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect(n, 4);
+    const at::Tensor &k = tensor(item(a[0], 0, 4, "LayerCache"), "layers.k"),
+                     &v = tensor(item(a[0], 1, 4, "LayerCache"), "layers.v");
+    const at::Tensor *ke = maybe(item(a[0], 2, 4, "LayerCache"), "layers.k_exp"),
+                     *ve = maybe(item(a[0], 3, 4, "LayerCache"), "layers.v_exp");
+    const Place at(k);
+    for (const at::Tensor* t : {&v, ke, ve})
+      if (t && !at.here(*t)) {
+        require_gpu(*t);
+        refuse(PyExc_ValueError, "the cache is on cuda:%d and on %s", (int)at.index, t->device().str().c_str());
+      }
+    const int64_t d = k.dim();
+    if ((d != 4 && d != 5) || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || !k.is_contiguous() ||
+        !v.is_contiguous())
+      refuse(PyExc_ValueError, "cache pages must be two contiguous tensors [pages, KV heads, page size, head dim], or of "
+                               "several layers [layers, pages, ...], got %s %s and %s %s", type_name(k), shape(k).c_str(),
+             type_name(v), shape(v).c_str());
+    const bool e8 = k.scalar_type() == at::kFloat8_e4m3fn;
+    for (const at::Tensor* e : {ke, ve}) {
+      if (e8 && (!e || e->scalar_type() != at::kChar || e->sizes() != k.sizes().slice(0, d - 1) || !e->is_contiguous()))
+        refuse(PyExc_ValueError, "a float8_e4m3fn cache needs contiguous int8 exponents of a token and head beside it");
+      if (!e8 && e) refuse(PyExc_TypeError, "a cache of %s has no exponents", type_name(k));
+    }
+    if (!is_draft(a[1])) refuse(PyExc_TypeError, "expected a DraftStep, got %s", Py_TYPE(a[1])->tp_name);
+    const at::Tensor &start = tensor(PyTuple_GET_ITEM(a[1], 0), "row_start"), &slots = tensor(PyTuple_GET_ITEM(a[1], 8), "slots");
+    const int64_t rows = integer(PyTuple_GET_ITEM(a[1], 3));
+    int32_table(start, "row_start", at, 1);
+    const int64_t B = start.size(0) - 1;
+    if (B < 1 || rows < 0 || slots.scalar_type() != at::kLong || slots.dim() != 1 || slots.size(0) < rows ||
+        !slots.is_contiguous() || !at.here(slots)) {
+      require_gpu(slots);
+      refuse(PyExc_ValueError, "slots must be a contiguous int64 tensor of the step's %lld rows on cuda:%d, got %s %s",
+             (long long)rows, (int)at.index, type_name(slots), shape(slots).c_str());
+    }
+    const at::Tensor &kept = tensor(a[2], "kept"), &counts = per_sequence(tensor(a[3], "counts"), "counts", B, at);
+    int32_table(kept, "kept", at, 2);
+    if (kept.size(0) != B)
+      refuse(PyExc_ValueError, "kept must be [%lld, nodes], got %s", (long long)B, shape(kept).c_str());
+    call("lz_kv_keep", p_keep, k.data_ptr(), v.data_ptr(), address(ke), address(ve), e8 ? LZ_E4M3 : code_of(k),
+         d == 5 ? k.size(0) : 1, k.size(d - 4), k.size(d - 2), k.size(d - 3), k.size(d - 1),
+         (const int64_t*)address<int64_t>(&slots), rows, (const int32_t*)address<int32_t>(&start), B,
+         (const int32_t*)address<int32_t>(&kept), kept.size(1), kept.size(1), (const int32_t*)address<int32_t>(&counts),
+         at.stream);
+    Py_RETURN_NONE;
+  });
+}
+
 template <typename P>
 void take(PyObject* addresses, const char* name, P& p) {
   PyObject* o = PyDict_GetItemString(addresses, name);
@@ -523,6 +756,13 @@ PyObject* bind(PyObject*, PyObject* args) {
     take(addresses, "lz_copy2d", p_copy);
     take(addresses, "lz_fill", p_fill);
     take(addresses, "lz_last_error", p_error);
+    take(addresses, "lz_kv_write_at", p_write_at);
+    take(addresses, "lz_kv_keep", p_keep);
+    take(addresses, "lz_tree_attn", p_tree);
+    take(addresses, "lz_tree_attn_workspace", p_tree_ws);
+    take(addresses, "lz_cache_tables", p_tables);
+    take(addresses, "lz_verify_draft", p_verify);
+    take(addresses, "lz_verify_workspace", p_verify_ws);
     take(addresses, "lz_kv_write", p_write);
     for (auto& [slot, o] : {std::pair<PyObject*&, PyObject*>{g_stream, stream}, {g_get, get}, {g_set, set}, {g_failure, failure}}) {
       Py_INCREF(o);
@@ -536,6 +776,7 @@ PyObject* bind(PyObject*, PyObject* args) {
 #define METHOD(name) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&name)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {METHOD(kv_cache_write), METHOD(kv_cache_read), METHOD(paged_attention), METHOD(process_logits),
+                          METHOD(cache_tables), METHOD(verify_draft), METHOD(kv_cache_keep),
                           {"bind", bind, METH_VARARGS, "bind(addresses, raw_stream, get_device, set_device, error)"},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torchcall", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

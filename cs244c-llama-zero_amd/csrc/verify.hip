@@ -1,0 +1,501 @@
+// Verification of drafted tokens against the model's logits, from given random
+// numbers.
+//
+// Row i of a sequence holds the logits of what follows its node i; with the
+// temperature T, p = softmax(x / T), or all of it on the arg-max where T <= 0.
+//
+//   without draft probabilities (a tree): t_i = the first token whose sum of p up
+//     to it is over u_i; from the root on, the walk goes to the first child that
+//     holds t_i, and ends with t_i where there is none.
+//   with them (a chain): node j, drawn from q_j, is kept while u_j q_j(x_j) <
+//     p_{j-1}(x_j); the token after the last kept one is chosen with u_0 from
+//     max(p - q, 0) of the node that was not kept, or from p after the last.
+//
+// A choice falls on another token where an error in the sums crosses a token's
+// border: in fp32 (2^-24) that is one row in a few hundred of a flat vocabulary of
+// 128000, so weights and sums are formed in fp64 (to 2^-41 or better).  A weight
+// is 2^((x - m) log2(e) / T), its fraction by the Taylor series of 2^f, |f| <= 1/2,
+// to the tenth power (2e-13).
+//
+// Every logit is read once: stats_kernel leaves each piece's largest logit and
+// its sum of weights, a wave for each piece and no meeting of waves.  What remains
+// works on pieces: a wave joins a row's sums, finds the piece that the choice falls
+// into and goes over that one alone.  All rows of a tree choose at the same time,
+// a wave each, and one wave walks through the choices in LDS.
+#include <type_traits>
+
+#include "kvcache.h"
+
+namespace {
+
+constexpr int kVec = 512;  // logits that a wave loads at a time, eight a lane
+
+struct Piece {
+  double sum;  // of 2^((x - top) log2(e) / T); NaN where no choice can be made
+  float top;
+  int arg;  // the first token with it
+};
+
+struct VerifyArgs {
+  const void* logits;
+  int64_t ld;
+  const int64_t* tokens;
+  const void* uniform;
+  const int32_t* row_start;
+  const float* heat;  // [B]; null: heat_s
+  const int32_t* parents;  // [B or 1][nodes], null: a chain
+  const float* probs;
+  int64_t ldp, ldq;
+  Piece* pieces;  // [rows][n_pieces]
+  double* rest;   // [B][n_pieces]
+  int32_t* stop;  // [B]: the last kept node
+  int32_t* counts;
+  int32_t* kept;   // [B][nodes]
+  int64_t* chosen;  // [B][nodes]
+  float heat_s;
+  int u_double, rows, B, V, nodes, n_pieces, piece, tree_nodes;
+};
+
+typedef uint32_t Words4 __attribute__((ext_vector_type(4), aligned(2)));  // of rows that start anywhere
+
+// 2^t for t <= 0 (NaN stays one).
+__device__ __forceinline__ double pow2_of(double t) {
+  t = t < -1100.0 ? -1100.0 : t;
+  const double n = rint(t), f = t - n;
+  // (ln 2)^k / k!
+  double p = 7.054911620801121e-09;
+  p = fma(p, f, 1.0178086009239696e-07);
+  p = fma(p, f, 1.3215486790144305e-06);
+  p = fma(p, f, 1.5252733804059838e-05);
+  p = fma(p, f, 0.00015403530393381606);
+  p = fma(p, f, 0.0013333558146428441);
+  p = fma(p, f, 0.009618129107628477);
+  p = fma(p, f, 0.055504108664821576);
+  p = fma(p, f, 0.2402265069591007);
+  p = fma(p, f, 0.6931471805599453);
+  p = fma(p, f, 1.0);
+  return ldexp(p, (int)n);
+}
+
+// log2(e) / T, or 0 where the arg-max is chosen.
+__device__ __forceinline__ double per_heat(const VerifyArgs& a, int b) {
+  const float t = a.heat ? a.heat[b] : a.heat_s;
+  return t > 0.f ? 1.4426950408889634 / (double)t : 0.0;
+}
+
+__device__ __forceinline__ double uniform_of(const VerifyArgs& a, int row) {
+  return a.u_double ? static_cast<const double*>(a.uniform)[row] : (double)static_cast<const float*>(a.uniform)[row];
+}
+
+// Eight logits of a row from v on; -inf past the vocabulary.
+template <typename T>
+__device__ __forceinline__ void load8(float (&x)[8], const T* row, int v, int V) {
+  if (v + 8 <= V) {
+    T raw[8];
+#pragma unroll
+    for (int w = 0; w < (int)sizeof(T) / 2; ++w)
+      reinterpret_cast<Words4*>(raw)[w] = reinterpret_cast<const Words4*>(row + v)[w];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = Elem<T>::load(raw, e);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = v + e < V ? Elem<T>::load(row, v + e) : -INFINITY;
+  }
+}
+
+// A token's weight beside the largest logit `top` (finite).
+__device__ __forceinline__ double weight(float x, float top, double c) {
+  return x == -INFINITY ? 0.0 : pow2_of(((double)x - (double)top) * c);
+}
+
+// Sum over the wave of the lanes up to this one.
+__device__ __forceinline__ double sum_up_to(double x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+// A row's rows of the call, bounded: lo .. lo + n - 1.
+struct Nodes {
+  int lo, n;
+  __device__ __forceinline__ Nodes(const VerifyArgs& a, int b) {
+    lo = min(max(a.row_start[b], 0), a.rows);
+    n = min(min(max(a.row_start[b + 1], lo), a.rows) - lo, a.nodes);
+  }
+};
+
+// NV vectors of a piece, a wave each.
+template <typename T, int NV>
+__global__ void __launch_bounds__(256) stats_kernel(VerifyArgs a) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t per_row = (uint32_t)(a.n_pieces + 3) / 4;
+  const int row = (int)(blockIdx.x / per_row), p = (int)(blockIdx.x % per_row) * 4 + wave;
+  if (p >= a.n_pieces) return;
+  const T* x_row = static_cast<const T*>(a.logits) + row * a.ld;
+  float x[NV][8];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) load8(x[k], x_row, (p * NV + k) * kVec + lane * 8, a.V);
+  const int b = a.heat ? lz_seq_of_row(a.row_start, a.B, a.rows, row) : 0;
+  const double c = b < 0 ? 0.0 : per_heat(a, b);
+
+  float top = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      top = fmaxf(top, x[k][e]);
+      nan |= x[k][e] != x[k][e];
+    }
+  top = wave_max(top);
+  nan = __ballot(nan) != 0;
+  int arg = INT32_MAX;
+#pragma unroll
+  for (int k = NV - 1; k >= 0; --k)
+#pragma unroll
+    for (int e = 7; e >= 0; --e)
+      if (x[k][e] == top) arg = (p * NV + k) * kVec + lane * 8 + e;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) arg = min(arg, __shfl_xor(arg, o, 64));
+  double sum = 0.0;
+  if (c != 0.0 && top > -INFINITY && top < INFINITY) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += weight(x[k][e], top, c);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  }
+  if (lane == 0) {
+    Piece s;
+    s.sum = nan || top == INFINITY ? __builtin_nan("") : sum;
+    s.top = nan ? __builtin_nanf("") : top;
+    s.arg = arg;
+    a.pieces[(int64_t)row * a.n_pieces + p] = s;
+  }
+}
+
+// A row's largest logit (NaN where there is one among them), the first token
+// that has it and the sum of its weights, with a whole wave.
+struct Row {
+  const Piece* pieces;
+  double c, sum;
+  float top;
+  int arg;
+
+  __device__ __forceinline__ Row(const VerifyArgs& a, int row, double c_, int lane)
+      : pieces(a.pieces + (int64_t)row * a.n_pieces), c(c_), sum(0.0), top(-INFINITY), arg(INT32_MAX) {
+    bool nan = false;
+    for (int p = lane; p < a.n_pieces; p += 64) {
+      const Piece s = pieces[p];
+      nan |= s.top != s.top;
+      if (s.top > top) {
+        top = s.top;
+        arg = s.arg;
+      }
+    }
+    const float all = wave_max(top);
+    arg = top == all ? arg : INT32_MAX;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) arg = min(arg, __shfl_xor(arg, o, 64));
+    top = __ballot(nan) ? __builtin_nanf("") : all;
+    if (c != 0.0) {
+      for (int p = lane; p < a.n_pieces; p += 64) sum += of_piece(p);
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    }
+  }
+  // a piece's sum beside the row's largest logit
+  __device__ __forceinline__ double of_piece(int p) const {
+    const Piece s = pieces[p];
+    return s.sum == 0.0 ? 0.0 : s.sum * pow2_of(((double)s.top - (double)top) * c);
+  }
+  // whether a token can be chosen
+  __device__ __forceinline__ bool fine() const {
+    return c == 0.0 ? top > -INFINITY : top > -INFINITY && top < INFINITY;  // not for NaN
+  }
+};
+
+// The first token whose sum up to it is over u times the sum of all, and the
+// last one with a weight where rounding leaves none; -1 where all are zero.
+// of_piece(p): a piece's sum; of_token(v, w): eight tokens' weights.
+template <typename OfPiece, typename OfTokens>
+__device__ __forceinline__ int pick(const VerifyArgs& a, double u, int lane, const OfPiece& of_piece, const OfTokens& of_tokens) {
+  double all = 0.0;
+  for (int p0 = 0; p0 < a.n_pieces; p0 += 64)
+    all += __shfl(sum_up_to(p0 + lane < a.n_pieces ? of_piece(p0 + lane) : 0.0, lane), 63, 64);
+  if (!(all > 0.0)) return -1;
+  double target = (u > 0.0 ? u : 0.0) * all, run = 0.0, before = 0.0;
+  int piece = -1, last = -1;
+  double before_last = 0.0;
+  for (int p0 = 0; p0 < a.n_pieces; p0 += 64) {
+    const double x = p0 + lane < a.n_pieces ? of_piece(p0 + lane) : 0.0, up_to = sum_up_to(x, lane);
+    const uint64_t over = __ballot(x > 0.0 && run + up_to > target), some = __ballot(x > 0.0);
+    if (over) {
+      const int l = __builtin_ctzll(over);
+      piece = p0 + l;
+      before = run + (__shfl(up_to, l, 64) - __shfl(x, l, 64));
+      break;
+    }
+    if (some) last = p0 + 63 - __builtin_clzll(some);
+    run += __shfl(up_to, 63, 64);
+  }
+  if (piece < 0) {  // u is 1 or just under it
+    piece = last;
+    target = INFINITY;
+  }
+  run = before;
+  int found = -1;
+  const int end = min((piece + 1) * a.piece, a.V);
+  for (int v0 = piece * a.piece; v0 < end; v0 += kVec) {
+    const int v = v0 + lane * 8;
+    double w[8], x = 0.0;
+    of_tokens(v, w);
+    int mine = -1;  // this lane's last token with a weight
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x += w[e];
+      mine = w[e] > 0.0 ? v + e : mine;
+    }
+    const double up_to = sum_up_to(x, lane);
+    const uint64_t over = __ballot(x > 0.0 && run + up_to > target), some = __ballot(x > 0.0);
+    if (over) {
+      const int l = __builtin_ctzll(over);
+      double at = run + (up_to - x);
+      bool done = false;
+      int token = mine;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        at += w[e];
+        if (!done && w[e] > 0.0 && at > target) {
+          token = v + e;
+          done = true;
+        }
+      }
+      return __shfl(token, l, 64);
+    }
+    if (some) found = __shfl(mine, 63 - __builtin_clzll(some), 64);
+    run += __shfl(up_to, 63, 64);
+  }
+  return found;
+}
+
+template <typename T>
+__device__ __forceinline__ int pick_row(const VerifyArgs& a, const Row& r, int row, double u, int lane) {
+  if (!r.fine()) return -1;
+  if (r.c == 0.0) return r.arg;
+  const T* x_row = static_cast<const T*>(a.logits) + row * a.ld;
+  return pick(a, u, lane, [&](int p) { return r.of_piece(p); },
+              [&](int v, double (&w)[8]) {
+                float x[8];
+                load8(x, x_row, v, a.V);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = weight(x[e], r.top, r.c);
+              });
+}
+
+constexpr int kMostNodes = 4096;
+
+// Without draft probabilities: one workgroup a sequence.
+template <typename T>
+__global__ void __launch_bounds__(1024) walk_kernel(VerifyArgs a) {
+  __shared__ int choice[kMostNodes], token[kMostNodes], parent[kMostNodes], path[kMostNodes];
+  __shared__ int n_path;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Nodes s(a, b);
+  const double c = per_heat(a, b);
+  for (int i = tid; i < s.n; i += 1024) {
+    const int64_t t = a.tokens[s.lo + i];
+    token[i] = t >= 0 && t < a.V ? (int)t : -2;
+    parent[i] = a.parents && i < a.tree_nodes ? a.parents[b * a.ldp + i] : -1;
+  }
+  for (int i = wave; i < s.n; i += 16) {
+    const int t = pick_row<T>(a, Row(a, s.lo + i, c, lane), s.lo + i, uniform_of(a, s.lo + i), lane);
+    if (lane == 0) choice[i] = t;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    int node = 0, count = 0;
+    while (node < s.n) {
+      if (lane == 0) path[count] = node;
+      ++count;
+      const int want = choice[node];
+      int next = s.n;
+      if (want < 0) break;
+      if (!a.parents) {
+        if (node + 1 < s.n && token[node + 1] == want) next = node + 1;
+      } else {
+        for (int i0 = node + 1; i0 < s.n; i0 += 64) {
+          const int i = i0 + lane;
+          const uint64_t ok = __ballot(i < s.n && parent[i] == node && token[i] == want);
+          if (ok) {
+            next = i0 + __builtin_ctzll(ok);
+            break;
+          }
+        }
+      }
+      node = next;
+    }
+    if (lane == 0) n_path = count;
+  }
+  __syncthreads();
+  const int count = n_path;
+  if (tid == 0) a.counts[b] = count;
+  for (int j = tid; j < a.nodes; j += 1024) {
+    a.kept[(int64_t)b * a.nodes + j] = j < count ? path[j] : -1;
+    a.chosen[(int64_t)b * a.nodes + j] = j < count ? choice[path[j]] : -1;
+  }
+}
+
+// With them: each workgroup of a sequence finds where its chain ends, four rows
+// at a time, and sums what is left of p beside q over four pieces of that row.
+template <typename T>
+__global__ void __launch_bounds__(256) rest_kernel(VerifyArgs a) {
+  __shared__ int kept[4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t groups = (uint32_t)(a.n_pieces + 3) / 4;
+  const int b = (int)(blockIdx.x / groups), p = (int)(blockIdx.x % groups) * 4 + wave;
+  const Nodes s(a, b);
+  if (s.n == 0) return;
+  const double c = per_heat(a, b);
+  int stop = 0;
+  for (bool more = true; more;) {
+    const int node = stop + wave + 1;  // is it kept?
+    bool ok = false;
+    if (node < s.n) {
+      const int64_t t = a.tokens[s.lo + node];
+      const int row = s.lo + node - 1;
+      const Row r(a, row, c, lane);
+      if (t >= 0 && t < a.V && r.fine()) {
+        const float x = Elem<T>::load(static_cast<const T*>(a.logits) + row * a.ld, t);
+        if (c == 0.0) ok = t == r.arg;
+        else ok = uniform_of(a, s.lo + node) * (double)a.probs[(s.lo + node) * a.ldq + t] < weight(x, r.top, c) / r.sum;
+      }
+    }
+    if (lane == 0) kept[wave] = ok;
+    __syncthreads();
+    int run = 0;
+    while (run < 4 && kept[run]) ++run;
+    __syncthreads();
+    stop += run;
+    more = run == 4;
+  }
+  if (threadIdx.x == 0 && p == 0) a.stop[b] = stop;
+  if (p >= a.n_pieces || c == 0.0) return;
+  const int row = s.lo + stop;
+  const Row r(a, row, c, lane);
+  double rest = 0.0;
+  if (stop + 1 < s.n && r.fine()) {
+    const T* x_row = static_cast<const T*>(a.logits) + row * a.ld;
+    const float* q_row = a.probs + (row + 1) * a.ldq;
+    const double per = 1.0 / r.sum;
+    for (int v = p * a.piece + lane * 8; v < min((p + 1) * a.piece, a.V); v += kVec) {
+      float x[8], q[8];
+      load8(x, x_row, v, a.V);
+      load8(q, q_row, v, a.V);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (v + e < a.V) rest += fmax(weight(x[e], r.top, c) * per - (double)q[e], 0.0);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) rest += __shfl_xor(rest, o, 64);
+  }
+  if (lane == 0) a.rest[(int64_t)b * a.n_pieces + p] = rest;
+}
+
+// The token after a chain's last kept one, a wave for each sequence.
+template <typename T>
+__global__ void __launch_bounds__(64) end_kernel(VerifyArgs a) {
+  const int b = blockIdx.x, lane = threadIdx.x;
+  const Nodes s(a, b);
+  int count = 0, last = -1;
+  if (s.n > 0) {
+    const int stop = a.stop[b], row = s.lo + stop;
+    const double c = per_heat(a, b), u = uniform_of(a, s.lo);
+    count = stop + 1;
+    const Row r(a, row, c, lane);
+    if (c != 0.0 && r.fine() && stop + 1 < s.n) {
+      const T* x_row = static_cast<const T*>(a.logits) + row * a.ld;
+      const float* q_row = a.probs + (row + 1) * a.ldq;
+      const double* rest = a.rest + (int64_t)b * a.n_pieces;
+      const double per = 1.0 / r.sum;
+      last = pick(a, u, lane, [&](int p) { return rest[p]; },
+                  [&](int v, double (&w)[8]) {
+                    float x[8], q[8];
+                    load8(x, x_row, v, a.V);
+                    load8(q, q_row, v, a.V);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                      w[e] = v + e < a.V ? fmax(weight(x[e], r.top, c) * per - (double)q[e], 0.0) : 0.0;
+                  });
+    }
+    if (last < 0) last = pick_row<T>(a, r, row, u, lane);  // nothing of q was not kept, or p is q
+  }
+  if (lane == 0) a.counts[b] = count;
+  for (int j = lane; j < a.nodes; j += 64) {
+    a.kept[(int64_t)b * a.nodes + j] = j < count ? j : -1;
+    a.chosen[(int64_t)b * a.nodes + j] = j + 1 < count ? a.tokens[s.lo + j + 1] : j + 1 == count ? last : -1;
+  }
+}
+
+// Pieces of 2048 where that makes more waves than the chip holds at a time, of
+// 512 where the wave's own chain is the time.
+int vectors(int64_t rows, int64_t V) { return rows * V >= (int64_t)lz_num_cus() * 8 * 2048 ? 4 : 1; }
+
+}  // namespace
+
+LZ_EXPORT int64_t lz_verify_workspace(int64_t rows, int64_t B, int64_t V, int drawn) {
+  if (rows <= 0 || B <= 0 || V <= 0 || V > (1 << 28)) return 0;
+  const int64_t pieces = lz_cdiv(V, kVec * vectors(rows, V));
+  return rows * pieces * (int64_t)sizeof(Piece) + (drawn ? B * pieces * 8 + B * 4 : 0);
+}
+
+LZ_EXPORT int lz_verify_draft(const void* logits, int64_t ld, int dtype, int64_t rows, int64_t V, const int64_t* tokens,
+                              const void* uniform, int u_double, const int32_t* row_start, int64_t B, int64_t nodes,
+                              const float* temperature, float temperature_s, const int32_t* parents, int64_t ldp,
+                              int64_t tree_nodes, const float* probs, int64_t ldq, int32_t* counts, int32_t* kept,
+                              int64_t* chosen, void* workspace, int64_t ws_bytes, void* stream) {
+  LZ_REQUIRE(dtype == LZ_BF16 || dtype == LZ_F16 || dtype == LZ_F32, "lz_verify_draft: bad dtype %d", dtype);
+  LZ_REQUIRE(rows >= 0 && rows <= INT32_MAX && V > 0 && V <= (1 << 28) && B > 0 && B <= INT32_MAX / 256,
+             "lz_verify_draft: bad shape");
+  LZ_REQUIRE(nodes > 0 && nodes <= kMostNodes, "lz_verify_draft: %lld nodes a sequence (1 to %d)", (long long)nodes, kMostNodes);
+  LZ_REQUIRE(!(parents && probs), "lz_verify_draft: draft probabilities are for chains");
+  LZ_REQUIRE(!parents || (tree_nodes > 0 && tree_nodes <= INT32_MAX && (ldp == 0 || ldp >= tree_nodes)),
+             "lz_verify_draft: trees of %lld nodes", (long long)tree_nodes);
+  LZ_REQUIRE(row_start && counts && kept && chosen, "lz_verify_draft: bad arguments");
+  LZ_REQUIRE(rows == 0 || (logits && tokens && uniform && (rows == 1 || (ld >= V && (!probs || ldq >= V)))),
+             "lz_verify_draft: bad rows");
+  const int nv = vectors(rows, V);
+  const int64_t pieces = lz_cdiv(V, kVec * nv), need = lz_verify_workspace(rows, B, V, probs != nullptr);
+  LZ_REQUIRE(need == 0 || (workspace && lz_aligned16(workspace) && ws_bytes >= need),
+             "lz_verify_draft: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
+  const int64_t stats = rows * lz_cdiv(pieces, 4), rests = B * lz_cdiv(pieces, 4);
+  LZ_REQUIRE(stats <= INT32_MAX / 256 && rests <= INT32_MAX / 256, "lz_verify_draft: too many rows");
+  Piece* at = static_cast<Piece*>(workspace);
+  double* rest = reinterpret_cast<double*>(at + rows * pieces);
+  VerifyArgs a{logits, ld, tokens, uniform, row_start, temperature, parents, probs, ldp, ldq, at, rest,
+               reinterpret_cast<int32_t*>(rest + B * pieces), counts, kept, chosen, temperature_s, u_double,
+               (int)rows, (int)B, (int)V, (int)nodes, (int)pieces, kVec * nv, (int)tree_nodes};
+  hipStream_t s = lz_stream(stream);
+#define RUN(T)                                                                              \
+  do {                                                                                      \
+    if (stats > 0) {                                                                        \
+      if (nv == 4) stats_kernel<T, 4><<<(uint32_t)stats, 256, 0, s>>>(a);                   \
+      else stats_kernel<T, 1><<<(uint32_t)stats, 256, 0, s>>>(a);                           \
+    }                                                                                       \
+    if (probs) {                                                                            \
+      rest_kernel<T><<<(uint32_t)rests, 256, 0, s>>>(a);                                    \
+      end_kernel<T><<<(uint32_t)B, 64, 0, s>>>(a);                                          \
+    } else {                                                                                \
+      walk_kernel<T><<<(uint32_t)B, 1024, 0, s>>>(a);                                       \
+    }                                                                                       \
+  } while (0)
+  if (dtype == LZ_BF16) RUN(uint16_t);
+  else if (dtype == LZ_F16) RUN(_Float16);
+  else RUN(float);
+#undef RUN
+  return lz_check_launch("lz_verify_draft");
+}

@@ -156,6 +156,41 @@ SIGNATURES = {
             _i64, _i64, _f32, _vp, _i64, _vp, _i64, _vp,
         ],
     ),
+    "lz_kv_write_at": (
+        _i32,
+        [
+            _vp, _i64, _i32, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _vp, _i64, _vp,
+            _vp, _vp, _i64, _i64, _i64, _i64, _vp,
+        ],
+    ),
+    "lz_kv_keep": (
+        _i32,
+        [_vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp],
+    ),
+    "lz_tree_attn_workspace": (_i64, [_i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "lz_tree_attn_plan": (_i64, [_i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "lz_tree_attn": (
+        _i32,
+        [
+            _vp, _i64, _i32, _i64, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
+            _i64, _i64, _i64, _i64, _f32, _vp, _i64, _vp, _i64, _vp,
+        ],
+    ),
+    "lz_cache_tables": (
+        _i32,
+        [
+            _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp,
+            _vp, _vp, _vp, _i64, _vp,
+        ],
+    ),
+    "lz_verify_workspace": (_i64, [_i64, _i64, _i64, _i32]),
+    "lz_verify_draft": (
+        _i32,
+        [
+            _vp, _i64, _i32, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _vp, _f32, _vp, _i64, _i64, _vp, _i64, _vp, _vp,
+            _vp, _vp, _i64, _vp,
+        ],
+    ),
     "lz_process_logits": (
         _i32,
         [

@@ -50,6 +50,40 @@ class CacheStep(NamedTuple):
     max_len: int
 
 
+class DraftStep(NamedTuple):
+    """A CacheStep whose new tokens may be the nodes of a tree for each
+    sequence, made by ops.cache_tables.  More device tensors: base [B] int32
+    (the tokens that all rows of a sequence see), positions [rows] int32 (that
+    rows are rotated to), slots [rows] int64 (where a row is cached: page * page
+    size + place in it, -1: nowhere), mask [rows, words] int32 (bit j of a row:
+    it sees the token in place base + j; None: what comes before it, as in a
+    CacheStep).  Rows of no sequence hold -1, -1 and 0."""
+
+    row_start: torch.Tensor
+    kv_len: torch.Tensor
+    page_table: torch.Tensor
+    rows: int
+    max_new: int
+    max_len: int
+    base: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+    mask: Optional[torch.Tensor] = None
+
+
+class PageTables(NamedTuple):
+    """Which pages the sequences hold, on the device (int32): page_table [B,
+    most pages of one], lengths [B] (sequence b holds the first ceil(lengths[b]
+    / page_size) entries of its row), and the free pages: free [pages], a stack
+    of which the first n_free [1] are free.  ops.cache_tables updates them."""
+
+    page_table: torch.Tensor
+    lengths: torch.Tensor
+    free: torch.Tensor
+    n_free: torch.Tensor
+    page_size: int
+
+
 class KVCache:
     """Pages for n_layers layers and up to `batch` sequences.
 

@@ -1222,7 +1222,8 @@ def kv_cache_write(qkv: torch.Tensor, layer, step, n_heads: int, cos: torch.Tens
 
     qkv: [rows, (n_heads + 2 * KV) * hd], the fused projection before RoPE;
     layer: LayerCache, layer.k of qkv's dtype or float8_e4m3fn; step:
-    CacheStep; cos/sin: RoPE tables [>= step.max_len, hd] in qkv's dtype; out:
+    CacheStep, or a DraftStep, whose rows are rotated to its positions; cos/sin:
+    RoPE tables [>= step.max_len, hd] in qkv's dtype; out:
     rows for the queries, where those of no sequence are left as they are; they
     may be qkv's own q columns and must not overlap it otherwise.  In new ones
     the rows from step.rows on are zeros; others of no sequence (row_start may
@@ -1246,7 +1247,9 @@ def paged_attention(q: torch.Tensor, layer, step, n_heads: int, scale: float,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of a step's rotated queries [rows, n_heads * hd] over the
     cached keys and values of their sequences (a step's own tokens included:
-    kv_cache_write comes first); causal within the new tokens; scale > 0.  A
+    kv_cache_write comes first); causal within the new tokens, or, with a
+    DraftStep that has a mask, each row seeing its sequence's first base[b]
+    tokens and of those after them what its mask says; scale > 0.  A
     row that sees nothing is zero, one whose scores are all -inf is NaN, as a
     softmax of them.  out: rows for the result, as kv_cache_write's; it may be
     q itself and must not overlap it otherwise.  No gradients: the result of a
@@ -1272,3 +1275,60 @@ def process_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = Non
     the vocabulary (padding) count for nothing."""
     return _lib.tensor_calls().process_logits(logits, tokens, lengths, prompt_lengths, repetition_penalty,
                                               presence_penalty, frequency_penalty, bias, mask)
+
+
+def cache_tables(tables, new: torch.Tensor, rows: int, max_new: int, max_len: int, *, keep: Optional[torch.Tensor] = None,
+                 base: Optional[torch.Tensor] = None, parents: Optional[torch.Tensor] = None):
+    """A step's tables (cache.DraftStep), made on the device: nothing of what
+    it depends on need be known to the host.
+
+    tables: cache.PageTables, which is updated; new: int32 [B], the tokens that
+    each sequence asks room for; keep: int32 [B], the tokens that it is cut to
+    first (None: all that it has), whose pages go back; rows, max_new, max_len:
+    bounds of all new tokens, and of the new and all tokens of a sequence.
+    Sequences are served in order: one whose tokens pass these bounds or the
+    table gets none, nor one that needs pages, or rows, where what it and those
+    before it ask for is more than there is (row_start says who got them).
+    parents: int32 [nodes] or [B, nodes], the new tokens as trees: node i is
+    the token in place base[b] + i (base: int32 [B]; None: the kept length), its
+    parent a node before it or -1.  Then rows see their ancestors alone and are
+    rotated to base + their depth.  Up to 4096 sequences."""
+    from .cache import DraftStep
+
+    start, length, at, positions, slots, mask = _lib.tensor_calls().cache_tables(tables, new, rows, max_new, max_len, keep,
+                                                                                 base, parents)
+    return DraftStep(start, length, tables[0], rows, max_new, max_len, at, positions, slots, mask)
+
+
+def verify_draft(logits: torch.Tensor, tokens: torch.Tensor, row_start: torch.Tensor, max_new: int, uniform: torch.Tensor, *,
+                 temperature=1.0, parents: Optional[torch.Tensor] = None, draft_probs: Optional[torch.Tensor] = None
+                 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(counts, kept, chosen): how many tokens each sequence gains, the nodes
+    that it keeps and the tokens.
+
+    Rows row_start[b] .. row_start[b + 1] - 1 (at most max_new, up to 4096) are
+    the nodes of sequence b: tokens [rows] int64 holds their tokens, the first
+    one the root (the text's last token), and logits [rows, V] what follows
+    each.  p is their softmax at `temperature` (a number or float32 [B]; <= 0:
+    the first of the largest logits); uniform: a number in [0, 1) for each row
+    (float32 or float64).  Without draft_probs a token is chosen from p at each
+    node with the node's number, and the child that holds it is kept (parents as
+    in cache_tables; None: a chain), which is the model's own choice at every
+    place whatever was drafted.  With draft_probs (float32 [rows, V], row r the
+    distribution that token r was drawn from), a chain's tokens are kept with
+    probability min(1, p / q) and the token after them is chosen with the
+    root's number from what is left of p.  counts: int32 [B], 0 for a sequence
+    without rows; kept: int32 [B, max_new], the root (0) and the kept nodes;
+    chosen: int64 [B, max_new], the kept nodes' tokens and the one that follows;
+    both -1 from counts[b] on.  A token that the logits do not choose (a NaN
+    among them, all -inf, infinity where it is sampled) is -1."""
+    return _lib.tensor_calls().verify_draft(logits, tokens, row_start, max_new, uniform, temperature, parents, draft_probs)
+
+
+def kv_cache_keep(layers, step, kept: torch.Tensor, counts: torch.Tensor) -> None:
+    """Moves what is kept of a draft to consecutive places: in each sequence,
+    node kept[b, j]'s keys and values to the place of the step's j-th new token,
+    for j < counts[b] (int32 [B, n], ascending, and int32 [B], as verify_draft
+    returns them).  layers: a LayerCache of one layer, or of several ([layers,
+    pages, ...]; KVCache.stacked); step: the DraftStep that wrote them."""
+    _lib.tensor_calls().kv_cache_keep(layers, step, kept, counts)

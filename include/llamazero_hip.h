@@ -443,6 +443,91 @@ int lz_paged_attn(const void* q, int64_t ldq, int dtype, int64_t rows, const voi
                   int64_t hd, int64_t max_new, int64_t max_len, float scale, void* o, int64_t ldo, void* workspace,
                   int64_t ws_bytes, void* stream);
 
+/* ---- drafted tokens over the cache ----------------------------------------
+ * A step's rows may be the nodes of a tree of drafted tokens for each sequence:
+ * node i is cached in place base + i, its parent comes before it, and its
+ * position is base + its depth.  The reference has no counterpart. */
+
+/* lz_kv_write with row_position[r] the position that row r is rotated to (it
+ * is cached in its place all the same; outside the tables: its query is zeros
+ * and nothing is cached). */
+int lz_kv_write_at(const void* qkv, int64_t ld, int dtype, int64_t rows, const void* cos_t, const void* sin_t,
+                   int64_t positions, void* q_out, int64_t ldq, void* k, void* v, void* k_exp, void* v_exp,
+                   int cache_dtype, int64_t pages, int64_t page_size, const int32_t* table, int64_t width,
+                   const int32_t* row_start, const int32_t* kv_len, const int32_t* row_position, int64_t B, int64_t H,
+                   int64_t KV, int64_t hd, void* stream);
+
+/* Attention of such rows: row r sees the first base[b] places of its sequence
+ * and, of those after them up to the last of kv_len[b], place base[b] + j where
+ * bit j of its `words` mask words is set (mask: [rows][words], lowest bit
+ * first; bits past them are clear).  The rest as lz_paged_attn, its workspace
+ * and plan too. */
+int64_t lz_tree_attn_workspace(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd,
+                               int64_t max_new, int64_t max_len);
+int64_t lz_tree_attn_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd,
+                          int64_t max_new, int64_t max_len);
+int lz_tree_attn(const void* q, int64_t ldq, int dtype, int64_t rows, const void* k, const void* v, const void* k_exp,
+                 const void* v_exp, int cache_dtype, int64_t pages, int64_t page_size, const int32_t* table,
+                 int64_t width, const int32_t* row_start, const int32_t* kv_len, const int32_t* base,
+                 const int32_t* mask, int64_t words, int64_t B, int64_t H, int64_t KV, int64_t hd, int64_t max_new,
+                 int64_t max_len, float scale, void* o, int64_t ldo, void* workspace, int64_t ws_bytes, void* stream);
+
+/* A step's tables from the sequences' lengths, without the host: each of the B
+ * (up to 4096) sequences is cut to keep[b] tokens (NULL: all; at most
+ * lengths[b]), its pages behind them go back on the stack `free` (`pages`
+ * values, of which n_free[0] are free), and it takes pages for add[b] more.
+ * Sequences are served in order: one whose tokens pass max_new, max_len or the
+ * table gets none, nor one that needs a page, or rows, where what it and those
+ * before it ask for is more than there is.  Pages go back so that the first
+ * sequence's first is on top, and are taken from the top in that order.
+ * table, lengths, free and n_free are updated (table entries without a page
+ * become -1); row_start (B + 1), kv_len and base (first[b]; NULL: the kept
+ * length) are written, and for each of the `rows` rows its position, its slot
+ * (page * page_size + place in it) and its mask, -1, -1 and 0 for rows of no
+ * sequence.  parents ([nodes] with ldp 0, or B rows of ldp): node i's, -1 or
+ * any value that is not below i for none; node i of a sequence is its place
+ * base[b] + i.  Without parents (and mask) a row's position is its place. */
+int lz_cache_tables(int32_t* table, int64_t width, int32_t* lengths, int32_t* free, int64_t pages, int32_t* n_free,
+                    int64_t page_size, const int32_t* add, const int32_t* keep, const int32_t* first,
+                    const int32_t* parents, int64_t ldp, int64_t nodes, int64_t B, int64_t rows, int64_t max_new,
+                    int64_t max_len, int32_t* row_start, int32_t* kv_len, int32_t* base, int32_t* positions,
+                    int64_t* slots, int32_t* mask, int64_t words, void* stream);
+
+/* Which drafted tokens are kept, given the logits of what follows each row
+ * (p = softmax(x / temperature), temperature[b] or, where that is NULL,
+ * temperature_s; <= 0: all of it on the first of the largest) and a uniform
+ * number in [0, 1) for each row (float, or double with u_double; below 0 counts
+ * as 0, from 1 on as just under it).  A sequence's rows are its nodes (up to
+ * `nodes`, at most 4096), the first one the root.
+ * probs NULL: at each node, from the root on, t = the first token whose sum of p
+ *   up to it is over the node's number times the sum of all; the first child
+ *   that holds t is kept and the walk goes on there (parents NULL: node i's
+ *   parent is i - 1).
+ * probs ([rows][ldq]): row r's token was drawn from probs row r (the root's row
+ *   is not read), in a chain; it is kept while number * q < p.  The token after
+ *   the last kept one is chosen with the root's number from max(p - q, 0), from
+ *   p where that is all zeros or every token was kept.
+ * counts[b] tokens are gained, as many as nodes kept: kept[b] holds the nodes
+ * (the root, 0, first) and chosen[b] the kept children's tokens and the one
+ * that follows, -1 behind them; -1 too for a token that the logits do not
+ * choose (a NaN among them, all -inf, or an infinite largest one that is
+ * sampled).  Sums are in double.  workspace: lz_verify_workspace bytes. */
+int64_t lz_verify_workspace(int64_t rows, int64_t B, int64_t V, int drawn);
+int lz_verify_draft(const void* logits, int64_t ld, int dtype, int64_t rows, int64_t V, const int64_t* tokens,
+                    const void* uniform, int u_double, const int32_t* row_start, int64_t B, int64_t nodes,
+                    const float* temperature, float temperature_s, const int32_t* parents, int64_t ldp,
+                    int64_t tree_nodes, const float* probs, int64_t ldq, int32_t* counts, int32_t* kept,
+                    int64_t* chosen, void* workspace, int64_t ws_bytes, void* stream);
+
+/* Moves the kept nodes of a step's sequences to its first places: node
+ * kept[b][j]'s keys and values to that of node j, for j < counts[b], in
+ * `layers` layers of `pages` pages that lie one after another.  slots, row_start:
+ * the step's; kept (rows of ldk, `nodes` of them) ascends; nodes that a
+ * sequence does not have and rows without a slot are left out. */
+int lz_kv_keep(void* k, void* v, void* k_exp, void* v_exp, int cache_dtype, int64_t layers, int64_t pages,
+               int64_t page_size, int64_t KV, int64_t hd, const int64_t* slots, int64_t rows, const int32_t* row_start,
+               int64_t B, const int32_t* kept, int64_t ldk, int64_t nodes, const int32_t* counts, void* stream);
+
 /* out (fp32, B rows of V) = logits after, in this order: the repetition
  * penalty of tokens in the row's text (x > 0 ? x / rep : x * rep), minus
  * freq * (occurrences after the prompt) and pres (if there are any), plus the
