@@ -19,6 +19,7 @@
 // up to four sequences in registers; where a page or a row belongs is found by
 // bisection in LDS.  The rows' positions, slots and masks follow in the same
 // launch where they are few, in rows_kernel where they are many.
+#include "draft.h"
 #include "kvcache.h"
 
 namespace {
@@ -45,43 +46,6 @@ struct TablesArgs {
   int nodes, words;
 };
 
-// The last b with start[b] <= x, of the B that there are (start[0] = 0 <= x).
-// __host__: tested there.
-__host__ __device__ __forceinline__ int last_at(const int32_t* start, int B, int x) {
-  int lo = 0, hi = B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (start[mid] <= x) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
-// A tree's node as its row: its mask (itself and its ancestors, written to
-// `mask` where that is not null) and its depth.  A parent that does not come
-// before its child is none.
-__host__ __device__ __forceinline__ int node_depth(const int32_t* parents, int nodes, int node, int32_t* mask, int words) {
-  if (mask)
-    for (int w = 0; w < words; ++w) mask[w] = 0;
-  if (node < 0 || node >= nodes) return -1;
-  int depth = 0;
-  uint32_t word = 0;
-  for (int at = node, w = node >> 5;; ++depth) {
-    if (at >> 5 != w) {
-      if (mask) mask[w] = (int32_t)word;
-      word = 0;
-      w = at >> 5;
-    }
-    word |= 1u << (at & 31);
-    const int up = parents[at];
-    if (up < 0 || up >= at) {
-      if (mask) mask[w] = (int32_t)word;
-      return depth;
-    }
-    at = up;
-  }
-}
-
 // Row r of the step, whose sequences' first rows and lengths are `start` (B + 1)
 // and `len`.
 __device__ __forceinline__ void row_of(const TablesArgs& a, const int32_t* start, const int32_t* len, int r) {
@@ -89,13 +53,14 @@ __device__ __forceinline__ void row_of(const TablesArgs& a, const int32_t* start
   int64_t slot = -1;
   int32_t* mask = a.mask ? a.mask + (int64_t)r * a.words : nullptr;
   if (r < start[a.B]) {
-    const int b = last_at(start, a.B, r), place = len[b] - start[b + 1] + r;
+    const int b = lz_last_at(start, a.B, r), place = len[b] - start[b + 1] + r;
     const LzPages pg{a.table, a.width, a.n_pages, a.log_size};
     const int page = pg.page_of(b, place);
     position = place;
     if (page >= 0) slot = ((int64_t)page << a.log_size) + (place & ((1 << a.log_size) - 1));
     if (mask) {
-      const int base = a.base[b], depth = node_depth(a.parents + b * a.ldp, a.nodes, place - base, mask, a.words);
+      const int base = a.base[b], depth = lz_node_depth(a.parents + b * a.ldp, a.nodes, (int)((uint32_t)place - (uint32_t)base), mask,
+                                                              a.words);
       if (depth >= 0) position = base + depth;
     }
   } else if (mask) {
@@ -199,7 +164,7 @@ __global__ void __launch_bounds__(kThreads) tables_kernel(TablesArgs a, int rows
   __syncthreads();
 
   for (int x = tid; x < (int)all_back; x += kThreads) {
-    const int b = last_at(gone, a.B, x);
+    const int b = lz_last_at(gone, a.B, x);
     int32_t* entry = a.table + (int64_t)b * a.width + left[b] + (x - gone[b]);
     const int64_t at = free0 + all_back - 1 - x;
     if (at < a.n_pages) a.free[at] = *entry;
@@ -207,7 +172,7 @@ __global__ void __launch_bounds__(kThreads) tables_kernel(TablesArgs a, int rows
   }
   __syncthreads();
   for (int x = tid; x < (int)all_taken; x += kThreads) {
-    const int b = last_at(taken, a.B, x);
+    const int b = lz_last_at(taken, a.B, x);
     a.table[(int64_t)b * a.width + left[b] + (x - taken[b])] = a.free[top - 1 - x];
   }
   if (rows == 0) return;  // the same for all
