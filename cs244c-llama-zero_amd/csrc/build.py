@@ -42,6 +42,7 @@ SOURCES = [
     "kvcache.hip",
     "paged_attn.hip",
     "paged_tile.hip",
+    "tree_attn.hip",
     "logits.hip",
     "tables.hip",
     "verify.hip",

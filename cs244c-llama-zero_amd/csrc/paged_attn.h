@@ -28,13 +28,17 @@ struct LzPagedArgs {
   const int32_t* base;    // [B]: the tokens that every row of the sequence sees
   const uint32_t* mask;   // [rows][words]: bit j of a row: it sees token base + j
   int words;
+  int bm, shares, least;  // tree_kernel: rows of a block; workgroups a kv head (0: one a block), keys of one at least
+  int32_t* parts;         // [B][nqb]: of the blocks
 };
 
 // paged_tile.hip: 16-bit rows in blocks of kPagedTileRows; `groups`
-// (1 or 2) of its waves share a block's keys; trees where a.mask is set.  LZ_OK
-// or a status.
+// (1 or 2) of its waves share a block's keys.  LZ_OK or a status.
 constexpr int kPagedTileRows = 128;
 int lz_paged_tile(const LzPagedArgs& a, int dtype, bool e4m3, int64_t hd, int groups, uint32_t blocks, hipStream_t stream);
+
+// tree_attn.hip: trees of 16-bit rows, in blocks of a.bm.
+int lz_tree_tiles(const LzPagedArgs& a, int dtype, bool e4m3, int64_t hd, uint32_t blocks, hipStream_t stream);
 
 namespace {
 
@@ -129,8 +133,13 @@ __host__ __device__ __forceinline__ bool sees_any(const PagedArgs& a, int b, int
 __host__ __device__ __forceinline__ bool sees_any(const PagedArgs& a, int b, int k_lo, int k_hi, const TreeRows& rw, int row) {
   if (sees_any(a, b, k_lo, k_hi, rw.ctx)) return true;
   const uint32_t* mask = a.mask + (int64_t)row * a.words;
-  for (int key = max(k_lo, rw.ctx); key < min(k_hi, rw.len); ++key)
-    if ((tree_bits(mask, a.words, key - rw.ctx) & 1) && a.pg.page_of(b, key) >= 0) return true;
+  const int end = min(k_hi, rw.len);
+  for (int key0 = max(k_lo, rw.ctx); key0 < end; key0 += 32) {
+    uint32_t bits = tree_bits(mask, a.words, key0 - rw.ctx);
+    if (end - key0 < 32) bits &= (1u << (end - key0)) - 1u;
+    for (; bits; bits &= bits - 1)
+      if (a.pg.page_of(b, key0 + __builtin_ctz(bits)) >= 0) return true;
+  }
   return false;
 }
 __host__ __device__ __forceinline__ bool sees_any(const PagedArgs& a, int b, int k_lo, int k_hi, const PagedRows& rw, int, int m) {
@@ -232,5 +241,18 @@ __device__ __forceinline__ bool nonfinite16(uint32_t w) {
   return (w & kExp) == kExp || ((w >> 16) & kExp) == kExp;
 }
 __device__ __forceinline__ bool nonfinite32(uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u; }
+
+// The fragment without its infinities and NaN.
+template <typename F>
+__device__ __forceinline__ bf16x8_t finite_part(const bf16x8_t& x) {
+  uint4 w = __builtin_bit_cast(uint4, x);
+  uint32_t* y = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (nonfinite16<F>(y[i] & 0xffffu)) y[i] &= 0xffff0000u;
+    if (nonfinite16<F>(y[i] & 0xffff0000u)) y[i] &= 0xffffu;
+  }
+  return __builtin_bit_cast(bf16x8_t, w);
+}
 
 }  // namespace

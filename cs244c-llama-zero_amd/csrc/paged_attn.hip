@@ -233,7 +233,7 @@ __device__ __forceinline__ void store_row4(const PagedArgs& a, int row, int head
   }
 }
 
-// Rows: PagedRows, or TreeRows, whose tiles from the first key that not all rows
+// Rows: PagedRows, or (fp32) TreeRows, whose tiles from the first key that not all rows
 // see on take each row's bits of its mask.
 template <typename T, int HD, bool k8, int NQ, typename Rows>
 __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
@@ -536,6 +536,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm, in
       const int m = (row - rw.row0) * rw.G + head % rw.G;
       rw.m0 = m / bm * bm;
       if (m < rw.count) n_parts = PagedRows::parts(a, rw.keys(bm));
+      if constexpr (std::is_same<Rows, TreeRows>::value)
+        if (a.shares && m < rw.count) n_parts = a.parts[(int64_t)b * a.nqb + m / bm];
     }
   }
   if (n_parts == 1) n_parts = 0;  // was written whole
@@ -588,7 +590,13 @@ struct Plan {
   int bm;  // rows of a block: 16 or 32 (paged_wave_kernel) or kPagedTileRows
   int groups;  // of the tile kernel's waves
   int nqb, nsplit, chunk;
+  int shares = 0, least = 0;  // tree_kernel
 };
+
+// Blocks of bm packed rows that have rows: not every sequence has max_new of them.
+int64_t blocks_of(int64_t bm, int64_t packed, int64_t rows, int64_t B, int64_t KV, int64_t G) {
+  return KV * std::min(B * lz_cdiv(packed, bm), std::min(B, rows) + rows * G / bm);
+}
 
 // Row blocks and parts.  Tiles of 128 rows where a sequence has 64 packed rows
 // or more and the work is not little: at most 1.5 blocks of 32 rows a CU which
@@ -624,8 +632,7 @@ Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, i
   const bool little = 2 * small <= 3 * cus && small * std::min<int64_t>(len, 1 << 20) <= 512 * cus;
   p.bm = packed <= 16 ? 16 : packed < 64 || little || dtype == LZ_F32 ? 32 : kPagedTileRows;
   p.nqb = (int)lz_cdiv(packed, p.bm);
-  // blocks that have rows: not every sequence has max_new of them
-  const int64_t blocks = KV * std::min(B * p.nqb, std::min(B, rows) + rows * G / p.bm);
+  const int64_t blocks = blocks_of(p.bm, packed, rows, B, KV, G);
   const int64_t one = std::max<int64_t>(1, cus / blocks);
   int64_t chunk = lz_cdiv(len, one);
   if (p.bm != kPagedTileRows) {
@@ -646,10 +653,46 @@ Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, i
   return p;
 }
 
+// Row blocks and shares of trees.  fp32: paged_wave_kernel, as above.  Else
+// tree_kernel: a block's keys whole where texts are short or blocks many, since
+// the share's arithmetic and the join cost 8 us (32 x 16 nodes over up to 2048,
+// 16/8 heads of 128: 38 us, shared out 45; 16 x 24 over 1024, 12/4 heads of 64: 13
+// and 17; 2 x 160 over 4096, 32/8 heads of 128, fp16: 47 and 52); elsewhere two
+// workgroups a CU of equal shares (8 x 15 over 4096, 32/8 heads: 35 us, whole 53;
+// 1 x 16 over 8192: 19 and 47), of 512 keys at least (in shares of 256: 22).
+// Blocks of 64 rows where a share is long and there are some for every eighth CU,
+// and for e4m3 heads of 128, whose converted tiles two waves share (32 rows of 32
+// sequences over up to 4096: 65 us, in blocks of 32 rows, whose bytes on the way
+// spill, 72).
+Plan make_tree_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd, int64_t max_new,
+                    int64_t max_len) {
+  Plan p = make_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
+  if (dtype == LZ_F32) return p;
+  const int64_t G = H / KV, packed = std::max<int64_t>(1, std::min(max_new, rows)) * G, cus = lz_num_cus();
+  const int64_t len = std::max<int64_t>(1, max_len), blocks = blocks_of(32, packed, rows, B, KV, G);
+  const bool shared = len > 512 && (4 * blocks < cus || (len > 2048 && (blocks < cus || B >= 8)));
+  const bool many = packed > 32 && 8 * blocks_of(64, packed, rows, B, KV, G) >= cus;
+  p.bm = shared && len >= 4096 && (many || (cache_dtype == LZ_E4M3 && hd == 128)) ? 64 : 32;
+  p.groups = 1;
+  p.nqb = (int)lz_cdiv(packed, p.bm);
+  p.nsplit = 1;
+  if (shared) {
+    p.least = 512;
+    p.shares = (int)std::max<int64_t>(1, 2 * cus / KV);
+    p.nsplit = (int)std::min<int64_t>(lz_cdiv(len, p.least) + 1, 33);
+  }
+  return p;
+}
+
 }  // namespace
 
 static bool plannable(int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t max_len) {
   return rows > 0 && B > 0 && H > 0 && KV > 0 && H % KV == 0 && max_len >= 0 && max_len <= INT32_MAX - 1024;
+}
+
+// Workspace of the parts and, for trees, of their counts.
+static int64_t part_bytes(const Plan& p, int64_t rows, int64_t B, int64_t H, int64_t hd) {
+  return p.nsplit > 1 ? rows * H * p.nsplit * (hd + 2) * 4 + (p.shares ? B * p.nqb * 4 : 0) : 0;
 }
 
 LZ_EXPORT int64_t lz_paged_attn_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV,
@@ -668,26 +711,35 @@ LZ_EXPORT int64_t lz_paged_attn_workspace(int dtype, int cache_dtype, int64_t ro
 
 LZ_EXPORT int64_t lz_tree_attn_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd,
                                     int64_t max_new, int64_t max_len) {
-  return lz_paged_attn_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
+  if (!plannable(rows, B, H, KV, max_len)) return 0;
+  const Plan p = make_tree_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
+  return p.bm | (p.bm == kPagedTileRows ? p.groups : 1) << 8 | (int64_t)p.nsplit << 16;
 }
 
 LZ_EXPORT int64_t lz_tree_attn_workspace(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV,
                                          int64_t hd, int64_t max_new, int64_t max_len) {
-  return lz_paged_attn_workspace(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
+  if (!plannable(rows, B, H, KV, max_len)) return 0;
+  const Plan p = make_tree_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
+  return part_bytes(p, rows, B, H, hd);
 }
 
 template <typename Rows>
-static void launch(const PagedArgs& a, const Plan& p, int dtype, int cache_dtype, int64_t hd, uint32_t blocks, uint32_t joins,
-                   int per, hipStream_t s) {
-#define RUN(T, HD, E8)                                                              \
-  do {                                                                              \
-    if (p.bm == 16) paged_wave_kernel<T, HD, E8, 1, Rows><<<blocks, 256, 0, s>>>(a); \
-    else paged_wave_kernel<T, HD, E8, 2, Rows><<<blocks, 256, 0, s>>>(a);           \
+static void run_waves(const PagedArgs& a, const Plan& p, int dtype, int cache_dtype, int64_t hd, uint32_t blocks,
+                      hipStream_t s) {
+#define RUN(T, HD, E8)                                                                                                   \
+  do {                                                                                                                   \
+    if constexpr (std::is_same<Rows, PagedRows>::value || std::is_same<T, float>::value) {                               \
+      if (p.bm == 16) paged_wave_kernel<T, HD, E8, 1, Rows><<<blocks, 256, 0, s>>>(a);                                   \
+      else paged_wave_kernel<T, HD, E8, 2, Rows><<<blocks, 256, 0, s>>>(a);                                              \
+    }                                                                                                                    \
   } while (0)
-  if (p.bm != kPagedTileRows) LZ_CACHE_CASES(dtype, cache_dtype, hd, RUN);
+  LZ_CACHE_CASES(dtype, cache_dtype, hd, RUN);
 #undef RUN
-#define RUN(T, HD, E8) paged_join_kernel<T, HD, Rows><<<joins, 256, 0, s>>>(a, p.bm, per)
-  if (p.nsplit > 1) LZ_CACHE_CASES(dtype, 0, hd, RUN);
+}
+template <typename Rows>
+static void run_join(const PagedArgs& a, int dtype, int64_t hd, uint32_t blocks, int per, hipStream_t s) {
+#define RUN(T, HD, E8) paged_join_kernel<T, HD, Rows><<<blocks, 256, 0, s>>>(a, a.bm, per)
+  LZ_CACHE_CASES(dtype, 0, hd, RUN);
 #undef RUN
 }
 
@@ -711,22 +763,35 @@ static int attend(const char* what, const void* q, int64_t ldq, int dtype, int64
                            ldo * esz % 16 == 0),
              "%s: rows must be 16-byte aligned", what);
   if (rows == 0) return LZ_OK;
-  const Plan p = make_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
-  const int64_t need = lz_paged_attn_workspace(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
+  const Plan p = mask ? make_tree_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len)
+                      : make_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
+  const int64_t need = part_bytes(p, rows, B, H, hd);
   LZ_REQUIRE(need == 0 || (workspace && lz_aligned16(workspace) && ws_bytes >= need),
              "%s: workspace of %lld bytes, %lld needed", what, (long long)ws_bytes, (long long)need);
-  const int64_t blocks = B * KV * p.nqb * p.nsplit, per = p.nsplit <= 4 ? 1 : p.nsplit <= 16 ? 4 : 8,
+  const int64_t blocks = p.shares ? KV * p.shares : B * KV * p.nqb * p.nsplit, per = p.nsplit <= 4 ? 1 : p.nsplit <= 16 ? 4 : 8,
                 joins = lz_cdiv(rows * H * (hd / 4) * per, 256);
+  LZ_REQUIRE(p.shares == 0 || B * p.nqb < INT32_MAX / (lz_cdiv(width * page_size, 128) + 1), "%s: too many rows and pages", what);
   LZ_REQUIRE(blocks <= INT32_MAX / 256 && joins <= INT32_MAX / 256, "%s: too many rows", what);
   PagedArgs a{q, ldq, k, v, (const int8_t*)k_exp, (const int8_t*)v_exp,
               LzPages{table, (int)width, (int)pages, lz_log2(page_size)}, row_start, kv_len, o, ldo, (float*)workspace,
               scale, (int)rows, (int)B, (int)H, (int)KV, p.nqb, p.nsplit, p.chunk,
-              (int)(std::min(max_new, rows) * (H / KV)), base, mask, (int)words};
+              (int)(std::min(max_new, rows) * (H / KV)), base, mask, (int)words, p.bm, p.shares, p.least,
+              p.shares ? (int32_t*)((float*)workspace + rows * H * p.nsplit * (hd + 2)) : nullptr};
   hipStream_t s = lz_stream(stream);
-  if (p.bm == kPagedTileRows)
-    if (int rc = lz_paged_tile(a, dtype, cache_dtype == LZ_E4M3, hd, p.groups, (uint32_t)blocks, s)) return rc;
-  if (mask) launch<TreeRows>(a, p, dtype, cache_dtype, hd, (uint32_t)blocks, (uint32_t)joins, (int)per, s);
-  else launch<PagedRows>(a, p, dtype, cache_dtype, hd, (uint32_t)blocks, (uint32_t)joins, (int)per, s);
+  const bool e8 = cache_dtype == LZ_E4M3;
+  if (mask && dtype != LZ_F32) {
+    if (int rc = lz_tree_tiles(a, dtype, e8, hd, (uint32_t)blocks, s)) return rc;
+  } else if (p.bm == kPagedTileRows) {
+    if (int rc = lz_paged_tile(a, dtype, e8, hd, p.groups, (uint32_t)blocks, s)) return rc;
+  } else if (mask) {
+    run_waves<TreeRows>(a, p, dtype, cache_dtype, hd, (uint32_t)blocks, s);
+  } else {
+    run_waves<PagedRows>(a, p, dtype, cache_dtype, hd, (uint32_t)blocks, s);
+  }
+  if (p.nsplit > 1) {
+    if (mask) run_join<TreeRows>(a, dtype, hd, (uint32_t)joins, (int)per, s);
+    else run_join<PagedRows>(a, dtype, hd, (uint32_t)joins, (int)per, s);
+  }
   return lz_check_launch(what);
 }
 

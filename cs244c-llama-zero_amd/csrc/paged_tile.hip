@@ -123,19 +123,6 @@ __device__ __forceinline__ void step_scores(f32x16_t (&s)[2], const TileOffsets<
     for (int t = 0; t < 2; ++t) s[t] = mfma16<F>(to.frag(kt, t, kk), qf[kk], s[t]);
 }
 
-// The fragment without its infinities and NaN.
-template <typename F>
-__device__ __forceinline__ bf16x8_t finite_part(const bf16x8_t& x) {
-  uint4 w = __builtin_bit_cast(uint4, x);
-  uint32_t* y = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (nonfinite16<F>(y[i] & 0xffffu)) y[i] &= 0xffff0000u;
-    if (nonfinite16<F>(y[i] & 0xffff0000u)) y[i] &= 0xffffu;
-  }
-  return __builtin_bit_cast(bf16x8_t, w);
-}
-
 // O^T += V^T . P^T of one step, each weight as two terms (weight_terms); vf: the
 // fragments of V^T for its first 16 keys, read ahead as the others are here.
 // ODD: infinities and NaN left out.
@@ -157,23 +144,13 @@ __device__ __forceinline__ void step_sum(f32x16_t (&o)[HD / 32], const f32x16_t 
   }
 }
 
-// A tree's row: bit k says whether it sees the step's key k.
-struct TreeSeen {
-  uint64_t bits;
-};
-// Whether a row does not see key `k` + 4 half of a step.
-__device__ __forceinline__ bool hidden(int lim, int k, int half) { return k + 4 * half >= lim; }
-__device__ __forceinline__ bool hidden(const TreeSeen& s, int k, int half) {
-  return !((s.bits >> (k & 32) >> (4 * half + (k & 31))) & 1);
-}
-
 // One step's softmax and its part of the sum.  s: scores of keys 32 t + 8 (r /
 // 4) + 4 half + r % 4 in register [t][r]; MASK: keys at or past `lim` (of this
-// lane's row, from the step's first key; TreeSeen: those without a bit) and 16-key tiles without their bit in
+// lane's row, from the step's first key) and 16-key tiles without their bit in
 // `here` are not seen.  ODD: see step_sum().
-template <typename F, int HD, bool MASK, bool ODD, typename Lim>
+template <typename F, int HD, bool MASK, bool ODD>
 __device__ __forceinline__ void step_softmax(f32x16_t (&s)[2], f32x16_t (&o)[HD / 32], float& m, float& l,
-                                             const TileOffsets<HD>& to, const char* vt, float unit, Lim lim,
+                                             const TileOffsets<HD>& to, const char* vt, float unit, int lim,
                                              uint32_t here, int half) {
   bf16x8_t vf[2][HD / 32];
 #pragma unroll
@@ -184,7 +161,8 @@ __device__ __forceinline__ void step_softmax(f32x16_t (&s)[2], f32x16_t (&o)[HD 
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       if constexpr (MASK) {
-        if (hidden(lim, 32 * t + 8 * (r >> 2) + (r & 3), half) || !((here >> (2 * t + (r >> 3))) & 1)) s[t][r] = -INFINITY;
+        const int key = 32 * t + 8 * (r >> 2) + 4 * half + (r & 3);
+        if (key >= lim || !((here >> (2 * t + (r >> 3))) & 1)) s[t][r] = -INFINITY;
       }
       mx = fmaxf(mx, s[t][r]);
     }
@@ -213,8 +191,8 @@ __device__ __forceinline__ void step_softmax(f32x16_t (&s)[2], f32x16_t (&o)[HD 
 }
 
 // What finite_part took out, added to the rows that see it.
-template <typename F, int HD, typename Lim>
-__device__ __forceinline__ void add_odd(f32x16_t (&o)[HD / 32], const f32x16_t (&s)[2], const char* vt, Lim lim,
+template <typename F, int HD>
+__device__ __forceinline__ void add_odd(f32x16_t (&o)[HD / 32], const f32x16_t (&s)[2], const char* vt, int lim,
                                         int lane) {
   const int half = lane >> 5, l32 = lane & 31;
 #pragma unroll 1
@@ -225,7 +203,7 @@ __device__ __forceinline__ void add_odd(f32x16_t (&o)[HD / 32], const f32x16_t (
 #pragma unroll
       for (int r = 0; r < 16; ++r) p = key >> 5 == t && 4 * ((key & 31) >> 3) + (key & 3) == r ? s[t][r] : p;
     p = __shfl(p, l32 + 32 * ((key >> 2) & 1), 64);
-    if (!hidden(lim, key, 0)) {
+    if (key < lim) {
 #pragma unroll
       for (int i = 0; i < HD / 32; ++i)
 #pragma unroll
@@ -243,7 +221,6 @@ __device__ __forceinline__ void add_odd(f32x16_t (&o)[HD / 32], const f32x16_t (
 // (eight prompts of up to 2048 tokens, 16 heads of 128, fp16: 121 us dealt in
 // turn, 102 sequence after sequence, 87 so).  Lane b of a wave counts sequence
 // b's blocks; a bisection finds the step count of the w-th one.
-template <typename Rows>
 struct ByLength {
   int b, m0;  // sequence and first row; b < 0: there are fewer blocks
 
@@ -259,10 +236,9 @@ struct ByLength {
 
   __device__ __forceinline__ ByLength(const PagedArgs& a, int w, int lane) {
     constexpr int BM = kPagedTileRows;
-    constexpr bool kTree = std::is_same<Rows, TreeRows>::value;
     if (a.B > 64) {  // sequence after sequence
       b = w / a.nqb;
-      const Rows rw(a, b, 0);
+      const PagedRows rw(a, b, 0);
       m0 = ((rw.count + BM - 1) / BM - 1 - w % a.nqb) * BM;
       if (m0 < 0) b = -1;
       return;
@@ -270,17 +246,15 @@ struct ByLength {
     int count = 0, base = 0, nq = 0;
     const int G = a.H / a.KV, cap = a.pg.width << a.pg.log_size;
     if (lane < a.B) {
-      const Rows rw(a, lane, 0);
+      const PagedRows rw(a, lane, 0);
       count = rw.count;
       base = (int)((uint32_t)rw.base + (uint32_t)rw.row0);  // keys that the sequence's first row sees
-      if constexpr (kTree) base = rw.len;
       nq = (count + BM - 1) / BM;
     }
     // this lane's first block with more than 64 s keys, nq: none; -1: all blocks
     auto first = [&](int s) {
       const uint32_t t = 64u * (uint32_t)s + 1u;
       if (s < 0) return 0;
-      if constexpr (kTree) return t > (uint32_t)base ? nq : 0;  // all blocks of a tree have the same keys
       const int d = (int)(t - (uint32_t)base);  // token of its first row that sees t keys
       if (t > (uint32_t)cap || nq == 0 || d > (count - 1) / G) return nq;
       return max(d, 0) * G / BM;
@@ -311,24 +285,23 @@ struct ByLength {
 
 // NG: groups of four waves that share the rows and take every NG-th step of
 // the keys, each with tiles of its own; they meet in LDS at the end.
-template <typename F, int HD, bool k8, int NG, typename Rows>
+template <typename F, int HD, bool k8, int NG>
 __global__ void __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(HD == 128 || NG == 2 ? 2 : 3, HD == 128 || NG == 2 ? 2 : 3)))
 paged_tile_kernel(PagedArgs a) {
   typedef Tiles<F, HD, k8> T;
   constexpr int BM = kPagedTileRows;
-  constexpr bool kTree = std::is_same<Rows, TreeRows>::value;
   __shared__ __attribute__((aligned(1024))) char smem[NG * 4 * T::kTile];
   __shared__ float stats[NG == 2 ? 4 : 1][64][2];
 
   // kv heads go to the XCDs in turn, so that a head's keys and values are
   // fetched into few L2s
   const uint32_t rest = blockIdx.x / (uint32_t)a.KV;
-  const ByLength<Rows> block(a, (int)(rest / (uint32_t)a.nsplit), threadIdx.x & 63);
+  const ByLength block(a, (int)(rest / (uint32_t)a.nsplit), threadIdx.x & 63);
   if (block.b < 0) return;
   const struct {
     int b, g, split;
   } at = {block.b, (int)(blockIdx.x % (uint32_t)a.KV), (int)(rest % (uint32_t)a.nsplit)};
-  const Rows rw(a, at.b, block.m0);
+  const PagedRows rw(a, at.b, block.m0);
   const int n_keys = rw.keys(BM), n_parts = PagedRows::parts(a, n_keys);
   if (at.split >= n_parts) return;
   const int k_lo = at.split * a.chunk, k_hi = at.split + 1 == n_parts ? n_keys : k_lo + a.chunk;
@@ -343,10 +316,10 @@ paged_tile_kernel(PagedArgs a) {
   TileOffsets<HD> to;
   to.init(lane);
 
-  // this wave's rows: all see the first `all` keys, the last sees `most`
+  // this wave's rows: the first sees `all` keys, the last `most`
   const int m_first = rw.m0 + 32 * tl.wave, m_last = min(m_first + 32, rw.count) - 1;
   const bool idle = m_first >= rw.count;
-  const int all = idle ? 0 : rw.all(m_first), most = idle ? 0 : rw.sees(m_last);
+  const int all = idle ? 0 : rw.sees(m_first), most = idle ? 0 : rw.sees(m_last);
   const int m = min(m_first + l32, rw.count - 1);  // rows past the last repeat it and are not stored
   const int row = rw.row(m), head = at.g * rw.G + m % rw.G, sees = rw.sees(m);
 
@@ -418,21 +391,10 @@ paged_tile_kernel(PagedArgs a) {
         const uint32_t here = open_round(std::false_type{});
         const int it = rt + grp;
         if (it < wave_end) {
-          auto seen = [&] {
-            if constexpr (kTree) {
-              const uint32_t* mask = a.mask + (int64_t)row * a.words;
-              const int off = 64 * it - all;
-              const uint64_t bits = tree_bits(mask, a.words, off) | (uint64_t)tree_bits(mask, a.words, off + 32) << 32;
-              const int left = sees - 64 * it;  // of the sequence's keys
-              return TreeSeen{left >= 64 ? bits : left > 0 ? bits & ((1ull << left) - 1) : 0};
-            } else {
-              return sees - 64 * it;
-            }
-          }();
           f32x16_t s[2];
           step_scores<F, HD>(s, to, tl.k_tile(), qf);
-          step_softmax<F, HD, true, ODD>(s, o, mx, l, to, tl.v_tile(), unit, seen, here, half);
-          if constexpr (ODD) add_odd<F, HD>(o, s, tl.v_tile(), seen, lane);
+          step_softmax<F, HD, true, ODD>(s, o, mx, l, to, tl.v_tile(), unit, sees - 64 * it, here, half);
+          if constexpr (ODD) add_odd<F, HD>(o, s, tl.v_tile(), sees - 64 * it, lane);
         }
         close_round();
       }
@@ -473,7 +435,7 @@ paged_tile_kernel(PagedArgs a) {
       for (int r = 0; r < 16; ++r) o[i][r] = fmaf(o[i][r], f, park[(16 * i + r) * 64] * f2);
   }
   if (m_first + l32 >= rw.count) return;
-  if (mx == -INFINITY && sees_any(a, at.b, k_lo, k_hi, rw, row, m)) mx = kAllInf;
+  if (mx == -INFINITY && sees_any(a, at.b, k_lo, k_hi, sees)) mx = kAllInf;
   if (n_parts == 1) {
     const float inv = mx == -INFINITY ? 0.f : 1.f / l;
     uint16_t* op = static_cast<uint16_t*>(a.o) + (int64_t)row * a.ldo + head * HD;
@@ -502,19 +464,16 @@ paged_tile_kernel(PagedArgs a) {
 
 }  // namespace
 
-namespace {
-
-template <typename Rows>
-void run_tiles(const LzPagedArgs& a, int dtype, bool e4m3, int64_t hd, int groups, uint32_t blocks, hipStream_t stream) {
+int lz_paged_tile(const LzPagedArgs& a, int dtype, bool e4m3, int64_t hd, int groups, uint32_t blocks, hipStream_t stream) {
 #define RUN(F, HD)                                                                      \
   do {                                                                                  \
     if (groups == 2) {                                                                  \
-      if (e4m3) paged_tile_kernel<F, HD, true, 2, Rows><<<blocks, 512, 0, stream>>>(a); \
-      else paged_tile_kernel<F, HD, false, 2, Rows><<<blocks, 512, 0, stream>>>(a);     \
+      if (e4m3) paged_tile_kernel<F, HD, true, 2><<<blocks, 512, 0, stream>>>(a);       \
+      else paged_tile_kernel<F, HD, false, 2><<<blocks, 512, 0, stream>>>(a);           \
     } else if (e4m3) {                                                                  \
-      paged_tile_kernel<F, HD, true, 1, Rows><<<blocks, 256, 0, stream>>>(a);           \
+      paged_tile_kernel<F, HD, true, 1><<<blocks, 256, 0, stream>>>(a);                 \
     } else {                                                                            \
-      paged_tile_kernel<F, HD, false, 1, Rows><<<blocks, 256, 0, stream>>>(a);          \
+      paged_tile_kernel<F, HD, false, 1><<<blocks, 256, 0, stream>>>(a);                \
     }                                                                                   \
   } while (0)
   if (dtype == LZ_F16) {
@@ -527,12 +486,5 @@ void run_tiles(const LzPagedArgs& a, int dtype, bool e4m3, int64_t hd, int group
     else RUN(FmtBF16, 128);
   }
 #undef RUN
-}
-
-}  // namespace
-
-int lz_paged_tile(const LzPagedArgs& a, int dtype, bool e4m3, int64_t hd, int groups, uint32_t blocks, hipStream_t stream) {
-  if (a.mask) run_tiles<TreeRows>(a, dtype, e4m3, hd, groups, blocks, stream);
-  else run_tiles<PagedRows>(a, dtype, e4m3, hd, groups, blocks, stream);
-  return lz_check_launch(a.mask ? "lz_tree_attn" : "lz_paged_attn");
+  return lz_check_launch("lz_paged_attn");
 }
