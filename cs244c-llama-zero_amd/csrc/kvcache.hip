@@ -213,7 +213,11 @@ struct KeepArgs {
 // it has written, and no other thread touches its bytes.
 template <bool k8>
 __global__ void __launch_bounds__(256) kv_keep_kernel(KeepArgs a, int chunks) {
+  constexpr int kAhead = 8;
   const int b = blockIdx.y;
+  int node[kAhead];  // fetched beside the counts that say which of them there are
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) node[i] = a.kept[b * a.ldk + min(i, a.nodes - 1)];
   const int lo = min(max(a.row_start[b], 0), a.rows), hi = min(max(a.row_start[b + 1], lo), a.rows), n = hi - lo;
   const int count = min(min(a.counts[b], n), a.nodes);
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
@@ -229,29 +233,36 @@ __global__ void __launch_bounds__(256) kv_keep_kernel(KeepArgs a, int chunks) {
   auto place = [&](int64_t slot) {  // of this head, in tokens
     return ((((slot >> a.log_size) * a.KV + g) << a.log_size) + (slot & mask));
   };
-  constexpr int kAhead = 8;
   for (int j0 = 0; j0 < count; j0 += kAhead) {
-    int64_t dst[kAhead];
+    // each of these rounds in flight together: nodes, slots, tokens
+    if (j0 > 0)
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) node[i] = a.kept[b * a.ldk + min(j0 + i, a.nodes - 1)];
+    int64_t from[kAhead], to[kAhead];
+    bool moves[kAhead];
     uint4 w[kAhead];
     int8_t we[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int j = j0 + i;
-      dst[i] = -1;
-      const int node = j < count ? a.kept[b * a.ldk + j] : -1;
-      if (node < 0 || node >= n || node == j) continue;
-      const int64_t from = a.slots[lo + node], to = a.slots[lo + j];
-      if (from < 0 || from >= a.slots_all || to < 0 || to >= a.slots_all) continue;
-      dst[i] = place(to);
-      const int64_t src = place(from);
-      w[i] = *reinterpret_cast<const uint4*>(x + src * chunks * 16);
-      if (k8 && c == 0) we[i] = e[src];
+      from[i] = a.slots[lo + min(max(node[i], 0), n - 1)];
+      to[i] = a.slots[lo + min(j0 + i, count - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      moves[i] = j0 + i < count && node[i] >= 0 && node[i] < n && node[i] != j0 + i && (uint64_t)from[i] < (uint64_t)a.slots_all &&
+                 (uint64_t)to[i] < (uint64_t)a.slots_all;
+      if (moves[i]) {  // the same for the workgroup
+        const int64_t src = place(from[i]);
+        w[i] = *reinterpret_cast<const uint4*>(x + src * chunks * 16);
+        if (k8) we[i] = e[src];
+      }
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
-      if (dst[i] >= 0) {
-        *reinterpret_cast<uint4*>(x + dst[i] * chunks * 16) = w[i];
-        if (k8 && c == 0) e[dst[i]] = we[i];
+      if (moves[i]) {
+        const int64_t dst = place(to[i]);
+        *reinterpret_cast<uint4*>(x + dst * chunks * 16) = w[i];
+        if (k8 && c == 0) e[dst] = we[i];
       }
   }
 }

@@ -484,8 +484,8 @@ int lz_tree_attn(const void* q, int64_t ldq, int dtype, int64_t rows, const void
  * become -1); row_start (B + 1), kv_len and base (first[b]; NULL: the kept
  * length) are written, and for each of the `rows` rows its position, its slot
  * (page * page_size + place in it) and its mask, -1, -1 and 0 for rows of no
- * sequence.  parents ([nodes] with ldp 0, or B rows of ldp): node i's, -1 or
- * any value that is not below i for none; node i of a sequence is its place
+ * sequence.  parents ([nodes] with ldp 0, or B rows of ldp = nodes): node
+ * i's, -1 or any value that is not below i for none; node i of a sequence is its place
  * base[b] + i.  Without parents (and mask) a row's position is its place. */
 int lz_cache_tables(int32_t* table, int64_t width, int32_t* lengths, int32_t* free, int64_t pages, int32_t* n_free,
                     int64_t page_size, const int32_t* add, const int32_t* keep, const int32_t* first,

@@ -51,7 +51,7 @@ KEEP = dict(k=P, v=P, k_exp=None, v_exp=None, cache=1, layers=2, pages=4, size=1
                             dict(scale=0.0), dict(max_new=-1), dict(size=24)]),
     ("lz_cache_tables", TABLES, [dict(size=24), dict(size=8), dict(B=0), dict(B=4097), dict(width=0), dict(width=2**30),
                                  dict(pages=0), dict(rows=-1), dict(rows=2**31), dict(max_new=-1), dict(max_len=2**31),
-                                 dict(mask=None), dict(parents=None), dict(words=1), dict(nodes=0), dict(ldp=32),
+                                 dict(mask=None), dict(parents=None), dict(words=1), dict(nodes=0), dict(ldp=32), dict(ldp=34),
                                  dict(table=None), dict(slots=None), dict(add=None)]),
     ("lz_verify_draft", VERIFY, [dict(dtype=5), dict(rows=-1), dict(V=0), dict(V=2**29), dict(B=0), dict(nodes=0),
                                  dict(nodes=4097), dict(probs=P), dict(tree=0), dict(ldp=2), dict(ld=7), dict(tokens=None),
