@@ -2,7 +2,9 @@
 
 LayerCache and CacheStep are what the kernels take (ops.kv_cache_write,
 ops.paged_attention, ops.kv_cache_read); KVCache owns the pages of a model's
-layers and hands them to sequences.  The reference has no cache: its generate
+layers and hands them to sequences.  DraftStep, PageTables and DraftCache are
+the same for steps whose lengths the device alone knows, as when drafted tokens
+are verified there.  The reference has no cache: its generate
 (model/llama.py:311-335) runs the whole window through the model for every
 token.
 """
@@ -10,7 +12,7 @@ from __future__ import annotations
 
 import itertools
 import operator
-from typing import List, NamedTuple, Optional, Sequence, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -116,11 +118,17 @@ class KVCache:
         exps: List[Optional[torch.Tensor]] = [None, None]
         if eight:
             exps = [torch.empty(shape[:4], dtype=torch.int8, device=self.device) for _ in range(2)]
+        self._exps = exps
         self.layers = [LayerCache(self._k[i], self._v[i], *(None if e is None else e[i] for e in exps))
                        for i in range(n_layers)]
         self.lengths = [0] * batch
         self._pages: List[List[int]] = [[] for _ in range(batch)]
         self._free = list(range(n_pages - 1, -1, -1))
+
+    @property
+    def stacked(self) -> LayerCache:
+        """All layers' pages in one: [layers, pages, ...] (ops.kv_cache_keep)."""
+        return LayerCache(self._k, self._v, *self._exps)
 
     @staticmethod
     def _page_table(pages: Sequence[List[int]]) -> List[List[int]]:
@@ -166,4 +174,63 @@ class KVCache:
         n, kv = self.lengths[b], self.layers[layer]
         flat = torch.tensor([0, n] + self._page_table([self._pages[b]])[0], dtype=torch.int32).to(self.device)
         k, v = ops.kv_cache_read(kv, flat[2:].view(1, -1), flat[:2], n, self.dtype)
+        return k.view(n, *kv.k.shape[1::2]), v.view(n, *kv.v.shape[1::2])
+
+
+class DraftCache(KVCache):
+    """KVCache whose page tables and lengths are kept on the device (`tables`),
+    for sequences of up to max_len tokens: a step does not need their lengths
+    on the host, and what is rejected of a draft goes back with the next one.
+
+    A sequence that the pages do not suffice for is left out of a step (its rows
+    in row_start are none) where KVCache.step raises."""
+
+    def __init__(self, *args, max_len: int, **kw) -> None:
+        super().__init__(*args, **kw)
+        if max_len < 1:
+            raise ValueError(f"sequences of up to {max_len} tokens")
+        batch, full = len(self.lengths), lambda *n: torch.full(n, -1, dtype=torch.int32, device=self.device)
+        self.max_len = max_len
+        self.tables = PageTables(full(batch, -(-max_len // self.page_size)), full(batch).zero_(),
+                                 torch.arange(self.n_pages, dtype=torch.int32, device=self.device),
+                                 full(1).fill_(self.n_pages), self.page_size)
+        del self.lengths, self._pages, self._free  # the host does not know them
+
+    def step(self, new: Union[Sequence[int], torch.Tensor], *, rows: Optional[int] = None, max_new: Optional[int] = None,
+             max_len: Optional[int] = None, keep: Optional[torch.Tensor] = None, base: Optional[torch.Tensor] = None,
+             parents: Optional[torch.Tensor] = None) -> DraftStep:
+        """Room for new[b] more tokens of every sequence, after each is cut to
+        keep[b] (see ops.cache_tables).  new: counts, or int32 [B] on the device
+        with bounds `rows` and max_new of their sum and of each; max_len: a bound
+        on the lengths (None: the cache's)."""
+        if not torch.is_tensor(new):
+            new = [operator.index(n) for n in new]
+            if len(new) != len(self.tables.lengths):
+                raise ValueError(f"{len(new)} counts of new tokens for {len(self.tables.lengths)} sequences")
+            if min(new) < 0:
+                raise ValueError("counts of new tokens must not be negative")
+            rows, max_new = sum(new), max(new)
+            new = torch.tensor(new, dtype=torch.int32).to(self.device)
+        elif rows is None or max_new is None:
+            raise ValueError("counts on the device need bounds: rows and max_new")
+        return ops.cache_tables(self.tables, new, rows, max_new, self.max_len if max_len is None else max_len, keep=keep,
+                                base=base, parents=parents)
+
+    def keep(self, step: DraftStep, kept: torch.Tensor, counts: torch.Tensor) -> None:
+        """Moves what ops.verify_draft kept of `step` to its first places, in
+        all layers; the next step's keep is base + counts."""
+        ops.kv_cache_keep(self.stacked, step, kept, counts)
+
+    def free(self, b: int) -> None:
+        """Ends sequence b: its pages go back, and its slot is empty."""
+        keep = self.tables.lengths.clone()
+        keep[b] = 0
+        self.step(torch.zeros_like(keep), rows=0, max_new=0, keep=keep)
+
+    def read(self, layer: int, b: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Sequence b's keys and values in one layer, [tokens, KV heads, head
+        dim] each, in the model's dtype.  Waits for the device."""
+        n, kv = int(self.tables.lengths[b]), self.layers[layer]
+        start = torch.tensor([0, n], dtype=torch.int32).to(self.device)
+        k, v = ops.kv_cache_read(kv, self.tables.page_table[b : b + 1].contiguous(), start, n, self.dtype)
         return k.view(n, *kv.k.shape[1::2]), v.view(n, *kv.v.shape[1::2])

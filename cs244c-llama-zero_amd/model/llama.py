@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import threading
 from dataclasses import dataclass
-from typing import Any, Callable, Optional, Tuple, Union
+from typing import Any, Callable, List, Optional, Sequence, Tuple, Union
 
 import torch
 import torch.nn as nn
@@ -21,7 +21,7 @@ from torch.utils.checkpoint import checkpoint as activation_checkpoint
 
 from lzhip import functional as LF
 from lzhip import ops
-from lzhip.cache import CacheStep, KVCache, LayerCache
+from lzhip.cache import CacheStep, DraftCache, DraftStep, KVCache, LayerCache
 
 from .config import ModelConfig
 
@@ -30,11 +30,39 @@ def _next_token(logits: torch.Tensor, temperature: float, top_k: Optional[int]) 
     """One token per row of [B, V] logits (see LlamaForCausalLM.generate)."""
     if temperature <= 0:
         return logits.argmax(dim=-1)
-    scaled = logits / temperature
-    if top_k is not None:
-        kth = torch.topk(scaled, min(top_k, scaled.size(-1))).values[:, -1:]
-        scaled = scaled.masked_fill(scaled < kth, float("-inf"))
+    scaled = _cut(logits / temperature, top_k)
     return torch.multinomial(torch.softmax(scaled, dim=-1), num_samples=1).squeeze(-1)
+
+
+def _cut(logits: torch.Tensor, top_k: Optional[int]) -> torch.Tensor:
+    """The rows' top_k largest logits, the others -inf."""
+    if top_k is None:
+        return logits
+    kth = torch.topk(logits, min(top_k, logits.size(-1))).values[:, -1:]
+    return logits.masked_fill(logits < kth, float("-inf"))
+
+
+class _Tree:
+    """Drafted tokens of one sequence: the root, and `widths[i]` children of
+    each node of level i.  Nodes are numbered level by level."""
+
+    def __init__(self, widths: Sequence[int]) -> None:
+        self.widths = list(widths)
+        self.levels, self.parents = [(0, 1)], [-1]
+        for w in self.widths:
+            lo, hi = self.levels[-1]
+            self.parents += [p for p in range(lo, hi) for _ in range(w)]
+            self.levels.append((hi, len(self.parents)))
+        self.nodes = len(self.parents)
+
+    def step_of(self, step: DraftStep, level: int) -> DraftStep:
+        """The rows of a level, of a step that made room for all nodes."""
+        lo, hi = self.levels[level]
+        B, n = step.kv_len.numel(), hi - lo
+        of = lambda t: t.view(B, self.nodes, *t.shape[1:])[:, lo:hi].reshape(B * n, *t.shape[1:]).contiguous()  # noqa: E731
+        return step._replace(row_start=torch.arange(0, B * n + 1, n, dtype=torch.int32, device=step.kv_len.device),
+                             kv_len=step.base + hi, rows=B * n, max_new=n, positions=of(step.positions), slots=of(step.slots),
+                             mask=None if step.mask is None else of(step.mask))
 
 
 def _require_choice(logits: torch.Tensor, t: int, temperature: float) -> None:
@@ -457,12 +485,18 @@ class LlamaForCausalLM(nn.Module):
                        device=w.device)
 
     @torch.no_grad()
-    def forward_cached(self, ids: torch.Tensor, cache: KVCache, step: CacheStep) -> torch.Tensor:
-        """Logits [B, V] of each sequence's last new token.  ids: the step's
-        new tokens, sequence after sequence ([rows] int64); step: what
-        cache.step(counts) returned for them.  Without dropout, whatever the
-        mode; forward hooks of the model, its blocks and their attention do not
-        run.  The row of a sequence that has no new tokens says nothing."""
+    def forward_cached(self, ids: torch.Tensor, cache: KVCache, step: Union[CacheStep, DraftStep], *,
+                       rows: str = "last") -> torch.Tensor:
+        """Logits [B, V] of each sequence's last new token, or of every new
+        token (rows="all": [step.rows, V]); rows="none" fills the cache alone
+        and returns the last block's output.  ids: the step's new tokens,
+        sequence after sequence ([rows] int64); step: what cache.step(counts)
+        returned for them.  Without dropout, whatever the mode; forward hooks of
+        the model, its blocks and their attention do not run.  The row of a
+        sequence that has no new tokens says nothing, nor do rows of no
+        sequence."""
+        if rows not in ("last", "all", "none"):
+            raise ValueError(f"rows must be 'last', 'all' or 'none', not {rows!r}")
         if self._zero3_executor is not None and not getattr(self._zero3_executor, "params_materialized", False):
             raise RuntimeError("a ZeRO-3 sharded model has no cached forward: gather its parameters first "
                                "(summon_full_params; a forward within it hands them back) or generate without use_cache")
@@ -475,8 +509,11 @@ class LlamaForCausalLM(nn.Module):
         x = self.tok_embeddings(ids)
         for layer, block in zip(cache.layers, self.layers):
             x = block.forward_cached(x, layer, step)
-        last = ops.embedding_fwd((step.row_start[1:] - 1).long(), x)  # rows of x
-        return self.lm_head(self.norm(last))
+        if rows == "none":
+            return x
+        if rows == "last":
+            x = ops.embedding_fwd((step.row_start[1:] - 1).long(), x)  # rows of x
+        return self.lm_head(self.norm(x))
 
     @torch.no_grad()
     def generate(
@@ -493,6 +530,8 @@ class LlamaForCausalLM(nn.Module):
         frequency_penalty: Union[float, torch.Tensor] = 0.0,
         logit_bias: Optional[torch.Tensor] = None,
         token_mask: Union[None, torch.Tensor, Callable[[torch.Tensor], torch.Tensor]] = None,
+        draft_model: Optional["LlamaForCausalLM"] = None,
+        draft_tokens: Union[int, Sequence[int]] = 4,
     ) -> torch.Tensor:
         """Autoregressive sampling with the reference's semantics
         (model/llama.py:311-335): each new token takes a full forward over the
@@ -509,8 +548,17 @@ class LlamaForCausalLM(nn.Module):
         ops.process_logits says, the prompt counting for repetition_penalty
         alone.  They are then looked at, for which the host waits for the
         device: a row without a token to choose (all -inf, or NaN; infinite
-        where a token is sampled) is a ValueError."""
-        if cache_dtype is not None and not use_cache:
+        where a token is sampled) is a ValueError.
+
+        draft_model (of the same vocabulary) drafts draft_tokens tokens ahead,
+        which one pass of this model then verifies: a chain that it draws from
+        its own distribution, or, given widths such as (3, 2, 1), a tree of its
+        likeliest tokens, that many children for each node of a level.  What is
+        generated is distributed as without it (temperature <= 0: the same
+        tokens, as far as the two ways to compute the logits agree).  Both
+        models keep caches; the whole text has to fit both's max_seq_len, and
+        penalties, logit_bias and token_mask are refused."""
+        if cache_dtype is not None and not use_cache and draft_model is None:
             raise ValueError("cache_dtype is for use_cache=True")
         self.eval()
         bsz, t0 = input_ids.shape
@@ -520,6 +568,10 @@ class LlamaForCausalLM(nn.Module):
         penalties = ((repetition_penalty, 1.0), (presence_penalty, 0.0), (frequency_penalty, 0.0))
         adjust = (any(torch.is_tensor(p) or p != none for p, none in penalties)
                   or logit_bias is not None or token_mask is not None)
+        if draft_model is not None:
+            if adjust:
+                raise ValueError("penalties, logit_bias and token_mask are not taken with a draft_model")
+            return self._generate_drafted(seq, t0, temperature, top_k, cache_dtype, draft_model, draft_tokens)
         prompts = torch.full((bsz,), t0, dtype=torch.int32, device=seq.device) if adjust else None
         cache, cached = None, 0
         if use_cache and 0 < t0 <= window and max_new_tokens > 0:
@@ -541,3 +593,80 @@ class LlamaForCausalLM(nn.Module):
                 _require_choice(last, t, temperature)
             seq[:, t] = _next_token(last.float(), temperature, top_k)
         return seq
+
+    def _generate_drafted(self, seq: torch.Tensor, t0: int, temperature: float, top_k: Optional[int],
+                          cache_dtype: Optional[torch.dtype], draft: "LlamaForCausalLM",
+                          draft_tokens: Union[int, Sequence[int]]) -> torch.Tensor:
+        """generate() with a draft model; seq: [B, t0 + new], its first t0 given."""
+        chain = isinstance(draft_tokens, int)
+        widths = [1] * draft_tokens if chain else [int(w) for w in draft_tokens]
+        B, total = seq.shape
+        if not widths or min(widths) < 1:
+            raise ValueError(f"draft_tokens must be positive, got {draft_tokens}")
+        if draft.cfg.vocab_size != self.cfg.vocab_size:
+            raise ValueError(f"a draft model of {draft.cfg.vocab_size} tokens for one of {self.cfg.vocab_size}")
+        if t0 < 1 or total > min(self.cfg.max_seq_len, draft.cfg.max_seq_len):
+            raise ValueError(f"{total} tokens (of which {t0} are given) do not fit both models' max_seq_len "
+                             f"({self.cfg.max_seq_len} and {draft.cfg.max_seq_len})")
+        if not chain and max(widths) > self.cfg.vocab_size:
+            raise ValueError(f"{max(widths)} children of a node from {self.cfg.vocab_size} tokens")
+        if total == t0:
+            return seq
+        draft.eval()
+        tree, dev = _Tree(widths), seq.device
+        N, models = tree.nodes, (self, draft)
+        page = 64
+        caches = [DraftCache(m.cfg.n_layers, m.cfg.n_kv_heads, m.cfg.head_dim, batch=B,
+                             n_pages=B * -(-(total + N) // page), page_size=page, dtype=m.tok_embeddings.weight.dtype,
+                             storage=cache_dtype, device=dev, max_len=total + N) for m in models]
+        if t0 > 1:
+            for m, cache in zip(models, caches):
+                step = cache.step([t0 - 1] * B, max_len=t0 - 1)
+                m.forward_cached(seq[:, : t0 - 1].reshape(-1), cache, step, rows="none")
+        parents = None if chain else torch.tensor(tree.parents, dtype=torch.int32, device=dev)
+        new = torch.full((B,), N, dtype=torch.int32, device=dev)
+        cached = torch.full((B,), t0 - 1, dtype=torch.int32, device=dev)  # tokens before the root
+        lengths = [t0] * B  # of the texts
+        drawn = chain and temperature > 0
+        i = torch.arange(N, device=dev)
+        text = torch.nn.functional.pad(seq, (0, N))  # room for what is cut off at the end
+        while min(lengths) < total:
+            bound = dict(rows=B * N, max_new=N, max_len=max(lengths) - 1 + N, keep=cached, parents=parents)
+            ids = torch.empty((B, N), dtype=torch.int64, device=dev)
+            ids[:, 0] = text.gather(1, cached.long()[:, None])[:, 0]
+            probs: List[torch.Tensor] = []
+            ahead = caches[1].step(new, **bound)
+            for level, (lo, hi) in enumerate(tree.levels):
+                step, last = tree.step_of(ahead, level), level == len(tree.widths)
+                x = draft.forward_cached(ids[:, lo:hi].reshape(-1), caches[1], step, rows="none" if last else "all")
+                if last:
+                    break
+                if drawn:
+                    probs.append(torch.softmax(_cut(x.float() / temperature, top_k), -1))
+                    ids[:, hi] = torch.multinomial(probs[-1], 1)[:, 0]
+                else:
+                    first, end = tree.levels[level + 1]
+                    ids[:, first:end] = x.topk(tree.widths[level]).indices.view(B, -1)
+            step = caches[0].step(new, **bound)
+            flat = ids.view(-1)
+            logits = self.forward_cached(flat, caches[0], step, rows="all")
+            if temperature > 0:
+                logits = _cut(logits.float(), top_k) if top_k is not None else logits
+            q = torch.stack([probs[0], *probs], 1).view(B * N, -1) if drawn else None  # the root's is not read
+            counts, kept, chosen = ops.verify_draft(
+                logits, flat, step.row_start, N, torch.rand(B * N, dtype=torch.float64, device=dev),
+                temperature=float(max(temperature, 0.0)), parents=parents, draft_probs=q)
+            # no further than the text goes; the last token of what is gained is the next root
+            counts = torch.minimum(counts, (total - 1 - cached).clamp(min=0))
+            if not chain:
+                for cache, made in zip(caches, (step, ahead)):
+                    cache.keep(made, kept, counts)
+            at = cached.long()[:, None] + 1 + i
+            gained = i < counts[:, None]
+            text.scatter_(1, at, torch.where(gained, chosen, text.gather(1, at)))
+            cached = cached + counts
+            *ends, none = torch.cat([cached, (gained & (chosen < 0)).any().view(1)]).tolist()  # waits, once a step
+            if none:
+                raise ValueError("a row's logits leave no token to choose (NaN, or infinite where it is sampled)")
+            lengths = [n + 1 for n in ends]
+        return text[:, :total]
