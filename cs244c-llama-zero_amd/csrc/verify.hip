@@ -74,17 +74,21 @@ __constant__ const double kRoots[32] = {
     1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
 };
 
-// A workgroup's table of them, in LDS, and 2^(t / 32).
+// A workgroup's table of them, in LDS, and 2^(t / 32).  With t = n + f the result
+// is 2^(n >> 5) 2^((n & 31) / 32) 2^(f / 32): the exponent is added to the table's
+// value, from which the part that n & 31 adds too is taken beforehand.
 struct Exp {
-  const double* roots;
+  const int2* roots;
 
   // With the whole workgroup, before any use.
-  __device__ __forceinline__ explicit Exp(double* lds) : roots(lds) {
-    if (threadIdx.x < 32) lds[threadIdx.x] = kRoots[threadIdx.x];
+  __device__ __forceinline__ explicit Exp(int2* lds) : roots(lds) {
+    const int k = threadIdx.x;
+    if (k < 32) lds[k] = make_int2(__double2loint(kRoots[k]), __double2hiint(kRoots[k]) - (k << 15));
     __syncthreads();
   }
-  // t <= 0; below -32000 as -32000 (no sum of weights up to 1 holds those), NaN too.
-  __device__ __forceinline__ double operator()(double t) const {
+  // t <= 0 as two factors; below -32000 as -32000 (no sum of weights up to 1 holds
+  // those), NaN too.
+  __device__ __forceinline__ void parts(double t, double& series, double& power) const {
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52
     t = fmax(t, -32000.0);
     const double z = t + kRound, f = t - (z - kRound);
@@ -93,9 +97,19 @@ struct Exp {
     p = fma(p, f, 1.6938509724371819e-06);
     p = fma(p, f, 0.00023459619820224677);
     p = fma(p, f, 0.02166084939249829);
-    p = fma(p, f, 1.0);
-    p *= roots[n & 31];
-    return __hiloint2double(__double2hiint(p) + (int)((uint32_t)(n >> 5) << 20), __double2loint(p));
+    series = fma(p, f, 1.0);
+    const int2 r = roots[n & 31];
+    power = __hiloint2double((int)(((uint32_t)n << 15) + (uint32_t)r.y), r.x);
+  }
+  __device__ __forceinline__ double operator()(double t) const {
+    double series, power;
+    parts(t, series, power);
+    return series * power;
+  }
+  __device__ __forceinline__ void add_to(double& sum, double t) const {
+    double series, power;
+    parts(t, series, power);
+    sum = fma(series, power, sum);
   }
 };
 
@@ -186,7 +200,7 @@ struct Nodes {
 // NV vectors of a piece, a wave each.
 template <typename T, int NV>
 __global__ void __launch_bounds__(256) stats_kernel(VerifyArgs a) {
-  __shared__ double roots[32];
+  __shared__ int2 roots[32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t per_row = (uint32_t)(a.n_pieces + 3) / 4;
   const int row = (int)(blockIdx.x / per_row), p = (int)(blockIdx.x % per_row) * 4 + wave;
@@ -222,10 +236,11 @@ __global__ void __launch_bounds__(256) stats_kernel(VerifyArgs a) {
     arg = least_of_wave(arg);
   } else if (top > -INFINITY && top < INFINITY) {
     // (tokens that may not be chosen add 2^-1000 beside a sum of 1 or more)
+    // (the largest's is 1: equal logits' sums are whole numbers)
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += exp(((double)x[k][e] - (double)top) * c);
+      for (int e = 0; e < 8; ++e) exp.add_to(sum, ((double)x[k][e] - (double)top) * c);
     sum = sum_of_wave(sum);
   }
   if (lane == 0) {
@@ -361,7 +376,7 @@ constexpr int kMostNodes = 4096;
 // Every row's choice, a wave each.
 template <typename T, int NV>
 __global__ void __launch_bounds__(256) pick_kernel(VerifyArgs a) {
-  __shared__ double roots[32];
+  __shared__ int2 roots[32];
   const Exp exp(roots);
   const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (row >= a.rows) return;
@@ -375,7 +390,7 @@ __global__ void __launch_bounds__(256) pick_kernel(VerifyArgs a) {
 // 16 rows of short vocabularies itself.
 template <typename T, int NV>
 __global__ void __launch_bounds__(1024) walk_kernel(VerifyArgs a) {
-  __shared__ double roots[32];
+  __shared__ int2 roots[32];
   __shared__ int choice[kMostNodes], token[kMostNodes], parent[kMostNodes], path[kMostNodes];
   __shared__ int n_path;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -430,7 +445,7 @@ __global__ void __launch_bounds__(1024) walk_kernel(VerifyArgs a) {
 // at a time, and sums what is left of p beside q over four pieces of that row.
 template <typename T>
 __global__ void __launch_bounds__(256) rest_kernel(VerifyArgs a) {
-  __shared__ double roots[32];
+  __shared__ int2 roots[32];
   __shared__ int kept[4];
   const Exp exp(roots);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -486,7 +501,7 @@ __global__ void __launch_bounds__(256) rest_kernel(VerifyArgs a) {
 // The token after a chain's last kept one, a wave for each sequence.
 template <typename T, int NV>
 __global__ void __launch_bounds__(64) end_kernel(VerifyArgs a) {
-  __shared__ double roots[32];
+  __shared__ int2 roots[32];
   const Exp exp(roots);
   const int b = blockIdx.x, lane = threadIdx.x;
   const Nodes s(a, b);
