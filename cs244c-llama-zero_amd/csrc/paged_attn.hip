@@ -655,24 +655,33 @@ Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, i
 
 // Row blocks and shares of trees.  fp32: paged_wave_kernel, as above.  Else
 // tree_kernel: a block's keys whole where texts are short or blocks many, since
-// the share's arithmetic and the join cost 8 us (32 x 16 nodes over up to 2048,
-// 16/8 heads of 128: 38 us, shared out 45; 16 x 24 over 1024, 12/4 heads of 64: 13
-// and 17; 2 x 160 over 4096, 32/8 heads of 128, fp16: 47 and 52); elsewhere two
-// workgroups a CU of equal shares (8 x 15 over 4096, 32/8 heads: 35 us, whole 53;
-// 1 x 16 over 8192: 19 and 47), of 512 keys at least (in shares of 256: 22).
+// the shares' arithmetic and the join cost 8 us (32 x 16 nodes over up to 2048,
+// 16/8 heads of 128: 37 us, shared out 45; 16 x 24 over 1024, 12/4 heads of 64: 13
+// and 20); elsewhere two workgroups a CU of equal shares (8 x 15 over 4096, 32/8
+// heads: 32 us, whole 50; 1 x 16 over 8192: 19 and 79), of 512 keys at least (that
+// one in shares of 256: 22).  Blocks for three quarters of the CUs, 16 bits, up to
+// 4096 keys: whole (3 x 100 over 4096, 32/8 heads: 43 us, shared out 51; 6 x 80,
+// 16/8 heads: 44 and 43; in e4m3 60 and 56); for up to a quarter more than there
+// are, whose second turn is nearly empty, longer texts in shares (2 x 160 over
+// 8192, 32/8 heads: 74 us, whole 79, in e4m3 83 and 108; 4 x 140 over 6000: 63 and
+// 61, 70 and 82; heads of 64: 42 and 46).
 // Blocks of 64 rows where a share is long and there are some for every eighth CU,
-// and for e4m3 heads of 128, whose converted tiles two waves share (32 rows of 32
-// sequences over up to 4096: 65 us, in blocks of 32 rows, whose bytes on the way
-// spill, 72).
+// and for e4m3 heads of 128, whose converted tiles two waves share (8 rows of 32
+// sequences over up to 4096, 32/8 heads: 60 us, in blocks of 32 rows, whose bytes
+// on the way spill, 72; 4 x 120 over 3000, 16/8 heads: 40 and 54; but 1 x 8 over
+// 2500 22 and 20).
 Plan make_tree_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd, int64_t max_new,
                     int64_t max_len) {
   Plan p = make_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
   if (dtype == LZ_F32) return p;
   const int64_t G = H / KV, packed = std::max<int64_t>(1, std::min(max_new, rows)) * G, cus = lz_num_cus();
   const int64_t len = std::max<int64_t>(1, max_len), blocks = blocks_of(32, packed, rows, B, KV, G);
-  const bool shared = len > 512 && (4 * blocks < cus || (len > 2048 && (blocks < cus || B >= 8)));
-  const bool many = packed > 32 && 8 * blocks_of(64, packed, rows, B, KV, G) >= cus;
-  p.bm = shared && len >= 4096 && (many || (cache_dtype == LZ_E4M3 && hd == 128)) ? 64 : 32;
+  const bool most = cache_dtype != LZ_E4M3 && hd == 128 && len <= 4096 && 4 * blocks >= 3 * cus;
+  const bool shared = len > 512 && (4 * blocks < cus || (len > 2048 && (B >= 8 || (blocks < cus && !most))) ||
+                                    (len > 4096 && 4 * blocks <= 5 * cus));
+  const bool many = 8 * blocks_of(64, packed, rows, B, KV, G) >= cus;
+  const bool converted = cache_dtype == LZ_E4M3 && hd == 128;
+  p.bm = shared && (len >= 4096 ? (packed > 32 && many) || converted : len > 2048 && many && converted) ? 64 : 32;
   p.groups = 1;
   p.nqb = (int)lz_cdiv(packed, p.bm);
   p.nsplit = 1;
@@ -713,7 +722,7 @@ LZ_EXPORT int64_t lz_tree_attn_plan(int dtype, int cache_dtype, int64_t rows, in
                                     int64_t max_new, int64_t max_len) {
   if (!plannable(rows, B, H, KV, max_len)) return 0;
   const Plan p = make_tree_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
-  return p.bm | (p.bm == kPagedTileRows ? p.groups : 1) << 8 | (int64_t)p.nsplit << 16;
+  return p.bm | (int64_t)(p.shares ? 1 : 0) << 8 | (int64_t)p.nsplit << 16;
 }
 
 LZ_EXPORT int64_t lz_tree_attn_workspace(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV,

@@ -19,9 +19,9 @@
 // RG = 2: the waves share stages of 64 keys, the next of which is on its way while
 //   this one is computed; two waves for each 32 rows, a half of the keys each.
 //   It reads K and V half as often where there are more rows, and its parts
-//   come together at a barrier a stage (64 packed rows of 8 sequences over up to
-//   16384, 32/8 heads of 128, e4m3: 64 us, with RG 1 80; 60 rows of 1 sequence over
-//   8192 19 and 26).
+//   come together at a barrier a stage (16 nodes of 8 sequences over up to 16384,
+//   32/8 heads of 128, e4m3: 63 us, with RG 1 84; 16 nodes of one over 8192, 16
+//   bits: 23 and 19).
 //   A third form, of 128 rows, won 5 to 15 % over texts of 32768 and lost up to
 //   half elsewhere; 64 rows in one wave's registers lost everywhere.
 #include <type_traits>

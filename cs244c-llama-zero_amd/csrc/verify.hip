@@ -17,8 +17,10 @@
 // 2^((x - m) log2(e) / T): its exponent in 32nds is rounded by adding 1.5 * 2^52,
 // 2^(k/32) comes from a table (32 doubles fill LDS's 64 banks once, so any lanes
 // read it without a conflict) and 2^(f/32), |f| <= 1/2, from the Taylor series to
-// the fourth power (1.3e-12; 1.9 T weights a second where the series of 2^f to the
-// tenth power makes 1.4).
+// the fourth power (1.3e-12; in a loop by itself 1.9 T weights a second, where the
+// series of 2^f to the tenth power makes 1.4).  That arithmetic bounds stats_kernel
+// (16 x 32 rows of 128256 in bf16: 33 us for 131 MB of logits; 8.3 to choose, 4.7 to
+// walk).
 //
 // Every logit is read once: stats_kernel leaves each piece's largest logit and
 // its sum of weights, a wave for each piece and no meeting of waves.  What remains
@@ -386,8 +388,8 @@ __global__ void __launch_bounds__(256) pick_kernel(VerifyArgs a) {
   if (lane == 0) a.choice[row] = t;
 }
 
-// Without draft probabilities: one workgroup a sequence, which chooses for up to
-// 16 rows of short vocabularies itself.
+// Without draft probabilities: one workgroup a sequence, which chooses for a few
+// rows itself.
 template <typename T, int NV>
 __global__ void __launch_bounds__(1024) walk_kernel(VerifyArgs a) {
   __shared__ int2 roots[32];
@@ -569,11 +571,13 @@ LZ_EXPORT int lz_verify_draft(const void* logits, int64_t ld, int dtype, int64_t
   LZ_REQUIRE(stats <= INT32_MAX / 256 && rests <= INT32_MAX / 256, "lz_verify_draft: too many rows");
   Piece* at = static_cast<Piece*>(workspace);
   double* rest = reinterpret_cast<double*>(at + rows * pieces);
-  // 4 x 5 rows of 32000, sampled: 11 us with the choices in the walk, 13 apart;
-  // 16 x 32 of 128256: 55 and 43
-  const bool apart = !probs && rows > 0 && (nodes > 16 || nv > 1);
+  // 4 x 5 rows of 32000, sampled: 9.0 us with the choices in the walk, 11.9 apart;
+  // 64 x 14 22.7 and 24.8, 16 x 32 21.9 and 20.2, 1 x 60 19.0 and 12.0; 64 x 8 of
+  // 128256 38 and 41, 16 x 16 33.5 and 32.4, 16 x 32 52 and 42
+  const bool apart = !probs && rows > 0 && nodes > 16;
   VerifyArgs a{logits, ld, tokens, uniform, row_start, temperature, parents, probs, ldp, ldq, at, rest,
-               reinterpret_cast<int32_t*>(rest + B * pieces), apart ? reinterpret_cast<int32_t*>(rest) : nullptr, counts, kept, chosen, temperature_s, u_double,
+               reinterpret_cast<int32_t*>(rest + B * pieces), apart ? reinterpret_cast<int32_t*>(rest) : nullptr, counts, kept,
+               chosen, temperature_s, u_double,
                (int)rows, (int)B, (int)V, (int)nodes, (int)pieces, kVec * nv, (int)tree_nodes};
   hipStream_t s = lz_stream(stream);
 #define RUN_PIECES(T, NV)                                                   \

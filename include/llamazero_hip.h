@@ -460,8 +460,9 @@ int lz_kv_write_at(const void* qkv, int64_t ld, int dtype, int64_t rows, const v
 /* Attention of such rows: row r sees the first base[b] places of its sequence
  * and, of those after them up to the last of kv_len[b], place base[b] + j where
  * bit j of its `words` mask words is set (mask: [rows][words], lowest bit
- * first; bits past them are clear).  The rest as lz_paged_attn, its workspace
- * and plan too. */
+ * first; bits past them are clear).  The rest as lz_paged_attn.  The plan: packed
+ * rows of a block, + 256 where the blocks' keys are dealt out in equal shares, +
+ * 65536 times the parts that a row may have. */
 int64_t lz_tree_attn_workspace(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd,
                                int64_t max_new, int64_t max_len);
 int64_t lz_tree_attn_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd,
@@ -482,11 +483,12 @@ int lz_tree_attn(const void* q, int64_t ldq, int dtype, int64_t rows, const void
  * sequence's first is on top, and are taken from the top in that order.
  * table, lengths, free and n_free are updated (table entries without a page
  * become -1); row_start (B + 1), kv_len and base (first[b]; NULL: the kept
- * length) are written, and for each of the `rows` rows its position, its slot
- * (page * page_size + place in it) and its mask, -1, -1 and 0 for rows of no
- * sequence.  parents ([nodes] with ldp 0, or B rows of ldp = nodes): node
- * i's, -1 or any value that is not below i for none; node i of a sequence is its place
- * base[b] + i.  Without parents (and mask) a row's position is its place. */
+ * length) are written, and for each of the `rows` (up to 2^28) rows its
+ * position, its slot (page * page_size + place in it) and its mask, -1, -1 and 0
+ * for rows of no sequence.  parents ([nodes] with ldp 0, or B rows of ldp =
+ * nodes): node i's, -1 or any value that is not below i for none; node i of a
+ * sequence is its place base[b] + i.  Without parents (and mask) a row's position
+ * is its place. */
 int lz_cache_tables(int32_t* table, int64_t width, int32_t* lengths, int32_t* free, int64_t pages, int32_t* n_free,
                     int64_t page_size, const int32_t* add, const int32_t* keep, const int32_t* first,
                     const int32_t* parents, int64_t ldp, int64_t nodes, int64_t B, int64_t rows, int64_t max_new,

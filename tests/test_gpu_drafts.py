@@ -140,21 +140,21 @@ def test_tree_attention(name, dtype, e4m3, hd):
         assert bool(((got - want).abs() <= tol).all()), (name, H, KV, page, float(((got - want).abs() - tol).max()))
 
 
-PLANS = {
-    # sequences, bases, heads, bound on the lengths, packed rows of a block, wave groups, parts
-    "wave, in parts": ([(8, 5000), (3, 700)], [4990, 690], (16, 8), 0, (16, 1, 8)),
-    "wave of 32, in parts": ([(13, 3000)], [2950], (4, 2), 0, (32, 1, 6)),
-    "tiles, one group": ([(160, 400)] * 9, [240] * 9, (32, 8), MUCH, (128, 1, 1)),
-    "tiles, two groups in parts": ([(64, 3000), (20, 100)], [2930, 77], (16, 4), 0, (128, 2, 6)),
+LONG = {
+    # sequences, bases, heads, bound on the lengths
+    "two texts": ([(8, 5000), (3, 700)], [4990, 690], (16, 8), 0),
+    "one text": ([(13, 3000)], [2950], (4, 2), 0),
+    "wide trees": ([(160, 400)] * 9, [240] * 9, (32, 8), MUCH),
+    "wide trees over long texts": ([(64, 3000), (20, 100)], [2930, 77], (16, 4), 0),
 }
 
 
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("dtype,e4m3", [(BF16, False), (F16, False), (BF16, True)])
-@pytest.mark.parametrize("name", sorted(PLANS))
+@pytest.mark.parametrize("name", sorted(LONG))
 def test_tree_attention_over_long_texts(name, dtype, e4m3, hd):
     """Texts that go in parts: the mask lies in the last of them, or over two."""
-    seqs, bases, (H, KV), most, _ = PLANS[name]
+    seqs, bases, (H, KV), most = LONG[name]
     c, bits = _tree_case(seqs, bases, KV, hd, 64, dtype, e4m3, seed=hd, most=most)
     q = torch.randn(c.rows, H * hd, generator=c.g).to(dtype)
     got = ops.paged_attention(q.to(DEV), c.layer, c.draft, H, hd**-0.5).double().cpu()
