@@ -537,14 +537,17 @@ __global__ void __launch_bounds__(64) end_kernel(VerifyArgs a) {
   }
 }
 
-// Pieces of 512 logits, of 2048 where those of 512 are more than a wave's lanes.
-int vectors(int64_t V) { return V > 64 * kVec ? 4 : 1; }
+// Pieces of 512 logits, of 2048 where those of 512 are more than a wave's lanes
+// and more than two for every wave that the CUs hold: large calls then join fewer
+// (32 chains of up to 8 over 128256 in fp32, drawn: 38.5 us, in short ones 45),
+// small ones have more waves (4 of up to 5: 21.8 and 19.2, sampled 13.3 and 11.8).
+int vectors(int64_t V, int64_t rows) { return V > 64 * kVec && rows * lz_cdiv(V, kVec) > 16384 ? 4 : 1; }
 
 }  // namespace
 
 LZ_EXPORT int64_t lz_verify_workspace(int64_t rows, int64_t B, int64_t V, int drawn) {
   if (rows <= 0 || B <= 0 || V <= 0 || V > (1 << 28)) return 0;
-  const int64_t pieces = lz_cdiv(V, kVec * vectors(V));
+  const int64_t pieces = lz_cdiv(V, kVec * vectors(V, rows));
   return rows * pieces * (int64_t)sizeof(Piece) + (drawn ? B * pieces * 8 + B * 4 : rows * 4);
 }
 
@@ -563,7 +566,7 @@ LZ_EXPORT int lz_verify_draft(const void* logits, int64_t ld, int dtype, int64_t
   LZ_REQUIRE(row_start && counts && kept && chosen, "lz_verify_draft: bad arguments");
   LZ_REQUIRE(rows == 0 || (logits && tokens && uniform && (rows == 1 || (ld >= V && (!probs || ldq >= V)))),
              "lz_verify_draft: bad rows");
-  const int nv = vectors(V);
+  const int nv = vectors(V, rows);
   const int64_t pieces = lz_cdiv(V, kVec * nv), need = lz_verify_workspace(rows, B, V, probs != nullptr);
   LZ_REQUIRE(need == 0 || (workspace && lz_aligned16(workspace) && ws_bytes >= need),
              "lz_verify_draft: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);

@@ -700,7 +700,7 @@ def test_drawn_tokens(dtype, new, V):
 
 
 def test_large_vocabularies():
-    """Enough rows for pieces of 2048, wide rows, uneven ends."""
+    """More pieces than lanes, uneven ends."""
     for V, new in ((128256, [8] * 5), (40001, [3] * 40), (151937, [30])):
         logits, tokens, parents, u = _drafted(V, new, V, BF16, scale=5.0, trees=True)
         _check_verify(logits, tokens, new, u, 1.0, parents)
@@ -709,6 +709,21 @@ def test_large_vocabularies():
     tokens = torch.multinomial(probs, 1).squeeze(1).tolist()
     counts = _check_verify(logits, tokens, [4] * 12, u, 1.0, None, probs)[0]
     assert sum(counts) == 48  # q = p: everything is kept
+
+
+@pytest.mark.parametrize("V,new,dtype", [(128256, [14] * 5, BF16), (33001, [20] * 14, F32), (33001, [60, 9, 200], F16)])
+@pytest.mark.parametrize("drawn", [False, True])
+def test_many_rows_of_large_vocabularies(V, new, dtype, drawn):
+    """Enough rows for pieces of 2048."""
+    logits, tokens, parents, u = _drafted(V, new, V, dtype, scale=5.0, trees=not drawn)
+    probs = None
+    if drawn:
+        g = torch.Generator().manual_seed(V)
+        noisy = logits.float() + torch.randn(logits.shape, generator=g)
+        probs = torch.softmax(noisy, -1).roll(1, 0).contiguous()
+        tokens = torch.multinomial(probs, 1, generator=g)[:, 0].tolist()
+    for heat in (1.0, [0.0 if b % 2 else 0.7 for b in range(len(new))]):
+        _check_verify(logits, tokens, new, u, heat, parents, probs)
 
 
 def test_strided_rows():
