@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(256, 2) paged_wave_kernel(PagedArgs a) {
 // one (row, head), each with every per-th part, all loads of a thread
 // independent; the groups meet in LDS in a fixed order.
 template <typename T, int HD, typename Rows>
-__global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm, int per) {
+__global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm, int per, int likely) {
   constexpr int kLanes = HD / 4;
   __shared__ float4 ys[256];
   __shared__ float ms[256], ls[256];
@@ -504,14 +504,17 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm, in
   const float* part = a.part + (int64_t)rh * a.nsplit * HD + d;
   const float* s2 = a.part + (int64_t)a.rows * a.H * a.nsplit * HD + (int64_t)rh * a.nsplit * 2;
   // A thread's first parts are fetched beside what says how many there are
-  // (parts that were not written hold anything and are not used).
+  // (parts that were not written hold anything and are not used); of trees, whose
+  // shares may leave few of nsplit parts, the `likely` ones, with two groups for
+  // up to 12 and four for more (4 x 64 nodes over 32768, 32/8 heads of 128: 7.6 us,
+  // with eight groups 12.5, with all of 33 parts 18.6).
   constexpr int kAhead = 4;
   float4 z[kAhead];
   float2 zs[kAhead];
 #pragma unroll
   for (int k = 0; k < kAhead; ++k) {
     const int i = grp + k * per;
-    if (row < a.rows && i < a.nsplit) {
+    if (row < a.rows && i < (std::is_same<Rows, TreeRows>::value ? likely : a.nsplit)) {
       z[k] = *reinterpret_cast<const float4*>(part + (int64_t)i * HD);
       zs[k] = *reinterpret_cast<const float2*>(s2 + 2 * i);
     }
@@ -541,6 +544,15 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int bm, in
     }
   }
   if (n_parts == 1) n_parts = 0;  // was written whole
+  if constexpr (std::is_same<Rows, TreeRows>::value)
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = grp + k * per;
+      if (i >= likely && i < n_parts) {
+        z[k] = *reinterpret_cast<const float4*>(part + (int64_t)i * HD);
+        zs[k] = *reinterpret_cast<const float2*>(s2 + 2 * i);
+      }
+    }
   float top = -INFINITY, l = 0.f;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](const float4& v, const float2& t) {
@@ -591,6 +603,7 @@ struct Plan {
   int groups;  // of the tile kernel's waves
   int nqb, nsplit, chunk;
   int shares = 0, least = 0;  // tree_kernel
+  int likely = 0;             // parts of most of its rows
 };
 
 // Blocks of bm packed rows that have rows: not every sequence has max_new of them.
@@ -673,6 +686,7 @@ Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, i
 Plan make_tree_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd, int64_t max_new,
                     int64_t max_len) {
   Plan p = make_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
+  p.likely = p.nsplit;
   if (dtype == LZ_F32) return p;
   const int64_t G = H / KV, packed = std::max<int64_t>(1, std::min(max_new, rows)) * G, cus = lz_num_cus();
   const int64_t len = std::max<int64_t>(1, max_len), blocks = blocks_of(32, packed, rows, B, KV, G);
@@ -689,6 +703,7 @@ Plan make_tree_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t
     p.least = 512;
     p.shares = (int)std::max<int64_t>(1, 2 * cus / KV);
     p.nsplit = (int)std::min<int64_t>(lz_cdiv(len, p.least) + 1, 33);
+    p.likely = (int)std::min<int64_t>(KV * p.shares / blocks_of(p.bm, packed, rows, B, KV, G) + 2, p.nsplit);
   }
   return p;
 }
@@ -746,8 +761,8 @@ static void run_waves(const PagedArgs& a, const Plan& p, int dtype, int cache_dt
 #undef RUN
 }
 template <typename Rows>
-static void run_join(const PagedArgs& a, int dtype, int64_t hd, uint32_t blocks, int per, hipStream_t s) {
-#define RUN(T, HD, E8) paged_join_kernel<T, HD, Rows><<<blocks, 256, 0, s>>>(a, a.bm, per)
+static void run_join(const PagedArgs& a, int dtype, int64_t hd, uint32_t blocks, int per, int likely, hipStream_t s) {
+#define RUN(T, HD, E8) paged_join_kernel<T, HD, Rows><<<blocks, 256, 0, s>>>(a, a.bm, per, likely)
   LZ_CACHE_CASES(dtype, 0, hd, RUN);
 #undef RUN
 }
@@ -777,8 +792,9 @@ static int attend(const char* what, const void* q, int64_t ldq, int dtype, int64
   const int64_t need = part_bytes(p, rows, B, H, hd);
   LZ_REQUIRE(need == 0 || (workspace && lz_aligned16(workspace) && ws_bytes >= need),
              "%s: workspace of %lld bytes, %lld needed", what, (long long)ws_bytes, (long long)need);
-  const int64_t blocks = p.shares ? KV * p.shares : B * KV * p.nqb * p.nsplit, per = p.nsplit <= 4 ? 1 : p.nsplit <= 16 ? 4 : 8,
-                joins = lz_cdiv(rows * H * (hd / 4) * per, 256);
+  const int64_t blocks = p.shares ? KV * p.shares : B * KV * p.nqb * p.nsplit;
+  const int64_t per = p.shares ? (p.likely <= 4 ? 1 : p.likely <= 12 ? 2 : 4) : p.nsplit <= 4 ? 1 : p.nsplit <= 16 ? 4 : 8;
+  const int64_t joins = lz_cdiv(rows * H * (hd / 4) * per, 256);
   LZ_REQUIRE(p.shares == 0 || B * p.nqb < INT32_MAX / (lz_cdiv(width * page_size, 128) + 1), "%s: too many rows and pages", what);
   LZ_REQUIRE(blocks <= INT32_MAX / 256 && joins <= INT32_MAX / 256, "%s: too many rows", what);
   PagedArgs a{q, ldq, k, v, (const int8_t*)k_exp, (const int8_t*)v_exp,
@@ -798,8 +814,8 @@ static int attend(const char* what, const void* q, int64_t ldq, int dtype, int64
     run_waves<PagedRows>(a, p, dtype, cache_dtype, hd, (uint32_t)blocks, s);
   }
   if (p.nsplit > 1) {
-    if (mask) run_join<TreeRows>(a, dtype, hd, (uint32_t)joins, (int)per, s);
-    else run_join<PagedRows>(a, dtype, hd, (uint32_t)joins, (int)per, s);
+    if (mask) run_join<TreeRows>(a, dtype, hd, (uint32_t)joins, (int)per, p.likely, s);
+    else run_join<PagedRows>(a, dtype, hd, (uint32_t)joins, (int)per, p.likely, s);
   }
   return lz_check_launch(what);
 }
