@@ -162,3 +162,47 @@ def test_drafted_generation_is_refused():
         bad.norm.weight.fill_(math.nan)
     with pytest.raises(ValueError, match="no token"):
         bad.generate(prompt, 3, temperature=1.0, draft_model=model)
+
+
+def test_a_servers_loop_of_trees():
+    """Steps whose lengths the host never sees: texts go on as the model writes
+    them, right guesses or wrong, shared tree or one for each."""
+    N, made = 6, 24
+    model = _model(F32, max_seq_len=128)  # generate() moves its window where a text passes it
+    prompts = [_ids(n, seed=20 + n) for n in (9, 17, 4)]
+    want = [model.generate(p[None], made + 2 * N, temperature=0, use_cache=True)[0, len(p):] for p in prompts]
+    right = torch.stack(want)
+    cache = _cache(model, 3, 17 + made + 3 * N)
+    model.forward_cached(torch.cat([p[:-1] for p in prompts]), cache, cache.step([len(p) - 1 for p in prompts]), rows="none")
+    root = torch.stack([p[-1] for p in prompts])
+    start = cached = cache.tables.lengths.clone()
+    new = torch.full((3,), N, dtype=torch.int32, device=DEV)
+    one = torch.tensor([-1, 0, 0, 2, 3, 2], dtype=torch.int32, device=DEV)
+    each = torch.stack([one, torch.tensor([-1, 0, 1, 1, 2, 4], device=DEV), torch.tensor([-1, 0, 1, 2, 3, 4], device=DEV)]).int()
+    texts, steps = [[], [], []], 0
+    while min(len(t) for t in texts) < made:
+        parents = each if steps % 2 else one
+        depth = torch.zeros(3, N, dtype=torch.int64, device=DEV)
+        for i in range(1, N):
+            up = parents[:, i] if steps % 2 else parents[i].expand(3)
+            depth[:, i] = depth.gather(1, up.long()[:, None])[:, 0] + 1
+        done = (cached - start).long()[:, None]
+        ids = right.gather(1, (done + depth - 1).clamp(0, right.shape[1] - 1))  # what follows, at each depth
+        wrong = torch.rand(3, N, generator=torch.Generator().manual_seed(steps)).to(DEV) < 0.3
+        ids = torch.where(wrong, (ids + 1) % 500, ids)
+        ids[:, 0] = root
+        step = cache.step(new, rows=3 * N, max_new=N, keep=cached, parents=parents)
+        logits = model.forward_cached(ids.view(-1), cache, step, rows="all")
+        u = torch.rand(3 * N, dtype=torch.float64, device=DEV)
+        counts, kept, chosen = ops.verify_draft(logits, ids.view(-1), step.row_start, N, u, temperature=0, parents=parents)
+        cache.keep(step, kept, counts)
+        root = chosen.gather(1, counts.long()[:, None] - 1)[:, 0]
+        cached = cached + counts
+        steps += 1
+        for t, c, n in zip(texts, chosen.tolist(), counts.tolist()):
+            t += c[:n]
+        if max(len(t) for t in texts) > made + N:
+            break
+    assert steps < made
+    for b, (t, w) in enumerate(zip(texts, want)):
+        assert t == w[: len(t)].tolist(), b
