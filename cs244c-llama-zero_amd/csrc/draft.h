@@ -3,6 +3,8 @@
 #pragma once
 #include "lz_common.h"
 
+constexpr int kMostNodes = 4096;  // of a tree
+
 // The last b with start[b] <= x, of the B that there are (ascending, start[0] <=
 // x): the sequence that entry x belongs to where start are sums before each.
 __host__ __device__ __forceinline__ int lz_last_at(const int32_t* start, int B, int x) {

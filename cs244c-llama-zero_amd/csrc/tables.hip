@@ -254,9 +254,9 @@ LZ_EXPORT int lz_cache_tables(int32_t* table, int64_t width, int32_t* lengths, i
                  rows <= (1 << 28) && max_new >= 0 && max_new <= INT32_MAX && max_len >= 0 && max_len <= INT32_MAX,
              "lz_cache_tables: bad shape");
   LZ_REQUIRE((mask == nullptr) == (parents == nullptr), "lz_cache_tables: a mask and no parents, or the reverse");
-  LZ_REQUIRE(!parents || (nodes > 0 && nodes <= (1 << 20) && words >= lz_cdiv(nodes, 32) && words <= (1 << 20) &&
+  LZ_REQUIRE(!parents || (nodes > 0 && nodes <= kMostNodes && words >= lz_cdiv(nodes, 32) && words <= (1 << 20) &&
                           (ldp == 0 || ldp == nodes)),
-             "lz_cache_tables: trees of %lld nodes in %lld mask words", (long long)nodes, (long long)words);
+             "lz_cache_tables: trees of %lld nodes (1 to %d) in %lld mask words", (long long)nodes, kMostNodes, (long long)words);
   LZ_REQUIRE(table && lengths && free && n_free && add && row_start && kv_len && base && (rows == 0 || (positions && slots)),
              "lz_cache_tables: bad arguments");
   TablesArgs a{table, lengths, free, n_free, add, keep, first, (int)width, (int)pages, lz_log2(page_size), (int)B,

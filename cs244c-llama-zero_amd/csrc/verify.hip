@@ -27,8 +27,10 @@
 // works on pieces: a wave joins a row's sums, finds the piece that the choice falls
 // into and goes over that one alone.  All rows of a tree choose at the same time,
 // a wave each, and one wave walks through the choices in LDS.
+#include <cfloat>
 #include <type_traits>
 
+#include "draft.h"
 #include "kvcache.h"
 
 namespace {
@@ -118,7 +120,7 @@ struct Exp {
 // 32 log2(e) / T, or 0 where the arg-max is chosen.
 __device__ __forceinline__ double per_heat(const VerifyArgs& a, int b) {
   const float t = a.heat ? a.heat[b] : a.heat_s;
-  return t > 0.f ? 46.16624130844683 / (double)t : 0.0;
+  return t > 0.f ? 46.16624130844683 / (double)fminf(t, FLT_MAX) : 0.0;  // (an infinite T, too, takes from all alike)
 }
 
 __device__ __forceinline__ double uniform_of(const VerifyArgs& a, int row) {
@@ -372,8 +374,6 @@ __device__ __forceinline__ int pick_row(const VerifyArgs& a, const Exp& exp, con
                     for (int e = 0; e < 8; ++e) w[e] = weight(exp, x[e], r.top, r.c);
                   });
 }
-
-constexpr int kMostNodes = 4096;
 
 // Every row's choice, a wave each.
 template <typename T, int NV>

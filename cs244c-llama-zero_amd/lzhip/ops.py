@@ -1289,7 +1289,7 @@ def cache_tables(tables, new: torch.Tensor, rows: int, max_new: int, max_len: in
     Sequences are served in order: one whose tokens pass these bounds or the
     table gets none, nor one that needs pages, or rows, where what it and those
     before it ask for is more than there is (row_start says who got them).
-    parents: int32 [nodes] or [B, nodes], the new tokens as trees: node i is
+    parents: int32 [nodes] or [B, nodes] (up to 4096), the new tokens as trees: node i is
     the token in place base[b] + i (base: int32 [B]; None: the kept length), its
     parent a node before it or -1.  Then rows see their ancestors alone and are
     rotated to base + their depth.  Up to 4096 sequences."""

@@ -486,7 +486,7 @@ int lz_tree_attn(const void* q, int64_t ldq, int dtype, int64_t rows, const void
  * length) are written, and for each of the `rows` (up to 2^28) rows its
  * position, its slot (page * page_size + place in it) and its mask, -1, -1 and 0
  * for rows of no sequence.  parents ([nodes] with ldp 0, or B rows of ldp =
- * nodes): node i's, -1 or any value that is not below i for none; node i of a
+ * nodes; up to 4096): node i's, -1 or any value that is not below i for none; node i of a
  * sequence is its place base[b] + i.  Without parents (and mask) a row's position
  * is its place. */
 int lz_cache_tables(int32_t* table, int64_t width, int32_t* lengths, int32_t* free, int64_t pages, int32_t* n_free,

@@ -579,7 +579,7 @@ def test_tables_are_refused():
     for bad in (lambda: call(t._replace(page_size=24)), lambda: call(t, new.long()), lambda: call(t, _i32([1])),
                 lambda: call(t, rows=-1), lambda: call(t, max_new=-1), lambda: call(t, keep=_i32([1])),
                 lambda: call(t, parents=_i32([[-1]])), lambda: call(t, max_new=3, parents=_i32([-1, 0])),
-                lambda: call(t, parents=_i32([])), lambda: call(t, new.cpu()), lambda: call(t._replace(n_free=_i32([1, 2]))),
+                lambda: call(t, parents=_i32([])), lambda: call(t, parents=torch.full((4097,), -1, dtype=torch.int32, device=DEV)), lambda: call(t, new.cpu()), lambda: call(t._replace(n_free=_i32([1, 2]))),
                 lambda: call(t._replace(page_table=t.page_table.t())), lambda: call(t._replace(free=t.free[:0]))):
         with pytest.raises((ValueError, RuntimeError)):
             bad()
@@ -752,6 +752,18 @@ def test_borders_and_ties():
     assert got[2][:, 0].tolist() == want and got[0].tolist() == [1] * 9
     got = ops.verify_draft(x.to(DEV), torch.zeros(9, dtype=torch.int64, device=DEV), _i32(list(range(10))), 1, u.to(DEV), temperature=0)
     assert got[2][:, 0].tolist() == [1] * 9
+
+
+def test_an_infinite_temperature_takes_from_all():
+    x = 3 * torch.randn(40, 4, generator=torch.Generator().manual_seed(6))
+    x[:, 2] = -math.inf
+    u = (torch.arange(40, dtype=torch.float64) + 0.5) / 40
+    got = ops.verify_draft(x.to(DEV), torch.zeros(40, dtype=torch.int64, device=DEV), _i32(list(range(41))), 1, u.to(DEV),
+                           temperature=torch.full((40,), math.inf, device=DEV))[2][:, 0].tolist()
+    assert got == [(0, 1, 3)[int(3 * v)] for v in u.tolist()]
+    with pytest.raises(ValueError, match="finite"):
+        ops.verify_draft(x.to(DEV), torch.zeros(40, dtype=torch.int64, device=DEV), _i32(list(range(41))), 1, u.to(DEV),
+                         temperature=math.inf)
 
 
 def test_each_token_has_its_share():
