@@ -30,6 +30,7 @@ struct LzPagedArgs {
   int words;
   int bm, shares, least;  // tree_kernel: rows of a block; workgroups a kv head (0: one a block), keys of one at least
   int32_t* parts;         // [B][nqb]: of the blocks
+  int waves;              // tree_kernel, blocks of 32 rows: 4 or 8
 };
 
 // paged_tile.hip: 16-bit rows in blocks of kPagedTileRows; `groups`

@@ -604,6 +604,7 @@ struct Plan {
   int nqb, nsplit, chunk;
   int shares = 0, least = 0;  // tree_kernel
   int likely = 0;             // parts of most of its rows
+  int waves = 4;              // tree_kernel, blocks of 32 rows
 };
 
 // Blocks of bm packed rows that have rows: not every sequence has max_new of them.
@@ -667,17 +668,21 @@ Plan make_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, i
 }
 
 // Row blocks and shares of trees.  fp32: paged_wave_kernel, as above.  Else
-// tree_kernel: a block's keys whole where texts are short or blocks many, since
-// the shares' arithmetic and the join cost 8 us (32 x 16 nodes over up to 2048,
-// 16/8 heads of 128: 37 us, shared out 45; 16 x 24 over 1024, 12/4 heads of 64: 13
-// and 20); elsewhere two workgroups a CU of equal shares (8 x 15 over 4096, 32/8
-// heads: 32 us, whole 50; 1 x 16 over 8192: 19 and 79), of 512 keys at least (that
-// one in shares of 256: 22).  Blocks for three quarters of the CUs, 16 bits, up to
-// 4096 keys: whole (3 x 100 over 4096, 32/8 heads: 43 us, shared out 51; 6 x 80,
-// 16/8 heads: 44 and 43; in e4m3 60 and 56); for up to a quarter more than there
-// are, whose second turn is nearly empty, longer texts in shares (2 x 160 over
-// 8192, 32/8 heads: 74 us, whole 79, in e4m3 83 and 108; 4 x 140 over 6000: 63 and
-// 61, 70 and 82; heads of 64: 42 and 46).
+// tree_kernel.  Up to a block a CU: a block's keys whole, by eight waves, up to a
+// length that grows with the blocks, since shares cost their arithmetic and the
+// join (16 bits, 32/8 heads of 128: 1 x 16 nodes over 2048 19 us whole, in shares
+// 16, over 3000 26 and 17; 16 x 10 over 2048 21 and 27; 3 x 100 over 4096 33 and 48; 8 x
+// 24 over 6000 55 and 43; 12/4 heads of 64 in e4m3: 1 x 16 over 1024 10.4 and 12.7);
+// half as long where each block converts e4m3 heads of 128 by itself (2 x 40 over
+// 2048: 28 and 23; 16 x 10 over 1024 24 and 36).  More blocks: shares where they are some sequences of uneven
+// lengths (32 x 8 over up to 4096, e4m3: 60 us, whole 70) or a second turn would be
+// nearly empty (2 x 160 over 8192: 74 us, whole 79, in e4m3 83 and 108; 4 x 140 over
+// 6000: 63 and 61, 70 and 82).  Shares: two workgroups a CU, of 512 keys at least
+// (1 x 16 over 8192 19 us, of 256: 22).
+// Eight waves also for two blocks a CU of heads of 32 and 64, whose tiles leave
+// room for a second workgroup (4 x 120 over 3000, 32/8 heads of 64: 23 us, four
+// waves 26; of 128, 64 x 8 over 1024: 39 and 37), and not for texts of a tile or two a
+// wave (1 x 8 over 128: 5.5 and 5.1).
 // Blocks of 64 rows where a share is long and there are some for every eighth CU,
 // and for e4m3 heads of 128, whose converted tiles two waves share (8 rows of 32
 // sequences over up to 4096, 32/8 heads: 60 us, in blocks of 32 rows, whose bytes
@@ -690,15 +695,15 @@ Plan make_tree_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t
   if (dtype == LZ_F32) return p;
   const int64_t G = H / KV, packed = std::max<int64_t>(1, std::min(max_new, rows)) * G, cus = lz_num_cus();
   const int64_t len = std::max<int64_t>(1, max_len), blocks = blocks_of(32, packed, rows, B, KV, G);
-  const bool most = cache_dtype != LZ_E4M3 && hd == 128 && len <= 4096 && 4 * blocks >= 3 * cus;
-  const bool shared = len > 512 && (4 * blocks < cus || (len > 2048 && (B >= 8 || (blocks < cus && !most))) ||
-                                    (len > 4096 && 4 * blocks <= 5 * cus));
-  const bool many = 8 * blocks_of(64, packed, rows, B, KV, G) >= cus;
   const bool converted = cache_dtype == LZ_E4M3 && hd == 128;
+  const int64_t whole = (1536 + 16 * blocks) / (converted ? 2 : 1);
+  const bool shared = blocks < cus ? len > whole : (len > 2048 && B >= 8) || (len > 4096 && 4 * blocks <= 5 * cus);
+  const bool many = 8 * blocks_of(64, packed, rows, B, KV, G) >= cus;
   p.bm = shared && (len >= 4096 ? (packed > 32 && many) || converted : len > 2048 && many && converted) ? 64 : 32;
   p.groups = 1;
   p.nqb = (int)lz_cdiv(packed, p.bm);
   p.nsplit = 1;
+  p.waves = !shared && len > 256 && blocks <= (hd == 128 ? 1 : 2) * cus ? 8 : 4;
   if (shared) {
     p.least = 512;
     p.shares = (int)std::max<int64_t>(1, 2 * cus / KV);
@@ -737,7 +742,7 @@ LZ_EXPORT int64_t lz_tree_attn_plan(int dtype, int cache_dtype, int64_t rows, in
                                     int64_t max_new, int64_t max_len) {
   if (!plannable(rows, B, H, KV, max_len)) return 0;
   const Plan p = make_tree_plan(dtype, cache_dtype, rows, B, H, KV, hd, max_new, max_len);
-  return p.bm | (int64_t)(p.shares ? 1 : 0) << 8 | (int64_t)p.nsplit << 16;
+  return p.bm | (int64_t)(p.shares ? 1 : 0) << 8 | (int64_t)(p.waves == 8 ? 1 : 0) << 9 | (int64_t)p.nsplit << 16;
 }
 
 LZ_EXPORT int64_t lz_tree_attn_workspace(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV,
@@ -801,7 +806,7 @@ static int attend(const char* what, const void* q, int64_t ldq, int dtype, int64
               LzPages{table, (int)width, (int)pages, lz_log2(page_size)}, row_start, kv_len, o, ldo, (float*)workspace,
               scale, (int)rows, (int)B, (int)H, (int)KV, p.nqb, p.nsplit, p.chunk,
               (int)(std::min(max_new, rows) * (H / KV)), base, mask, (int)words, p.bm, p.shares, p.least,
-              p.shares ? (int32_t*)((float*)workspace + rows * H * p.nsplit * (hd + 2)) : nullptr};
+              p.shares ? (int32_t*)((float*)workspace + rows * H * p.nsplit * (hd + 2)) : nullptr, p.waves};
   hipStream_t s = lz_stream(stream);
   const bool e8 = cache_dtype == LZ_E4M3;
   if (mask && dtype != LZ_F32) {

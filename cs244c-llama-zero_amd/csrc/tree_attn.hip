@@ -13,9 +13,12 @@
 // (direct-to-LDS loads; e4m3 through registers), V^T is read transposed.  Only the
 // tiles behind the text carry masks.
 //
-// RG = 1: each of the four waves takes every fourth tile of 32 keys, which is its
+// RG = 1: each of the W waves (4, 8) takes every W-th tile of 32 keys, which is its
 //   own: the next K is on its way as soon as this one's scores are formed, the next
-//   V after this one's sum, and no wave waits for another until the end.
+//   V after this one's sum, and no wave waits for another until the end.  What is
+//   on its way bounds it: a CU with four waves reads 43 GB/s, so that eight are
+//   faster where a CU has one block (16 x 12 nodes over up to 2048, 16/8 heads of
+//   128: 20.7 us, with four 25.5).
 // RG = 2: the waves share stages of 64 keys, the next of which is on its way while
 //   this one is computed; two waves for each 32 rows, a half of the keys each.
 //   It reads K and V half as often where there are more rows, and its parts
@@ -40,12 +43,12 @@ __device__ __forceinline__ void loads_left() {
 __device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // A block's tiles: a wave's own (RG 1) or the workgroup's.
-template <typename F, int HD, bool k8, int RG>
+template <typename F, int HD, bool k8, int RG, int W>
 struct TreeTiles {
   static constexpr bool kOwn = RG == 1;
   static constexpr int kKeys = kOwn ? 32 : 64;      // of a tile
   static constexpr int kTile = kKeys * HD * 2;      // bytes of K or V
-  static constexpr int kSmem = 4 * 2 * 32 * HD * 2; // four waves' K and V, or two stages of K and V
+  static constexpr int kSmem = W * 2 * 32 * HD * 2; // the waves' K and V, or two stages of K and V
   static constexpr int kRowsPerLoad = 1024 / (HD * 2), kChunks = HD / 8, kPer = 16 / kRowsPerLoad;
   static constexpr int kLoads = 2 * kPer;  // RG 1: of a K or V tile
   static constexpr int kIds = kKeys / 16, kBatch = 64 / kIds;  // pages of a tile, tiles whose pages are held
@@ -60,7 +63,7 @@ struct TreeTiles {
   int ex[2][k8 ? kMine : 1];
 
   __device__ __forceinline__ char* tile(int side, int t) const { return lds + (kOwn ? side : 2 * (t & 1) + side) * kTile; }
-  __device__ __forceinline__ int key_of(int t) const { return k_lo + (kOwn ? (4 * t + wave) * 32 : 64 * t); }
+  __device__ __forceinline__ int key_of(int t) const { return k_lo + (kOwn ? (W * t + wave) * 32 : 64 * t); }
   __device__ __forceinline__ int key_of_id(int t0) const { return key_of(t0 + lane / kIds) + 16 * (lane % kIds); }
   __device__ __forceinline__ int look_up(const PagedArgs& a, int b, int t0) const {
     const int key = key_of_id(t0);
@@ -228,12 +231,12 @@ struct Share {
   }
 };
 
-template <typename F, int HD, bool k8, int RG>
-__global__ void __launch_bounds__(256, 2) tree_kernel(PagedArgs a) {
-  typedef TreeTiles<F, HD, k8, RG> T;
-  constexpr int BM = 32 * RG, KG = 4 / RG;
+template <typename F, int HD, bool k8, int RG, int W>
+__global__ void __launch_bounds__(64 * W, 2) tree_kernel(PagedArgs a) {
+  typedef TreeTiles<F, HD, k8, RG, W> T;
+  constexpr int BM = 32 * RG, KG = W / RG;
   __shared__ __attribute__((aligned(1024))) char smem[T::kSmem];
-  __shared__ float ml[4][32][2];
+  __shared__ float ml[W][32][2];
   T tl;
   const int tid = threadIdx.x;
   tl.lane = tid & 63;
@@ -264,10 +267,10 @@ __global__ void __launch_bounds__(256, 2) tree_kernel(PagedArgs a) {
     for (int kk = 0; kk < HD / 16; ++kk) qf[kk] = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(qp + kk * 16));
     f32x16_t o[HD / 32];
     float mx, l;
-    const int span = tl.k_hi - tl.key_of(0), n_tiles = span > 0 ? (T::kOwn ? (span + 127) / 128 : (span + 63) / 64) : 0;
+    const int span = tl.k_hi - tl.key_of(0), n_tiles = span > 0 ? (T::kOwn ? (span + 32 * W - 1) / (32 * W) : (span + 63) / 64) : 0;
     // tiles that every row sees whole
     const int free_span = min(rw.ctx, tl.k_hi) - tl.key_of(0);
-    const int free_tiles = free_span >= T::kKeys ? (T::kOwn ? (free_span - 32) / 128 + 1 : free_span / 64) : 0;
+    const int free_tiles = free_span >= T::kKeys ? (T::kOwn ? (free_span - 32) / (32 * W) + 1 : free_span / 64) : 0;
     uint64_t there = 0;
     bool odd = false;
 
@@ -478,7 +481,7 @@ __global__ void __launch_bounds__(256, 2) tree_kernel(PagedArgs a) {
       ml[tl.wave][l32][1] = l;
     }
     __syncthreads();
-    for (int e = tid; e < BM * (HD / 4); e += 256) {
+    for (int e = tid; e < BM * (HD / 4); e += 64 * W) {
       const int x = e / (HD / 4) % 32, y_rg = e / (HD / 4) / 32, d4 = e % (HD / 4), mm = rw.m0 + 32 * y_rg + x;
       if (mm >= rw.count) break;
       float top = -INFINITY;
@@ -526,8 +529,9 @@ __global__ void __launch_bounds__(256, 2) tree_kernel(PagedArgs a) {
 
 template <typename F, int HD, bool k8>
 void run(const LzPagedArgs& a, uint32_t blocks, hipStream_t s) {
-  if (a.bm == 32) tree_kernel<F, HD, k8, 1><<<blocks, 256, 0, s>>>(a);
-  else tree_kernel<F, HD, k8, 2><<<blocks, 256, 0, s>>>(a);
+  if (a.bm != 32) tree_kernel<F, HD, k8, 2, 4><<<blocks, 256, 0, s>>>(a);
+  else if (a.waves == 8) tree_kernel<F, HD, k8, 1, 8><<<blocks, 512, 0, s>>>(a);
+  else tree_kernel<F, HD, k8, 1, 4><<<blocks, 256, 0, s>>>(a);
 }
 
 }  // namespace

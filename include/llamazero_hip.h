@@ -462,7 +462,8 @@ int lz_kv_write_at(const void* qkv, int64_t ld, int dtype, int64_t rows, const v
  * bit j of its `words` mask words is set (mask: [rows][words], lowest bit
  * first; bits past them are clear).  The rest as lz_paged_attn.  The plan: packed
  * rows of a block, + 256 where the blocks' keys are dealt out in equal shares, +
- * 65536 times the parts that a row may have. */
+ * 512 where eight waves share a block, + 65536 times the parts that a row may
+ * have. */
 int64_t lz_tree_attn_workspace(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd,
                                int64_t max_new, int64_t max_len);
 int64_t lz_tree_attn_plan(int dtype, int cache_dtype, int64_t rows, int64_t B, int64_t H, int64_t KV, int64_t hd,

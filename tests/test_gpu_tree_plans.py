@@ -25,10 +25,13 @@ def _ragged(n, new, length):
 
 
 PLANS = {
-    # types, head dims, heads, sequences, (rows of a block, shared out, parts)
-    "whole texts": (B16 + B8, [32, 64, 128], (16, 8), _ragged(33, 16, 1000), (32, 0, 1)),
-    "short": (B16 + B8, [64], (8, 2), [(40, 500), (3, 10)], (32, 0, 1)),
-    "for most of the CUs": (B16, [128], (32, 8), [(100, 2200), (70, 1200), (40, 900)], (32, 0, 1)),
+    # types, head dims, heads, sequences, (rows of a block, 1: shared out, 2: eight waves, parts)
+    "whole texts": (B16 + B8, [128], (16, 8), _ragged(33, 16, 1000), (32, 0, 1)),
+    "whole texts, small heads": (B16 + B8, [32, 64], (16, 8), _ragged(33, 16, 1000), (32, 2, 1)),
+    "very many": (B16 + B8, [32, 64], (16, 8), _ragged(80, 9, 300), (32, 0, 1)),
+    "shortest": (B16 + B8, [32, 64, 128], (8, 2), [(40, 200), (3, 10)], (32, 0, 1)),
+    "short": (B16 + B8, [32, 64, 128], (8, 2), [(40, 500), (3, 10)], (32, 2, 1)),
+    "for most of the CUs": (B16, [128], (32, 8), [(100, 2200), (70, 1200), (40, 900)], (32, 2, 1)),
     "one long text": (B16, [32, 64, 128], (32, 8), [(16, 8192)], (32, 1, 17)),
     "parts end at 33": (B16, [64], (8, 1), [(4, 20000), (1, 5), (3, 17000)], (32, 1, 33)),
     "wide trees": (B16 + B8, [32, 64, 128], (16, 4), _ragged(8, 30, 4500), (64, 1, 10)),
