@@ -1004,3 +1004,39 @@ def test_a_captured_step_on_its_own_stream():
             assert torch.equal(x, y)
         assert torch.equal(ca.k, cb.k) and torch.equal(ca.v, cb.v) and torch.equal(ka, kb)
         assert torch.equal(ta.page_table, tb.page_table) and torch.equal(ta.free[: int(ta.n_free)], tb.free[: int(tb.n_free)])
+
+
+def test_two_graphs_on_two_streams():
+    """Calls with workspaces, captured twice and replayed at the same time."""
+    H, KV, hd, V = 16, 4, 64, 40001
+    cases, graphs, outs, wants = [], [], [], []
+    for seed in range(2):
+        c, _ = _tree_case([(16, 4500), (9, 3000), (0, 70)], [4484, 2990, 70], KV, hd, 64, BF16, seed=seed)
+        q = torch.randn(c.rows, H * hd, generator=c.g).to(BF16).to(DEV)
+        logits = 3 * torch.randn(c.rows, V, generator=c.g).to(DEV)
+        probs = torch.softmax(logits.roll(1, 0) + torch.randn(c.rows, V, generator=c.g).to(DEV), -1)
+        tokens, u = torch.multinomial(probs, 1)[:, 0], torch.rand(c.rows, generator=c.g).to(DEV)
+        cases.append((c, q, logits, probs, tokens, u))
+
+    def run(c, q, logits, probs, tokens, u):
+        return [ops.paged_attention(q, c.layer, c.draft, H, hd**-0.5),
+                *ops.verify_draft(logits, tokens, c.draft.row_start, 16, u, draft_probs=probs),
+                *ops.verify_draft(logits, tokens, c.draft.row_start, 16, u)]
+
+    for case in cases:
+        wants.append(run(*case))
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(run(*case))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for s, g, out in zip(streams, graphs, outs):
+            with torch.cuda.stream(s):
+                for o in out:
+                    o.zero_()
+                g.replay()
+        again = run(*cases[0])  # beside them
+        torch.cuda.synchronize()
+        for out, want in zip([*outs, again], [*wants, wants[0]]):
+            assert all(torch.equal(x, y) for x, y in zip(out, want))
