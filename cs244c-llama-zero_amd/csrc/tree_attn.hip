@@ -492,8 +492,9 @@ __global__ void __launch_bounds__(64 * W, 2) tree_kernel(PagedArgs a) {
 #pragma unroll
       for (int i = 0; i < KG; ++i) {
         const int from = y_rg + RG * i;
-        if (ml[from][x][0] == -INFINITY) continue;  // a wave that saw nothing
-        const float f = KG == 1 ? 1.f : __builtin_amdgcn_exp2f(ml[from][x][0] - top);
+        // a wave that saw nothing holds zeros; one whose scores are NaN has no
+        // maximum either, and its sums are NaN
+        const float f = ml[from][x][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[from][x][0] - top);
         const float4 z = reinterpret_cast<const float4*>(smem + from * 64 * HD * 2)[d4 * 32 + (x ^ (d4 & 31))];
         sum = fmaf(f, ml[from][x][1], sum);
         y.x = fmaf(f, z.x, y.x);

@@ -237,6 +237,64 @@ def test_an_infinity_reaches_those_that_see_it(dtype, most, odd):
     assert bool((got[hit].isnan() if math.isnan(odd) else got[hit] == odd).all())
 
 
+NANS = {
+    # sequence of (new, all) tokens, base, heads, bound on the length, (rows of a block, 1: shared out, 2: eight
+    # waves), keys that are NaN
+    "alone in a wave's tile": ((1, 33), 32, (4, 2), 0, (32, 0), lambda k: k == 32),
+    "every tile of a wave": ((9, 250), 241, (4, 2), 0, (32, 0), lambda k: k // 32 % 4 == 2),
+    "every tile of one wave in eight": ((9, 500), 480, (4, 2), 0, (32, 2), lambda k: k // 32 % 8 == 1),
+    "one node": ((9, 500), 480, (4, 2), 0, (32, 2), lambda k: k == 485),
+    "a whole share": ((16, 8192), 8100, (32, 8), 0, (32, 1), lambda k: k // 512 == 3),
+    "half of the tiles of shared stages": ((160, 6000), 5840, (32, 8), 0, (64, 1), lambda k: k // 32 % 2 == 1),
+}
+
+
+@pytest.mark.parametrize("dtype,e4m3,odd", [(BF16, False, math.nan), (F16, False, math.nan), (F16, False, math.inf),
+                                            (F32, False, math.nan), (BF16, True, math.nan)])
+@pytest.mark.parametrize("name", sorted(NANS))
+def test_a_score_of_nan_reaches_the_rows_that_see_it(name, dtype, e4m3, odd):
+    """However the keys fall to waves and shares.  (A key of infinities gives it
+    too: its products with a query of both signs do not add up.)"""
+    (n, l), base, (H, KV), most, plan, which = NANS[name]
+    hd = 64
+    c, bits = _tree_case([(n, l)], [base], KV, hd, 64, dtype, e4m3, seed=13, most=most, fill=0.0)
+    code = {F32: 0, BF16: 1, F16: 2}[dtype]
+    p = _lib.query("lz_tree_attn_plan", code, 8 if e4m3 else code, c.rows, 1, H, KV, hd, c.step.max_new, c.step.max_len)
+    assert dtype == F32 or (p & 255, p >> 8 & 255) == plan
+    q = torch.randn(c.rows, H * hd, generator=c.g).to(dtype).to(DEV)
+    clean = ops.paged_attention(q, c.layer, c.draft, H, hd**-0.5)
+    keys = torch.tensor([k for k in range(l) if which(k)])
+    k = c.layer.k.clone()
+    stored = k.view(torch.uint8) if e4m3 else k
+    stored[c.table[0, keys // 64].long().to(DEV), KV - 1, (keys % 64).to(DEV)] = 0x7F if e4m3 else odd
+    got = ops.paged_attention(q, c.layer._replace(k=k), c.draft, H, hd**-0.5).view(n, H, hd)
+    hit = torch.zeros(n, H, dtype=torch.bool)
+    hit[:, H - H // KV :] = _seen(c, [base], bits)[0][:, keys].any(1)[:, None]
+    assert bool(hit.any())
+    hit = hit.to(DEV)
+    assert bool(got[hit].isnan().all())
+    assert torch.equal(got[~hit], clean.view(n, H, hd)[~hit])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_scores_of_nan_in_a_chain_are_the_causal_calls(dtype):
+    H, KV, hd, n, l = 8, 2, 64, 20, 500
+    c = Case([(n, l)], KV, hd, 64, dtype, seed=3)
+    bits = torch.ones(n, n).tril().bool()
+    s = c.step
+    draft = DraftStep(*s, _i32([l - n]), torch.zeros(n, dtype=torch.int32, device=DEV),
+                      torch.zeros(n, dtype=torch.int64, device=DEV), _pack(bits).to(DEV))
+    q = torch.randn(n, H * hd, generator=c.g).to(dtype).to(DEV)
+    for keys in ([l - n + 7], [0], [k for k in range(l) if k // 32 % 8 == 3]):
+        k = c.layer.k.clone()
+        for key in keys:
+            k[int(c.table[0, key // 64]), :, key % 64] = math.nan
+        layer = LayerCache(k, c.layer.v)
+        got, want = ops.paged_attention(q, layer, draft, H, hd**-0.5), ops.paged_attention(q, layer, s, H, hd**-0.5)
+        assert torch.equal(got.isnan(), want.isnan())
+        assert bool(got.view(n, -1).isnan().all(1)[max(0, keys[0] - (l - n)) :].all())
+
+
 def test_rows_of_no_sequence_and_past_the_bounds_are_left():
     H, KV, hd = 4, 2, 32
     c, bits = _tree_case([(6, 20), (9, 40)], [14, 31], KV, hd, 16, BF16, seed=2)
