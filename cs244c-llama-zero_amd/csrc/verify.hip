@@ -143,9 +143,12 @@ __device__ __forceinline__ void load8(float (&x)[8], const T* row, int v, int V)
   }
 }
 
-// A token's weight beside the largest logit `top` (finite).
+// A token's weight beside the largest logit `top` (finite).  Where it is no double
+// above 0 (under 2^-1075), as a mask of the type's lowest value makes it, there is
+// none: a number of 0 would choose it.
 __device__ __forceinline__ double weight(const Exp& exp, float x, float top, double c) {
-  return x == -INFINITY ? 0.0 : exp(((double)x - (double)top) * c);
+  const double t = ((double)x - (double)top) * c;  // -inf too
+  return t < -34400.0 ? 0.0 : exp(t);
 }
 
 // Sums over the wave of the lanes up to this one, with DPP (row_shr 1, 2, 4, 8,
@@ -293,7 +296,7 @@ struct Row {
   // a piece's sum beside the row's largest logit
   __device__ __forceinline__ double of_piece(const Exp& exp, int p) const {
     const Piece s = pieces[p];
-    return s.top == -INFINITY ? 0.0 : s.sum * exp(((double)s.top - (double)top) * c);
+    return s.sum * weight(exp, s.top, top, c);
   }
   // whether a token can be chosen
   __device__ __forceinline__ bool fine() const {

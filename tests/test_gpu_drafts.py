@@ -812,6 +812,29 @@ def test_borders_and_ties():
     assert got[2][:, 0].tolist() == [1] * 9
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("V", [700, 40000])
+def test_tokens_at_the_types_lowest_value_are_not_chosen(dtype, V):
+    """A mask of finite values: their probability is zero, for numbers at either
+    end of the range too, in sampling and in what is kept of a draft."""
+    n = 200 if V == 700 else 40
+    x = (3 * torch.randn(n, V, generator=torch.Generator().manual_seed(V))).to(dtype)
+    x[:, V - 200 :] = torch.finfo(dtype).min
+    x[:, :5] = torch.finfo(dtype).min
+    x = x.to(DEV)
+    tokens = torch.zeros(n, dtype=torch.int64, device=DEV)
+    for u in (0.0, math.nextafter(1.0, 0.0), 1.0):
+        uniform = torch.full((n,), u, dtype=torch.float64, device=DEV)
+        chosen = ops.verify_draft(x, tokens, _i32(list(range(n + 1))), 1, uniform)[2]
+        assert bool(((chosen >= 5) & (chosen < V - 200)).all()), u
+        # chains of one drafted token that the mask forbids, with a number of 0, and what follows
+        probs = torch.full((n, V), 1.0 / V, device=DEV)
+        uniform[1::2] = 0.0
+        counts, _, chosen = ops.verify_draft(x, tokens, _i32(list(range(0, n + 1, 2))), 2, uniform, draft_probs=probs)
+        assert bool((counts == 1).all())
+        assert bool(((chosen[:, 0] >= 5) & (chosen[:, 0] < V - 200)).all())
+
+
 def test_an_infinite_temperature_takes_from_all():
     x = 3 * torch.randn(40, 4, generator=torch.Generator().manual_seed(6))
     x[:, 2] = -math.inf
