@@ -123,8 +123,10 @@ __device__ __forceinline__ double per_heat(const VerifyArgs& a, int b) {
   return t > 0.f ? 46.16624130844683 / (double)fminf(t, FLT_MAX) : 0.0;  // (an infinite T, too, takes from all alike)
 }
 
+// A row's number: below 0, and NaN, as 0; from 1 on as the double under it.
 __device__ __forceinline__ double uniform_of(const VerifyArgs& a, int row) {
-  return a.u_double ? static_cast<const double*>(a.uniform)[row] : (double)static_cast<const float*>(a.uniform)[row];
+  const double u = a.u_double ? static_cast<const double*>(a.uniform)[row] : (double)static_cast<const float*>(a.uniform)[row];
+  return fmin(fmax(u, 0.0), 0x1.fffffffffffffp-1);
 }
 
 // Eight logits of a row from v on; -inf past the vocabulary.
@@ -314,7 +316,7 @@ __device__ __forceinline__ int pick(const VerifyArgs& a, double u, int lane, con
   double all = of_lane(up0, 63);
   for (int p0 = 64; p0 < a.n_pieces; p0 += 64) all += sum_of_wave(piece_sum(p0));
   if (!(all > 0.0)) return -1;
-  double target = (u > 0.0 ? u : 0.0) * all, run = 0.0;
+  double target = u * all, run = 0.0;
   int piece = -1, last = 0;
   for (int p0 = 0; p0 < a.n_pieces; p0 += 64) {
     const double x = p0 ? piece_sum(p0) : x0, up_to = p0 ? sum_up_to(x) : up0;
@@ -328,7 +330,7 @@ __device__ __forceinline__ int pick(const VerifyArgs& a, double u, int lane, con
     if (some) last = p0 + 63 - __builtin_clzll(some);
     run += of_lane(up_to, 63);
   }
-  if (piece < 0) {  // u is 1 or just under it
+  if (piece < 0) {  // u is just under 1
     piece = last;
     target = INFINITY;
   }

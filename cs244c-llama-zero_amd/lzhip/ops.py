@@ -1311,8 +1311,8 @@ def verify_draft(logits: torch.Tensor, tokens: torch.Tensor, row_start: torch.Te
     one the root (the text's last token), and logits [rows, V] what follows
     each.  p is their softmax at `temperature` (a number or float32 [B]; <= 0:
     the first of the largest logits); uniform: a number in [0, 1) for each row
-    (float32 or float64).  Without draft_probs a token is chosen from p at each
-    node with the node's number, and the child that holds it is kept (parents as
+    (float32 or float64; below 0, and NaN, counts as 0, from 1 on as just under
+    it).  Without draft_probs a token is chosen from p at each node with the node's number, and the child that holds it is kept (parents as
     in cache_tables; None: a chain), which is the model's own choice at every
     place whatever was drafted.  With draft_probs (float32 [rows, V], row r the
     distribution that token r was drawn from), a chain's tokens are kept with

@@ -499,8 +499,8 @@ int lz_cache_tables(int32_t* table, int64_t width, int32_t* lengths, int32_t* fr
 /* Which drafted tokens are kept, given the logits of what follows each row
  * (p = softmax(x / temperature), temperature[b] or, where that is NULL,
  * temperature_s; <= 0: all of it on the first of the largest) and a uniform
- * number in [0, 1) for each row (float, or double with u_double; below 0 counts
- * as 0, from 1 on as just under it).  A sequence's rows are its nodes (up to
+ * number in [0, 1) for each row (float, or double with u_double; below 0, and NaN,
+ * counts as 0, from 1 on as just under it, in choices and in what is kept).  A sequence's rows are its nodes (up to
  * `nodes`, at most 4096), the first one the root.
  * probs NULL: at each node, from the root on, t = the first token whose sum of p
  *   up to it is over the node's number times the sum of all; the first child

@@ -812,6 +812,24 @@ def test_borders_and_ties():
     assert got[2][:, 0].tolist() == [1] * 9
 
 
+def test_numbers_outside_of_the_range_keep_as_those_at_its_ends():
+    """Below 0 and NaN as 0: what p does not hold is not kept, the rest is.  From
+    1 on as just under it: where p is q, everything is kept."""
+    V = 8
+    x = torch.full((2, V), -math.inf)
+    x[:, :4] = 1.0  # p = 1/4 each
+    q = torch.zeros(2, V)
+    q[:, :4] = 0.25
+    q[:, 4:] = 0.5
+    just = math.nextafter(1.0, 0.0)
+    for u, token, counts in ((-3.0, 5, 1), (-3.0, 2, 2), (-math.inf, 5, 1), (math.nan, 5, 1), (math.nan, 2, 2), (0.0, 2, 2), (0.0, 5, 1),
+                             (just, 3, 2), (1.0, 3, 2), (7.0, 3, 2), (math.inf, 3, 2), (1.0, 5, 1)):
+        for kind in (torch.float64, torch.float32):
+            got = ops.verify_draft(x.to(DEV), torch.tensor([0, token], device=DEV), _i32([0, 2]), 2,
+                                   torch.tensor([0.5, u], dtype=kind, device=DEV), draft_probs=q.to(DEV))
+            assert got[0].tolist() == [counts], (u, token, kind)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("V", [700, 40000])
 def test_tokens_at_the_types_lowest_value_are_not_chosen(dtype, V):
