@@ -641,8 +641,9 @@ class LlamaForCausalLM(nn.Module):
                 x = draft.forward_cached(ids[:, lo:hi].reshape(-1), caches[1], step, rows="none" if last else "all")
                 if last:
                     break
-                if drawn:
-                    probs.append(torch.softmax(_cut(x.float() / temperature, top_k), -1))
+                if drawn:  # logits that have no softmax draw from all alike (drawing from NaN would end the process)
+                    law = torch.softmax(_cut(x.float() / temperature, top_k), -1)
+                    probs.append(law.nan_to_num_(nan=1.0 / law.size(-1)))
                     ids[:, hi] = torch.multinomial(probs[-1], 1)[:, 0]
                 else:
                     first, end = tree.levels[level + 1]

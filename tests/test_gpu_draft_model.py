@@ -206,3 +206,16 @@ def test_a_servers_loop_of_trees():
     assert steps < made
     for b, (t, w) in enumerate(zip(texts, want)):
         assert t == w[: len(t)].tolist(), b
+
+
+@pytest.mark.parametrize("top_k", [None, 4])
+def test_a_draft_without_a_law_draws_from_all(top_k):
+    """A draft model that has gone NaN costs tokens, and changes none."""
+    model, draft = _model(F32), _model(F32, dim=128, n_layers=1, n_heads=2, n_kv_heads=1)
+    with torch.no_grad():
+        draft.norm.weight.fill_(math.nan)
+    prompt = _ids(2, 17)
+    out = model.generate(prompt, 9, temperature=1.0, top_k=top_k, draft_model=draft, draft_tokens=3)
+    assert out.shape == (2, 26) and torch.equal(out[:, :17], prompt) and bool(((out >= 0) & (out < 500)).all())
+    want = model.generate(prompt, 9, temperature=0.0)
+    assert torch.equal(model.generate(prompt, 9, temperature=1.0, top_k=1, draft_model=draft, draft_tokens=3), want)
