@@ -185,7 +185,11 @@ class DraftCache(KVCache):
     A sequence that the pages do not suffice for is left out of a step (its rows
     in row_start are none) where KVCache.step raises."""
 
+    MOST = 4096  # sequences of ops.cache_tables, and nodes of a tree there and in ops.verify_draft
+
     def __init__(self, *args, max_len: int, **kw) -> None:
+        if kw.get("batch", 0) > self.MOST:
+            raise ValueError(f"{kw['batch']} sequences in one cache of tables on the device: up to {self.MOST}")
         super().__init__(*args, **kw)
         if max_len < 1:
             raise ValueError(f"sequences of up to {max_len} tokens")

@@ -11,6 +11,8 @@ no CPU compute path.
 """
 from __future__ import annotations
 
+import itertools
+import operator
 import threading
 from dataclasses import dataclass
 from typing import Any, Callable, List, Optional, Sequence, Tuple, Union
@@ -556,8 +558,9 @@ class LlamaForCausalLM(nn.Module):
         likeliest tokens, that many children for each node of a level.  What is
         generated is distributed as without it (temperature <= 0: the same
         tokens, as far as the two ways to compute the logits agree).  Both
-        models keep caches; the whole text has to fit both's max_seq_len, and
-        penalties, logit_bias and token_mask are refused."""
+        models keep caches; the whole text has to fit both's max_seq_len, there
+        are up to 4096 sequences and drafted tokens of each (the text's last one
+        counts), and penalties, logit_bias and token_mask are refused."""
         if cache_dtype is not None and not use_cache and draft_model is None:
             raise ValueError("cache_dtype is for use_cache=True")
         self.eval()
@@ -610,6 +613,10 @@ class LlamaForCausalLM(nn.Module):
                              f"({self.cfg.max_seq_len} and {draft.cfg.max_seq_len})")
         if not chain and max(widths) > self.cfg.vocab_size:
             raise ValueError(f"{max(widths)} children of a node from {self.cfg.vocab_size} tokens")
+        nodes = 1 + sum(itertools.accumulate(widths, operator.mul))
+        if B > DraftCache.MOST or nodes > DraftCache.MOST:
+            raise ValueError(f"{B} sequences with a draft of {nodes} tokens each (the root among them): up to "
+                             f"{DraftCache.MOST} of both are taken with a draft_model")
         if total == t0:
             return seq
         draft.eval()

@@ -208,6 +208,19 @@ def test_a_servers_loop_of_trees():
         assert t == w[: len(t)].tolist(), b
 
 
+def test_more_than_a_step_takes_is_refused_before_anything_is_made():
+    """4096 sequences, and as many nodes of a tree."""
+    model = _model(F32)
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    for batch, tokens in ((4097, 2), (1, 4096), (1, (500, 8))):
+        with pytest.raises(ValueError, match="4096"):
+            model.generate(_ids(batch, 3), 2, draft_model=model, draft_tokens=tokens)
+    with pytest.raises(ValueError, match="4096"):
+        _cache(model, 4097, 16)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20  # the caches of 4097 sequences alone are 1 GB
+
+
 @pytest.mark.parametrize("top_k", [None, 4])
 def test_a_draft_without_a_law_draws_from_all(top_k):
     """A draft model that has gone NaN costs tokens, and changes none."""
