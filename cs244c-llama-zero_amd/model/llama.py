@@ -677,4 +677,4 @@ class LlamaForCausalLM(nn.Module):
             if none:
                 raise ValueError("a row's logits leave no token to choose (NaN, or infinite where it is sampled)")
             lengths = [n + 1 for n in ends]
-        return text[:, :total]
+        return text[:, :total].contiguous()

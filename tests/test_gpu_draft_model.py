@@ -208,6 +208,16 @@ def test_a_servers_loop_of_trees():
         assert t == w[: len(t)].tolist(), b
 
 
+def test_drafted_rows_are_adjacent():
+    """As generate's without a draft: they can be viewed as one row of tokens."""
+    model = _model(F32)
+    prompt = _ids(3, 17)
+    want = model.generate(prompt, 9, temperature=0.0)
+    for tokens in (3, (2, 1)):
+        out = model.generate(prompt, 9, temperature=0.0, draft_model=model, draft_tokens=tokens)
+        assert out.is_contiguous() and torch.equal(out.view(-1), want.view(-1))
+
+
 def test_more_than_a_step_takes_is_refused_before_anything_is_made():
     """4096 sequences, and as many nodes of a tree."""
     model = _model(F32)
