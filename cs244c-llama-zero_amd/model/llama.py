@@ -12,6 +12,7 @@ no CPU compute path.
 from __future__ import annotations
 
 import itertools
+import numbers
 import operator
 import threading
 from dataclasses import dataclass
@@ -601,8 +602,8 @@ class LlamaForCausalLM(nn.Module):
                           cache_dtype: Optional[torch.dtype], draft: "LlamaForCausalLM",
                           draft_tokens: Union[int, Sequence[int]]) -> torch.Tensor:
         """generate() with a draft model; seq: [B, t0 + new], its first t0 given."""
-        chain = isinstance(draft_tokens, int)
-        widths = [1] * draft_tokens if chain else [int(w) for w in draft_tokens]
+        chain = isinstance(draft_tokens, numbers.Integral)  # NumPy's too
+        widths = [1] * int(draft_tokens) if chain else [int(w) for w in draft_tokens]
         B, total = seq.shape
         if not widths or min(widths) < 1:
             raise ValueError(f"draft_tokens must be positive, got {draft_tokens}")

@@ -218,6 +218,15 @@ def test_drafted_rows_are_adjacent():
         assert out.is_contiguous() and torch.equal(out.view(-1), want.view(-1))
 
 
+def test_counts_of_drafted_tokens_of_other_integer_types():
+    np = pytest.importorskip("numpy")
+    model = _model(F32)
+    prompt = _ids(2, 17)
+    want = model.generate(prompt, 9, temperature=0.0, draft_model=model, draft_tokens=3)
+    for tokens in (np.int64(3), np.uint8(3), np.array([2, 1]), [np.int32(2), 1]):
+        assert torch.equal(model.generate(prompt, 9, temperature=0.0, draft_model=model, draft_tokens=tokens), want)
+
+
 def test_more_than_a_step_takes_is_refused_before_anything_is_made():
     """4096 sequences, and as many nodes of a tree."""
     model = _model(F32)
