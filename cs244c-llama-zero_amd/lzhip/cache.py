@@ -236,5 +236,5 @@ class DraftCache(KVCache):
         dim] each, in the model's dtype.  Waits for the device."""
         n, kv = int(self.tables.lengths[b]), self.layers[layer]
         start = torch.tensor([0, n], dtype=torch.int32).to(self.device)
-        k, v = ops.kv_cache_read(kv, self.tables.page_table[b : b + 1].contiguous(), start, n, self.dtype)
+        k, v = ops.kv_cache_read(kv, self.tables.page_table[b][None], start, n, self.dtype)
         return k.view(n, *kv.k.shape[1::2]), v.view(n, *kv.v.shape[1::2])

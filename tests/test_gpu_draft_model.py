@@ -240,6 +240,15 @@ def test_more_than_a_step_takes_is_refused_before_anything_is_made():
     assert torch.cuda.max_memory_allocated() - before < 1 << 20  # the caches of 4097 sequences alone are 1 GB
 
 
+def test_reading_the_cache_counts_from_its_end_too():
+    model = _model(F32)
+    cache = _cache(model, 3, 40)
+    model.forward_cached(_ids(31), cache, cache.step([11, 9, 11]), rows="none")
+    for b in range(3):
+        for x, y in zip(cache.read(0, b - 3), cache.read(0, b)):
+            assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize("top_k", [None, 4])
 def test_a_draft_without_a_law_draws_from_all(top_k):
     """A draft model that has gone NaN costs tokens, and changes none."""
