@@ -8,6 +8,8 @@
 //   top = n_free + sum(held - left)
 //   served: (need = 0 or sum_{c <= b} need_c <= top) and sum_{c <= b} new_c <= rows
 //
+// (new_b that by itself passes max_new, max_len, the table or `rows` counts as 0
+// in these sums: it could not be served in any order and holds up nobody)
 // and row_start is the sum of the served sequences' new tokens.  Pages go back
 // so that the first sequence's first one is on top, and are taken from the top in
 // the same order: a step that keeps nothing of the last one's drafts gets the

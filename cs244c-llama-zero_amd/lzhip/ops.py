@@ -1286,13 +1286,14 @@ def cache_tables(tables, new: torch.Tensor, rows: int, max_new: int, max_len: in
     each sequence asks room for; keep: int32 [B], the tokens that it is cut to
     first (None: all that it has), whose pages go back; rows, max_new, max_len:
     bounds of all new tokens, and of the new and all tokens of a sequence.
-    Sequences are served in order: one whose tokens pass these bounds or the
-    table gets none, nor one that needs pages, or rows, where what it and those
-    before it ask for is more than there is (row_start says who got them).
-    parents: int32 [nodes] or [B, nodes] (up to 4096), the new tokens as trees: node i is
-    the token in place base[b] + i (base: int32 [B]; None: the kept length), its
-    parent a node before it or -1.  Then rows see their ancestors alone and are
-    rotated to base + their depth.  Up to 4096 sequences."""
+    Sequences are served in order: one whose own tokens pass one of these bounds
+    or the table gets none and counts for nothing; nor does one get any that
+    needs pages, or rows, where what it and those before it ask for is more than
+    there is (row_start says who got them).  parents: int32 [nodes] or [B,
+    nodes] (up to 4096), the new tokens as trees: node i is the token in place
+    base[b] + i (base: int32 [B]; None: the kept length), its parent a node
+    before it or -1.  Then rows see their ancestors alone and are rotated to
+    base + their depth.  Up to 4096 sequences."""
     from .cache import DraftStep
 
     start, length, at, positions, slots, mask = _lib.tensor_calls().cache_tables(tables, new, rows, max_new, max_len, keep,
@@ -1312,9 +1313,10 @@ def verify_draft(logits: torch.Tensor, tokens: torch.Tensor, row_start: torch.Te
     each.  p is their softmax at `temperature` (a number or float32 [B]; <= 0:
     the first of the largest logits); uniform: a number in [0, 1) for each row
     (float32 or float64; below 0, and NaN, counts as 0, from 1 on as just under
-    it).  Without draft_probs a token is chosen from p at each node with the node's number, and the child that holds it is kept (parents as
-    in cache_tables; None: a chain), which is the model's own choice at every
-    place whatever was drafted.  With draft_probs (float32 [rows, V], row r the
+    it).  Without draft_probs a token is chosen from p at each node with the
+    node's number, and the child that holds it is kept (parents as in
+    cache_tables; None: a chain), which is the model's own choice at every place
+    whatever was drafted.  With draft_probs (float32 [rows, V], row r the
     distribution that token r was drawn from), a chain's tokens are kept with
     probability min(1, p / q) and the token after them is chosen with the
     root's number from what is left of p.  counts: int32 [B], 0 for a sequence

@@ -478,10 +478,11 @@ int lz_tree_attn(const void* q, int64_t ldq, int dtype, int64_t rows, const void
  * (up to 4096) sequences is cut to keep[b] tokens (NULL: all; at most
  * lengths[b]), its pages behind them go back on the stack `free` (`pages`
  * values, of which n_free[0] are free), and it takes pages for add[b] more.
- * Sequences are served in order: one whose tokens pass max_new, max_len or the
- * table gets none, nor one that needs a page, or rows, where what it and those
- * before it ask for is more than there is.  Pages go back so that the first
- * sequence's first is on top, and are taken from the top in that order.
+ * Sequences are served in order: one whose own tokens pass max_new, max_len, the
+ * table or `rows` gets none and counts for nothing; nor does one get any that
+ * needs a page, or rows, where what it and those before it ask for is more than
+ * there is.  Pages go back so that the first sequence's first is on top, and are
+ * taken from the top in that order.
  * table, lengths, free and n_free are updated (table entries without a page
  * become -1); row_start (B + 1), kv_len and base (first[b]; NULL: the kept
  * length) are written, and for each of the `rows` (up to 2^28) rows its

@@ -549,6 +549,17 @@ def test_tables_over_many_steps(B):
         assert (step.rows, step.max_new, step.max_len) == tuple(args) and step.page_table is tables.page_table
 
 
+def test_an_ask_of_more_than_all_rows_holds_up_nobody():
+    """It could not be served in any order, so it counts for nothing; one that
+    does not fit beside those before it counts, and those behind it wait."""
+    for new, want in (([70, 3], [0, 0, 3]), ([6, 5], [0, 0, 5]), ([3, 3, 2], [0, 3, 3, 3])):
+        pool = Pool([4] * len(new), 8, 16, spare=16)
+        tables = pool.device()
+        step = ops.cache_tables(tables, _i32(new), 5, 70, 128)
+        assert step.row_start.tolist() == want
+        pool.check(tables, step, pool.step(new, 5, 70, 128))
+
+
 def test_tables_of_prompts():
     """More rows than one workgroup describes, sequences that do not all fit."""
     rng = random.Random(1)
