@@ -59,7 +59,10 @@ class DraftStep(NamedTuple):
     rows are rotated to), slots [rows] int64 (where a row is cached: page * page
     size + place in it, -1: nowhere), mask [rows, words] int32 (bit j of a row:
     it sees the token in place base + j; None: what comes before it, as in a
-    CacheStep).  Rows of no sequence hold -1, -1 and 0."""
+    CacheStep).  Rows of no sequence hold -1, -1 and 0.
+
+    page_table is that of the PageTables, not a copy: a step is for use before
+    the next ops.cache_tables on them, which may give its pages to others."""
 
     row_start: torch.Tensor
     kv_len: torch.Tensor

@@ -1282,7 +1282,8 @@ def cache_tables(tables, new: torch.Tensor, rows: int, max_new: int, max_len: in
     """A step's tables (cache.DraftStep), made on the device: nothing of what
     it depends on need be known to the host.
 
-    tables: cache.PageTables, which is updated; new: int32 [B], the tokens that
+    tables: cache.PageTables, which is updated (a step made of it before, whose
+    page_table it is, ends with this call); new: int32 [B], the tokens that
     each sequence asks room for; keep: int32 [B], the tokens that it is cut to
     first (None: all that it has), whose pages go back; rows, max_new, max_len:
     bounds of all new tokens, and of the new and all tokens of a sequence.
