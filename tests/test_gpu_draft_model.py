@@ -260,3 +260,46 @@ def test_a_draft_without_a_law_draws_from_all(top_k):
     assert out.shape == (2, 26) and torch.equal(out[:, :17], prompt) and bool(((out >= 0) & (out < 500)).all())
     want = model.generate(prompt, 9, temperature=0.0)
     assert torch.equal(model.generate(prompt, 9, temperature=1.0, top_k=1, draft_model=draft, draft_tokens=3), want)
+
+
+def test_a_servers_loop_in_which_sequences_end():
+    """One reaches the cache's max_len, and gets no rows from then on; those of
+    the others move up, and their texts go on as the model writes them."""
+    N, limit, steps = 5, 60, 9
+    model = _model(F32, max_seq_len=128)
+    prompts = [_ids(n, seed=30 + n) for n in (30, 50, 6)]
+    want = [model.generate(p[None], limit, temperature=0, use_cache=True)[0, len(p):] for p in prompts]
+    cache = _cache(model, 3, limit)
+    model.forward_cached(torch.cat([p[:-1] for p in prompts]), cache, cache.step([len(p) - 1 for p in prompts]), rows="none")
+    root = torch.stack([p[-1] for p in prompts])
+    start = cached = cache.tables.lengths.clone()
+    new = torch.full((3,), N, dtype=torch.int32, device=DEV)
+    parents = torch.tensor([-1, 0, 0, 2, 3], dtype=torch.int32, device=DEV)
+    depth = torch.tensor([0, 1, 1, 2, 3], device=DEV)
+    right = torch.stack(want)
+    texts, unserved = [[], [], []], 0
+    for _ in range(steps):
+        ids = right.gather(1, ((cached - start).long()[:, None] + depth - 1).clamp(0, limit - 1))
+        ids[:, 1] = (ids[:, 1] + 1) % 500  # a wrong branch beside the right one
+        ids[:, 0] = root
+        step = cache.step(new, rows=3 * N, max_new=N, keep=cached, parents=parents)
+        served = step.row_start.diff()
+        ids = ids[served.argsort(descending=True, stable=True)].view(-1)
+        logits = model.forward_cached(ids, cache, step, rows="all")
+        u = torch.rand(3 * N, dtype=torch.float64, device=DEV)
+        counts, kept, chosen = ops.verify_draft(logits, ids, step.row_start, N, u, temperature=0, parents=parents)
+        cache.keep(step, kept, counts)
+        last = chosen.gather(1, (counts.long() - 1).clamp(min=0)[:, None])[:, 0]
+        root = torch.where(served > 0, last, root)
+        cached = cached + counts
+        unserved += int((served == 0).sum())
+        for t, c, n in zip(texts, chosen.tolist(), counts.tolist()):
+            t += c[:n]
+    assert unserved > 0 and len(texts[1]) < len(texts[0]) and len(texts[2]) > 20
+    assert cached.tolist() == [len(p) - 1 + len(t) for p, t in zip(prompts, texts)] and max(cached.tolist()) <= limit
+    for t, w in zip(texts, want):
+        assert t == w[: len(t)].tolist()
+    cache.free(1)
+    new[1] = 0
+    first = N * (int(cached[0]) + N <= limit)
+    assert cache.step(new, rows=3 * N, max_new=N, keep=cached, parents=parents).row_start.tolist() == [0, first, first, first + N]
