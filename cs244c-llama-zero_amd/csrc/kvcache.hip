@@ -208,9 +208,17 @@ struct KeepArgs {
 // Moves the kept nodes of each sequence to its first slots of the step: node
 // kept[j]'s keys and values to slot j.  One thread per (layer, keys or values, kv
 // head, 16 bytes of a token), and gridDim.y for the sequences: it goes over the
-// nodes in their order, eight at a time, whose loads are in flight together.
+// nodes in their order, eight at a time, all of which it reads before it writes.
 // kept ascends, so kept[j] >= j: what a thread still has to read lies behind what
 // it has written, and no other thread touches its bytes.
+//
+// The eight are not in flight together: as compiled each one's 16 bytes go to
+// scratch (144 bytes a thread) and wait for the load, and that chain of loads
+// bounds it (32 sequences of up to 32 nodes, 32 layers of 8 heads of 128 in bf16:
+// 10.7 us for 22 MB).  Whether a node moves stands apart in moves[]: with -1 in
+// to[] for it and `continue` in place of the condition, hipcc of ROCm 7.2 held to[]
+// in one run of registers, wrote a comparison's operand into those of to[0] ahead
+// of a branch, and a token went to place slots_all.
 template <bool k8>
 __global__ void __launch_bounds__(256) kv_keep_kernel(KeepArgs a, int chunks) {
   constexpr int kAhead = 8;
@@ -234,7 +242,7 @@ __global__ void __launch_bounds__(256) kv_keep_kernel(KeepArgs a, int chunks) {
     return ((((slot >> a.log_size) * a.KV + g) << a.log_size) + (slot & mask));
   };
   for (int j0 = 0; j0 < count; j0 += kAhead) {
-    // each of these rounds in flight together: nodes, slots, tokens
+    // nodes, their slots, their tokens
     if (j0 > 0)
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) node[i] = a.kept[b * a.ldk + min(j0 + i, a.nodes - 1)];
