@@ -118,6 +118,14 @@ __host__ __device__ __forceinline__ uint32_t tree_bits(const uint32_t* row, int 
   return lo >> s | hi << (32 - s);
 }
 
+// Where the w-th stretch of `per` units of a list of `all` begins (all: there is
+// none).  Lengths on the device past the call's bound may make `per` as large as the
+// table, and w times that passes 32 bits.
+__host__ __device__ __forceinline__ int lz_stretch(int w, int per, int all) {
+  const int64_t at = (int64_t)w * per;
+  return at < all ? (int)at : all;
+}
+
 // Whether a row that sees `sees` keys sees one of k_lo .. k_hi - 1 (of pages
 // that there are).  A maximum of -inf says that it does not or that all its
 // scores are -inf: the former's output is zeros, the latter's NaN (0 / 0).  The

@@ -192,8 +192,8 @@ struct Share {
       most = max(most, __builtin_amdgcn_readlane(scan(units, 0, larger), 63));
     }
     per = max(max((all + a.shares - 1) / a.shares, (most + a.nsplit - 2) / (a.nsplit - 1)), a.least >> 7);
-    at = w * per;  // no more than all, or behind it
-    end = min(at + per, all);
+    at = lz_stretch(w, per, all);
+    end = lz_stretch(w + 1, per, all);
   }
 
   struct Block {

@@ -132,3 +132,29 @@ int main() {
 
 def test_lookups_stay_inside(tmp_path):
     run_on_host(tmp_path, LOOKUPS)
+
+
+STRETCHES = r"""
+#include "paged_attn.h"
+#include <cstdio>
+int main() {
+  int bad = 0;
+  // a list of any length, dealt out in order, inside it and without gaps
+  for (int all : {0, 1, 4, 127, 16777208, 2147483000, 2147483647})
+    for (int per : {1, 4, 4194303, 8388604, 16777208, 2147483647}) {
+      bad += lz_stretch(0, per, all) != 0;
+      for (int w = 0; w < 512; ++w) {
+        const int at = lz_stretch(w, per, all), end = lz_stretch(w + 1, per, all);
+        bad += at < 0 || at > end || end > all || (end < all && (long)end - at != per);
+      }
+    }
+  printf("%d\n", bad);
+  return bad != 0;
+}
+"""
+
+
+def test_shares_stay_inside(tmp_path):
+    """Lengths past the call's bound make shares as long as the page table: 512 of
+    8388604 units of 128 keys pass 32 bits."""
+    run_on_host(tmp_path, STRETCHES)
