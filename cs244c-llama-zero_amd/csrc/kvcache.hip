@@ -215,7 +215,8 @@ struct KeepArgs {
 // The eight are not in flight together: as compiled each one's 16 bytes go to
 // scratch (144 bytes a thread) and wait for the load, and that chain of loads
 // bounds it (32 sequences of up to 32 nodes, 32 layers of 8 heads of 128 in bf16:
-// 10.7 us for 22 MB).  Whether a node moves stands apart in moves[]: with -1 in
+// 10.7 us for 22 MB; a trial that kept them in registers, with a vector type for
+// uint4 and loads that no branch surrounds, took 6.6).  Whether a node moves stands apart in moves[]: with -1 in
 // to[] for it and `continue` in place of the condition, hipcc of ROCm 7.2 held to[]
 // in one run of registers, wrote a comparison's operand into those of to[0] ahead
 // of a branch, and a token went to place slots_all.
