@@ -429,6 +429,40 @@ def test_kept_branches_move(name, dtype, layers):
         assert torch.equal(got.view(want.dtype).cpu(), back)
 
 
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_kept_branches_move_whichever_of_them_are_left_out(dtype):
+    """Up to three rounds of eight nodes, of which any may have no slot, or one
+    past the pages, or be no node: the moves of the others do not change."""
+    KV, hd, page, n_pages, B = 2, 32, 16, 12, 4
+    bits = torch.uint8 if dtype == E4M3 else torch.int16
+    for seed in range(40):
+        rng, g = random.Random(seed), torch.Generator().manual_seed(seed)
+        new = [rng.randint(0, 24) for _ in range(B)]
+        rows, starts = sum(new), [sum(new[:b]) for b in range(B + 1)]
+        order = torch.randperm(n_pages * page, generator=g)[:rows].tolist()
+        odd = rng.choice([0.0, 0.1, 0.5])
+        slots = [rng.choice([-1, n_pages * page, 2**40]) if rng.random() < odd else s for s in order]
+        kept = [sorted(rng.sample(range(n), rng.randint(min(n, 1), n))) for n in new]
+        counts = [len(k) for k in kept]
+        kept = [[rng.choice([-1, 99, 2**31 - 1]) if rng.random() < odd else x for x in k] + [-1] * (24 - len(k)) for k in kept]
+        cpu = [torch.randint(0, 127, (n_pages, KV, page, hd), generator=g).to(bits) for _ in range(2)]
+        exps = [torch.randint(-9, 9, (n_pages, KV, page), generator=g).to(torch.int8) for _ in range(2)] if dtype == E4M3 else []
+        layer = LayerCache(*(t.to(DEV).view(dtype) for t in cpu), *([e.to(DEV) for e in exps] or [None, None]))
+        step = DraftStep(_i32(starts), _i32(new), _i32([[0]] * B), rows, 24, 64, _i32([0] * B), _i32([0] * rows),
+                         torch.tensor(slots, dtype=torch.int64, device=DEV))
+        ops.kv_cache_keep(layer, step, _i32(kept), _i32(counts))
+        inside = lambda x: 0 <= x < n_pages * page  # noqa: E731
+        for got, want in zip([x for x in layer if x is not None], [*cpu, *exps]):
+            flat = want.transpose(1, 2).reshape(n_pages * page, -1).clone()
+            old = flat.clone()
+            for b, n in enumerate(new):
+                for j in range(counts[b]):
+                    if 0 <= kept[b][j] < n and inside(src := slots[starts[b] + kept[b][j]]) and inside(dst := slots[starts[b] + j]):
+                        flat[dst] = old[src]
+            back = flat.view(n_pages, page, KV, *want.shape[3:]).transpose(1, 2)
+            assert torch.equal(got.view(want.dtype).cpu(), back), seed
+
+
 def test_keep_is_refused():
     layer = LayerCache(*(torch.zeros(4, 2, 16, 32, dtype=BF16, device=DEV) for _ in range(2)))
     step = DraftStep(_i32([0, 3]), _i32([3]), _i32([[0]]), 3, 3, 16, _i32([0]), _i32([0] * 3),
